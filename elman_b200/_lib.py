@@ -90,6 +90,9 @@ SIGNATURES = {
     "elman_e1_lm_token_workspace": (_Z, [_I] * 3),
     "elman_e1_lm_token": (_I, [_I] * 5 + [_P] * 5 + [_F] * 3 + [_P, _P, _Z, _P]),
     "elman_adamw_step": (_I, [_I, _L, _P, _P, _P, _P] + [_c.c_float] * 5 + [_P, _P, _P]),
+    "elman_gated_linear_workspace": (_Z, [_I] * 4),
+    "elman_gated_linear_forward": (_I, [_I] * 5 + [_P] * 9 + [_P, _Z, _P]),
+    "elman_gated_linear_backward": (_I, [_I] * 4 + [_P] * 12 + [_P, _Z, _P]),
     "elman_projection": (_I, [_I, _I, _I, _I, _P, _I, _P, _I, _P, _P, _I, _I, _P]),
 }
 

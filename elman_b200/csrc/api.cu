@@ -1694,3 +1694,83 @@ int elman_adamw_step(int dtype, long n, void* params, const void* grads, void* e
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------
+// gated linear recurrence
+// ---------------------------------------------------------------------------
+// No two elements of a [T, B, d] output may share an address.
+static bool distinct_elements(int T, int B, int d, const long* s) {
+  if (T > 1 && s[0] < d) return false;
+  if (B > 1 && s[1] < d) return false;
+  if (T <= 1 || B <= 1) return true;
+  return s[0] >= (B - 1) * s[1] + d || s[1] >= (T - 1) * s[0] + d;
+}
+
+static int check_gated_linear(int dtype, int T, int B, int d, const long* strides, int n_in, int n_out) {
+  ELMAN_RETURN_IF(check_common(dtype, T, B, d));
+  REQUIRE_PTR(strides);
+  for (int k = 0; k < 2 * (n_in + n_out); ++k)
+    ELMAN_ARG_CHECK(strides[k] >= 0, "negative stride");
+  for (int k = n_in; k < n_in + n_out; ++k)
+    ELMAN_ARG_CHECK(distinct_elements(T, B, d, strides + 2 * k), "an output's rows overlap");
+  return ELMAN_OK;
+}
+
+extern "C" {
+
+size_t elman_gated_linear_workspace(int dtype, int T, int B, int d) {
+  if (T < 0 || B < 0 || d < 0) return 0;
+  return gated_linear_workspace(dtype, T, B, d);
+}
+
+int elman_gated_linear_forward(int dtype, int training, int T, int B, int d, const void* f,
+                               const void* c, const void* z, const float* h0,
+                               const unsigned char* reset, const long* strides, void* y,
+                               float* h_last, float* saved, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  ELMAN_RETURN_IF(check_gated_linear(dtype, T, B, d, strides, 3, 1));
+  if ((long)B * d == 0) return ELMAN_OK;
+  REQUIRE_PTR(h_last);
+  if (T > 0) {
+    REQUIRE_PTR(f); REQUIRE_PTR(c); REQUIRE_PTR(z); REQUIRE_PTR(y);
+    if (training) REQUIRE_PTR(saved);
+  }
+  const size_t need = gated_linear_workspace(dtype, T, B, d);
+  if (need > 0) REQUIRE_PTR(workspace);
+  if (workspace_bytes < need)
+    return set_error(ELMAN_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  GatedLinearArgs a{};
+  a.T = T; a.B = B; a.d = d; a.f = f; a.c = c; a.z = z;
+  a.f_strides = strides; a.c_strides = strides + 2; a.z_strides = strides + 4; a.y_strides = strides + 6;
+  a.df_strides = a.dc_strides = a.dz_strides = strides + 6;
+  a.reset = reset; a.saved = training ? saved : nullptr; a.h0 = h0; a.y = y; a.h_last = h_last;
+  a.workspace = workspace;
+  return gated_linear_fwd(dtype, a, (cudaStream_t)stream);
+}
+
+int elman_gated_linear_backward(int dtype, int T, int B, int d, const void* f, const void* c,
+                                const void* z, const float* saved, const void* d_output,
+                                const float* dh_last, const unsigned char* reset, const long* strides,
+                                void* df, void* dc, void* dz, float* dh0, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  ELMAN_RETURN_IF(check_gated_linear(dtype, T, B, d, strides, 4, 3));
+  if ((long)B * d == 0) return ELMAN_OK;
+  REQUIRE_PTR(dh0);
+  if (T > 0) {
+    REQUIRE_PTR(f); REQUIRE_PTR(c); REQUIRE_PTR(z); REQUIRE_PTR(saved); REQUIRE_PTR(d_output);
+    REQUIRE_PTR(df); REQUIRE_PTR(dc); REQUIRE_PTR(dz);
+  }
+  const size_t need = gated_linear_workspace(dtype, T, B, d);
+  if (need > 0) REQUIRE_PTR(workspace);
+  if (workspace_bytes < need)
+    return set_error(ELMAN_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  GatedLinearArgs a{};
+  a.T = T; a.B = B; a.d = d; a.f = f; a.c = c; a.z = z; a.dy = d_output;
+  a.f_strides = strides; a.c_strides = strides + 2; a.z_strides = strides + 4; a.y_strides = strides + 6;
+  a.df_strides = strides + 8; a.dc_strides = strides + 10; a.dz_strides = strides + 12;
+  a.reset = reset; a.saved = const_cast<float*>(saved); a.dh_last = dh_last;
+  a.df = df; a.dc = dc; a.dz = dz; a.dh0 = dh0; a.workspace = workspace;
+  return gated_linear_bwd(dtype, a, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -365,6 +365,24 @@ int lowrank_tc(const LowRankTcArgs& a, cudaStream_t stream);
 int gemm_tc_dual_tn(int M, int N, int K, const bf16* A, const bf16* B1, const bf16* B2, void* C1,
                     void* C2, cudaStream_t stream);
 
+// Gated linear recurrence (gated_linear.cu).  Strides are element strides over (t, b); channels are dense.
+constexpr int GL_CHUNK = ELMAN_GATED_LINEAR_CHUNK;
+struct GatedLinearArgs {
+  int T, B, d;
+  const void *f, *c, *z;
+  const long *f_strides, *c_strides, *z_strides, *y_strides;   // y_strides: y, or dy in the backward pass
+  const unsigned char* reset;                                  // [T, B] or null
+  float* saved;                                                // [ceil(T / GL_CHUNK), B, d] or null (forward)
+  const float* h0; void* y; float* h_last;                     // forward
+  const void* dy; const float* dh_last;                        // backward
+  void *df, *dc, *dz; float* dh0;
+  const long *df_strides, *dc_strides, *dz_strides;
+  void* workspace;
+};
+size_t gated_linear_workspace(int dtype, int T, int B, int d);
+int gated_linear_fwd(int dtype, const GatedLinearArgs& a, cudaStream_t stream);
+int gated_linear_bwd(int dtype, const GatedLinearArgs& a, cudaStream_t stream);
+
 // Spectral normalisation of a [d, d] matrix (csrc/spectral.cu): three power-iteration steps
 // from u (advanced in place), v and sigma saved for the backward pass.
 int spectral_norm_fwd(int dtype, int d, const void* W, void* u, float* v, float* sigma, void* W_eff,

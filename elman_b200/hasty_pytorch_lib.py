@@ -14,6 +14,8 @@ to this module, so the reference's model files pick it up unchanged.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -45,6 +47,10 @@ def _shape(fn, t, shape, name):
 
 def _ptr(t):
     return None if t is None or t.numel() == 0 else t.data_ptr()
+
+
+def _opt(t):
+    return None if t is None else t.data_ptr()
 
 
 def _workspace(nbytes, device):
@@ -801,3 +807,127 @@ def e33_self_gate_backward(W_x, W_h, x, h, v, d_output):
         _lib.check(rc, fn)
         ws.record_stream(torch.cuda.current_stream(x.device))
     return [dx, dW_x, dW_h, db]
+
+
+# --------------------------------------------------------------------------- gated linear recurrence
+
+GATED_LINEAR_CHUNK = 64   # ELMAN_GATED_LINEAR_CHUNK: steps between the states kept for the backward pass
+
+
+def _check_sequences(fn, ref, **tensors):
+    """[T, B, d] tensors of one dtype and device whose channels are dense; the strides over t and b are
+    free (slices of one projection, batch-major tensors seen through transpose(0, 1))."""
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{fn}: {name} must be a Tensor")
+        if not t.is_cuda:
+            raise RuntimeError(f"{fn}: {name} must be a CUDA tensor")
+        if t.dim() != 3:
+            raise RuntimeError(f"{fn}: {name} must be [T, B, dim]")
+        if t.dtype != ref.dtype:
+            raise RuntimeError(f"{fn}: {name} has dtype {t.dtype}, expected {ref.dtype}")
+        if t.device != ref.device:
+            raise RuntimeError(f"{fn}: {name} is on {t.device}, expected {ref.device}")
+        _shape(fn, t, ref.shape, name)
+        if t.shape[2] > 1 and t.stride(2) != 1:
+            raise RuntimeError(f"{fn}: {name} must have dense channels (stride 1 over the last dimension)")
+    if ref.dtype not in _DT:
+        raise RuntimeError(f"{fn}: dtype {ref.dtype} is not supported (float32 and bfloat16 are)")
+    return _DT[ref.dtype]
+
+
+def _check_state(fn, t, name, shape, device):
+    """An fp32 state [B, d] (None: zeros)."""
+    if t is None:
+        return
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device != device:
+        raise RuntimeError(f"{fn}: {name} must be a CUDA tensor on {device}")
+    if t.dtype != torch.float32:
+        raise RuntimeError(f"{fn}: {name} has dtype {t.dtype}; states are float32")
+    _shape(fn, t, shape, name)
+    if not t.is_contiguous():
+        raise RuntimeError(f"{fn}: {name} must be contiguous")
+
+
+def _check_reset(fn, reset, T, B, device):
+    if reset is None:
+        return
+    if not isinstance(reset, torch.Tensor) or reset.dtype != torch.bool or reset.device != device:
+        raise RuntimeError(f"{fn}: reset must be a bool tensor on {device}")
+    _shape(fn, reset, (T, B), "reset")
+    if not reset.is_contiguous():
+        raise RuntimeError(f"{fn}: reset must be contiguous")
+
+
+def _sequence_like(x):
+    """A dense [T, B, d] tensor in x's order of t and b (batch-major x: a view of a [B, T, d] one)."""
+    T, B, d = x.shape
+    if T > 1 and B > 1 and x.stride(0) < x.stride(1):
+        return torch.empty(B, T, d, dtype=x.dtype, device=x.device).transpose(0, 1)
+    return torch.empty(T, B, d, dtype=x.dtype, device=x.device)
+
+
+def _tb_strides(*tensors):
+    flat = [s for t in tensors for s in (t.stride(0), t.stride(1))]
+    return (ctypes.c_long * len(flat))(*flat)
+
+
+def gated_linear_forward(training, f, c, z, h0=None, reset=None):
+    """u = sigmoid(-f), h_t = p_t + u_t (c_t - p_t) with p_t = h_{t-1} (0 where reset[t,b]), y = h silu(z)
+    -> [y [T,B,d], h_last [B,d] float32, saved (for the backward pass; empty if not training)].
+
+    f, c, z: [T,B,d] with dense channels and any strides over t and b; h0 [B,d] float32 or None (zeros);
+    reset [T,B] bool or None.  The state is float32 whatever the dtype: generation feeds h_last back as
+    h0, one token a call.  No counterpart in the reference."""
+    fn = "gated_linear_forward"
+    dt = _check_sequences(fn, f, f=f, c=c, z=z)
+    T, B, d = f.shape
+    _check_state(fn, h0, "h0", (B, d), f.device)
+    _check_reset(fn, reset, T, B, f.device)
+    lib = _lib.load()
+    with torch.cuda.device(f.device):
+        y = _sequence_like(f)
+        h_last = torch.empty(B, d, dtype=torch.float32, device=f.device)
+        rows = -(-T // GATED_LINEAR_CHUNK) if training else 0
+        saved = torch.empty((rows, B, d) if training else (0,), dtype=torch.float32, device=f.device)
+        ws = _workspace(lib.elman_gated_linear_workspace(dt, T, B, d), f.device)
+        rc = lib.elman_gated_linear_forward(
+            dt, 1 if training else 0, T, B, d, f.data_ptr(), c.data_ptr(), z.data_ptr(), _opt(h0),
+            _opt(reset), _tb_strides(f, c, z, y), y.data_ptr(), h_last.data_ptr(), saved.data_ptr(),
+            ws.data_ptr(), ws.numel(), _stream(f.device))
+        _lib.check(rc, fn)
+    return [y, h_last, saved]
+
+
+def gated_linear_backward(f, c, z, saved, d_output, dh_last=None, reset=None, out=None):
+    """-> [df, dc, dz, dh0 [B,d] float32] for the forward call on the same f, c, z and reset.
+
+    dh_last [B,d] float32 or None: gradient of the last state.  out: three [T,B,d] tensors with dense
+    channels to write df, dc, dz to (slices of one gradient buffer), sharing no storage with the inputs."""
+    fn = "gated_linear_backward"
+    dt = _check_sequences(fn, f, f=f, c=c, z=z, d_output=d_output)
+    T, B, d = f.shape
+    _check_state(fn, dh_last, "dh_last", (B, d), f.device)
+    _check_reset(fn, reset, T, B, f.device)
+    if T > 0 and saved.numel() == 0 and B * d > 0:
+        raise RuntimeError(f"{fn}: saved is empty: run the forward pass with training=True")
+    _check_state(fn, saved, "saved", (-(-T // GATED_LINEAR_CHUNK), B, d), f.device)
+    lib = _lib.load()
+    with torch.cuda.device(f.device):
+        if out is None:
+            df, dc, dz = (_sequence_like(f) for _ in range(3))
+        else:
+            df, dc, dz = out
+            _check_sequences(fn, f, df=df, dc=dc, dz=dz)
+            used = {t.untyped_storage().data_ptr() for t in (f, c, z, saved, d_output)}
+            if any(t.untyped_storage().data_ptr() in used for t in out if t.numel() > 0):
+                raise RuntimeError(f"{fn}: out must not share storage with the inputs")
+        dh0 = torch.empty(B, d, dtype=torch.float32, device=f.device)
+        ws = _workspace(lib.elman_gated_linear_workspace(dt, T, B, d), f.device)
+        rc = lib.elman_gated_linear_backward(
+            dt, T, B, d, f.data_ptr(), c.data_ptr(), z.data_ptr(), saved.data_ptr(),
+            d_output.data_ptr(), _opt(dh_last), _opt(reset),
+            _tb_strides(f, c, z, d_output, df, dc, dz), df.data_ptr(), dc.data_ptr(), dz.data_ptr(),
+            dh0.data_ptr(), ws.data_ptr(), ws.numel(), _stream(f.device))
+        _lib.check(rc, fn)
+    return [df, dc, dz, dh0]

@@ -569,6 +569,35 @@ int elman_e1_lm_token(int dtype, int depth, int B, int d, int vocab, const long 
                       const void* head, float eps, float target_radius, float spectral_eps,
                       void* logits, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Gated linear recurrence: the Elman recurrence with an elementwise, input-gated linear state in place
+ * of tanh(W_h h), and E1's output gate (an extension without a counterpart in the reference).  Per
+ * channel, with an fp32 state:
+ *     u_t = sigmoid(-f_t);  p_t = reset[t,b] ? 0 : h_{t-1};  h_t = p_t + u_t (c_t - p_t)
+ *     y_t = h_t silu(z_t)
+ * f, c, z, y, d_output, df, dc, dz are [T,B,d] of `dtype` with dense channels and any element strides
+ * over t and b: `strides` holds a (t, b) pair for f, c, z, y (forward) resp. f, c, z, d_output, df, dc,
+ * dz (backward), read on the host.  Slices of one projection and batch-major tensors are read in place.
+ * Outputs must not overlap anything else of the call.  The states are fp32 in either dtype: h0 [B,d] (NULL:
+ * zeros), h_last [B,d] (the state after step T-1), dh_last [B,d] (NULL: zeros), dh0 [B,d].
+ * reset [T,B] (NULL: none): non-zero where step t starts a new sequence and forgets the state.
+ * saved [ceil(T / ELMAN_GATED_LINEAR_CHUNK), B, d] fp32: written by the forward call with `training`, read
+ * by the backward call, which takes the inputs of that forward call again.  T = 1 is the generation step.
+ * elman_gated_linear_workspace covers both directions; 0 bytes: none is needed.
+ */
+#define ELMAN_GATED_LINEAR_CHUNK 64
+size_t elman_gated_linear_workspace(int dtype, int T, int B, int d);
+int elman_gated_linear_forward(int dtype, int training, int T, int B, int d, const void* f,
+                               const void* c, const void* z, const float* h0,
+                               const unsigned char* reset, const long* strides, void* y,
+                               float* h_last, float* saved, void* workspace, size_t workspace_bytes,
+                               void* stream);
+int elman_gated_linear_backward(int dtype, int T, int B, int d, const void* f, const void* c,
+                                const void* z, const float* saved, const void* d_output,
+                                const float* dh_last, const unsigned char* reset, const long* strides,
+                                void* df, void* dc, void* dz, float* dh0, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
