@@ -92,7 +92,8 @@ int* device_status_ptr();   // device-side alias, or nullptr if unavailable
 
 // kernel ids recorded in the status word
 enum KernelId { KID_REC_SIMT = 1, KID_REC_TC_FWD = 2, KID_REC_TC_BWD = 3, KID_GEMM_TC = 4,
-                KID_LOWRANK_SIMT = 5, KID_WAIT_PROBE = 6, KID_LOWRANK_TC = 7, KID_LM_TOKEN = 8 };
+                KID_LOWRANK_SIMT = 5, KID_WAIT_PROBE = 6, KID_LOWRANK_TC = 7, KID_LM_TOKEN = 8,
+                KID_GATED_LINEAR = 9 };
 
 // ---------------------------------------------------------------------------
 // device helpers
