@@ -134,42 +134,112 @@ struct GlChain {             // workspace; all of it starts as NOT_YET
 };
 
 struct Pair { float R, H; };
-__device__ __forceinline__ float pass(float S, Pair a) { return a.R < 0.f ? a.H : S + fmaf(-a.R, S, a.H); }
-__device__ __forceinline__ Pair join(Pair a, Pair b) {       // a, then b
-  if (b.R < 0.f) return b;
-  return Pair{a.R < 0.f ? -1.f : a.R + fmaf(-b.R, a.R, b.R), a.H + fmaf(-b.R, a.H, b.H)};
+template <bool RESET> __device__ __forceinline__ float pass(float S, Pair a) {
+  return RESET && a.R < 0.f ? a.H : S + fmaf(-a.R, S, a.H);
+}
+template <bool RESET> __device__ __forceinline__ Pair join(Pair a, Pair b) {       // a, then b
+  const Pair ab = Pair{RESET && a.R < 0.f ? -1.f : a.R + fmaf(-b.R, a.R, b.R), a.H + fmaf(-b.R, a.H, b.H)};
+  return RESET && b.R < 0.f ? b : ab;
+}
+
+// The V channels of a lane; two of them are one packed fp32x2 operand (half the instructions: at HBM
+// speed the forward kernel has 44 issue slots for a warp's 32 elements, the backward kernel 76).
+template <int V> struct Vec;
+template <> struct Vec<1> {
+  float x;
+  __device__ __forceinline__ Vec() {}
+  __device__ __forceinline__ explicit Vec(float s) : x(s) {}
+  __device__ __forceinline__ float get(int) const { return x; }
+  __device__ __forceinline__ void set(int, float s) { x = s; }
+};
+template <> struct Vec<2> {
+  float x[2];
+  __device__ __forceinline__ Vec() {}
+  __device__ __forceinline__ explicit Vec(float s) { x[0] = x[1] = s; }
+  __device__ __forceinline__ float get(int v) const { return x[v]; }
+  __device__ __forceinline__ void set(int v, float s) { x[v] = s; }
+};
+__device__ __forceinline__ Vec<1> vfma(Vec<1> a, Vec<1> b, Vec<1> c) { return Vec<1>(fmaf(a.x, b.x, c.x)); }
+__device__ __forceinline__ Vec<1> vmul(Vec<1> a, Vec<1> b) { return Vec<1>(a.x * b.x); }
+__device__ __forceinline__ Vec<1> vadd(Vec<1> a, Vec<1> b) { return Vec<1>(a.x + b.x); }
+__device__ __forceinline__ Vec<1> vsub(Vec<1> a, Vec<1> b) { return Vec<1>(a.x - b.x); }
+#define ELMAN_PACKED(op, ...)                                                                        \
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"                                                               \
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t" op ";\n\t"         \
+      "mov.b64 {%0, %1}, d;\n\t}"                                                                    \
+      : "=f"(r.x[0]), "=f"(r.x[1])                                                                   \
+      : __VA_ARGS__)
+#define ELMAN_HALVES(v) "f"((v).x[0]), "f"((v).x[1])
+__device__ __forceinline__ Vec<2> vfma(Vec<2> a, Vec<2> b, Vec<2> c) {
+  Vec<2> r;
+  ELMAN_PACKED("fma.rn.f32x2 d, a, b, c", ELMAN_HALVES(a), ELMAN_HALVES(b), ELMAN_HALVES(c));
+  return r;
+}
+__device__ __forceinline__ Vec<2> vmul(Vec<2> a, Vec<2> b) {
+  Vec<2> r;
+  ELMAN_PACKED("mul.rn.f32x2 d, a, b", ELMAN_HALVES(a), ELMAN_HALVES(b), ELMAN_HALVES(b));
+  return r;
+}
+__device__ __forceinline__ Vec<2> vadd(Vec<2> a, Vec<2> b) {
+  Vec<2> r;
+  ELMAN_PACKED("add.rn.f32x2 d, a, b", ELMAN_HALVES(a), ELMAN_HALVES(b), ELMAN_HALVES(b));
+  return r;
+}
+__device__ __forceinline__ Vec<2> vsub(Vec<2> a, Vec<2> b) { return vfma(b, Vec<2>(-1.f), a); }   // exact product: one rounding
+
+__device__ __forceinline__ float exp2_(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+// 1 / (1 + exp2(x)); e receives exp2(x)
+template <int V> __device__ __forceinline__ Vec<V> gate_of(Vec<V> x, Vec<V>& e) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) e.set(v, exp2_(x.get(v)));
+  const Vec<V> den = vadd(e, Vec<V>(1.f));
+  Vec<V> r;
+#pragma unroll
+  for (int v = 0; v < V; ++v) r.set(v, rcp_(den.get(v)));
+  return r;
 }
 
 template <typename T, int V> struct Lane;                    // V adjacent channels as they are in memory
 template <> struct Lane<float, 1> {
   typedef float Raw;
-  static __device__ __forceinline__ void get(Raw r, float (&x)[1]) { x[0] = r; }
-  static __device__ __forceinline__ Raw put(const float (&x)[1]) { return x[0]; }
+  static __device__ __forceinline__ Vec<1> get(Raw r) { return Vec<1>(r); }
+  static __device__ __forceinline__ Raw put(Vec<1> v) { return v.x; }
 };
 template <> struct Lane<bf16, 1> {
   typedef unsigned short Raw;
-  static __device__ __forceinline__ void get(Raw r, float (&x)[1]) { x[0] = __uint_as_float((uint32_t)r << 16); }
-  static __device__ __forceinline__ Raw put(const float (&x)[1]) { return __bfloat16_as_ushort(__float2bfloat16_rn(x[0])); }
+  static __device__ __forceinline__ Vec<1> get(Raw r) { return Vec<1>(__uint_as_float((uint32_t)r << 16)); }
+  static __device__ __forceinline__ Raw put(Vec<1> v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v.x)); }
 };
 template <> struct Lane<bf16, 2> {
   typedef uint32_t Raw;
-  static __device__ __forceinline__ void get(Raw r, float (&x)[2]) {
-    x[0] = __uint_as_float(r << 16);
-    x[1] = __uint_as_float(r & 0xFFFF0000u);
+  static __device__ __forceinline__ Vec<2> get(Raw r) {
+    Vec<2> v;
+    v.x[0] = __uint_as_float(r << 16);
+    v.x[1] = __uint_as_float(r & 0xFFFF0000u);
+    return v;
   }
-  static __device__ __forceinline__ Raw put(const float (&x)[2]) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(x[0], x[1]);
-    return *reinterpret_cast<const Raw*>(&v);
+  static __device__ __forceinline__ Raw put(Vec<2> v) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(v.x[0], v.x[1]);
+    return *reinterpret_cast<const Raw*>(&p);
   }
 };
 
 __device__ __forceinline__ uint32_t word_of(float x) { return x != x ? 0x7FFFFFFFu : __float_as_uint(x); }
-template <int V> __device__ __forceinline__ void publish(float2* at, const Pair (&a)[V]) {
-  if constexpr (V == 2)
-    asm volatile("st.relaxed.gpu.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(at), "r"(word_of(a[0].R)), "r"(word_of(a[0].H)),
-                 "r"(word_of(a[1].R)), "r"(word_of(a[1].H)) : "memory");
-  else
-    asm volatile("st.relaxed.gpu.global.v2.b32 [%0], {%1, %2};" ::"l"(at), "r"(word_of(a[0].R)), "r"(word_of(a[0].H)) : "memory");
+__device__ __forceinline__ void publish(float2* at, Pair a) {
+  asm volatile("st.relaxed.gpu.global.v2.b32 [%0], {%1, %2};" ::"l"(at), "r"(word_of(a.R)), "r"(word_of(a.H)) : "memory");
+}
+__device__ __forceinline__ void publish(float* at, float x) {
+  asm volatile("st.relaxed.gpu.global.b32 [%0], %1;" ::"l"(at), "r"(word_of(x)) : "memory");
 }
 template <int N> __device__ __forceinline__ bool look(const void* at, uint32_t (&w)[N]) {
   if constexpr (N == 4)
@@ -210,80 +280,74 @@ template <int N> __device__ __forceinline__ bool await(const void* at, uint32_t 
   return true;
 }
 
-// Where a tile stands in the chain: `n` counts tiles from the end of time the scan starts at.
-template <int V, int W> struct Chain {
-  struct Shared {
-    Pair own[2][W][32 * V];             // the warps' pairs (two tiles' worth: a slow warp may still read the last one's)
-    Pair before[2][GROUP - 1][32 * V];  // pairs of the tiles before in the group
-    float start[2][32 * V];             // state at the group's start
-    int next;
-    int gave_up;
-  };
-  // From the warp's own pair to the state that enters it.  All W warps (w = order in the scan's
-  // direction) call it; `initial` is the state at the scan's start.  False: a wait gave up.
-  static __device__ __forceinline__ bool enter(Shared& sh, int buf, int w, int warps, const Pair (&mine)[V], int n,
-                                               int tiles, long col, long cols, bool lane_on, const float (&initial)[V],
-                                               const GlChain& ch, int ticket, uint32_t* grabbed, float (&S)[V]) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int v = 0; v < V; ++v) sh.own[buf][w][lane * V + v] = mine[v];
-    __syncthreads();
-    const int first = n / GROUP * GROUP, in_group = n - first;
-    const bool last_of_group = in_group == GROUP - 1;
-    if (tiles > 1) {
-      bool ok = true;
-      if (w == 0 && n + 1 < tiles && !last_of_group && ticket != ch.stall) {
-        Pair all[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          all[v] = sh.own[buf][0][lane * V + v];
-          for (int k = 1; k < warps; ++k) all[v] = join(all[v], sh.own[buf][k][lane * V + v]);
-        }
-        if (lane_on) publish<V>(ch.pairs + (long)n * cols + col, all);
-      }
-      for (int k = w; k < in_group && ok; k += warps) {
-        uint32_t x[2 * V];
-        ok = await<2 * V>(ch.pairs + (long)(first + k) * cols + col, x, ch, n);
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          sh.before[buf][k][lane * V + v] = Pair{__uint_as_float(x[2 * v]), __uint_as_float(x[2 * v + 1])};
-      }
-      if (w == warps - 1) {
-        uint32_t x[V];
-        if (first > 0 && ok) ok = await<V>(ch.states + (long)(first / GROUP - 1) * cols + col, x, ch, n);
-#pragma unroll
-        for (int v = 0; v < V; ++v) sh.start[buf][lane * V + v] = first > 0 ? __uint_as_float(x[v]) : initial[v];
-      }
-      if (!ok && lane == 0) sh.gave_up = 1;
-      if (threadIdx.x == 0) sh.next = (int)(*grabbed + 1u);
-      __syncthreads();
-      if (sh.gave_up) return false;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        S[v] = sh.start[buf][lane * V + v];
-        for (int k = 0; k < in_group; ++k) S[v] = pass(S[v], sh.before[buf][k][lane * V + v]);
-      }
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) S[v] = initial[v];
-    }
-    if (w == 0 && last_of_group && n + 1 < tiles && ticket != ch.stall) {
-      float end[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        end[v] = S[v];
-        for (int k = 0; k < warps; ++k) end[v] = pass(end[v], sh.own[buf][k][lane * V + v]);
-        if (lane_on)
-          asm volatile("st.relaxed.gpu.global.b32 [%0], %1;" ::"l"(ch.states + (long)(first / GROUP) * cols + col + v),
-                       "r"(word_of(end[v])) : "memory");
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      for (int k = 0; k < w; ++k) S[v] = pass(S[v], sh.own[buf][k][lane * V + v]);
-    return true;
-  }
+// What the warps of a block share.  Two buffers: a slow warp may still read the last tile's.
+template <int V, int W> struct Shared {
+  Pair own[2][W][32 * V];             // the warps' pairs, in the scan's direction
+  Pair before[2][GROUP - 1][32 * V];  // pairs of the tiles before in the group
+  float start[2][32 * V];             // state at the group's start
+  float enters[2][W][32 * V];         // state that enters each warp
+  int next;                           // the block's next tile
+  int gave_up;
 };
+
+// From the warps' pairs to the state that enters each: all threads call it; `n` counts tiles and `w` warps in
+// the scan's direction; lane's channels start at `col`; `initial` is the state at the scan's start.  False: a
+// wait gave up.
+template <int V, int W, bool RESET>
+__device__ __forceinline__ bool enter(Shared<V, W>& sh, int buf, int w, int warps, Vec<V> R, Vec<V> H, int n, int tiles,
+                                      long col, long cols, bool lane_on, Vec<V> initial, const GlChain& ch, int ticket,
+                                      uint32_t grabbed, Vec<V>& S) {
+  const int lane = threadIdx.x & 31, x = threadIdx.x;
+#pragma unroll
+  for (int v = 0; v < V; ++v) sh.own[buf][w][lane * V + v] = Pair{R.get(v), H.get(v)};
+  const int first = n / GROUP * GROUP, in_group = n - first;
+  const bool ends_group = in_group == GROUP - 1, more = n + 1 < tiles && ticket != ch.stall;
+  if (w == 0 && first == 0) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) sh.start[buf][lane * V + v] = initial.get(v);
+  }
+  __syncthreads();
+  const long base = col - lane * V, mine = base + x;     // one thread per channel from here to the last barrier
+  const bool on = x < 32 * V && mine < cols;
+  if (on && more && !ends_group) {
+    Pair all = sh.own[buf][0][x];
+    for (int k = 1; k < warps; ++k) all = join<RESET>(all, sh.own[buf][k][x]);
+    publish(ch.pairs + (long)n * cols + mine, all);
+  }
+  if (in_group > 0 || first > 0) {
+    bool ok = true;
+    for (int k = w; k < in_group && ok; k += warps) {
+      uint32_t g[2 * V];
+      ok = await<2 * V>(ch.pairs + (long)(first + k) * cols + (lane_on ? col : cols - V), g, ch, n);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        sh.before[buf][k][lane * V + v] = Pair{__uint_as_float(g[2 * v]), __uint_as_float(g[2 * v + 1])};
+    }
+    if (w == warps - 1 && first > 0 && ok) {
+      uint32_t g[V];
+      ok = await<V>(ch.states + (long)(first / GROUP - 1) * cols + (lane_on ? col : cols - V), g, ch, n);
+#pragma unroll
+      for (int v = 0; v < V; ++v) sh.start[buf][lane * V + v] = __uint_as_float(g[v]);
+    }
+    if (!ok && lane == 0) sh.gave_up = 1;
+  }
+  if (tiles > 1 && x == 0) sh.next = (int)(grabbed + 1u);
+  if (tiles > 1) __syncthreads();
+  if (sh.gave_up) return false;
+  if (x < 32 * V) {
+    float s = sh.start[buf][x];
+    for (int k = 0; k < in_group; ++k) s = pass<RESET>(s, sh.before[buf][k][x]);
+    for (int k = 0; k < warps; ++k) {
+      sh.enters[buf][k][x] = s;
+      s = pass<RESET>(s, sh.own[buf][k][x]);
+    }
+    if (on && more && ends_group) publish(ch.states + (long)(first / GROUP) * cols + mine, s);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < V; ++v) S.set(v, sh.enters[buf][w][lane * V + v]);
+  return true;
+}
 
 // Steps of a warp whose document starts anew, as bits (lanes of one batch row agree).
 template <int L> __device__ __forceinline__ uint32_t reset_bits(const GlParams& p, int t0, int b) {
@@ -293,16 +357,62 @@ template <int L> __device__ __forceinline__ uint32_t reset_bits(const GlParams& 
     if (t0 + l < p.T && p.reset[(long)(t0 + l) * p.B + b] != 0) bits |= 1u << l;
   return bits;
 }
+template <int V> __device__ __forceinline__ Vec<V> unless(bool cut, Vec<V> x) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) x.set(v, cut ? 0.f : x.get(v));
+  return x;
+}
 
-constexpr int FW = 8, FL = 16;      // forward tile: 128 steps
+// L rows of a tensor, this lane's channels; rows past the end repeat the last one.
+template <typename T, int V, int L>
+__device__ __forceinline__ void load_rows(typename Lane<T, V>::Raw (&r)[L], const void* base, Strides s, int t0, int T_, int b, int i) {
+  typedef typename Lane<T, V>::Raw Raw;
+  const char* at = (const char*)base + (b * s.b + i) * (long)sizeof(T);
+  const long step = s.t * (long)sizeof(T);
+  if (t0 + L <= T_) {
+    at += t0 * step;
+#pragma unroll
+    for (int l = 0; l < L; ++l) r[l] = __ldcs(reinterpret_cast<const Raw*>(at + l * step));
+  } else {
+#pragma unroll
+    for (int l = 0; l < L; ++l) r[l] = __ldcs(reinterpret_cast<const Raw*>(at + (t0 + l < T_ ? t0 + l : T_ - 1) * step));
+  }
+}
+
+#ifndef GLV_FW
+#define GLV_FW 8
+#define GLV_FL 16
+#define GLV_FB 2
+#define GLV_BB 2
+#endif
+constexpr int FW = GLV_FW, FL = GLV_FL;      // forward tile: 128 steps
 constexpr int BW = 8, BL = 8;       // backward tile: GL_CHUNK steps, so that it starts at a saved state
 static_assert(BW * BL == GL_CHUNK && GL_CHUNK % FL == 0, "saved states lie on tile and warp edges");
 
+// What both kernels know of the tile they are at.
+template <int V> struct Tile {
+  int n, b, i;
+  long col, base;
+  bool on;
+  __device__ __forceinline__ Tile(int ticket, int col_groups, const GlParams& p) {
+    const int lane = threadIdx.x & 31;
+    const long cols = (long)p.B * p.d;
+    n = ticket / col_groups;
+    base = (long)(ticket - n * col_groups) * (32 * V);
+    col = base + lane * V;
+    on = col < cols;
+    const long at = on ? col : cols - V;      // lanes past the last channel read it and write nothing
+    b = (int)(at / p.d);
+    i = (int)(at - (long)b * p.d);
+  }
+};
+
 template <typename T, int V, bool RESET>
-__global__ void __launch_bounds__(32 * FW, 2) gl_forward_tile_kernel(GlParams p, GlChain ch, int tiles, int col_groups) {
-  typedef typename Lane<T, V>::Raw Raw;
-  __shared__ typename Chain<V, FW>::Shared sh;
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+__global__ void __launch_bounds__(32 * FW, GLV_FB) gl_forward_tile_kernel(GlParams p, GlChain ch, int tiles, int col_groups) {
+  typedef Lane<T, V> Ln;
+  typedef Vec<V> F;
+  __shared__ Shared<V, FW> sh;
+  const int w = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const long cols = (long)p.B * p.d;
   const int total = tiles * col_groups;
   if (threadIdx.x == 0) {
@@ -313,83 +423,62 @@ __global__ void __launch_bounds__(32 * FW, 2) gl_forward_tile_kernel(GlParams p,
   for (int ticket = sh.next, buf = 0; ticket < total; buf ^= 1) {
     uint32_t grabbed = 0;
     if (tiles > 1 && threadIdx.x == 0) grabbed = atomicAdd(ch.ctrl, 1u);
-    const int n = ticket / col_groups;
-    const long mine = (long)(ticket - n * col_groups) * (32 * V) + lane * V;
-    const bool lane_on = mine < cols;
-    const long col = lane_on ? mine : cols - V;
-    const int b = (int)(col / p.d), i = (int)(col - (long)b * p.d);
-    const int t0 = n * (FW * FL) + w * FL;
-    const Raw* f = reinterpret_cast<const Raw*>((const T*)p.f + (long)t0 * p.sf.t + b * p.sf.b + i);
-    const Raw* c = reinterpret_cast<const Raw*>((const T*)p.c + (long)t0 * p.sc.t + b * p.sc.b + i);
-    const Raw* z = reinterpret_cast<const Raw*>((const T*)p.z + (long)t0 * p.sz.t + b * p.sz.b + i);
-    const int steps = p.T - t0;            // of this warp, L at most
-    Raw rf[FL], rc[FL], rz[FL];
+    const Tile<V> at(ticket, col_groups, p);
+    const int t0 = at.n * (FW * FL) + w * FL, steps = p.T - t0;
+    typename Ln::Raw rf[FL], rc[FL], rz[FL];
+    load_rows<T, V, FL>(rf, p.f, p.sf, t0, p.T, at.b, at.i);
+    load_rows<T, V, FL>(rc, p.c, p.sc, t0, p.T, at.b, at.i);
+    load_rows<T, V, FL>(rz, p.z, p.sz, t0, p.T, at.b, at.i);
+    const uint32_t cut = RESET ? reset_bits<FL>(p, t0, at.b) : 0;
+    F u[FL], e, initial(0.f);
+    if (w == 0 && at.n < GROUP && p.h0 != nullptr && at.on) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) initial.set(v, p.h0[at.col + v]);
+    }
+#pragma unroll
+    for (int l = 0; l < FL; ++l) u[l] = gate_of(vmul(Ln::get(rf[l]), F(LOG2E)), e);
+    if (steps < FL) {
+#pragma unroll
+      for (int l = 0; l < FL; ++l)
+        if (l >= steps) u[l] = F(0.f);        // beyond the end: the state stays
+    }
+    F H(0.f), R(0.f);
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
-      rf[l] = Raw(0); rc[l] = Raw(0); rz[l] = Raw(0);
-      if (l < steps) {
-        rf[l] = __ldcs(f + l * (p.sf.t / V));
-        rc[l] = __ldcs(c + l * (p.sc.t / V));
-        rz[l] = __ldcs(z + l * (p.sz.t / V));
-      }
+      if (RESET) H = unless(cut >> l & 1, H);
+      H = vfma(u[l], vsub(Ln::get(rc[l]), H), H);
+      R = vfma(u[l], vsub(F(1.f), R), R);
     }
-    const uint32_t cut = RESET ? reset_bits<FL>(p, t0, b) : 0;
-    float u[FL][V], H[V], R[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) H[v] = R[v] = 0.f;
-#pragma unroll
-    for (int l = 0; l < FL; ++l) {
-      float fx[V], cx[V], e;
-      Lane<T, V>::get(rf[l], fx);
-      Lane<T, V>::get(rc[l], cx);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        u[l][v] = l < steps ? keep_gate(fx[v], e) : 0.f;     // beyond the end: the state stays
-        if (RESET && (cut >> l & 1)) H[v] = 0.f;
-        H[v] = fmaf(u[l][v], cx[v] - H[v], H[v]);
-        R[v] = fmaf(u[l][v], 1.f - R[v], R[v]);
-      }
-    }
-    Pair own[V];
-    float h[V], initial[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      own[v] = Pair{RESET && cut ? -1.f : R[v], H[v]};
-      initial[v] = n < GROUP && p.h0 != nullptr ? p.h0[col + v] : 0.f;
-    }
-    if (!Chain<V, FW>::enter(sh, buf, w, warps, own, n, tiles, col, cols, lane_on, initial, ch, ticket, &grabbed, h)) return;
+    if (RESET && cut) R = F(-1.f);
+    F h;
+    if (!enter<V, FW, RESET>(sh, buf, w, warps, R, H, at.n, tiles, at.col, cols, at.on, initial, ch, ticket, grabbed, h)) return;
     ticket = tiles > 1 ? sh.next : total;
-    if (lane_on && steps > 0) {
-      if (p.saved != nullptr && t0 % GL_CHUNK == 0) {
+    if (at.on && p.saved != nullptr && t0 % GL_CHUNK == 0 && steps > 0) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) p.saved[(long)(t0 / GL_CHUNK) * cols + col + v] = h[v];
-      }
-      Raw* y = reinterpret_cast<Raw*>((T*)p.y + (long)t0 * p.sy.t + b * p.sy.b + i);
+      for (int v = 0; v < V; ++v) p.saved[(long)(t0 / GL_CHUNK) * cols + at.col + v] = h.get(v);
+    }
+    char* y = (char*)p.y + ((long)t0 * p.sy.t + at.b * p.sy.b + at.i) * (long)sizeof(T);
+    const long step = p.sy.t * (long)sizeof(T);
 #pragma unroll
-      for (int l = 0; l < FL; ++l) {
-        float cx[V], zx[V], out[V];
-        Lane<T, V>::get(rc[l], cx);
-        Lane<T, V>::get(rz[l], zx);
+    for (int l = 0; l < FL; ++l) {
+      if (RESET) h = unless(cut >> l & 1, h);
+      h = vfma(u[l], vsub(Ln::get(rc[l]), h), h);
+      const F z = Ln::get(rz[l]);
+      const F out = vmul(h, vmul(z, gate_of(vmul(z, F(-LOG2E)), e)));
+      if (at.on && l < steps) __stcs(reinterpret_cast<typename Ln::Raw*>(y + l * step), Ln::put(out));
+    }
+    if (at.on && steps > 0 && steps <= FL) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          if (RESET && (cut >> l & 1)) h[v] = 0.f;
-          h[v] = fmaf(u[l][v], cx[v] - h[v], h[v]);
-          out[v] = h[v] * siluf_(zx[v]);
-        }
-        if (l < steps) __stcs(y + l * (p.sy.t / V), Lane<T, V>::put(out));
-      }
-      if (steps <= FL) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) p.h_last[col + v] = h[v];
-      }
+      for (int v = 0; v < V; ++v) p.h_last[at.col + v] = h.get(v);
     }
   }
 }
 
 template <typename T, int V, bool RESET>
-__global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p, GlChain ch, int tiles, int col_groups) {
-  typedef typename Lane<T, V>::Raw Raw;
-  __shared__ typename Chain<V, BW>::Shared sh;
+__global__ void __launch_bounds__(32 * BW, GLV_BB) gl_backward_tile_kernel(GlParams p, GlChain ch, int tiles, int col_groups) {
+  typedef Lane<T, V> Ln;
+  typedef Vec<V> F;
+  __shared__ Shared<V, BW> sh;
   __shared__ Pair ahead[2][BW][32 * V];      // the warps' pairs of the forward scan
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const long cols = (long)p.B * p.d;
@@ -402,120 +491,107 @@ __global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p
   for (int ticket = sh.next, buf = 0; ticket < total; buf ^= 1) {
     uint32_t grabbed = 0;
     if (tiles > 1 && threadIdx.x == 0) grabbed = atomicAdd(ch.ctrl, 1u);
-    const int n = ticket / col_groups, chunk = tiles - 1 - n;
-    const long mine = (long)(ticket - n * col_groups) * (32 * V) + lane * V;
-    const bool lane_on = mine < cols;
-    const long col = lane_on ? mine : cols - V;
-    const int b = (int)(col / p.d), i = (int)(col - (long)b * p.d);
-    const int t0 = chunk * GL_CHUNK + w * BL;
-    const Raw* f = reinterpret_cast<const Raw*>((const T*)p.f + (long)t0 * p.sf.t + b * p.sf.b + i);
-    const Raw* c = reinterpret_cast<const Raw*>((const T*)p.c + (long)t0 * p.sc.t + b * p.sc.b + i);
-    const Raw* z = reinterpret_cast<const Raw*>((const T*)p.z + (long)t0 * p.sz.t + b * p.sz.b + i);
-    const Raw* dy = reinterpret_cast<const Raw*>((const T*)p.dy + (long)t0 * p.sy.t + b * p.sy.b + i);
-    const int steps = p.T - t0;
-    Raw rf[BL], rc[BL], rz[BL], rdy[BL];
+    const Tile<V> at(ticket, col_groups, p);
+    const int chunk = tiles - 1 - at.n, t0 = chunk * GL_CHUNK + w * BL, steps = p.T - t0;
+    typename Ln::Raw rf[BL], rc[BL], rz[BL], rdy[BL];
+    load_rows<T, V, BL>(rf, p.f, p.sf, t0, p.T, at.b, at.i);
+    load_rows<T, V, BL>(rc, p.c, p.sc, t0, p.T, at.b, at.i);
+    load_rows<T, V, BL>(rz, p.z, p.sz, t0, p.T, at.b, at.i);
+    load_rows<T, V, BL>(rdy, p.dy, p.sy, t0, p.T, at.b, at.i);
+    F h(0.f), initial(0.f);
+    if (at.on) {
 #pragma unroll
-    for (int l = 0; l < BL; ++l) {
-      rf[l] = Raw(0); rc[l] = Raw(0); rz[l] = Raw(0); rdy[l] = Raw(0);
-      if (l < steps) {
-        rf[l] = __ldcs(f + l * (p.sf.t / V));
-        rc[l] = __ldcs(c + l * (p.sc.t / V));
-        rz[l] = __ldcs(z + l * (p.sz.t / V));
-        rdy[l] = __ldcs(dy + l * (p.sy.t / V));
+      for (int v = 0; v < V; ++v) h.set(v, p.saved[(long)chunk * cols + at.col + v]);
+      if (w == warps - 1 && at.n < GROUP && p.dh_last != nullptr) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) initial.set(v, p.dh_last[at.col + v]);
       }
     }
-    float h[V], D[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      h[v] = p.saved[(long)chunk * cols + col + v];
-      D[v] = n < GROUP && p.dh_last != nullptr ? p.dh_last[col + v] : 0.f;
-    }
-    const uint32_t cut = RESET ? reset_bits<BL>(p, t0, b) : 0;
+    const uint32_t cut = RESET ? reset_bits<BL>(p, t0, at.b) : 0;
     // the states before the warp's steps
-    float u[BL][V], a[BL][V], H[V], R[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) H[v] = R[v] = 0.f;
+    F u[BL], a[BL];
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
-      float fx[V], cx[V];
-      Lane<T, V>::get(rf[l], fx);
-      Lane<T, V>::get(rc[l], cx);
+      // exp2's argument is held at 115 (u = 2^-115), so that u (1 - u) = e u^2 stays a number; NaN passes
+      F x = vmul(Ln::get(rf[l]), F(LOG2E)), e;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float e;
-        u[l][v] = keep_gate(fx[v], e);
-        a[l][v] = e * u[l][v] * u[l][v];                      // u (1 - u)
-        if (l >= steps) u[l][v] = 0.f;
-        if (RESET && (cut >> l & 1)) H[v] = 0.f;
-        H[v] = fmaf(u[l][v], cx[v] - H[v], H[v]);
-        R[v] = fmaf(u[l][v], 1.f - R[v], R[v]);
+        float m;
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x.get(v)), "f"(115.f));
+        x.set(v, m);
       }
+      u[l] = gate_of(x, e);
+      a[l] = vmul(vmul(e, u[l]), u[l]);
     }
+    if (steps < BL) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      R[v] = RESET && cut ? -1.f : R[v];
-      ahead[buf][w][lane * V + v] = Pair{R[v], H[v]};
+      for (int l = 0; l < BL; ++l)
+        if (l >= steps) u[l] = F(0.f);
     }
+    F H(0.f), R(0.f);
+#pragma unroll
+    for (int l = 0; l < BL; ++l) {
+      if (RESET) H = unless(cut >> l & 1, H);
+      H = vfma(u[l], vsub(Ln::get(rc[l]), H), H);
+      R = vfma(u[l], vsub(F(1.f), R), R);
+    }
+    if (RESET && cut) R = F(-1.f);
+#pragma unroll
+    for (int v = 0; v < V; ++v) ahead[buf][w][lane * V + v] = Pair{R.get(v), H.get(v)};
     __syncthreads();
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      for (int k = 0; k < w; ++k) h[v] = pass(h[v], ahead[buf][k][lane * V + v]);
+    for (int v = 0; v < V; ++v) {
+      float s = h.get(v);
+      for (int k = 0; k < w; ++k) s = pass<RESET>(s, ahead[buf][k][lane * V + v]);
+      h.set(v, s);
+    }
     // forward through the warp's steps: dz, and what the scan back needs
-    Raw* dz = reinterpret_cast<Raw*>((T*)p.dz + (long)t0 * p.sdz.t + b * p.sdz.b + i);
-    float q[BL][V], prev[BL][V];
+    char* dz = (char*)p.dz + ((long)t0 * p.sdz.t + at.b * p.sdz.b + at.i) * (long)sizeof(T);
+    const long step_z = p.sdz.t * (long)sizeof(T);
+    F q[BL], prev[BL];
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
-      float cx[V], zx[V], gx[V], out[V];
-      Lane<T, V>::get(rc[l], cx);
-      Lane<T, V>::get(rz[l], zx);
-      Lane<T, V>::get(rdy[l], gx);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (RESET && (cut >> l & 1)) h[v] = 0.f;
-        prev[l][v] = h[v] - cx[v];
-        h[v] = fmaf(u[l][v], cx[v] - h[v], h[v]);
-        const float sg = sigmoidf_(zx[v]);
-        q[l][v] = gx[v] * zx[v] * sg;
-        out[v] = gx[v] * h[v] * sg * (1.f + zx[v] * (1.f - sg));
-      }
-      if (lane_on && l < steps) __stcs(dz + l * (p.sdz.t / V), Lane<T, V>::put(out));
+      if (RESET) h = unless(cut >> l & 1, h);
+      prev[l] = vsub(h, Ln::get(rc[l]));
+      h = vfma(u[l], vsub(F(0.f), prev[l]), h);
+      const F z = Ln::get(rz[l]), dy = Ln::get(rdy[l]);
+      F e;
+      const F s = gate_of(vmul(z, F(-LOG2E)), e), zs = vmul(z, s);
+      q[l] = vmul(dy, zs);
+      const F out = vmul(vmul(dy, h), vfma(zs, vsub(F(1.f), s), s));
+      if (at.on && l < steps) __stcs(reinterpret_cast<typename Ln::Raw*>(dz + l * step_z), Ln::put(out));
     }
-    Pair own[V];
+    if (steps < BL) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float E = 0.f;
-#pragma unroll
-      for (int l = BL - 1; l >= 0; --l) {
-        const float g = q[l][v] + E;
-        E = RESET && (cut >> l & 1) ? 0.f : fmaf(-u[l][v], g, g);
-      }
-      own[v] = Pair{R[v], E};
+      for (int l = 0; l < BL; ++l)
+        if (l >= steps) q[l] = F(0.f);
     }
-    float start[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) start[v] = D[v];
-    if (!Chain<V, BW>::enter(sh, buf, warps - 1 - w, warps, own, n, tiles, col, cols, lane_on, start, ch, ticket, &grabbed, D)) return;
-    ticket = tiles > 1 ? sh.next : total;
-    Raw* df = reinterpret_cast<Raw*>((T*)p.df + (long)t0 * p.sdf.t + b * p.sdf.b + i);
-    Raw* dc = reinterpret_cast<Raw*>((T*)p.dc + (long)t0 * p.sdc.t + b * p.sdc.b + i);
+    F E(0.f), D;
 #pragma unroll
     for (int l = BL - 1; l >= 0; --l) {
-      float of[V], oc[V];
+      const F g = vadd(q[l], E);
+      E = vsub(g, vmul(u[l], g));
+      if (RESET) E = unless(cut >> l & 1, E);
+    }
+    if (!enter<V, BW, RESET>(sh, buf, warps - 1 - w, warps, R, E, at.n, tiles, at.col, cols, at.on, initial, ch, ticket, grabbed, D)) return;
+    ticket = tiles > 1 ? sh.next : total;
+    char* df = (char*)p.df + ((long)t0 * p.sdf.t + at.b * p.sdf.b + at.i) * (long)sizeof(T);
+    char* dc = (char*)p.dc + ((long)t0 * p.sdc.t + at.b * p.sdc.b + at.i) * (long)sizeof(T);
+    const long step_f = p.sdf.t * (long)sizeof(T), step_c = p.sdc.t * (long)sizeof(T);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float g = q[l][v] + D[v];
-        oc[v] = g * u[l][v];
-        of[v] = g * prev[l][v] * a[l][v];
-        D[v] = RESET && (cut >> l & 1) ? 0.f : fmaf(-u[l][v], g, g);
-      }
-      if (lane_on && l < steps) {
-        __stcs(dc + l * (p.sdc.t / V), Lane<T, V>::put(oc));
-        __stcs(df + l * (p.sdf.t / V), Lane<T, V>::put(of));
+    for (int l = BL - 1; l >= 0; --l) {
+      const F g = vadd(q[l], D), gu = vmul(g, u[l]);
+      const F of = vmul(vmul(g, prev[l]), a[l]);
+      D = vsub(g, gu);
+      if (RESET) D = unless(cut >> l & 1, D);
+      if (at.on && l < steps) {
+        __stcs(reinterpret_cast<typename Ln::Raw*>(dc + l * step_c), Ln::put(gu));
+        __stcs(reinterpret_cast<typename Ln::Raw*>(df + l * step_f), Ln::put(of));
       }
     }
-    if (lane_on && t0 == 0) {
+    if (at.on && t0 == 0) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) p.dh0[col + v] = D[v];
+      for (int v = 0; v < V; ++v) p.dh0[at.col + v] = D.get(v);
     }
   }
 }
@@ -558,7 +634,8 @@ int launch_tiles(const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
   const long cols = (long)a.B * a.d;
   const int per_warp = bwd ? BL : FL, tile = bwd ? BW * BL : FW * FL;
   const int tiles = tiles_of(a.T, tile);
-  const int warps = tiles > 1 ? tile / per_warp : tiles_of(a.T, per_warp);
+  // (a thread for each of the tile's channels at least)
+  const int needed = tiles_of(a.T, per_warp), warps = tiles > 1 ? tile / per_warp : needed < V ? V : needed;
   const long col_groups = (cols + 32 * V - 1) / (32 * V);
   const long total = col_groups * tiles;
   ELMAN_ARG_CHECK(total + 148 * 8 < (1L << 31), "too many channels for one call");
