@@ -9,7 +9,13 @@
 //
 // Bound by HBM: forward 4 values an element, backward 7 (each of f, c, z, dy read once, each result
 // written once); the backward pass recomputes the states from one in GL_CHUNK that the forward saved.
+#include <string.h>
+
+#include <mutex>
+
 #include "common.cuh"
+#include "sm100_ptx.cuh"
+#include "tc_helpers.cuh"
 
 namespace elman {
 
@@ -280,73 +286,90 @@ template <int N> __device__ __forceinline__ bool await(const void* at, uint32_t 
   return true;
 }
 
-// What the warps of a block share.  Two buffers: a slow warp may still read the last tile's.
+// What the scanning warps of a block share.  Every member is read between barriers that lie after the
+// write and before the next tile's write.
 template <int V, int W> struct Shared {
-  Pair own[2][W][32 * V];             // the warps' pairs, in the scan's direction
-  Pair before[2][GROUP - 1][32 * V];  // pairs of the tiles before in the group
-  float start[2][32 * V];             // state at the group's start
-  float enters[2][W][32 * V];         // state that enters each warp
-  int next;                           // the block's next tile
+  Pair own[W][32 * V];             // the warps' pairs, in the scan's direction
+  Pair before[GROUP - 1][32 * V];  // pairs of the tiles before in the group
+  float start[32 * V];             // state at the group's start
+  float enters[W][32 * V];         // state that enters each warp
+  int next;                        // the block's next tile
   int gave_up;
 };
+// Barrier of the block's first `warps` warps.
+__device__ __forceinline__ void warps_sync(int warps) {
+  asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
+}
 
 // From the warps' pairs to the state that enters each: all threads call it; `n` counts tiles and `w` warps in
-// the scan's direction; lane's channels start at `col`; `initial` is the state at the scan's start.  False: a
+// the scan's direction; `initial` is the state at the scan's start.  False: a
 // wait gave up.
 template <int V, int W, bool RESET>
-__device__ __forceinline__ bool enter(Shared<V, W>& sh, int buf, int w, int warps, Vec<V> R, Vec<V> H, int n, int tiles,
-                                      long col, long cols, bool lane_on, Vec<V> initial, const GlChain& ch, int ticket,
+__device__ __forceinline__ bool enter(Shared<V, W>& sh, int w, int warps, Vec<V> R, Vec<V> H, int n, int tiles,
+                                      long base, long cols, Vec<V> initial, const GlChain& ch, int ticket,
                                       uint32_t grabbed, Vec<V>& S) {
   const int lane = threadIdx.x & 31, x = threadIdx.x;
 #pragma unroll
-  for (int v = 0; v < V; ++v) sh.own[buf][w][lane * V + v] = Pair{R.get(v), H.get(v)};
+  for (int v = 0; v < V; ++v) sh.own[w][lane * V + v] = Pair{R.get(v), H.get(v)};
   const int first = n / GROUP * GROUP, in_group = n - first;
   const bool ends_group = in_group == GROUP - 1, more = n + 1 < tiles && ticket != ch.stall;
   if (w == 0 && first == 0) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) sh.start[buf][lane * V + v] = initial.get(v);
+    for (int v = 0; v < V; ++v) sh.start[lane * V + v] = initial.get(v);
   }
-  __syncthreads();
-  const long base = col - lane * V, mine = base + x;     // one thread per channel from here to the last barrier
+  warps_sync(warps);
+  // `base` is the tile's first of `cols` channels; one thread per channel folds from here to the last barrier
+  const long mine = base + x, col = base + lane * V, seen = col < cols ? col : cols - V;
   const bool on = x < 32 * V && mine < cols;
   if (on && more && !ends_group) {
-    Pair all = sh.own[buf][0][x];
-    for (int k = 1; k < warps; ++k) all = join<RESET>(all, sh.own[buf][k][x]);
+    Pair all = sh.own[0][x];
+    for (int k = 1; k < warps; ++k) all = join<RESET>(all, sh.own[k][x]);
     publish(ch.pairs + (long)n * cols + mine, all);
   }
   if (in_group > 0 || first > 0) {
     bool ok = true;
     for (int k = w; k < in_group && ok; k += warps) {
       uint32_t g[2 * V];
-      ok = await<2 * V>(ch.pairs + (long)(first + k) * cols + (lane_on ? col : cols - V), g, ch, n);
+      ok = await<2 * V>(ch.pairs + (long)(first + k) * cols + seen, g, ch, n);
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        sh.before[buf][k][lane * V + v] = Pair{__uint_as_float(g[2 * v]), __uint_as_float(g[2 * v + 1])};
+        sh.before[k][lane * V + v] = Pair{__uint_as_float(g[2 * v]), __uint_as_float(g[2 * v + 1])};
     }
     if (w == warps - 1 && first > 0 && ok) {
       uint32_t g[V];
-      ok = await<V>(ch.states + (long)(first / GROUP - 1) * cols + (lane_on ? col : cols - V), g, ch, n);
+      ok = await<V>(ch.states + (long)(first / GROUP - 1) * cols + seen, g, ch, n);
 #pragma unroll
-      for (int v = 0; v < V; ++v) sh.start[buf][lane * V + v] = __uint_as_float(g[v]);
+      for (int v = 0; v < V; ++v) sh.start[lane * V + v] = __uint_as_float(g[v]);
     }
     if (!ok && lane == 0) sh.gave_up = 1;
   }
-  if (tiles > 1 && x == 0) sh.next = (int)(grabbed + 1u);
-  if (tiles > 1) __syncthreads();
+  if (x == 0) sh.next = (int)(grabbed + 1u);
+  if (tiles > 1) warps_sync(warps);
   if (sh.gave_up) return false;
   if (x < 32 * V) {
-    float s = sh.start[buf][x];
-    for (int k = 0; k < in_group; ++k) s = pass<RESET>(s, sh.before[buf][k][x]);
+    float s = sh.start[x];
+    for (int k = 0; k < in_group; ++k) s = pass<RESET>(s, sh.before[k][x]);
     for (int k = 0; k < warps; ++k) {
-      sh.enters[buf][k][x] = s;
-      s = pass<RESET>(s, sh.own[buf][k][x]);
+      sh.enters[k][x] = s;
+      s = pass<RESET>(s, sh.own[k][x]);
     }
     if (on && more && ends_group) publish(ch.states + (long)(first / GROUP) * cols + mine, s);
   }
-  __syncthreads();
+  warps_sync(warps);
 #pragma unroll
-  for (int v = 0; v < V; ++v) S.set(v, sh.enters[buf][w][lane * V + v]);
+  for (int v = 0; v < V; ++v) S.set(v, sh.enters[w][lane * V + v]);
   return true;
+}
+
+// exp2's argument held at 115 (u = 2^-115), so that u (1 - u) = e u^2 stays a number; NaN passes.
+template <int V> __device__ __forceinline__ Vec<V> held(Vec<V> x) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float m;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x.get(v)), "f"(115.f));
+    x.set(v, m);
+  }
+  return x;
 }
 
 // Steps of a warp whose document starts anew, as bits (lanes of one batch row agree).
@@ -379,13 +402,7 @@ __device__ __forceinline__ void load_rows(typename Lane<T, V>::Raw (&r)[L], cons
   }
 }
 
-#ifndef GLV_FW
-#define GLV_FW 8
-#define GLV_FL 16
-#define GLV_FB 2
-#define GLV_BB 2
-#endif
-constexpr int FW = GLV_FW, FL = GLV_FL;      // forward tile: 128 steps
+constexpr int FW = 8, FL = 16;      // forward tile: 128 steps
 constexpr int BW = 8, BL = 8;       // backward tile: GL_CHUNK steps, so that it starts at a saved state
 static_assert(BW * BL == GL_CHUNK && GL_CHUNK % FL == 0, "saved states lie on tile and warp edges");
 
@@ -408,7 +425,7 @@ template <int V> struct Tile {
 };
 
 template <typename T, int V, bool RESET>
-__global__ void __launch_bounds__(32 * FW, GLV_FB) gl_forward_tile_kernel(GlParams p, GlChain ch, int tiles, int col_groups) {
+__global__ void __launch_bounds__(32 * FW, 2) gl_forward_tile_kernel(GlParams p, GlChain ch, int tiles, int col_groups) {
   typedef Lane<T, V> Ln;
   typedef Vec<V> F;
   __shared__ Shared<V, FW> sh;
@@ -420,7 +437,7 @@ __global__ void __launch_bounds__(32 * FW, GLV_FB) gl_forward_tile_kernel(GlPara
     sh.next = tiles > 1 ? (int)(atomicAdd(ch.ctrl, 1u) + 1u) : (int)blockIdx.x;
   }
   __syncthreads();
-  for (int ticket = sh.next, buf = 0; ticket < total; buf ^= 1) {
+  for (int ticket = sh.next; ticket < total;) {
     uint32_t grabbed = 0;
     if (tiles > 1 && threadIdx.x == 0) grabbed = atomicAdd(ch.ctrl, 1u);
     const Tile<V> at(ticket, col_groups, p);
@@ -451,7 +468,7 @@ __global__ void __launch_bounds__(32 * FW, GLV_FB) gl_forward_tile_kernel(GlPara
     }
     if (RESET && cut) R = F(-1.f);
     F h;
-    if (!enter<V, FW, RESET>(sh, buf, w, warps, R, H, at.n, tiles, at.col, cols, at.on, initial, ch, ticket, grabbed, h)) return;
+    if (!enter<V, FW, RESET>(sh, w, warps, R, H, at.n, tiles, at.base, cols, initial, ch, ticket, grabbed, h)) return;
     ticket = tiles > 1 ? sh.next : total;
     if (at.on && p.saved != nullptr && t0 % GL_CHUNK == 0 && steps > 0) {
 #pragma unroll
@@ -475,11 +492,11 @@ __global__ void __launch_bounds__(32 * FW, GLV_FB) gl_forward_tile_kernel(GlPara
 }
 
 template <typename T, int V, bool RESET>
-__global__ void __launch_bounds__(32 * BW, GLV_BB) gl_backward_tile_kernel(GlParams p, GlChain ch, int tiles, int col_groups) {
+__global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p, GlChain ch, int tiles, int col_groups) {
   typedef Lane<T, V> Ln;
   typedef Vec<V> F;
   __shared__ Shared<V, BW> sh;
-  __shared__ Pair ahead[2][BW][32 * V];      // the warps' pairs of the forward scan
+  __shared__ Pair ahead[BW][32 * V];      // the warps' pairs of the forward scan
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const long cols = (long)p.B * p.d;
   const int total = tiles * col_groups;
@@ -488,7 +505,7 @@ __global__ void __launch_bounds__(32 * BW, GLV_BB) gl_backward_tile_kernel(GlPar
     sh.next = tiles > 1 ? (int)(atomicAdd(ch.ctrl, 1u) + 1u) : (int)blockIdx.x;
   }
   __syncthreads();
-  for (int ticket = sh.next, buf = 0; ticket < total; buf ^= 1) {
+  for (int ticket = sh.next; ticket < total;) {
     uint32_t grabbed = 0;
     if (tiles > 1 && threadIdx.x == 0) grabbed = atomicAdd(ch.ctrl, 1u);
     const Tile<V> at(ticket, col_groups, p);
@@ -512,15 +529,8 @@ __global__ void __launch_bounds__(32 * BW, GLV_BB) gl_backward_tile_kernel(GlPar
     F u[BL], a[BL];
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
-      // exp2's argument is held at 115 (u = 2^-115), so that u (1 - u) = e u^2 stays a number; NaN passes
-      F x = vmul(Ln::get(rf[l]), F(LOG2E)), e;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float m;
-        asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x.get(v)), "f"(115.f));
-        x.set(v, m);
-      }
-      u[l] = gate_of(x, e);
+      F e;
+      u[l] = gate_of(held(vmul(Ln::get(rf[l]), F(LOG2E))), e);
       a[l] = vmul(vmul(e, u[l]), u[l]);
     }
     if (steps < BL) {
@@ -537,12 +547,12 @@ __global__ void __launch_bounds__(32 * BW, GLV_BB) gl_backward_tile_kernel(GlPar
     }
     if (RESET && cut) R = F(-1.f);
 #pragma unroll
-    for (int v = 0; v < V; ++v) ahead[buf][w][lane * V + v] = Pair{R.get(v), H.get(v)};
+    for (int v = 0; v < V; ++v) ahead[w][lane * V + v] = Pair{R.get(v), H.get(v)};
     __syncthreads();
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float s = h.get(v);
-      for (int k = 0; k < w; ++k) s = pass<RESET>(s, ahead[buf][k][lane * V + v]);
+      for (int k = 0; k < w; ++k) s = pass<RESET>(s, ahead[k][lane * V + v]);
       h.set(v, s);
     }
     // forward through the warp's steps: dz, and what the scan back needs
@@ -573,7 +583,7 @@ __global__ void __launch_bounds__(32 * BW, GLV_BB) gl_backward_tile_kernel(GlPar
       E = vsub(g, vmul(u[l], g));
       if (RESET) E = unless(cut >> l & 1, E);
     }
-    if (!enter<V, BW, RESET>(sh, buf, warps - 1 - w, warps, R, E, at.n, tiles, at.col, cols, at.on, initial, ch, ticket, grabbed, D)) return;
+    if (!enter<V, BW, RESET>(sh, warps - 1 - w, warps, R, E, at.n, tiles, at.base, cols, initial, ch, ticket, grabbed, D)) return;
     ticket = tiles > 1 ? sh.next : total;
     char* df = (char*)p.df + ((long)t0 * p.sdf.t + at.b * p.sdf.b + at.i) * (long)sizeof(T);
     char* dc = (char*)p.dc + ((long)t0 * p.sdc.t + at.b * p.sdc.b + at.i) * (long)sizeof(T);
@@ -593,6 +603,323 @@ __global__ void __launch_bounds__(32 * BW, GLV_BB) gl_backward_tile_kernel(GlPar
 #pragma unroll
       for (int v = 0; v < V; ++v) p.dh0[at.col + v] = D.get(v);
     }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The same tiles fed by TMA, for tensors whose base and row strides are multiples of 16 bytes: the next
+// tile's rows arrive in one shared-memory stage while this tile is scanned from the other, so the loads
+// never pause for the arithmetic, and results leave from the stage as bulk stores.  One producer thread
+// takes tiles from the counter, loads, and stores; the other warps scan.  A lane owns the same 4-byte
+// word of every row (two bf16 channels or one fp32 channel) throughout, so results overwrite the inputs
+// that made them.  A tile lies within one batch row; rows past T and channels past d are zero-filled
+// and clipped by the copies.
+// ---------------------------------------------------------------------------
+constexpr int ROW_BYTES = 128;
+template <int IN, int ROWS> struct Stages {
+  static constexpr int TENSOR = ROWS * ROW_BYTES, STAGE = IN * TENSOR, BYTES = 2 * STAGE + 128;   // + alignment
+};
+struct GlTma {
+  int tiles, groups_per_row, total;   // tiles in time; channel groups of a batch row; all tiles
+  long cols;                          // channels as the chain counts them: whole groups
+};
+struct Feed {                          // shared: producer <-> scanning warps
+  uint64_t full[2], done[2];
+  int ticket[2];
+  int gave_up;
+};
+
+template <int IN, int OUT, int ROWS, int SCAN_WARPS>
+__device__ __forceinline__ void produce(Feed& fd, uint8_t* smem, const CUtensorMap* const (&in)[IN],
+                                        const CUtensorMap* const (&out)[OUT], int channels, bool backward,
+                                        const GlTma& g, const GlChain& ch) {
+  constexpr int TENSOR = Stages<IN, ROWS>::TENSOR, STAGE = Stages<IN, ROWS>::STAGE;
+  volatile int* gave_up = &fd.gave_up;
+  int ticket[2] = {-1, -1};
+  for (int it = 0;; ++it) {
+    const int s = it & 1;
+    uint8_t* stage = smem + s * STAGE;
+    auto corner = [&](int tk, int& c0, int& c1, int& c2) {
+      const int n = tk / g.groups_per_row / (g.total / g.tiles / g.groups_per_row);
+      const int group = tk - n * (g.total / g.tiles);
+      c1 = group / g.groups_per_row;
+      c0 = (group - c1 * g.groups_per_row) * channels;
+      c2 = (backward ? g.tiles - 1 - n : n) * ROWS;
+    };
+    int c0, c1, c2;
+    if (it >= 2) {                                  // the tile that was here: its results leave
+      if (!ptx::mbar_wait(&fd.done[s], (uint32_t)((it >> 1) - 1) & 1u, ch.spin_limit * 8, gave_up)) break;
+      corner(ticket[s], c0, c1, c2);
+#pragma unroll
+      for (int k = 0; k < OUT; ++k) tch::tma_store_3d(out[k], stage + k * TENSOR, c0, c1, c2);
+      tch::bulk_commit();
+      tch::bulk_wait_read_all();
+    }
+    const uint32_t next = g.tiles > 1 ? atomicAdd(ch.ctrl, 1u) + 1u
+                                      : (uint32_t)(it == 0 ? blockIdx.x : g.total);
+    const bool any = next < (uint32_t)g.total;
+    ticket[s] = any ? (int)next : -1;
+    fd.ticket[s] = ticket[s];
+    if (!any) {
+      ptx::mbar_arrive(&fd.full[s]);                // nothing more: the scanning warps end here
+      if (it >= 1 && ticket[s ^ 1] >= 0) {          // the last tile's results
+        if (ptx::mbar_wait(&fd.done[s ^ 1], (uint32_t)((it - 1) >> 1) & 1u, ch.spin_limit * 8, gave_up)) {
+          corner(ticket[s ^ 1], c0, c1, c2);
+#pragma unroll
+          for (int k = 0; k < OUT; ++k) tch::tma_store_3d(out[k], smem + (s ^ 1) * STAGE + k * TENSOR, c0, c1, c2);
+          tch::bulk_commit();
+        }
+      }
+      break;
+    }
+    corner(ticket[s], c0, c1, c2);
+    ptx::mbar_arrive_expect_tx(&fd.full[s], STAGE);
+#pragma unroll
+    for (int k = 0; k < IN; ++k) tch::tma_load_3d(stage + k * TENSOR, in[k], c0, c1, c2, &fd.full[s]);
+  }
+  if (*gave_up != 0)
+    for (int i = 0; i < 2000; ++i) __nanosleep(100);   // loads in flight land before the shared memory goes
+  tch::bulk_wait_read_all();
+}
+
+// What a scanning warp knows of the tile it is at.
+template <int V> struct TmaTile {
+  int n, b, i;
+  long base;
+  __device__ __forceinline__ TmaTile(int ticket, const GlTma& g) {
+    const int per_time = g.total / g.tiles;
+    n = ticket / per_time;
+    const int group = ticket - n * per_time;
+    base = (long)group * (32 * V);
+    b = group / g.groups_per_row;
+    i = (group - b * g.groups_per_row) * (32 * V) + (threadIdx.x & 31) * V;
+  }
+};
+template <int V> __device__ __forceinline__ Vec<V> read_state(const float* from, int b, int i, int d) {
+  Vec<V> x(0.f);
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (from != nullptr && i + v < d) x.set(v, from[(long)b * d + i + v]);
+  return x;
+}
+template <int V> __device__ __forceinline__ void write_state(float* to, int b, int i, int d, Vec<V> x) {
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (i + v < d) to[(long)b * d + i + v] = x.get(v);
+}
+template <typename T, int V> __device__ __forceinline__ Vec<V> word_at(uint32_t addr) {
+  uint32_t w;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(addr));
+  typename Lane<T, V>::Raw r;
+  memcpy(&r, &w, 4);
+  return Lane<T, V>::get(r);
+}
+template <typename T, int V> __device__ __forceinline__ void word_to(uint32_t addr, Vec<V> x) {
+  const typename Lane<T, V>::Raw r = Lane<T, V>::put(x);
+  uint32_t w;
+  memcpy(&w, &r, 4);
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(w) : "memory");
+}
+
+template <typename T, int V, bool RESET>
+__global__ void __launch_bounds__(32 * FW + 32, 2)
+gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_constant__ CUtensorMap tc,
+                      const __grid_constant__ CUtensorMap tz, const __grid_constant__ CUtensorMap ty, GlParams p,
+                      GlChain ch, GlTma g) {
+  typedef Vec<V> F;
+  static_assert(32 * V * sizeof(T) == ROW_BYTES, "a lane owns 4 bytes of a row");
+  constexpr int ROWS = FW * FL, TENSOR = Stages<3, ROWS>::TENSOR, STAGE = Stages<3, ROWS>::STAGE;
+  extern __shared__ uint8_t raw[];
+  __shared__ Shared<V, FW> sh;
+  __shared__ Feed fd;
+  uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 127) & ~(uintptr_t)127);
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    sh.gave_up = 0;
+    fd.gave_up = 0;
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(&fd.full[s], 1);
+      ptx::mbar_init(&fd.done[s], FW);
+    }
+    ptx::mbar_fence_init();
+  }
+  __syncthreads();
+  if (w == FW) {
+    if (lane == 0) {
+      const CUtensorMap* const in[3] = {&tf, &tc, &tz};
+      const CUtensorMap* const out[1] = {&ty};
+      produce<3, 1, ROWS, FW>(fd, smem, in, out, 32 * V, false, g, ch);
+    }
+    return;
+  }
+  for (int it = 0;; ++it) {
+    const int s = it & 1;
+    const bool here = ptx::mbar_wait(&fd.full[s], (uint32_t)(it >> 1) & 1u, ch.spin_limit * 8, &fd.gave_up);
+    if (!__all_sync(0xFFFFFFFFu, here)) {
+      fd.gave_up = 1;
+      report_timeout(ch.status, KID_GATED_LINEAR, 0xFFFF);
+      return;
+    }
+    const int ticket = fd.ticket[s];
+    if (ticket < 0) return;
+    const TmaTile<V> at(ticket, g);
+    const int t0 = at.n * ROWS + w * FL, steps = p.T - t0;
+    const uint32_t row = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * FL * ROW_BYTES + lane * 4);
+    const uint32_t cut = RESET ? reset_bits<FL>(p, t0, at.b) : 0;
+    F u[FL], e, initial(0.f);
+    if (w == 0 && at.n < GROUP) initial = read_state<V>(p.h0, at.b, at.i, p.d);
+#pragma unroll
+    for (int l = 0; l < FL; ++l) u[l] = gate_of(vmul(word_at<T, V>(row + l * ROW_BYTES), F(LOG2E)), e);
+    if (steps < FL) {
+#pragma unroll
+      for (int l = 0; l < FL; ++l)
+        if (l >= steps) u[l] = F(0.f);
+    }
+    F H(0.f), R(0.f), h;
+#pragma unroll
+    for (int l = 0; l < FL; ++l) {
+      if (RESET) H = unless(cut >> l & 1, H);
+      H = vfma(u[l], vsub(word_at<T, V>(row + TENSOR + l * ROW_BYTES), H), H);
+      R = vfma(u[l], vsub(F(1.f), R), R);
+    }
+    if (RESET && cut) R = F(-1.f);
+    if (!enter<V, FW, RESET>(sh, w, FW, R, H, at.n, g.tiles, at.base, g.cols, initial, ch, ticket, 0u, h)) {
+      fd.gave_up = 1;
+      return;
+    }
+    if (p.saved != nullptr && t0 % GL_CHUNK == 0 && steps > 0)
+      write_state<V>(p.saved + (long)(t0 / GL_CHUNK) * p.B * p.d, at.b, at.i, p.d, h);
+#pragma unroll
+    for (int l = 0; l < FL; ++l) {
+      if (RESET) h = unless(cut >> l & 1, h);
+      h = vfma(u[l], vsub(word_at<T, V>(row + TENSOR + l * ROW_BYTES), h), h);
+      const F z = word_at<T, V>(row + 2 * TENSOR + l * ROW_BYTES);
+      word_to<T, V>(row + l * ROW_BYTES, vmul(h, vmul(z, gate_of(vmul(z, F(-LOG2E)), e))));
+    }
+    if (steps > 0 && steps <= FL) write_state<V>(p.h_last, at.b, at.i, p.d, h);
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(&fd.done[s]);
+  }
+}
+
+template <typename T, int V, bool RESET>
+__global__ void __launch_bounds__(32 * BW + 32, 2)
+gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_constant__ CUtensorMap tc,
+                       const __grid_constant__ CUtensorMap tz, const __grid_constant__ CUtensorMap tdy,
+                       const __grid_constant__ CUtensorMap tdf, const __grid_constant__ CUtensorMap tdc,
+                       const __grid_constant__ CUtensorMap tdz, GlParams p, GlChain ch, GlTma g) {
+  typedef Vec<V> F;
+  constexpr int ROWS = BW * BL, TENSOR = Stages<4, ROWS>::TENSOR, STAGE = Stages<4, ROWS>::STAGE;
+  extern __shared__ uint8_t raw[];
+  __shared__ Shared<V, BW> sh;
+  __shared__ Pair ahead[BW][32 * V];
+  __shared__ Feed fd;
+  uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 127) & ~(uintptr_t)127);
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    sh.gave_up = 0;
+    fd.gave_up = 0;
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(&fd.full[s], 1);
+      ptx::mbar_init(&fd.done[s], BW);
+    }
+    ptx::mbar_fence_init();
+  }
+  __syncthreads();
+  if (w == BW) {
+    if (lane == 0) {
+      const CUtensorMap* const in[4] = {&tf, &tc, &tz, &tdy};
+      const CUtensorMap* const out[3] = {&tdf, &tdc, &tdz};
+      produce<4, 3, ROWS, BW>(fd, smem, in, out, 32 * V, true, g, ch);
+    }
+    return;
+  }
+  for (int it = 0;; ++it) {
+    const int s = it & 1;
+    const bool here = ptx::mbar_wait(&fd.full[s], (uint32_t)(it >> 1) & 1u, ch.spin_limit * 8, &fd.gave_up);
+    if (!__all_sync(0xFFFFFFFFu, here)) {
+      fd.gave_up = 1;
+      report_timeout(ch.status, KID_GATED_LINEAR, 0xFFFF);
+      return;
+    }
+    const int ticket = fd.ticket[s];
+    if (ticket < 0) return;
+    const TmaTile<V> at(ticket, g);
+    const int chunk = g.tiles - 1 - at.n, t0 = chunk * ROWS + w * BL, steps = p.T - t0;
+    const uint32_t row = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * BL * ROW_BYTES + lane * 4);
+    const uint32_t cut = RESET ? reset_bits<BL>(p, t0, at.b) : 0;
+    F h = read_state<V>(p.saved + (long)chunk * p.B * p.d, at.b, at.i, p.d), initial(0.f);
+    if (w == BW - 1 && at.n < GROUP) initial = read_state<V>(p.dh_last, at.b, at.i, p.d);
+    F u[BL], a[BL];
+#pragma unroll
+    for (int l = 0; l < BL; ++l) {
+      F e;
+      u[l] = gate_of(held(vmul(word_at<T, V>(row + l * ROW_BYTES), F(LOG2E))), e);
+      a[l] = vmul(vmul(e, u[l]), u[l]);
+    }
+    if (steps < BL) {
+#pragma unroll
+      for (int l = 0; l < BL; ++l)
+        if (l >= steps) u[l] = F(0.f);
+    }
+    F H(0.f), R(0.f);
+#pragma unroll
+    for (int l = 0; l < BL; ++l) {
+      if (RESET) H = unless(cut >> l & 1, H);
+      H = vfma(u[l], vsub(word_at<T, V>(row + TENSOR + l * ROW_BYTES), H), H);
+      R = vfma(u[l], vsub(F(1.f), R), R);
+    }
+    if (RESET && cut) R = F(-1.f);
+#pragma unroll
+    for (int v = 0; v < V; ++v) ahead[w][lane * V + v] = Pair{R.get(v), H.get(v)};
+    warps_sync(BW);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float x = h.get(v);
+      for (int k = 0; k < w; ++k) x = pass<RESET>(x, ahead[k][lane * V + v]);
+      h.set(v, x);
+    }
+    F q[BL], prev[BL];
+#pragma unroll
+    for (int l = 0; l < BL; ++l) {
+      if (RESET) h = unless(cut >> l & 1, h);
+      prev[l] = vsub(h, word_at<T, V>(row + TENSOR + l * ROW_BYTES));
+      h = vfma(u[l], vsub(F(0.f), prev[l]), h);
+      const F z = word_at<T, V>(row + 2 * TENSOR + l * ROW_BYTES), dy = word_at<T, V>(row + 3 * TENSOR + l * ROW_BYTES);
+      F e;
+      const F sg = gate_of(vmul(z, F(-LOG2E)), e), zs = vmul(z, sg);
+      q[l] = vmul(dy, zs);
+      word_to<T, V>(row + 2 * TENSOR + l * ROW_BYTES, vmul(vmul(dy, h), vfma(zs, vsub(F(1.f), sg), sg)));
+    }
+    if (steps < BL) {
+#pragma unroll
+      for (int l = 0; l < BL; ++l)
+        if (l >= steps) q[l] = F(0.f);
+    }
+    F E(0.f), D;
+#pragma unroll
+    for (int l = BL - 1; l >= 0; --l) {
+      const F gt = vadd(q[l], E);
+      E = vsub(gt, vmul(u[l], gt));
+      if (RESET) E = unless(cut >> l & 1, E);
+    }
+    if (!enter<V, BW, RESET>(sh, BW - 1 - w, BW, R, E, at.n, g.tiles, at.base, g.cols, initial, ch, ticket, 0u, D)) {
+      fd.gave_up = 1;
+      return;
+    }
+#pragma unroll
+    for (int l = BL - 1; l >= 0; --l) {
+      const F gt = vadd(q[l], D), gu = vmul(gt, u[l]);
+      word_to<T, V>(row + l * ROW_BYTES, vmul(vmul(gt, prev[l]), a[l]));
+      word_to<T, V>(row + TENSOR + l * ROW_BYTES, gu);
+      D = vsub(gt, gu);
+      if (RESET) D = unless(cut >> l & 1, D);
+    }
+    if (t0 == 0) write_state<V>(p.dh0, at.b, at.i, p.d, D);
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(&fd.done[s]);
   }
 }
 
@@ -628,6 +955,89 @@ bool pairs_of_channels(const GatedLinearArgs& a, bool bwd) {
   return ok;
 }
 
+// Channels as a chain of whole TMA groups counts them: 128 bytes of a row each, within a batch row.
+long whole_groups(int dtype, int d) {
+  const int width = dtype == ELMAN_F32 ? 32 : 64;
+  return ((long)d + width - 1) / width * width;
+}
+// TMA copies need rows that start on 16 bytes; a batch row's last group should not be mostly empty.
+bool tma_width(int dtype, int d) { return whole_groups(dtype, d) <= d + d / 4; }
+bool tma_rows(int dtype, const GatedLinearArgs& a, bool bwd) {
+  if (!tma_width(dtype, a.d) || a.T > (1 << 30) || a.B > (1 << 30)) return false;
+  const long per16 = dtype == ELMAN_F32 ? 4 : 8, most = (1L << 39) / 4;
+  bool ok = true;
+  auto see = [&](const void* base, const long* s) {
+    ok = ok && ((uintptr_t)base & 15) == 0 && s[0] % per16 == 0 && s[0] < most &&
+         (a.B <= 1 || (s[1] % per16 == 0 && s[1] > 0 && s[1] < most)) && s[0] > 0;
+  };
+  see(a.f, a.f_strides); see(a.c, a.c_strides); see(a.z, a.z_strides);
+  see(bwd ? a.dy : a.y, a.y_strides);
+  if (bwd) { see(a.df, a.df_strides); see(a.dc, a.dc_strides); see(a.dz, a.dz_strides); }
+  return ok;
+}
+
+void prepare_chain(GlChain& ch, const GatedLinearArgs& a, int tiles, long cols) {
+  char* ws = (char*)a.workspace;
+  ch.status = device_status_ptr();
+  ch.spin_limit = options().spin_limit;
+  ch.stall = (int)options().test_stall_step;
+  if (tiles <= 1) return;
+  ch.ctrl = (uint32_t*)ws;
+  ch.pairs = (float2*)(ws + 256);
+  ch.states = (float*)(ws + 256 + (size_t)tiles * cols * sizeof(float2));
+}
+
+template <typename T, int V, bool RESET>
+int launch_tma(int dtype, const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
+  static std::mutex mutex;
+  static bool sized[2][64];      // the kernel's shared-memory limit is set, per direction and device
+  const int rows = bwd ? BW * BL : FW * FL;
+  GlTma g{};
+  g.tiles = tiles_of(a.T, rows);
+  g.groups_per_row = (int)(whole_groups(dtype, a.d) / (32 * V));
+  const long total = (long)g.groups_per_row * a.B * g.tiles;
+  ELMAN_ARG_CHECK(total + 148 * 8 < (1L << 31), "too many channels for one call");
+  g.total = (int)total;
+  g.cols = (long)g.groups_per_row * a.B * 32 * V;
+  const int smem = bwd ? Stages<4, BW * BL>::BYTES : Stages<3, FW * FL>::BYTES;
+  const void* kernel = bwd ? (const void*)&gl_backward_tma_kernel<T, V, RESET> : (const void*)&gl_forward_tma_kernel<T, V, RESET>;
+  int dev = 0;
+  ELMAN_CUDA_CHECK(cudaGetDevice(&dev));
+  {
+    std::lock_guard<std::mutex> lock(mutex);
+    if (dev >= 64 || !sized[bwd][dev]) {
+      ELMAN_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      if (dev < 64) sized[bwd][dev] = true;
+    }
+  }
+  CUtensorMap m[7];
+  auto map = [&](int k, const void* base, const long* s) {
+    const uint64_t one = a.B > 1 ? s[1] : s[0];     // (a single batch row: any valid stride)
+    return make_tmap_3d(&m[k], dtype, base, a.d, a.B, a.T, one, s[0], 32 * V, 1, rows);
+  };
+  ELMAN_RETURN_IF(map(0, a.f, a.f_strides));
+  ELMAN_RETURN_IF(map(1, a.c, a.c_strides));
+  ELMAN_RETURN_IF(map(2, a.z, a.z_strides));
+  ELMAN_RETURN_IF(map(3, bwd ? a.dy : a.y, a.y_strides));
+  if (bwd) {
+    ELMAN_RETURN_IF(map(4, a.df, a.df_strides));
+    ELMAN_RETURN_IF(map(5, a.dc, a.dc_strides));
+    ELMAN_RETURN_IF(map(6, a.dz, a.dz_strides));
+  }
+  GlChain ch{};
+  prepare_chain(ch, a, g.tiles, g.cols);
+  if (g.tiles > 1) ELMAN_CUDA_CHECK(cudaMemsetAsync(a.workspace, 0xFF, chain_bytes(g.tiles, g.cols), st));
+  const GlParams p = params_of(a);
+  const unsigned grid = (unsigned)(g.tiles > 1 && total > 148 * 2 ? 148 * 2 : total);
+  if (bwd)
+    gl_backward_tma_kernel<T, V, RESET><<<grid, 32 * BW + 32, smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], p, ch, g);
+  else
+    gl_forward_tma_kernel<T, V, RESET><<<grid, 32 * FW + 32, smem, st>>>(m[0], m[1], m[2], m[3], p, ch, g);
+  count_launch(false);
+  ELMAN_CUDA_CHECK(cudaGetLastError());
+  return ELMAN_OK;
+}
+
 template <typename T, int V, bool RESET>
 int launch_tiles(const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
   auto* kernel = bwd ? &gl_backward_tile_kernel<T, V, RESET> : &gl_forward_tile_kernel<T, V, RESET>;
@@ -640,17 +1050,11 @@ int launch_tiles(const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
   const long total = col_groups * tiles;
   ELMAN_ARG_CHECK(total + 148 * 8 < (1L << 31), "too many channels for one call");
   GlChain ch{};
+  prepare_chain(ch, a, tiles, cols);
   long grid = total;
   if (tiles > 1) {
-    char* ws = (char*)a.workspace;
-    ch.ctrl = (uint32_t*)ws;
-    ch.pairs = (float2*)(ws + 256);
-    ch.states = (float*)(ws + 256 + (size_t)tiles * cols * sizeof(float2));
-    ch.status = device_status_ptr();
-    ch.spin_limit = options().spin_limit;
-    ch.stall = (int)options().test_stall_step;
-    ELMAN_CUDA_CHECK(cudaMemsetAsync(ws, 0xFF, chain_bytes(tiles, cols), st));
-    const long resident = 148 * 4;       // more than stay resident: the counter hands out the tiles
+    ELMAN_CUDA_CHECK(cudaMemsetAsync(a.workspace, 0xFF, chain_bytes(tiles, cols), st));
+    const long resident = 148 * 2;       // the counter hands out the tiles
     if (grid > resident) grid = resident;
   }
   GlParams p = params_of(a);
@@ -662,6 +1066,8 @@ int launch_tiles(const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
 
 template <bool RESET>
 int launch_tiles(int dtype, const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
+  if (tma_rows(dtype, a, bwd))
+    return dtype == ELMAN_F32 ? launch_tma<float, 1, RESET>(dtype, a, bwd, st) : launch_tma<bf16, 2, RESET>(dtype, a, bwd, st);
   if (dtype == ELMAN_F32) return launch_tiles<float, 1, RESET>(a, bwd, st);
   if (pairs_of_channels(a, bwd)) return launch_tiles<bf16, 2, RESET>(a, bwd, st);
   return launch_tiles<bf16, 1, RESET>(a, bwd, st);
@@ -696,9 +1102,8 @@ int gated_linear_bwd(int dtype, const GatedLinearArgs& a, cudaStream_t st) {
 }
 
 size_t gated_linear_workspace(int dtype, int T, int B, int d) {
-  (void)dtype;
   // the backward pass has the shorter tiles
-  return T > SEQ_STEPS ? chain_bytes(tiles_of(T, BW * BL), (long)B * d) : 0;
+  return T > SEQ_STEPS ? chain_bytes(tiles_of(T, BW * BL), B * (tma_width(dtype, d) ? whole_groups(dtype, d) : (long)d)) : 0;
 }
 
 }  // namespace elman

@@ -977,6 +977,26 @@ int make_tmap_bf16_sw128(CUtensorMap* out, const void* base, uint64_t rows, uint
   return ELMAN_OK;
 }
 
+int make_tmap_3d(CUtensorMap* out, int dtype, const void* base, uint64_t n0, uint64_t n1, uint64_t n2, uint64_t s1,
+                 uint64_t s2, uint32_t b0, uint32_t b1, uint32_t b2) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr)
+    return set_error(ELMAN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const uint64_t es = dtype == ELMAN_F32 ? 4 : 2;
+  cuuint64_t dims[3] = {n0, n1, n2};
+  cuuint64_t strides[2] = {s1 * es, s2 * es};
+  cuuint32_t box[3] = {b0, b1, b2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult rc = fn(out, dtype == ELMAN_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                   const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS)
+    return set_error(ELMAN_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for [%llu x %llu x %llu]", (int)rc,
+                     (unsigned long long)n2, (unsigned long long)n1, (unsigned long long)n0);
+  return ELMAN_OK;
+}
+
 bool gemm_tc_supported(int M, int N, int K, const void* A, int lda, const void* W, int ldw,
                        const void* C, int ldc, int c_is_f32) {
   (void)C; (void)ldc; (void)c_is_f32;

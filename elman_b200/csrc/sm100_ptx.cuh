@@ -352,5 +352,9 @@ __device__ __forceinline__ bool elect_one() {
 // matrix [rows, cols] with row stride `ld` elements; box = box_rows x 64 columns.
 int make_tmap_bf16_sw128(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols,
                          uint64_t ld, uint32_t box_rows);
+// 3D tensor map over [n2, n1, n0] elements of `dtype` (n0 dense, s1 and s2 the element strides of the outer
+// dimensions), box b2 x b1 x b0, without swizzle.
+int make_tmap_3d(CUtensorMap* out, int dtype, const void* base, uint64_t n0, uint64_t n1, uint64_t n2, uint64_t s1,
+                 uint64_t s2, uint32_t b0, uint32_t b1, uint32_t b2);
 
 }  // namespace elman
