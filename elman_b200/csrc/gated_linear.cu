@@ -159,36 +159,35 @@ template <> struct Vec<1> {
   __device__ __forceinline__ void set(int, float s) { x = s; }
 };
 template <> struct Vec<2> {
-  float x[2];
+  unsigned long long x;                // one register pair from load to store: packing costs nothing
   __device__ __forceinline__ Vec() {}
-  __device__ __forceinline__ explicit Vec(float s) { x[0] = x[1] = s; }
-  __device__ __forceinline__ float get(int v) const { return x[v]; }
-  __device__ __forceinline__ void set(int v, float s) { x[v] = s; }
+  __device__ __forceinline__ explicit Vec(float s) : Vec(s, s) {}
+  __device__ __forceinline__ Vec(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ void halves(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+  __device__ __forceinline__ float get(int v) const {
+    float lo, hi;
+    halves(lo, hi);
+    return v == 0 ? lo : hi;
+  }
+  __device__ __forceinline__ void set(int v, float s) { *this = v == 0 ? Vec(s, get(1)) : Vec(get(0), s); }
 };
 __device__ __forceinline__ Vec<1> vfma(Vec<1> a, Vec<1> b, Vec<1> c) { return Vec<1>(fmaf(a.x, b.x, c.x)); }
 __device__ __forceinline__ Vec<1> vmul(Vec<1> a, Vec<1> b) { return Vec<1>(a.x * b.x); }
 __device__ __forceinline__ Vec<1> vadd(Vec<1> a, Vec<1> b) { return Vec<1>(a.x + b.x); }
 __device__ __forceinline__ Vec<1> vsub(Vec<1> a, Vec<1> b) { return Vec<1>(a.x - b.x); }
-#define ELMAN_PACKED(op, ...)                                                                        \
-  asm("{\n\t.reg .b64 a, b, c, d;\n\t"                                                               \
-      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t" op ";\n\t"         \
-      "mov.b64 {%0, %1}, d;\n\t}"                                                                    \
-      : "=f"(r.x[0]), "=f"(r.x[1])                                                                   \
-      : __VA_ARGS__)
-#define ELMAN_HALVES(v) "f"((v).x[0]), "f"((v).x[1])
 __device__ __forceinline__ Vec<2> vfma(Vec<2> a, Vec<2> b, Vec<2> c) {
   Vec<2> r;
-  ELMAN_PACKED("fma.rn.f32x2 d, a, b, c", ELMAN_HALVES(a), ELMAN_HALVES(b), ELMAN_HALVES(c));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.x) : "l"(a.x), "l"(b.x), "l"(c.x));
   return r;
 }
 __device__ __forceinline__ Vec<2> vmul(Vec<2> a, Vec<2> b) {
   Vec<2> r;
-  ELMAN_PACKED("mul.rn.f32x2 d, a, b", ELMAN_HALVES(a), ELMAN_HALVES(b), ELMAN_HALVES(b));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.x) : "l"(a.x), "l"(b.x));
   return r;
 }
 __device__ __forceinline__ Vec<2> vadd(Vec<2> a, Vec<2> b) {
   Vec<2> r;
-  ELMAN_PACKED("add.rn.f32x2 d, a, b", ELMAN_HALVES(a), ELMAN_HALVES(b), ELMAN_HALVES(b));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.x) : "l"(a.x), "l"(b.x));
   return r;
 }
 __device__ __forceinline__ Vec<2> vsub(Vec<2> a, Vec<2> b) { return vfma(b, Vec<2>(-1.f), a); }   // exact product: one rounding
@@ -229,13 +228,12 @@ template <> struct Lane<bf16, 1> {
 template <> struct Lane<bf16, 2> {
   typedef uint32_t Raw;
   static __device__ __forceinline__ Vec<2> get(Raw r) {
-    Vec<2> v;
-    v.x[0] = __uint_as_float(r << 16);
-    v.x[1] = __uint_as_float(r & 0xFFFF0000u);
-    return v;
+    return Vec<2>(__uint_as_float(r << 16), __uint_as_float(r & 0xFFFF0000u));
   }
   static __device__ __forceinline__ Raw put(Vec<2> v) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(v.x[0], v.x[1]);
+    float lo, hi;
+    v.halves(lo, hi);
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const Raw*>(&p);
   }
 };
@@ -259,30 +257,42 @@ template <int N> __device__ __forceinline__ bool look(const void* at, uint32_t (
   for (int k = 0; k < N; ++k) there = there && w[k] != NOT_YET;
   return there;
 }
-// The whole warp waits until every lane's N words are there; false: gave up.
-template <int N> __device__ __forceinline__ bool await(const void* at, uint32_t (&w)[N], const GlChain& ch, int step) {
+__device__ __forceinline__ void look_if(bool wanted, const float2* at, uint32_t (&w)[2]) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t@p ld.relaxed.gpu.global.v2.b32 {%0, %1}, [%2];\n\t}"
+               : "+r"(w[0]), "+r"(w[1]) : "l"(at), "r"((uint32_t)wanted));
+}
+__device__ __forceinline__ void look_if(bool wanted, const float* at, uint32_t& w) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p ld.relaxed.gpu.global.b32 %0, [%1];\n\t}"
+               : "+r"(w) : "l"(at), "r"((uint32_t)wanted));
+}
+
+// Bounds a polling loop that a whole warp runs together.
+struct Patience {
   long spins = 0;
   unsigned long long t0 = 0;
-  while (!__all_sync(0xFFFFFFFFu, look<N>(at, w))) {
+  __device__ __forceinline__ bool left(const GlChain& ch, int step) {
     ++spins;
     bool stop = spins > ch.spin_limit;
     if ((spins & 255) == 0) {
       uint32_t aborted[1];
       look<1>(ch.ctrl + 1, aborted);
-      stop = stop || aborted[0] == 0;
-      unsigned long long now;
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+      const unsigned long long now = ptx::globaltimer_ns();
       if (t0 == 0) t0 = now;
-      else if (now - t0 > 2000000000ull) stop = true;
+      stop = stop || aborted[0] == 0 || now - t0 > ptx::kWaitDeadlineNs;
     }
-    if (__any_sync(0xFFFFFFFFu, stop)) {
-      if ((threadIdx.x & 31) == 0) {
-        asm volatile("st.relaxed.gpu.global.b32 [%0], %1;" ::"l"(ch.ctrl + 1), "r"(0) : "memory");
-        report_timeout(ch.status, KID_GATED_LINEAR, step);
-      }
-      return false;
+    if (!__any_sync(0xFFFFFFFFu, stop)) return true;
+    if ((threadIdx.x & 31) == 0) {
+      asm volatile("st.relaxed.gpu.global.b32 [%0], %1;" ::"l"(ch.ctrl + 1), "r"(0) : "memory");
+      report_timeout(ch.status, KID_GATED_LINEAR, step);
     }
+    return false;
   }
+};
+// The whole warp waits until every lane's N words are there; false: gave up.
+template <int N> __device__ __forceinline__ bool await(const void* at, uint32_t (&w)[N], const GlChain& ch, int step) {
+  Patience patience;
+  while (!__all_sync(0xFFFFFFFFu, look<N>(at, w)))
+    if (!patience.left(ch, step)) return false;
   return true;
 }
 
@@ -629,7 +639,7 @@ struct Feed {                          // shared: producer <-> scanning warps
   int gave_up;
 };
 
-template <int IN, int OUT, int ROWS, int SCAN_WARPS>
+template <int IN, int OUT, int ROWS>
 __device__ __forceinline__ void produce(Feed& fd, uint8_t* smem, const CUtensorMap* const (&in)[IN],
                                         const CUtensorMap* const (&out)[OUT], int channels, bool backward,
                                         const GlTma& g, const GlChain& ch) {
@@ -721,8 +731,106 @@ template <typename T, int V> __device__ __forceinline__ void word_to(uint32_t ad
   asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(w) : "memory");
 }
 
+// What the warps of a TMA block share.  The scanning warps leave their pairs (barrier 1, where they only
+// arrive), warps of their own link the tile into the chain, one thread per channel, and hand back the
+// state that enters each scanning warp (barrier 2).  Meanwhile the scanning warps work on what needs no
+// state.  (The general kernel below 128-bit rows folds in the scanning warps: the pass over the pairs was
+// a third of the instructions of the backward tile.)
+template <int V, int W> struct Links {
+  Pair own[W][32 * V];             // the warps' pairs, in the scan's direction
+  float enters[W][32 * V];         // state that enters each warp
+  int gave_up;
+};
+template <int V, int W> __device__ __forceinline__ void leave_pair(Links<V, W>& sh, int w, Vec<V> R, Vec<V> H) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int v = 0; v < V; ++v) sh.own[w][lane * V + v] = Pair{R.get(v), H.get(v)};
+  asm volatile("bar.arrive 1, %0;" ::"n"(32 * (W + V)) : "memory");
+}
+template <int V, int W> __device__ __forceinline__ bool take_state(Links<V, W>& sh, int w, Vec<V>& S) {
+  const int lane = threadIdx.x & 31;
+  asm volatile("bar.sync 2, %0;" ::"n"(32 * (W + V)) : "memory");
+#pragma unroll
+  for (int v = 0; v < V; ++v) S.set(v, sh.enters[w][lane * V + v]);
+  return sh.gave_up == 0;
+}
+// One linking warp, one tile; x is the thread's channel in the tile.  False: a wait gave up.
+template <int V, int W, bool RESET>
+__device__ __forceinline__ bool link(Links<V, W>& sh, int x, int n, int tiles, long base, long cols, float initial,
+                                     const GlChain& ch, int ticket) {
+  const int first = n / GROUP * GROUP, in_group = n - first;
+  const bool ends_group = in_group == GROUP - 1, more = n + 1 < tiles && ticket != ch.stall;
+  const float2* pairs = ch.pairs + (long)first * cols + base + x;
+  const float* state = ch.states + (long)(first / GROUP - 1) * cols + base + x;
+  uint32_t g[GROUP - 1][2], at_start = first > 0 ? NOT_YET : __float_as_uint(initial);
+#pragma unroll
+  for (int k = 0; k < GROUP - 1; ++k) g[k][0] = g[k][1] = k < in_group ? NOT_YET : 0u;
+  auto fetch = [&]() {                             // what is missing: every load in flight before any is looked at
+    look_if(at_start == NOT_YET, state, at_start);
+#pragma unroll
+    for (int k = 0; k < GROUP - 1; ++k) look_if(g[k][0] == NOT_YET || g[k][1] == NOT_YET, pairs + (long)k * cols, g[k]);
+  };
+  auto complete = [&]() {
+    bool there = at_start != NOT_YET;
+#pragma unroll
+    for (int k = 0; k < GROUP - 1; ++k) there = there && g[k][0] != NOT_YET && g[k][1] != NOT_YET;
+    return there;
+  };
+  fetch();                                         // while the scanning warps scan
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * (W + V)) : "memory");
+  Pair own[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) own[k] = sh.own[k][x];
+  if (more && !ends_group) {
+    Pair all = own[0];
+#pragma unroll
+    for (int k = 1; k < W; ++k) all = join<RESET>(all, own[k]);
+    publish(ch.pairs + (long)n * cols + base + x, all);
+  }
+  Patience patience;
+  bool ok = true;
+  while (ok && !__all_sync(0xFFFFFFFFu, complete())) {
+    fetch();
+    ok = patience.left(ch, n);
+  }
+  float s = __uint_as_float(at_start);
+#pragma unroll
+  for (int k = 0; k < GROUP - 1; ++k)
+    if (k < in_group) s = pass<RESET>(s, Pair{__uint_as_float(g[k][0]), __uint_as_float(g[k][1])});
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    sh.enters[k][x] = s;
+    s = pass<RESET>(s, own[k]);
+  }
+  if (more && ends_group) publish(ch.states + (long)(first / GROUP) * cols + base + x, s);
+  if (!ok) sh.gave_up = 1;
+  asm volatile("bar.sync 2, %0;" ::"n"(32 * (W + V)) : "memory");
+  return sh.gave_up == 0;
+}
+// The linking warps' loop over the block's tiles.
+template <int V, int W, bool RESET>
+__device__ __forceinline__ void link_tiles(Links<V, W>& sh, Feed& fd, const GlParams& p, const GlChain& ch, const GlTma& g,
+                                           const float* initial) {
+  const int x = threadIdx.x - 32 * W;
+  for (int it = 0;; ++it) {
+    const int s = it & 1;
+    const bool here = ptx::mbar_wait(&fd.full[s], (uint32_t)(it >> 1) & 1u, ch.spin_limit * 8, &fd.gave_up);
+    if (!__all_sync(0xFFFFFFFFu, here)) return;      // (the scanning warps see it too)
+    const int ticket = fd.ticket[s];
+    if (ticket < 0) return;
+    const int per_time = g.total / g.tiles, n = ticket / per_time, group = ticket - n * per_time;
+    const int b = group / g.groups_per_row, i = (group - b * g.groups_per_row) * (32 * V) + x;
+    const float start = n < GROUP && initial != nullptr && i < p.d ? initial[(long)b * p.d + i] : 0.f;
+    const bool ok = link<V, W, RESET>(sh, x, n, g.tiles, (long)group * (32 * V), g.cols, start, ch, ticket);
+    if (threadIdx.x % 32 == 0) ptx::mbar_arrive(&fd.done[s]);
+    if (!ok) return;
+  }
+}
+
+constexpr int TMA_THREADS_EXTRA = 32;     // the producer's warp, after the linking ones
+
 template <typename T, int V, bool RESET>
-__global__ void __launch_bounds__(32 * FW + 32, 2)
+__global__ void __launch_bounds__(32 * (FW + V) + TMA_THREADS_EXTRA, 2)
 gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_constant__ CUtensorMap tc,
                       const __grid_constant__ CUtensorMap tz, const __grid_constant__ CUtensorMap ty, GlParams p,
                       GlChain ch, GlTma g) {
@@ -730,7 +838,7 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
   static_assert(32 * V * sizeof(T) == ROW_BYTES, "a lane owns 4 bytes of a row");
   constexpr int ROWS = FW * FL, TENSOR = Stages<3, ROWS>::TENSOR, STAGE = Stages<3, ROWS>::STAGE;
   extern __shared__ uint8_t raw[];
-  __shared__ Shared<V, FW> sh;
+  __shared__ Links<V, FW> sh;
   __shared__ Feed fd;
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 127) & ~(uintptr_t)127);
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -739,17 +847,21 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
     fd.gave_up = 0;
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(&fd.full[s], 1);
-      ptx::mbar_init(&fd.done[s], FW);
+      ptx::mbar_init(&fd.done[s], FW + V);
     }
     ptx::mbar_fence_init();
   }
   __syncthreads();
-  if (w == FW) {
+  if (w == FW + V) {
     if (lane == 0) {
       const CUtensorMap* const in[3] = {&tf, &tc, &tz};
       const CUtensorMap* const out[1] = {&ty};
-      produce<3, 1, ROWS, FW>(fd, smem, in, out, 32 * V, false, g, ch);
+      produce<3, 1, ROWS>(fd, smem, in, out, 32 * V, false, g, ch);
     }
+    return;
+  }
+  if (w >= FW) {
+    link_tiles<V, FW, RESET>(sh, fd, p, ch, g, p.h0);
     return;
   }
   for (int it = 0;; ++it) {
@@ -766,8 +878,7 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
     const int t0 = at.n * ROWS + w * FL, steps = p.T - t0;
     const uint32_t row = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * FL * ROW_BYTES + lane * 4);
     const uint32_t cut = RESET ? reset_bits<FL>(p, t0, at.b) : 0;
-    F u[FL], e, initial(0.f);
-    if (w == 0 && at.n < GROUP) initial = read_state<V>(p.h0, at.b, at.i, p.d);
+    F u[FL], zs[FL], e;
 #pragma unroll
     for (int l = 0; l < FL; ++l) u[l] = gate_of(vmul(word_at<T, V>(row + l * ROW_BYTES), F(LOG2E)), e);
     if (steps < FL) {
@@ -783,7 +894,13 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
       R = vfma(u[l], vsub(F(1.f), R), R);
     }
     if (RESET && cut) R = F(-1.f);
-    if (!enter<V, FW, RESET>(sh, w, FW, R, H, at.n, g.tiles, at.base, g.cols, initial, ch, ticket, 0u, h)) {
+    leave_pair<V, FW>(sh, w, R, H);
+#pragma unroll
+    for (int l = 0; l < FL; ++l) {
+      const F z = word_at<T, V>(row + 2 * TENSOR + l * ROW_BYTES);
+      zs[l] = vmul(z, gate_of(vmul(z, F(-LOG2E)), e));
+    }
+    if (!take_state<V, FW>(sh, w, h)) {
       fd.gave_up = 1;
       return;
     }
@@ -793,8 +910,7 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
     for (int l = 0; l < FL; ++l) {
       if (RESET) h = unless(cut >> l & 1, h);
       h = vfma(u[l], vsub(word_at<T, V>(row + TENSOR + l * ROW_BYTES), h), h);
-      const F z = word_at<T, V>(row + 2 * TENSOR + l * ROW_BYTES);
-      word_to<T, V>(row + l * ROW_BYTES, vmul(h, vmul(z, gate_of(vmul(z, F(-LOG2E)), e))));
+      word_to<T, V>(row + l * ROW_BYTES, vmul(h, zs[l]));
     }
     if (steps > 0 && steps <= FL) write_state<V>(p.h_last, at.b, at.i, p.d, h);
     ptx::fence_proxy_async_smem();
@@ -804,7 +920,7 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
 }
 
 template <typename T, int V, bool RESET>
-__global__ void __launch_bounds__(32 * BW + 32, 2)
+__global__ void __launch_bounds__(32 * (BW + V) + TMA_THREADS_EXTRA, 2)
 gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_constant__ CUtensorMap tc,
                        const __grid_constant__ CUtensorMap tz, const __grid_constant__ CUtensorMap tdy,
                        const __grid_constant__ CUtensorMap tdf, const __grid_constant__ CUtensorMap tdc,
@@ -812,7 +928,7 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
   typedef Vec<V> F;
   constexpr int ROWS = BW * BL, TENSOR = Stages<4, ROWS>::TENSOR, STAGE = Stages<4, ROWS>::STAGE;
   extern __shared__ uint8_t raw[];
-  __shared__ Shared<V, BW> sh;
+  __shared__ Links<V, BW> sh;
   __shared__ Pair ahead[BW][32 * V];
   __shared__ Feed fd;
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 127) & ~(uintptr_t)127);
@@ -822,17 +938,21 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
     fd.gave_up = 0;
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(&fd.full[s], 1);
-      ptx::mbar_init(&fd.done[s], BW);
+      ptx::mbar_init(&fd.done[s], BW + V);
     }
     ptx::mbar_fence_init();
   }
   __syncthreads();
-  if (w == BW) {
+  if (w == BW + V) {
     if (lane == 0) {
       const CUtensorMap* const in[4] = {&tf, &tc, &tz, &tdy};
       const CUtensorMap* const out[3] = {&tdf, &tdc, &tdz};
-      produce<4, 3, ROWS, BW>(fd, smem, in, out, 32 * V, true, g, ch);
+      produce<4, 3, ROWS>(fd, smem, in, out, 32 * V, true, g, ch);
     }
+    return;
+  }
+  if (w >= BW) {
+    link_tiles<V, BW, RESET>(sh, fd, p, ch, g, p.dh_last);
     return;
   }
   for (int it = 0;; ++it) {
@@ -849,8 +969,7 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
     const int chunk = g.tiles - 1 - at.n, t0 = chunk * ROWS + w * BL, steps = p.T - t0;
     const uint32_t row = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * BL * ROW_BYTES + lane * 4);
     const uint32_t cut = RESET ? reset_bits<BL>(p, t0, at.b) : 0;
-    F h = read_state<V>(p.saved + (long)chunk * p.B * p.d, at.b, at.i, p.d), initial(0.f);
-    if (w == BW - 1 && at.n < GROUP) initial = read_state<V>(p.dh_last, at.b, at.i, p.d);
+    F h = read_state<V>(p.saved + (long)chunk * p.B * p.d, at.b, at.i, p.d);
     F u[BL], a[BL];
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
@@ -873,19 +992,20 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
     if (RESET && cut) R = F(-1.f);
 #pragma unroll
     for (int v = 0; v < V; ++v) ahead[w][lane * V + v] = Pair{R.get(v), H.get(v)};
-    warps_sync(BW);
+    asm volatile("bar.sync 3, %0;" ::"n"(32 * BW) : "memory");
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float x = h.get(v);
-      for (int k = 0; k < w; ++k) x = pass<RESET>(x, ahead[k][lane * V + v]);
-      h.set(v, x);
-    }
-    F q[BL], prev[BL];
+    for (int k = 0; k < BW - 1; ++k)
+      if (k < w) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) h.set(v, pass<RESET>(h.get(v), ahead[k][lane * V + v]));
+      }
+    F q[BL];                              // a becomes (p - c) u (1 - u): df = g a
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
       if (RESET) h = unless(cut >> l & 1, h);
-      prev[l] = vsub(h, word_at<T, V>(row + TENSOR + l * ROW_BYTES));
-      h = vfma(u[l], vsub(F(0.f), prev[l]), h);
+      const F prev = vsub(h, word_at<T, V>(row + TENSOR + l * ROW_BYTES));
+      a[l] = vmul(a[l], prev);
+      h = vsub(h, vmul(u[l], prev));
       const F z = word_at<T, V>(row + 2 * TENSOR + l * ROW_BYTES), dy = word_at<T, V>(row + 3 * TENSOR + l * ROW_BYTES);
       F e;
       const F sg = gate_of(vmul(z, F(-LOG2E)), e), zs = vmul(z, sg);
@@ -904,14 +1024,15 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
       E = vsub(gt, vmul(u[l], gt));
       if (RESET) E = unless(cut >> l & 1, E);
     }
-    if (!enter<V, BW, RESET>(sh, BW - 1 - w, BW, R, E, at.n, g.tiles, at.base, g.cols, initial, ch, ticket, 0u, D)) {
+    leave_pair<V, BW>(sh, BW - 1 - w, R, E);
+    if (!take_state<V, BW>(sh, BW - 1 - w, D)) {
       fd.gave_up = 1;
       return;
     }
 #pragma unroll
     for (int l = BL - 1; l >= 0; --l) {
       const F gt = vadd(q[l], D), gu = vmul(gt, u[l]);
-      word_to<T, V>(row + l * ROW_BYTES, vmul(vmul(gt, prev[l]), a[l]));
+      word_to<T, V>(row + l * ROW_BYTES, vmul(gt, a[l]));
       word_to<T, V>(row + TENSOR + l * ROW_BYTES, gu);
       D = vsub(gt, gu);
       if (RESET) D = unless(cut >> l & 1, D);
@@ -1030,9 +1151,9 @@ int launch_tma(int dtype, const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
   const GlParams p = params_of(a);
   const unsigned grid = (unsigned)(g.tiles > 1 && total > 148 * 2 ? 148 * 2 : total);
   if (bwd)
-    gl_backward_tma_kernel<T, V, RESET><<<grid, 32 * BW + 32, smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], p, ch, g);
+    gl_backward_tma_kernel<T, V, RESET><<<grid, 32 * (BW + V) + TMA_THREADS_EXTRA, smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], p, ch, g);
   else
-    gl_forward_tma_kernel<T, V, RESET><<<grid, 32 * FW + 32, smem, st>>>(m[0], m[1], m[2], m[3], p, ch, g);
+    gl_forward_tma_kernel<T, V, RESET><<<grid, 32 * (FW + V) + TMA_THREADS_EXTRA, smem, st>>>(m[0], m[1], m[2], m[3], p, ch, g);
   count_launch(false);
   ELMAN_CUDA_CHECK(cudaGetLastError());
   return ELMAN_OK;
