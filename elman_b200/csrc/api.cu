@@ -1774,3 +1774,56 @@ int elman_gated_linear_backward(int dtype, int T, int B, int d, const void* f, c
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Newton-Schulz orthogonalisation and the Muon update
+// ---------------------------------------------------------------------------
+static int check_newton_schulz(int dtype, int count, int m, int n, int steps, float a, float b, float c,
+                               float eps, const void* workspace, size_t workspace_bytes) {
+  ELMAN_ARG_CHECK(dtype == ELMAN_F32 || dtype == ELMAN_BF16, "unknown dtype %d", dtype);
+  ELMAN_ARG_CHECK(count >= 0 && m >= 0 && n >= 0, "negative size (count=%d m=%d n=%d)", count, m, n);
+  ELMAN_ARG_CHECK(count <= 65535 && m <= (1 << 20) && n <= (1 << 20) &&
+                      (double)count * m * n < (double)(1L << 40), "matrices too large");
+  ELMAN_ARG_CHECK(steps >= 1 && steps <= 100, "steps must be in 1..100");
+  ELMAN_ARG_CHECK(eps >= 0.f, "eps must not be negative");
+  ELMAN_ARG_CHECK(newton_schulz_in_range(steps, a, b, c),
+                  "these coefficients take singular values in [0, 1] beyond 3.5 (or b s^2 + c s^4 beyond 60)");
+  ELMAN_RETURN_IF(check_status_on_entry());
+  if (count == 0 || m == 0 || n == 0) return ELMAN_OK;
+  REQUIRE_PTR(workspace);
+  const size_t need = newton_schulz_workspace(dtype, count, m, n);
+  if (workspace_bytes < need)
+    return set_error(ELMAN_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  ELMAN_ARG_CHECK(((uintptr_t)workspace & 255) == 0, "workspace must be 256-byte aligned");
+  return ELMAN_OK;
+}
+
+extern "C" {
+
+size_t elman_newton_schulz_workspace(int dtype, int count, int m, int n) {
+  if (count <= 0 || m <= 0 || n <= 0) return 0;
+  return newton_schulz_workspace(dtype, count, m, n);
+}
+
+int elman_newton_schulz(int dtype, int count, int m, int n, const void* in, void* out, int steps, float a,
+                        float b, float c, float eps, void* workspace, size_t workspace_bytes, void* stream) {
+  ELMAN_RETURN_IF(check_newton_schulz(dtype, count, m, n, steps, a, b, c, eps, workspace, workspace_bytes));
+  if (count == 0 || m == 0 || n == 0) return ELMAN_OK;
+  REQUIRE_PTR(in); REQUIRE_PTR(out);
+  const NewtonSchulzArgs args{dtype, count, m, n, steps, a, b, c, eps, in, out, workspace};
+  return newton_schulz(args, (cudaStream_t)stream);
+}
+
+int elman_muon_step(int dtype, int count, int m, int n, const long long* offsets, void* params,
+                    const void* grads, float* momentum, float lr, float mu, int nesterov,
+                    float weight_decay, float scale, const float* grad_scale, int steps, float a, float b,
+                    float c, float eps, void* workspace, size_t workspace_bytes, void* stream) {
+  ELMAN_RETURN_IF(check_newton_schulz(dtype, count, m, n, steps, a, b, c, eps, workspace, workspace_bytes));
+  if (count == 0 || m == 0 || n == 0) return ELMAN_OK;
+  REQUIRE_PTR(offsets); REQUIRE_PTR(params); REQUIRE_PTR(grads); REQUIRE_PTR(momentum);
+  const NewtonSchulzArgs args{dtype, count, m, n, steps, a, b, c, eps, nullptr, nullptr, workspace};
+  const MuonArgs u{offsets, params, grads, momentum, lr, mu, weight_decay, scale, nesterov, grad_scale};
+  return muon_step(args, u, (cudaStream_t)stream);
+}
+
+}  // extern "C"

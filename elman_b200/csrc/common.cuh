@@ -93,7 +93,7 @@ int* device_status_ptr();   // device-side alias, or nullptr if unavailable
 // kernel ids recorded in the status word
 enum KernelId { KID_REC_SIMT = 1, KID_REC_TC_FWD = 2, KID_REC_TC_BWD = 3, KID_GEMM_TC = 4,
                 KID_LOWRANK_SIMT = 5, KID_WAIT_PROBE = 6, KID_LOWRANK_TC = 7, KID_LM_TOKEN = 8,
-                KID_GATED_LINEAR = 9 };
+                KID_GATED_LINEAR = 9, KID_NEWTON_SCHULZ = 10 };
 
 // ---------------------------------------------------------------------------
 // device helpers
@@ -383,6 +383,25 @@ struct GatedLinearArgs {
 size_t gated_linear_workspace(int dtype, int T, int B, int d);
 int gated_linear_fwd(int dtype, const GatedLinearArgs& a, cudaStream_t stream);
 int gated_linear_bwd(int dtype, const GatedLinearArgs& a, cudaStream_t stream);
+
+// Newton-Schulz orthogonalisation of `count` matrices [m, n] and the Muon update (newton_schulz.cu).
+struct NewtonSchulzArgs {
+  int dtype, count, m, n, steps;
+  float a, b, c, eps;
+  const void* in; void* out;          // [count, m, n]; not used by muon_step
+  void* workspace;
+};
+struct MuonArgs {
+  const long long* offsets;           // device: element where each matrix starts in params and grads
+  void* params; const void* grads; float* momentum;   // momentum [count, m, n]
+  float lr, mu, weight_decay, scale;
+  int nesterov;
+  const float* grad_scale;            // device, or null
+};
+size_t newton_schulz_workspace(int dtype, int count, int m, int n);
+bool newton_schulz_in_range(int steps, float a, float b, float c);
+int newton_schulz(const NewtonSchulzArgs& a, cudaStream_t stream);
+int muon_step(const NewtonSchulzArgs& a, const MuonArgs& u, cudaStream_t stream);
 
 // Spectral normalisation of a [d, d] matrix (csrc/spectral.cu): three power-iteration steps
 // from u (advanced in place), v and sigma saved for the backward pass.

@@ -176,6 +176,11 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N) {
          ((uint32_t)(M >> 4) << 24);
 }
 
+// The same with A and B fp16 (the instruction itself does not differ).
+__host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
 // D[tmem] (+)= A[smem] * B[smem]; issued by one thread.
 __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
                                           uint32_t idesc, uint32_t accumulate) {
@@ -352,6 +357,10 @@ __device__ __forceinline__ bool elect_one() {
 // matrix [rows, cols] with row stride `ld` elements; box = box_rows x 64 columns.
 int make_tmap_bf16_sw128(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols,
                          uint64_t ld, uint32_t box_rows);
+// 3D fp16 tensor map with 128-byte swizzle over `count` row-major matrices [rows, cols] of row stride `ld` and
+// matrix stride `stride` (elements, multiples of 8); box 1 x 64 x 64.
+int make_tmap_f16_sw128(CUtensorMap* out, const void* base, uint64_t cols, uint64_t rows, uint64_t count, uint64_t ld,
+                        uint64_t stride);
 // 3D tensor map over [n2, n1, n0] elements of `dtype` (n0 dense, s1 and s2 the element strides of the outer
 // dimensions), box b2 x b1 x b0, without swizzle.
 int make_tmap_3d(CUtensorMap* out, int dtype, const void* base, uint64_t n0, uint64_t n1, uint64_t n2, uint64_t s1,

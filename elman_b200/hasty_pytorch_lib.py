@@ -931,3 +931,29 @@ def gated_linear_backward(f, c, z, saved, d_output, dh_last=None, reset=None, ou
             dh0.data_ptr(), ws.data_ptr(), ws.numel(), _stream(f.device))
         _lib.check(rc, fn)
     return [df, dc, dz, dh0]
+
+
+# --------------------------------------------------------------------------- orthogonalisation
+
+NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # singular values of (0, 1] go to about [0.7, 1.2] in five steps
+
+
+def newton_schulz(G, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7):
+    """The matrices G [..., m, n] with their singular values moved towards one and their singular vectors kept:
+    X = G / (|G| + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T.  float32 or bfloat16,
+    contiguous; returns a tensor like G.  No counterpart in the reference."""
+    fn = "newton_schulz"
+    dt = _check_inputs(fn, G, G=G)
+    if G.dim() < 2:
+        raise RuntimeError(f"{fn}: G must be [..., m, n]")
+    m, n = G.shape[-2:]
+    count = G.numel() // (m * n) if m * n > 0 else 0
+    a, b, c = coefficients
+    lib = _lib.load()
+    with torch.cuda.device(G.device):
+        out = torch.empty_like(G)
+        ws = _workspace(lib.elman_newton_schulz_workspace(dt, count, m, n), G.device)
+        rc = lib.elman_newton_schulz(dt, count, m, n, G.data_ptr(), out.data_ptr(), int(steps), float(a), float(b),
+                                     float(c), float(eps), ws.data_ptr(), ws.numel(), _stream(G.device))
+        _lib.check(rc, fn)
+    return out

@@ -598,6 +598,29 @@ int elman_gated_linear_backward(int dtype, int T, int B, int d, const void* f, c
                                 void* df, void* dc, void* dz, float* dh0, void* workspace,
                                 size_t workspace_bytes, void* stream);
 
+/*
+ * Newton-Schulz orthogonalisation of `count` dense row-major matrices in[count,m,n] (an extension without a
+ * counterpart in the reference): X = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A A) X with
+ * A = X X^T, which moves every singular value by s -> a s + b s^3 + c s^5 and keeps the singular
+ * vectors; out[count,m,n] of `dtype` (may be `in`).  Products take fp16 operands with fp32 sums (fp32
+ * matrices: two fp16 numbers an element), so coefficients that take singular values beyond 3.5 are refused.
+ * A zero matrix stays zero; a matrix with a NaN or an infinity becomes NaN; the others of the call
+ * are not touched by it.
+ *
+ * elman_muon_step: the Muon update of `count` equally shaped matrices that lie in flat parameter and
+ * gradient buffers; matrix k starts at element offsets[k] (device) of both.  momentum [count,m,n] is fp32:
+ *     g = grads * (*grad_scale);  momentum += (1 - mu) (g - momentum)
+ *     u = nesterov ? g + mu (momentum - g) : momentum
+ *     params = params (1 - lr weight_decay) - lr scale newton_schulz(u)
+ */
+size_t elman_newton_schulz_workspace(int dtype, int count, int m, int n);
+int elman_newton_schulz(int dtype, int count, int m, int n, const void* in, void* out, int steps, float a,
+                        float b, float c, float eps, void* workspace, size_t workspace_bytes, void* stream);
+int elman_muon_step(int dtype, int count, int m, int n, const long long* offsets, void* params,
+                    const void* grads, float* momentum, float lr, float mu, int nesterov,
+                    float weight_decay, float scale, const float* grad_scale, int steps, float a, float b,
+                    float c, float eps, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
