@@ -1,8 +1,7 @@
 // Orthogonalising matrices by Newton-Schulz products, and the Muon update built on it:
 //   X = G / (|G|_F + eps);  steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X
 // (tall matrices: A = X^T X and X <- a X + X B, so that A has the smaller of the two extents, r).
-// A and B are symmetric: only the tiles on and above the diagonal are computed, the others are their
-// mirror images.  Per step 3 r^2 q + r^3 flops with q the larger extent: bound by the tensor cores.
+// A and B are symmetric: only the tiles on and above the diagonal are computed and stored.  Per step 3 r^2 q + r^3 flops with q the larger extent: bound by the tensor cores.
 //
 // Numbers.  The operands are fp16 (11 significant bits; bf16 has 8), scaled by powers of two into its
 // range: X by 2^12, A by 2^12, B by 2^10; every sum is fp32.  The polynomial multiplies small singular
@@ -35,6 +34,13 @@ constexpr float SX = 4096.f, SA = 4096.f, SB = 1024.f;
 constexpr int NORM_PARTS = 64;                        // partial sums of squares a matrix
 
 enum Product { GRAM, SQUARE, UPDATE, LAST };
+// An operand block of rows x K: stored [rows, K]; stored [K, rows] and read MN-major in place; or part of a
+// symmetric matrix of which only the tiles on and above the diagonal are stored: below it the block is the
+// mirrored one, read MN-major.
+enum Form { ROWS_K, K_ROWS, UPPER };
+__device__ __forceinline__ bool mn_major(int form, int row0, int k0) {
+  return form == K_ROWS || (form == UPPER && row0 / TILE > k0 / TILE);
+}
 
 struct Split { __half* hi; __half* lo; };             // lo may be null
 
@@ -51,7 +57,7 @@ struct NsSource {
 struct NsParams {
   int kind, m, n;            // extents of the output
   int K, parts;              // contraction extent; 1, or 3 products of high and low parts
-  int a_mn, b_mn;            // operand stored [K, rows]: read MN-major
+  int a_form, b_form;        // how an operand lies in memory: Form
   int symmetric;
   long ld;                   // row stride of the fp16 output (and of `same`)
   long stride;               // elements between matrices of the output (and of `same`)
@@ -129,41 +135,76 @@ __global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n,
 
 // ------------------------------------------------------------------ products
 
-__device__ __forceinline__ float same_at(const NsParams& p, long at) {
-  return __half2float(p.same.hi[at]) + (p.same.lo != nullptr ? __half2float(p.same.lo[at]) : 0.f);
+__device__ __forceinline__ void add_halves(float (&f)[8], uint4 x, float k) {
+  const __half2* h = reinterpret_cast<const __half2*>(&x);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float2 v = __half22float2(h[q]);
+    f[2 * q] = fmaf(k, v.x, f[2 * q]);
+    f[2 * q + 1] = fmaf(k, v.y, f[2 * q + 1]);
+  }
+}
+__device__ __forceinline__ uint4 to_halves(const float (&f)[8]) {
+  uint4 x;
+  __half2* h = reinterpret_cast<__half2*>(&x);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) h[q] = __floats2half2_rn(f[2 * q], f[2 * q + 1]);
+  return x;
+}
+// Eight adjacent values of the result: X, or the parameters moved by it.
+template <typename T> __device__ __forceinline__ void store8(const NsParams& p, T* dst, const float (&f)[8], int cols) {
+  if (cols >= 8 && ((uintptr_t)dst & 15) == 0) {
+    uint4 x[sizeof(T) / 2];
+    T* v = reinterpret_cast<T*>(x);
+    if (p.muon) {
+#pragma unroll
+      for (int q = 0; q < (int)sizeof(T) / 2; ++q) x[q] = reinterpret_cast<const uint4*>(dst)[q];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = from_f<T>(p.muon ? to_f(v[j]) * p.decay - p.lr * p.scale * f[j] : f[j]);
+#pragma unroll
+    for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(dst)[q] = x[q];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < cols) dst[j] = from_f<T>(p.muon ? to_f(dst[j]) * p.decay - p.lr * p.scale * f[j] : f[j]);
+  }
 }
 
-// 32 columns of one output row as they come out of tensor memory.
+// 32 columns of one output row as they come out of tensor memory.  Rows of the fp16 matrices are whole groups of
+// eight: what lies past the last column is written with it and read by nobody.
 template <typename T>
-__device__ __forceinline__ void finish_row(const NsParams& p, int mat, int row, int col0, const uint32_t (&r)[32], bool mirror) {
-  const bool on = row < p.m;
-  const int cols = p.n - col0 < 32 ? p.n - col0 : 32;
+__device__ __forceinline__ void finish_row(const NsParams& p, int mat, int row, int col0, const uint32_t (&r)[32]) {
+  if (row >= p.m) return;
   const long at = (long)mat * p.stride + (long)row * p.ld + col0;
-  float v[32];
+  uint4 hi[4], lo[4];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    v[j] = p.k_acc * __uint_as_float(r[j]);
-    if (p.kind != GRAM && on && j < cols) v[j] = fmaf(p.k_same, same_at(p, at + j), v[j]);
-  }
-  if (p.kind == LAST) {
-    if (!on) return;
-    T* dst = (T*)p.result + (p.offsets != nullptr ? p.offsets[mat] : (long)mat * p.m * p.n) + (long)row * p.n + col0;
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < cols) dst[j] = p.muon ? from_f<T>(to_f(dst[j]) * p.decay - p.lr * p.scale * v[j]) : from_f<T>(v[j]);
-    return;
+  for (int g = 0; g < 4; ++g) {
+    hi[g] = lo[g] = make_uint4(0, 0, 0, 0);
+    if (p.kind != GRAM && col0 + 8 * g < p.n) {
+      hi[g] = *reinterpret_cast<const uint4*>(p.same.hi + at + 8 * g);
+      if (p.same.lo != nullptr) lo[g] = *reinterpret_cast<const uint4*>(p.same.lo + at + 8 * g);
+    }
   }
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    if (!on || j >= cols) continue;
-    __half hi, lo;
-    split_half(v[j], hi, lo);
-    p.out.hi[at + j] = hi;
-    if (p.out.lo != nullptr) p.out.lo[at + j] = lo;
-    if (mirror) {
-      const long to = (long)mat * p.stride + (long)(col0 + j) * p.ld + row;
-      p.out.hi[to] = hi;
-      if (p.out.lo != nullptr) p.out.lo[to] = lo;
+  for (int g = 0; g < 4; ++g) {
+    const int cols = p.n - col0 - 8 * g;
+    if (cols <= 0) break;
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = p.k_acc * __uint_as_float(r[8 * g + j]);
+    add_halves(f, hi[g], p.k_same);
+    add_halves(f, lo[g], p.k_same);
+    if (p.kind == LAST) {
+      store8(p, (T*)p.result + (p.offsets != nullptr ? p.offsets[mat] : (long)mat * p.m * p.n) + (long)row * p.n + col0 + 8 * g,
+             f, cols);
+      continue;
+    }
+    const uint4 h = to_halves(f);
+    *reinterpret_cast<uint4*>(p.out.hi + at + 8 * g) = h;
+    if (p.out.lo != nullptr) {
+      add_halves(f, h, -1.f);
+      *reinterpret_cast<uint4*>(p.out.lo + at + 8 * g) = to_halves(f);
     }
   }
 }
@@ -225,22 +266,21 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constant
         }
         ptx::mbar_arrive_expect_tx(&full_bar[s], 2 * OPERAND_BYTES);
         if (i == p.stall && blockIdx.x == 0 && mat == 0) continue;
+        const bool a_mn = mn_major(p.a_form, m0, k0), b_mn = mn_major(p.b_form, n0, k0);
         const CUtensorMap* A = part == 2 ? &tAl : &tAh;      // high x high, high x low, low x high
         const CUtensorMap* B = part == 1 ? &tBl : &tBh;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          tch::tma_load_3d(sA + s * OPERAND_BYTES + h * BLOCK_BYTES, A, p.a_mn ? m0 + 64 * h : k0, p.a_mn ? k0 : m0 + 64 * h,
-                           mat, &full_bar[s]);
-          tch::tma_load_3d(sB + s * OPERAND_BYTES + h * BLOCK_BYTES, B, p.b_mn ? n0 + 64 * h : k0, p.b_mn ? k0 : n0 + 64 * h,
-                           mat, &full_bar[s]);
+          tch::tma_load_3d(sA + s * OPERAND_BYTES + h * BLOCK_BYTES, A, a_mn ? m0 + 64 * h : k0, a_mn ? k0 : m0 + 64 * h, mat,
+                           &full_bar[s]);
+          tch::tma_load_3d(sB + s * OPERAND_BYTES + h * BLOCK_BYTES, B, b_mn ? n0 + 64 * h : k0, b_mn ? k0 : n0 + 64 * h, mat,
+                           &full_bar[s]);
         }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc = ptx::umma_idesc_f16(TILE, TILE) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u);
-      const uint64_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;
       bool ok = true;
       for (int i = 0; i < iters && ok; ++i) {
         const int s = i % STAGES;
@@ -252,8 +292,12 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constant
         }
         ptx::tc_fence_after();
         const uint32_t a_addr = ptx::smem_u32(sA + s * OPERAND_BYTES), b_addr = ptx::smem_u32(sB + s * OPERAND_BYTES);
-        const uint64_t da = p.a_mn ? ptx::umma_desc_mn_sw128(a_addr, BLOCK_BYTES) : ptx::umma_desc_k_sw128(a_addr);
-        const uint64_t db = p.b_mn ? ptx::umma_desc_mn_sw128(b_addr, BLOCK_BYTES) : ptx::umma_desc_k_sw128(b_addr);
+        const int k0 = (i % nk) * BK;
+        const bool a_mn = mn_major(p.a_form, m0, k0), b_mn = mn_major(p.b_form, n0, k0);
+        const uint32_t idesc = ptx::umma_idesc_f16(TILE, TILE) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+        const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
+        const uint64_t da = a_mn ? ptx::umma_desc_mn_sw128(a_addr, BLOCK_BYTES) : ptx::umma_desc_k_sw128(a_addr);
+        const uint64_t db = b_mn ? ptx::umma_desc_mn_sw128(b_addr, BLOCK_BYTES) : ptx::umma_desc_k_sw128(b_addr);
         const int sum = p.parts == 1 ? 0 : i < nk ? i % 3 : 3;
         const bool opens = p.parts == 1 ? i == 0 : i < 3 ? i < nk || i == nk : i == nk;
 #pragma unroll
@@ -285,7 +329,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constant
 #pragma unroll
         for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(more[j]));
       }
-      if (n0 + c * 32 < p.n) finish_row<T>(p, mat, m0 + warp * 32 + lane, n0 + c * 32, r, p.symmetric && ti != tj);
+      if (n0 + c * 32 < p.n) finish_row<T>(p, mat, m0 + warp * 32 + lane, n0 + c * 32, r);
     }
   }
   if (abort_flag != 0)
@@ -410,12 +454,12 @@ int run(int dtype, int count, int m, int n, const NsSource& src, int steps, floa
   for (int step = 0; step < steps; ++step) {
     const int at = step & 1;
     // A = X X^T, or X^T X
-    p.kind = GRAM; p.m = p.n = r; p.K = tall ? m : n; p.a_mn = p.b_mn = tall; p.symmetric = 1;
+    p.kind = GRAM; p.m = p.n = r; p.K = tall ? m : n; p.a_form = p.b_form = tall ? K_ROWS : ROWS_K; p.symmetric = 1;
     p.ld = buf.ldr; p.stride = (long)r * buf.ldr; p.k_acc = SA / (SX * SX); p.k_same = 0.f; p.out = buf.A;
     ns_product_kernel<T><<<dim3(triangle, count), 128, NS_SMEM, st>>>(mx[at][0], mx[at][1], mx[at][0], mx[at][1], p);
     count_launch(true);
     // B = b A + c A A
-    p.kind = SQUARE; p.K = r; p.a_mn = p.b_mn = 0; p.k_acc = c * SB / (SA * SA); p.k_same = b * SB / SA;
+    p.kind = SQUARE; p.K = r; p.a_form = p.b_form = UPPER; p.k_acc = c * SB / (SA * SA); p.k_same = b * SB / SA;
     p.same = buf.A; p.out = buf.B;
     ns_product_kernel<T><<<dim3(triangle, count), 128, NS_SMEM, st>>>(ma[0], ma[1], ma[0], ma[1], p);
     count_launch(true);
@@ -428,9 +472,10 @@ int run(int dtype, int count, int m, int n, const NsSource& src, int steps, floa
     if (!takes_low(step)) p.same.lo = nullptr;
     if (!ends && !takes_low(step + 1)) p.out.lo = nullptr;
     if (tall) {
+      p.a_form = ROWS_K;
       ns_product_kernel<T><<<dim3(all, count), 128, NS_SMEM, st>>>(mx[at][0], mx[at][1], mb[0], mb[1], p);
     } else {
-      p.b_mn = 1;
+      p.b_form = K_ROWS;
       ns_product_kernel<T><<<dim3(all, count), 128, NS_SMEM, st>>>(mb[0], mb[1], mx[at][0], mx[at][1], p);
     }
     count_launch(true);
