@@ -26,9 +26,12 @@ namespace elman {
 
 namespace {
 
-constexpr int TILE = 128, BK = 64, STAGES = 3;
+// One block's share of a tile is 128 rows of the product; a pair of blocks (cta_group::2) makes a tile of 256 x 256,
+// a block by itself one of 128 x 128.  Either way a block loads 128 rows of each operand a stage.
+constexpr int BK = 64, STAGES = 6, TICKETS = 4;
+constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
 constexpr int BLOCK_BYTES = 64 * BK * 2;              // one TMA box: 64 x 64 fp16
-constexpr int OPERAND_BYTES = TILE * BK * 2;
+constexpr int OPERAND_BYTES = 128 * BK * 2;
 constexpr int NS_SMEM = STAGES * 2 * OPERAND_BYTES + 1024;
 constexpr float SX = 4096.f, SA = 4096.f, SB = 1024.f;
 constexpr int NORM_PARTS = 64;                        // partial sums of squares a matrix
@@ -38,8 +41,8 @@ enum Product { GRAM, SQUARE, UPDATE, LAST };
 // symmetric matrix of which only the tiles on and above the diagonal are stored: below it the block is the
 // mirrored one, read MN-major.
 enum Form { ROWS_K, K_ROWS, UPPER };
-__device__ __forceinline__ bool mn_major(int form, int row0, int k0) {
-  return form == K_ROWS || (form == UPPER && row0 / TILE > k0 / TILE);
+__device__ __forceinline__ bool mn_major(int form, int row0, int k0, int edge) {
+  return form == K_ROWS || (form == UPPER && row0 / edge > k0 / edge);
 }
 
 struct Split { __half* hi; __half* lo; };             // lo may be null
@@ -54,23 +57,70 @@ struct NsSource {
   const float* grad_scale;   // device, or null
 };
 
-struct NsParams {
-  int kind, m, n;            // extents of the output
-  int K, parts;              // contraction extent; 1, or 3 products of high and low parts
-  int a_form, b_form;        // how an operand lies in memory: Form
-  int symmetric;
-  long ld;                   // row stride of the fp16 output (and of `same`)
-  long stride;               // elements between matrices of the output (and of `same`)
-  float k_acc, k_same;       // output = k_acc * product + k_same * same
-  Split same, out;
-  void* result;              // LAST: [count, m, n], or the flat parameters
+struct NsMaps { CUtensorMap x[2][2], a[2], b[2]; };   // [buffer][high, low part]
+
+// The whole iteration as one list of tiles: step by step, in a step all Gram tiles of all matrices, then the squares',
+// then the updates'.
+struct NsPlan {
+  int count, m, n, r, tall, steps, parts;
+  int triangle, all;         // tiles of a symmetric product and of an update
+  int per_step, total;       // items of the list
+  float a, b, c;
+  Split X[2], A, B;
+  long ldx, ldr;
+  void* result;              // [count, m, n], or the flat parameters
   const long long* offsets;
   int muon;
   float lr, decay, scale;    // Muon: p = p decay - lr scale X
+  int* ticket;               // items handed out
+  int* done;                 // [count]: blocks' shares of tiles finished
   int* status;
   long spin_limit;
-  int stall;
+  int stall;                 // test hook
 };
+__host__ __device__ inline bool takes_low(int step, int steps, int parts) { return parts > 1 || step < steps - 2; }
+
+// One item of the list.
+struct NsItem {
+  int kind, mat, ti, tj, step;
+  int m, n, K, a_form, b_form;
+  int need;                  // tiles of this matrix that have to be finished before
+};
+__device__ __forceinline__ NsItem item_of(const NsPlan& p, int index, int edge) {
+  NsItem it;
+  it.step = index / p.per_step;
+  int w = index - it.step * p.per_step;
+  const int gram = p.count * p.triangle, before = it.step * (2 * p.triangle + p.all);
+  if (w < 2 * gram) {
+    const bool square = w >= gram;
+    if (square) w -= gram;
+    it.kind = square ? SQUARE : GRAM;
+    it.mat = w / p.triangle;
+    const int t = w - it.mat * p.triangle;     // the tiles (i, j >= i), column by column
+    it.tj = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+    while ((it.tj + 1) * (it.tj + 2) / 2 <= t) ++it.tj;
+    while (it.tj * (it.tj + 1) / 2 > t) --it.tj;
+    it.ti = t - it.tj * (it.tj + 1) / 2;
+    it.m = it.n = p.r;
+    it.K = square ? p.r : p.tall ? p.m : p.n;
+    it.a_form = it.b_form = square ? UPPER : p.tall ? K_ROWS : ROWS_K;
+    it.need = before + (square ? p.triangle : 0);
+  } else {
+    w -= 2 * gram;
+    it.kind = it.step == p.steps - 1 ? LAST : UPDATE;
+    it.mat = w / p.all;
+    const int t = w - it.mat * p.all, tiles_n = (p.n + edge - 1) / edge;
+    it.ti = t / tiles_n;
+    it.tj = t - it.ti * tiles_n;
+    it.m = p.m;
+    it.n = p.n;
+    it.K = p.r;
+    it.a_form = p.tall ? ROWS_K : UPPER;       // X B, or B X
+    it.b_form = p.tall ? UPPER : K_ROWS;
+    it.need = before + 2 * p.triangle;
+  }
+  return it;
+}
 
 __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
   hi = __float2half_rn(v);
@@ -93,7 +143,11 @@ template <typename T> __device__ __forceinline__ float source_at(const NsSource&
 
 // Sums of squares in fp64: a sum over millions of elements, of numbers whose squares leave fp32's range.
 template <typename T>
-__global__ void __launch_bounds__(256) ns_norm_kernel(NsSource s, long size, double* partial) {
+__global__ void __launch_bounds__(256) ns_norm_kernel(NsSource s, long size, double* partial, int* ticket, int* done) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    done[blockIdx.y] = 0;
+    if (blockIdx.y == 0) *ticket = 0;
+  }
   const long base = s.offsets != nullptr ? s.offsets[blockIdx.y] : (long)blockIdx.y * size;
   const float gs = s.grad_scale != nullptr ? *s.grad_scale : 1.f;
   double sum = 0.;
@@ -152,7 +206,7 @@ __device__ __forceinline__ uint4 to_halves(const float (&f)[8]) {
   return x;
 }
 // Eight adjacent values of the result: X, or the parameters moved by it.
-template <typename T> __device__ __forceinline__ void store8(const NsParams& p, T* dst, const float (&f)[8], int cols) {
+template <typename T> __device__ __forceinline__ void store8(const NsPlan& p, T* dst, const float (&f)[8], int cols) {
   if (cols >= 8 && ((uintptr_t)dst & 15) == 0) {
     uint4 x[sizeof(T) / 2];
     T* v = reinterpret_cast<T*>(x);
@@ -171,172 +225,353 @@ template <typename T> __device__ __forceinline__ void store8(const NsParams& p, 
   }
 }
 
+// What becomes of a product's rows: k_acc * product + k_same * same.
+struct Finish {
+  float k_acc, k_same;
+  Split same, out;
+  long ld;
+};
+__device__ __forceinline__ Finish finish_of(const NsPlan& p, const NsItem& it) {
+  Finish f;
+  const int at = it.step & 1;
+  if (it.kind == GRAM || it.kind == SQUARE) {
+    f.ld = p.ldr;
+    f.same = p.A;
+    f.out = it.kind == GRAM ? p.A : p.B;
+    f.k_acc = it.kind == GRAM ? SA / (SX * SX) : p.c * (SB / (SA * SA));
+    f.k_same = p.b * (SB / SA);
+  } else {
+    f.ld = p.ldx;
+    f.same = p.X[at];
+    f.out = p.X[at ^ 1];
+    if (!takes_low(it.step, p.steps, p.parts)) f.same.lo = nullptr;
+    if (!takes_low(it.step + 1, p.steps, p.parts)) f.out.lo = nullptr;
+    f.k_acc = it.kind == LAST ? 1.f / (SB * SX) : 1.f / SB;
+    f.k_same = it.kind == LAST ? p.a / SX : p.a;
+  }
+  const long off = (long)it.mat * it.m * f.ld;
+  f.same.hi += off;
+  f.out.hi += off;
+  if (f.same.lo != nullptr) f.same.lo += off;
+  if (f.out.lo != nullptr) f.out.lo += off;
+  return f;
+}
+
 // 32 columns of one output row as they come out of tensor memory.  Rows of the fp16 matrices are whole groups of
 // eight: what lies past the last column is written with it and read by nobody.
 template <typename T>
-__device__ __forceinline__ void finish_row(const NsParams& p, int mat, int row, int col0, const uint32_t (&r)[32]) {
-  if (row >= p.m) return;
-  const long at = (long)mat * p.stride + (long)row * p.ld + col0;
+__device__ __forceinline__ void finish_row(const NsPlan& p, const NsItem& it, const Finish& fin, int row, int col0, const uint32_t (&r)[32]) {
+  if (row >= it.m) return;
+  const long at = (long)row * fin.ld + col0;
   uint4 hi[4], lo[4];
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     hi[g] = lo[g] = make_uint4(0, 0, 0, 0);
-    if (p.kind != GRAM && col0 + 8 * g < p.n) {
-      hi[g] = *reinterpret_cast<const uint4*>(p.same.hi + at + 8 * g);
-      if (p.same.lo != nullptr) lo[g] = *reinterpret_cast<const uint4*>(p.same.lo + at + 8 * g);
+    if (it.kind != GRAM && col0 + 8 * g < it.n) {
+      hi[g] = *reinterpret_cast<const uint4*>(fin.same.hi + at + 8 * g);
+      if (fin.same.lo != nullptr) lo[g] = *reinterpret_cast<const uint4*>(fin.same.lo + at + 8 * g);
     }
   }
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const int cols = p.n - col0 - 8 * g;
+    const int cols = it.n - col0 - 8 * g;
     if (cols <= 0) break;
     float f[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = p.k_acc * __uint_as_float(r[8 * g + j]);
-    add_halves(f, hi[g], p.k_same);
-    add_halves(f, lo[g], p.k_same);
-    if (p.kind == LAST) {
-      store8(p, (T*)p.result + (p.offsets != nullptr ? p.offsets[mat] : (long)mat * p.m * p.n) + (long)row * p.n + col0 + 8 * g,
+    for (int j = 0; j < 8; ++j) f[j] = fin.k_acc * __uint_as_float(r[8 * g + j]);
+    add_halves(f, hi[g], fin.k_same);
+    if (fin.same.lo != nullptr) add_halves(f, lo[g], fin.k_same);
+    if (it.kind == LAST) {
+      store8(p, (T*)p.result + (p.offsets != nullptr ? p.offsets[it.mat] : (long)it.mat * p.m * p.n) + (long)row * p.n + col0 + 8 * g,
              f, cols);
       continue;
     }
     const uint4 h = to_halves(f);
-    *reinterpret_cast<uint4*>(p.out.hi + at + 8 * g) = h;
-    if (p.out.lo != nullptr) {
+    *reinterpret_cast<uint4*>(fin.out.hi + at + 8 * g) = h;
+    if (fin.out.lo != nullptr) {
       add_halves(f, h, -1.f);
-      *reinterpret_cast<uint4*>(p.out.lo + at + 8 * g) = to_halves(f);
+      *reinterpret_cast<uint4*>(fin.out.lo + at + 8 * g) = to_halves(f);
     }
   }
 }
 
-// One block: one 128 x 128 tile.  Thread 0 of warp 0 loads, thread 0 of warp 1 issues the products, all
-// four warps finish the rows.
-template <typename T>
-__global__ void __launch_bounds__(128, 2)
-ns_product_kernel(const __grid_constant__ CUtensorMap tAh, const __grid_constant__ CUtensorMap tAl,
-                  const __grid_constant__ CUtensorMap tBh, const __grid_constant__ CUtensorMap tBl, NsParams p) {
+// All steps in one launch.  Blocks (or pairs) take items from a counter in the list's order; an item starts once the
+// products it reads are finished (`done` of its matrix), which were handed out before it, so whoever waits, waits
+// for someone who runs: no block has to be resident for another's sake, and launches may overlap.  With more than a
+// few matrices the wait is over before it begins.
+// Warp 0 takes the items (the even block of a pair) and loads, warp 1 issues the products (for both blocks), the others
+// finish the rows: two accumulators, so a tile is finished under the next one's products.
+template <typename T, bool PAIR>
+__global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ NsMaps maps, const NsPlan p) {
+  constexpr int EDGE = PAIR ? 256 : 128, BLOCKS = PAIR ? 2 : 1;
   extern __shared__ uint8_t raw[];
-  __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_bar;
+  __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2], tk_full[TICKETS], tk_empty[TICKETS];
+  __shared__ int tk[TICKETS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, mat = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = PAIR ? tch::cluster_ctarank() : 0;
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * OPERAND_BYTES;
-  int ti, tj;
-  const int tiles_n = (p.n + TILE - 1) / TILE;
-  if (p.symmetric) {             // blocks count the tiles (i, j >= i) column by column
-    tj = (int)((sqrtf(8.f * blockIdx.x + 1.f) - 1.f) * 0.5f);
-    while ((tj + 1) * (tj + 2) / 2 <= (int)blockIdx.x) ++tj;
-    while (tj * (tj + 1) / 2 > (int)blockIdx.x) --tj;
-    ti = blockIdx.x - tj * (tj + 1) / 2;
-  } else {
-    ti = blockIdx.x / tiles_n;
-    tj = blockIdx.x - ti * tiles_n;
-  }
-  const int m0 = ti * TILE, n0 = tj * TILE;
-  const int nk = (p.K + BK - 1) / BK, iters = nk * p.parts;
   if (tid == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
       ptx::mbar_init(&full_bar[s], 1);
       ptx::mbar_init(&empty_bar[s], 1);
     }
-    ptx::mbar_init(&acc_bar, 1);
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(&acc_full[b], 1);
+      ptx::mbar_init(&acc_empty[b], BLOCKS * EPI_WARPS);
+    }
+    for (int k = 0; k < TICKETS; ++k) {
+      ptx::mbar_init(&tk_full[k], 1);
+      ptx::mbar_init(&tk_empty[k], 1 + BLOCKS * EPI_WARPS + (BLOCKS - 1));   // products, rows, the odd block's loads
+    }
     ptx::mbar_fence_init();
   }
-  const uint32_t tmem_cols = p.parts > 1 ? 4 * TILE : TILE;
-  if (warp == 0) {
-    ptx::tmem_alloc(&tmem_slot, tmem_cols);
-    ptx::tmem_relinquish();
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      ptx::tmem_alloc_pair(&tmem_slot, 512);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(&tmem_slot, 512);
+      ptx::tmem_relinquish();
+    }
   }
   ptx::tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) tch::cluster_sync_all();
   ptx::tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
   volatile int* abortp = &abort_flag;
+  const int sums = p.parts > 1 ? 1 : 2;              // accumulators in turn (fp32: one of four partial sums)
+  auto give_up = [&](int where) {
+    abort_flag = 1;
+    if constexpr (PAIR)
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tch::mapa(ptx::smem_u32(&abort_flag), rank ^ 1u)), "r"(1) : "memory");
+    report_timeout(p.status, KID_NEWTON_SCHULZ, where);
+  };
+  auto wait_ticket = [&](int q) {                     // (cluster-wide acquire: a pair's come from the even block)
+    long spins = 0;
+    unsigned long long t0 = 0;
+    while (!tch::mbar_try_wait_cluster(&tk_full[q % TICKETS], (uint32_t)(q / TICKETS) & 1u)) {
+      if (++spins > p.spin_limit * 8 || *abortp != 0) return false;
+      if ((spins & 1023) == 0) {
+        const unsigned long long now = ptx::globaltimer_ns();
+        if (t0 == 0) t0 = now;
+        else if (now - t0 > ptx::kWaitDeadlineNs) return false;
+      }
+    }
+    return true;
+  };
+  auto free_ticket = [&](int q) {
+    if constexpr (PAIR) ptx::mbar_arrive_cluster(tch::mapa(ptx::smem_u32(&tk_empty[q % TICKETS]), 0));
+    else ptx::mbar_arrive(&tk_empty[q % TICKETS]);
+  };
+
   if (warp == 0) {
     if (lane == 0) {
-      for (int i = 0; i < iters; ++i) {
-        const int s = i % STAGES, part = i / nk, k0 = (i - part * nk) * BK;
-        if (!ptx::mbar_wait(&empty_bar[s], ((uint32_t)(i / STAGES) & 1u) ^ 1u, p.spin_limit, abortp)) {
-          abort_flag = 1;
-          report_timeout(p.status, KID_NEWTON_SCHULZ, i);
-          break;
+      uint32_t s = 0, ph = 0;
+      long iteration = 0;
+      for (int q = 0; abort_flag == 0; ++q) {
+        const int k = q % TICKETS;
+        int index;
+        if (rank == 0) {
+          if (!ptx::mbar_wait(&tk_empty[k], ((uint32_t)(q / TICKETS) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFB); break; }
+          index = atomicAdd(p.ticket, 1);
+          if (index >= p.total) index = -1;
+          tk[k] = index;
+          ptx::mbar_arrive(&tk_full[k]);
+          if constexpr (PAIR) {
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tch::mapa(ptx::smem_u32(&tk[k]), 1)), "r"(index) : "memory");
+            ptx::mbar_arrive_cluster(tch::mapa(ptx::smem_u32(&tk_full[k]), 1));
+          }
+        } else {
+          if (!wait_ticket(q)) { give_up(0xFFFC); break; }
+          index = tk[k];
+          free_ticket(q);
         }
-        ptx::mbar_arrive_expect_tx(&full_bar[s], 2 * OPERAND_BYTES);
-        if (i == p.stall && blockIdx.x == 0 && mat == 0) continue;
-        const bool a_mn = mn_major(p.a_form, m0, k0), b_mn = mn_major(p.b_form, n0, k0);
-        const CUtensorMap* A = part == 2 ? &tAl : &tAh;      // high x high, high x low, low x high
-        const CUtensorMap* B = part == 1 ? &tBl : &tBh;
+        if (index < 0) break;
+        const NsItem it = item_of(p, index, EDGE);
+        if (it.need > 0) {                            // the products this one reads
+          long spins = 0;
+          unsigned long long t0 = 0;
+          bool ok = true;
+          while (ld_acquire_gpu(p.done + it.mat) < it.need * BLOCKS) {
+            if (++spins > p.spin_limit || abort_flag != 0) { ok = false; break; }
+            if ((spins & 255) == 0) {
+              const unsigned long long now = ptx::globaltimer_ns();
+              if (t0 == 0) t0 = now;
+              else if (now - t0 > ptx::kWaitDeadlineNs) { ok = false; break; }
+            }
+          }
+          if (!ok) { give_up(0xFFFA); break; }
+        }
+        ptx::fence_proxy_async();                     // written by other blocks' stores, read here by TMA
+        const int m0 = it.ti * EDGE + 128 * (int)rank, n0 = it.tj * EDGE + 128 * (int)rank;
+        const int nk = (it.K + BK - 1) / BK, at = it.step & 1;
+        const CUtensorMap *A, *B;
+        if (it.kind == GRAM) A = B = maps.x[at];
+        else if (it.kind == SQUARE) A = B = maps.a;
+        else { A = p.tall ? maps.x[at] : maps.b; B = p.tall ? maps.b : maps.x[at]; }
+        bool ok = true;
+        for (int i = 0; i < nk * p.parts; ++i, ++iteration) {
+          const int part = i / nk, k0 = (i - part * nk) * BK;    // high x high, high x low, low x high
+          if (!ptx::mbar_wait(&empty_bar[s], ph ^ 1u, p.spin_limit, abortp)) { give_up(i); ok = false; break; }
+          if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[s], BLOCKS * 2 * OPERAND_BYTES);
+          const bool a_mn = mn_major(it.a_form, m0, k0, EDGE), b_mn = mn_major(it.b_form, n0, k0, EDGE);
+          if (!(iteration == p.stall && blockIdx.x == 0)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          tch::tma_load_3d(sA + s * OPERAND_BYTES + h * BLOCK_BYTES, A, a_mn ? m0 + 64 * h : k0, a_mn ? k0 : m0 + 64 * h, mat,
-                           &full_bar[s]);
-          tch::tma_load_3d(sB + s * OPERAND_BYTES + h * BLOCK_BYTES, B, b_mn ? n0 + 64 * h : k0, b_mn ? k0 : n0 + 64 * h, mat,
-                           &full_bar[s]);
+            for (int h = 0; h < 2; ++h) {
+              uint8_t* da = sA + s * OPERAND_BYTES + h * BLOCK_BYTES;
+              uint8_t* db = sB + s * OPERAND_BYTES + h * BLOCK_BYTES;
+              const int ax = a_mn ? m0 + 64 * h : k0, ay = a_mn ? k0 : m0 + 64 * h;
+              const int bx = b_mn ? n0 + 64 * h : k0, by = b_mn ? k0 : n0 + 64 * h;
+              if constexpr (PAIR) {
+                const uint32_t bar = tch::mapa(ptx::smem_u32(&full_bar[s]), 0);
+                ptx::tma_load_3d_pair(da, A + (part == 2), ax, ay, it.mat, bar);
+                ptx::tma_load_3d_pair(db, B + (part == 1), bx, by, it.mat, bar);
+              } else {
+                tch::tma_load_3d(da, A + (part == 2), ax, ay, it.mat, &full_bar[s]);
+                tch::tma_load_3d(db, B + (part == 1), bx, by, it.mat, &full_bar[s]);
+              }
+            }
+          }
+          if (++s == STAGES) { s = 0; ph ^= 1u; }
         }
+        if (!ok) break;
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      bool ok = true;
-      for (int i = 0; i < iters && ok; ++i) {
-        const int s = i % STAGES;
-        if (!ptx::mbar_wait(&full_bar[s], (uint32_t)(i / STAGES) & 1u, p.spin_limit, abortp)) {
-          abort_flag = 1;
-          report_timeout(p.status, KID_NEWTON_SCHULZ, i);
-          ok = false;
-          break;
-        }
+    if (lane == 0 && rank == 0) {
+      uint32_t s = 0, ph = 0;
+      bool ready = false, ok = true;
+      for (int q = 0; ok; ++q) {
+        if (!wait_ticket(q)) { give_up(0xFFFD); break; }
+        const int index = tk[q % TICKETS];
+        free_ticket(q);
+        if (index < 0) break;
+        const NsItem it = item_of(p, index, EDGE);
+        const int m0 = it.ti * EDGE, n0 = it.tj * EDGE, nk = (it.K + BK - 1) / BK, iters = nk * p.parts;
+        const int b = q % sums;
+        if (!ptx::mbar_wait(&acc_empty[b], ((uint32_t)(q / sums) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFE); break; }
         ptx::tc_fence_after();
-        const uint32_t a_addr = ptx::smem_u32(sA + s * OPERAND_BYTES), b_addr = ptx::smem_u32(sB + s * OPERAND_BYTES);
-        const int k0 = (i % nk) * BK;
-        const bool a_mn = mn_major(p.a_form, m0, k0), b_mn = mn_major(p.b_form, n0, k0);
-        const uint32_t idesc = ptx::umma_idesc_f16(TILE, TILE) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
-        const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
-        const uint64_t da = a_mn ? ptx::umma_desc_mn_sw128(a_addr, BLOCK_BYTES) : ptx::umma_desc_k_sw128(a_addr);
-        const uint64_t db = b_mn ? ptx::umma_desc_mn_sw128(b_addr, BLOCK_BYTES) : ptx::umma_desc_k_sw128(b_addr);
-        const int sum = p.parts == 1 ? 0 : i < nk ? i % 3 : 3;
-        const bool opens = p.parts == 1 ? i == 0 : i < 3 ? i < nk || i == nk : i == nk;
+        int k0 = 0;
+        for (int i = 0; i < iters; ++i) {
+          if (!ready && !ptx::mbar_wait(&full_bar[s], ph, p.spin_limit, abortp)) { give_up(i); ok = false; break; }
+          const bool a_mn = mn_major(it.a_form, m0, k0, EDGE), b_mn = mn_major(it.b_form, n0, k0, EDGE);
+          const uint32_t idesc = ptx::umma_idesc_f16(EDGE, EDGE) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+          const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
+          const uint32_t a_addr = ptx::smem_u32(sA) + s * OPERAND_BYTES, b_addr = ptx::smem_u32(sB) + s * OPERAND_BYTES;
+          const uint64_t da = a_mn ? ptx::umma_desc_mn_sw128(a_addr, BLOCK_BYTES) : ptx::umma_desc_k_sw128(a_addr);
+          const uint64_t db = b_mn ? ptx::umma_desc_mn_sw128(b_addr, BLOCK_BYTES) : ptx::umma_desc_k_sw128(b_addr);
+          uint32_t s_next = s + 1, ph_next = ph;
+          if (s_next == STAGES) { s_next = 0; ph_next ^= 1u; }
+          if constexpr (PAIR) {
+            ready = ptx::umma_stage_pair(tmem_base + (uint32_t)(b * EDGE), da, db, a_step, b_step, idesc, i > 0 ? 1u : 0u,
+                                         &empty_bar[s], &full_bar[s_next], ph_next);
+          } else {
+            // fp32: the large products take turns in three sums, the others have a fourth
+            const int sum = p.parts == 1 ? b : i < nk ? i % 3 : 3;
+            const bool opens = p.parts == 1 ? i == 0 : i < 3 ? i <= nk : i == nk;
+            ptx::tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k)
-          ptx::umma_bf16(tmem_base + (uint32_t)(sum * TILE), da + a_step * k, db + b_step * k, idesc, opens && k == 0 ? 0u : 1u);
-        ptx::umma_commit(&empty_bar[s]);
+            for (int j = 0; j < BK / 16; ++j)
+              ptx::umma_bf16(tmem_base + (uint32_t)(sum * EDGE), da + a_step * j, db + b_step * j, idesc, opens && j == 0 ? 0u : 1u);
+            ptx::umma_commit(&empty_bar[s]);
+            ready = false;
+          }
+          s = s_next;
+          ph = ph_next;
+          k0 += BK;
+          if (k0 >= it.K) k0 = 0;
+        }
+        if (ok) {
+          if constexpr (PAIR) ptx::umma_commit_pair(&acc_full[b], 3);
+          else ptx::umma_commit(&acc_full[b]);
+        }
       }
-      if (ok) ptx::umma_commit(&acc_bar);
     }
     __syncwarp();
-  }
-  bool ok = ptx::mbar_wait(&acc_bar, 0, p.spin_limit * 8, abortp);
-  if (!ok && abort_flag == 0) {
-    abort_flag = 1;
-    report_timeout(p.status, KID_NEWTON_SCHULZ, 0xFFFF);
-  }
-  ok = __all_sync(0xffffffffu, ok);
-  ptx::tc_fence_after();
-  if (ok) {
-    for (int c = 0; c < TILE / 32; ++c) {
-      uint32_t r[32];
-      ptx::tmem_ld32(tmem_base + ((uint32_t)(warp * 32) << 16) + (uint32_t)(c * 32), r);
-      ptx::tmem_ld_wait();
-      for (int sum = 1; sum < 4 && p.parts > 1; ++sum) {
-        if (sum < 3 && sum >= nk) continue;
-        uint32_t more[32];
-        ptx::tmem_ld32(tmem_base + ((uint32_t)(warp * 32) << 16) + (uint32_t)(sum * TILE + c * 32), more);
-        ptx::tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(more[j]));
+  } else {
+    // warp w may read TMEM lanes [32 (w % 4), +32); the two warps of a quarter split the tile's columns
+    const int quarter = warp & 3, half = (warp - 2) >> 2, et = tid - 64;
+    constexpr int CH = EDGE / 32 / 2;
+    for (int q = 0;; ++q) {
+      bool ok = wait_ticket(q);
+      const int index = tk[q % TICKETS];
+      NsItem it;
+      int b = 0;
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (ok) {
+        if (lane == 0) free_ticket(q);
+        if (index < 0) break;
+        it = item_of(p, index, EDGE);
+        b = q % sums;
+        ok = ptx::mbar_wait(&acc_full[b], (uint32_t)(q / sums) & 1u, p.spin_limit * 8, abortp);
       }
-      if (n0 + c * 32 < p.n) finish_row<T>(p, mat, m0 + warp * 32 + lane, n0 + c * 32, r);
+      if (!ok && abort_flag == 0) give_up(0xFFFF);
+      uint32_t stop;                                  // one verdict for all of them
+      asm volatile(
+          "{\n\t.reg .pred pp, qq;\n\t"
+          "setp.ne.b32 pp, %1, 0;\n\t"
+          "bar.red.or.pred qq, 1, %2, pp;\n\t"
+          "selp.b32 %0, 1, 0, qq;\n\t}"
+          : "=r"(stop)
+          : "r"((uint32_t)(!ok || abort_flag != 0)), "n"(32 * EPI_WARPS)
+          : "memory");
+      if (stop) break;
+      ptx::tc_fence_after();
+      if (lane == 0) (void)ld_acquire_gpu(p.done + it.mat);     // (the loads waited for the value)
+      __syncwarp();
+      const Finish fin = finish_of(p, it);
+      const int row = it.ti * EDGE + 128 * (int)rank + quarter * 32 + lane;
+      const int col0 = it.tj * EDGE + half * (EDGE / 2);
+      const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((p.parts > 1 ? 0 : b * EDGE) + half * (EDGE / 2));
+      const int nk = (it.K + BK - 1) / BK;
+#pragma unroll 1
+      for (int c = 0; c < CH; ++c) {
+        uint32_t r[32];
+        ptx::tmem_ld32(tsrc + (uint32_t)(c * 32), r);
+        ptx::tmem_ld_wait();
+        for (int sum = 1; sum < 4 && p.parts > 1; ++sum) {
+          if (sum < 3 && sum >= nk) continue;
+          uint32_t more[32];
+          ptx::tmem_ld32(tsrc + (uint32_t)(sum * EDGE + c * 32), more);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(more[j]));
+        }
+        if (c == CH - 1) {                            // the accumulator is free again
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (PAIR) ptx::mbar_arrive_cluster(tch::mapa(ptx::smem_u32(&acc_empty[b]), 0));
+            else ptx::mbar_arrive(&acc_empty[b]);
+          }
+        }
+        if (col0 + c * 32 < it.n) finish_row<T>(p, it, fin, row, col0 + c * 32, r);
+      }
+      if (it.kind != LAST) {
+        ptx::fence_proxy_async();
+        __threadfence();
+        asm volatile("bar.sync 2, %0;" ::"n"(32 * EPI_WARPS) : "memory");
+        if (et == 0) red_release_gpu_add(p.done + it.mat, 1);
+      }
     }
   }
   if (abort_flag != 0)
     for (int i = 0; i < 2000; ++i) __nanosleep(100);   // copies in flight land before the shared memory goes
   ptx::tc_fence_before();
   __syncthreads();
-  if (warp == 0) ptx::tmem_dealloc(tmem_base, tmem_cols);
+  if constexpr (PAIR) {
+    tch::cluster_sync_all();                           // the pair's MMAs read both blocks' operands
+    if (warp == 1) ptx::tmem_dealloc_pair(tmem_base, 512);
+  } else {
+    if (warp == 1) ptx::tmem_dealloc(tmem_base, 512);
+  }
 }
 
 // ------------------------------------------------------------------ host
@@ -346,6 +581,8 @@ long padded(long x) { return (x + 7) / 8 * 8; }       // rows start on 16 bytes
 struct NsBuffers {
   Split X[2], A, B;
   double* partial;
+  int* ticket;
+  int* done;
   long ldx, ldr;
   size_t bytes;
 };
@@ -373,6 +610,8 @@ NsBuffers carve(void* ws, int dtype, int count, int m, int n) {
     b.B.lo = (__half*)take(a);
   }
   b.partial = (double*)take((size_t)count * NORM_PARTS * sizeof(double));
+  b.ticket = (int*)take(sizeof(int));
+  b.done = (int*)take((size_t)count * sizeof(int));
   b.bytes = off;
   return b;
 }
@@ -407,12 +646,20 @@ bool stays_in_range(int steps, double a, double b, double c) {
   return true;
 }
 
-template <typename T>
-int run(int dtype, int count, int m, int n, const NsSource& src, int steps, float a, float b, float c, float eps, NsParams last,
-        void* ws, cudaStream_t st) {
-  const NsBuffers buf = carve(ws, dtype, count, m, n);
-  const bool split = dtype == ELMAN_F32, tall = m > n;
-  const int r = tall ? n : m;
+// Pairs run the tensor cores at their full rate, single blocks (128 columns a product) at about half of it, but
+// in tiles a quarter the size: fewer wasted rows and more blocks where there are few tiles.
+bool pays_as_pairs(const NsPlan& p) {
+  if (p.parts > 1) return false;
+  auto rounds = [&](int edge, int units) {     // rounds of tiles a step, in K steps of a tile
+    const double side = (p.r + edge - 1) / edge, q = (p.tall ? p.m : p.n);
+    const double tri = p.count * side * (side + 1) / 2, all = p.count * side * ceil(q / edge);
+    return ceil(tri / units) * q + ceil(tri / units) * p.r + ceil(all / units) * p.r;
+  };
+  return rounds(256, 74) * 512 < rounds(128, 148) * 440;
+}
+
+template <typename T, bool PAIR>
+int launch(const NsMaps& maps, const NsPlan& p, cudaStream_t st) {
   static std::mutex mutex;
   static bool sized[64];
   int dev = 0;
@@ -420,68 +667,71 @@ int run(int dtype, int count, int m, int n, const NsSource& src, int steps, floa
   {
     std::lock_guard<std::mutex> lock(mutex);
     if (dev >= 64 || !sized[dev]) {
-      ELMAN_CUDA_CHECK(cudaFuncSetAttribute(ns_product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM));
+      ELMAN_CUDA_CHECK(cudaFuncSetAttribute(ns_kernel<T, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM));
       if (dev < 64) sized[dev] = true;
     }
   }
-  auto takes_low = [&](int step) { return split || step < steps - 2; };
-  ns_norm_kernel<T><<<dim3(NORM_PARTS, count), 256, 0, st>>>(src, (long)m * n, buf.partial);
-  count_launch(false);
-  const long blocks = ((long)m * n + 256 * 8 - 1) / (256 * 8);
-  Split x0 = buf.X[0];
-  if (!takes_low(0)) x0.lo = nullptr;
-  ns_scale_kernel<T><<<dim3((unsigned)(blocks < 1024 ? blocks : 1024), count), 256, 0, st>>>(src, m, n, buf.ldx, eps, buf.partial, x0);
-  count_launch(false);
-  CUtensorMap mx[2][2], ma[2], mb[2];
-  auto map = [&](CUtensorMap* out, const __half* base, int rows, int cols, long ld) {
-    return make_tmap_f16_sw128(out, base, cols, rows, count, ld, (long)rows * ld);
-  };
-  for (int k = 0; k < 2; ++k) {
-    ELMAN_RETURN_IF(map(&mx[k][0], buf.X[k].hi, m, n, buf.ldx));
-    ELMAN_RETURN_IF(map(&mx[k][1], split ? buf.X[k].lo : buf.X[k].hi, m, n, buf.ldx));
-  }
-  ELMAN_RETURN_IF(map(&ma[0], buf.A.hi, r, r, buf.ldr));
-  ELMAN_RETURN_IF(map(&ma[1], split ? buf.A.lo : buf.A.hi, r, r, buf.ldr));
-  ELMAN_RETURN_IF(map(&mb[0], buf.B.hi, r, r, buf.ldr));
-  ELMAN_RETURN_IF(map(&mb[1], split ? buf.B.lo : buf.B.hi, r, r, buf.ldr));
-  const int side = (r + TILE - 1) / TILE, triangle = side * (side + 1) / 2;
-  const int all = ((m + TILE - 1) / TILE) * ((n + TILE - 1) / TILE);
-  NsParams p = last;
-  p.parts = split ? 3 : 1;
+  const int blocks = PAIR ? 2 : 1, units = 148 / blocks;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(blocks * (p.total < units ? p.total : units)));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = NS_SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = blocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  ELMAN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ns_kernel<T, PAIR>, maps, p));
+  count_launch(true);
+  return ELMAN_OK;
+}
+
+template <typename T>
+int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t st) {
+  const NsBuffers buf = carve(g.workspace, g.dtype, g.count, g.m, g.n);
+  p.count = g.count; p.m = g.m; p.n = g.n; p.tall = g.m > g.n;
+  p.r = p.tall ? g.n : g.m;
+  p.steps = g.steps;
+  p.parts = g.dtype == ELMAN_F32 ? 3 : 1;
+  p.a = g.a; p.b = g.b; p.c = g.c;
+  p.X[0] = buf.X[0]; p.X[1] = buf.X[1]; p.A = buf.A; p.B = buf.B;
+  p.ldx = buf.ldx; p.ldr = buf.ldr;
+  p.ticket = buf.ticket; p.done = buf.done;
   p.status = device_status_ptr();
   p.spin_limit = options().spin_limit;
   p.stall = (int)options().test_stall_step;
-  for (int step = 0; step < steps; ++step) {
-    const int at = step & 1;
-    // A = X X^T, or X^T X
-    p.kind = GRAM; p.m = p.n = r; p.K = tall ? m : n; p.a_form = p.b_form = tall ? K_ROWS : ROWS_K; p.symmetric = 1;
-    p.ld = buf.ldr; p.stride = (long)r * buf.ldr; p.k_acc = SA / (SX * SX); p.k_same = 0.f; p.out = buf.A;
-    ns_product_kernel<T><<<dim3(triangle, count), 128, NS_SMEM, st>>>(mx[at][0], mx[at][1], mx[at][0], mx[at][1], p);
-    count_launch(true);
-    // B = b A + c A A
-    p.kind = SQUARE; p.K = r; p.a_form = p.b_form = UPPER; p.k_acc = c * SB / (SA * SA); p.k_same = b * SB / SA;
-    p.same = buf.A; p.out = buf.B;
-    ns_product_kernel<T><<<dim3(triangle, count), 128, NS_SMEM, st>>>(ma[0], ma[1], ma[0], ma[1], p);
-    count_launch(true);
-    // X <- a X + B X, or a X + X B
-    const bool ends = step == steps - 1;
-    p.kind = ends ? LAST : UPDATE; p.m = m; p.n = n; p.symmetric = 0; p.ld = buf.ldx; p.stride = (long)m * buf.ldx;
-    p.k_acc = 1.f / SB; p.k_same = a;
-    if (ends) { p.k_acc /= SX; p.k_same /= SX; }
-    p.same = buf.X[at]; p.out = buf.X[at ^ 1];
-    if (!takes_low(step)) p.same.lo = nullptr;
-    if (!ends && !takes_low(step + 1)) p.out.lo = nullptr;
-    if (tall) {
-      p.a_form = ROWS_K;
-      ns_product_kernel<T><<<dim3(all, count), 128, NS_SMEM, st>>>(mx[at][0], mx[at][1], mb[0], mb[1], p);
-    } else {
-      p.b_form = K_ROWS;
-      ns_product_kernel<T><<<dim3(all, count), 128, NS_SMEM, st>>>(mb[0], mb[1], mx[at][0], mx[at][1], p);
-    }
-    count_launch(true);
+  const bool pair = pays_as_pairs(p);
+  const int edge = pair ? 256 : 128, side = (p.r + edge - 1) / edge;
+  p.triangle = side * (side + 1) / 2;
+  p.all = ((p.m + edge - 1) / edge) * ((p.n + edge - 1) / edge);
+  const double total = (double)p.steps * p.count * (2. * p.triangle + p.all);
+  ELMAN_ARG_CHECK(total + 1024 < (double)(1L << 31), "matrices too large");
+  p.per_step = p.count * (2 * p.triangle + p.all);
+  p.total = p.steps * p.per_step;
+  NsMaps maps;
+  auto map = [&](CUtensorMap* out, const __half* base, int rows, int cols, long ld) {
+    return make_tmap_f16_sw128(out, base, cols, rows, p.count, ld, (long)rows * ld);
+  };
+  const bool split = p.parts > 1;
+  for (int k = 0; k < 2; ++k) {
+    ELMAN_RETURN_IF(map(&maps.x[k][0], buf.X[k].hi, p.m, p.n, buf.ldx));
+    ELMAN_RETURN_IF(map(&maps.x[k][1], split ? buf.X[k].lo : buf.X[k].hi, p.m, p.n, buf.ldx));
   }
+  ELMAN_RETURN_IF(map(&maps.a[0], buf.A.hi, p.r, p.r, buf.ldr));
+  ELMAN_RETURN_IF(map(&maps.a[1], split ? buf.A.lo : buf.A.hi, p.r, p.r, buf.ldr));
+  ELMAN_RETURN_IF(map(&maps.b[0], buf.B.hi, p.r, p.r, buf.ldr));
+  ELMAN_RETURN_IF(map(&maps.b[1], split ? buf.B.lo : buf.B.hi, p.r, p.r, buf.ldr));
+  const long size = (long)p.m * p.n, blocks = (size + 256 * 8 - 1) / (256 * 8);
+  Split x0 = buf.X[0];
+  if (!takes_low(0, p.steps, p.parts)) x0.lo = nullptr;
+  ns_norm_kernel<T><<<dim3(NORM_PARTS, p.count), 256, 0, st>>>(src, size, buf.partial, buf.ticket, buf.done);
+  count_launch(false);
+  ns_scale_kernel<T><<<dim3((unsigned)(blocks < 1024 ? blocks : 1024), p.count), 256, 0, st>>>(src, p.m, p.n, buf.ldx, g.eps, buf.partial, x0);
+  count_launch(false);
   ELMAN_CUDA_CHECK(cudaGetLastError());
-  return ELMAN_OK;
+  return pair ? launch<T, true>(maps, p, st) : launch<T, false>(maps, p, st);
 }
 
 }  // namespace
@@ -492,10 +742,9 @@ bool newton_schulz_in_range(int steps, float a, float b, float c) { return stays
 int newton_schulz(const NewtonSchulzArgs& a, cudaStream_t st) {
   NsSource src{};
   src.in = a.in;
-  NsParams last{};
-  last.result = a.out;
-  return a.dtype == ELMAN_F32 ? run<float>(a.dtype, a.count, a.m, a.n, src, a.steps, a.a, a.b, a.c, a.eps, last, a.workspace, st)
-                              : run<bf16>(a.dtype, a.count, a.m, a.n, src, a.steps, a.a, a.b, a.c, a.eps, last, a.workspace, st);
+  NsPlan p{};
+  p.result = a.out;
+  return a.dtype == ELMAN_F32 ? run<float>(a, src, p, st) : run<bf16>(a, src, p, st);
 }
 
 int muon_step(const NewtonSchulzArgs& a, const MuonArgs& u, cudaStream_t st) {
@@ -506,15 +755,14 @@ int muon_step(const NewtonSchulzArgs& a, const MuonArgs& u, cudaStream_t st) {
   src.mu = u.mu;
   src.nesterov = u.nesterov;
   src.grad_scale = u.grad_scale;
-  NsParams last{};
-  last.result = u.params;
-  last.offsets = u.offsets;
-  last.muon = 1;
-  last.lr = u.lr;
-  last.decay = 1.f - u.lr * u.weight_decay;
-  last.scale = u.scale;
-  return a.dtype == ELMAN_F32 ? run<float>(a.dtype, a.count, a.m, a.n, src, a.steps, a.a, a.b, a.c, a.eps, last, a.workspace, st)
-                              : run<bf16>(a.dtype, a.count, a.m, a.n, src, a.steps, a.a, a.b, a.c, a.eps, last, a.workspace, st);
+  NsPlan p{};
+  p.result = u.params;
+  p.offsets = u.offsets;
+  p.muon = 1;
+  p.lr = u.lr;
+  p.decay = 1.f - u.lr * u.weight_decay;
+  p.scale = u.scale;
+  return a.dtype == ELMAN_F32 ? run<float>(a, src, p, st) : run<bf16>(a, src, p, st);
 }
 
 }  // namespace elman
