@@ -28,11 +28,13 @@ namespace {
 
 // One block's share of a tile is 128 rows of the product; a pair of blocks (cta_group::2) makes a tile of 256 x 256,
 // a block by itself one of 128 x 128.  Either way a block loads 128 rows of each operand a stage.
-constexpr int BK = 64, STAGES = 6, TICKETS = 4;
+constexpr int BK = 64, STAGES = 5, TICKETS = 4;
 constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
 constexpr int BLOCK_BYTES = 64 * BK * 2;              // one TMA box: 64 x 64 fp16
 constexpr int OPERAND_BYTES = 128 * BK * 2;
-constexpr int NS_SMEM = STAGES * 2 * OPERAND_BYTES + 1024;
+// Rows are finished in boxes of 32 x 32 through shared memory: two buffers a warp, each a box's high and low parts.
+constexpr int BOX_BYTES = 32 * 64, BUFFER_BYTES = 2 * BOX_BYTES;
+constexpr int NS_SMEM = STAGES * 2 * OPERAND_BYTES + EPI_WARPS * 2 * BUFFER_BYTES + 1024;
 constexpr float SX = 4096.f, SA = 4096.f, SB = 1024.f;
 constexpr int NORM_PARTS = 64;                        // partial sums of squares a matrix
 
@@ -57,7 +59,11 @@ struct NsSource {
   const float* grad_scale;   // device, or null
 };
 
-struct NsMaps { CUtensorMap x[2][2], a[2], b[2]; };   // [buffer][high, low part]
+// [buffer][high, low part]; operands in boxes of 64 x 64, results in boxes of 32 x 32.
+struct NsMaps {
+  CUtensorMap x[2][2], a[2], b[2];
+  CUtensorMap rx[2][2], ra[2], rb[2];
+};
 
 // The whole iteration as one list of tiles: step by step, in a step all Gram tiles of all matrices, then the squares',
 // then the updates'.
@@ -73,7 +79,7 @@ struct NsPlan {
   int muon;
   float lr, decay, scale;    // Muon: p = p decay - lr scale X
   int* ticket;               // items handed out
-  int* done;                 // [count]: blocks' shares of tiles finished
+  int* done;                 // [count]: warps' shares of tiles finished
   int* status;
   long spin_limit;
   int stall;                 // test hook
@@ -205,93 +211,60 @@ __device__ __forceinline__ uint4 to_halves(const float (&f)[8]) {
   for (int q = 0; q < 4; ++q) h[q] = __floats2half2_rn(f[2 * q], f[2 * q + 1]);
   return x;
 }
-// Eight adjacent values of the result: X, or the parameters moved by it.
-template <typename T> __device__ __forceinline__ void store8(const NsPlan& p, T* dst, const float (&f)[8], int cols) {
-  if (cols >= 8 && ((uintptr_t)dst & 15) == 0) {
-    uint4 x[sizeof(T) / 2];
-    T* v = reinterpret_cast<T*>(x);
-    if (p.muon) {
-#pragma unroll
-      for (int q = 0; q < (int)sizeof(T) / 2; ++q) x[q] = reinterpret_cast<const uint4*>(dst)[q];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = from_f<T>(p.muon ? to_f(v[j]) * p.decay - p.lr * p.scale * f[j] : f[j]);
-#pragma unroll
-    for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(dst)[q] = x[q];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < cols) dst[j] = from_f<T>(p.muon ? to_f(dst[j]) * p.decay - p.lr * p.scale * f[j] : f[j]);
-  }
+__device__ __forceinline__ void sts_u4(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// What becomes of a product's rows: k_acc * product + k_same * same.
+// What becomes of a product: k_acc * product + k_same * same.
 struct Finish {
   float k_acc, k_same;
-  Split same, out;
-  long ld;
+  const CUtensorMap *same, *out;    // [high, low]
+  bool same_low, out_low;
 };
-__device__ __forceinline__ Finish finish_of(const NsPlan& p, const NsItem& it) {
+__device__ __forceinline__ Finish finish_of(const NsPlan& p, const NsMaps& maps, const NsItem& it) {
   Finish f;
   const int at = it.step & 1;
   if (it.kind == GRAM || it.kind == SQUARE) {
-    f.ld = p.ldr;
-    f.same = p.A;
-    f.out = it.kind == GRAM ? p.A : p.B;
+    f.same = maps.ra;
+    f.out = it.kind == GRAM ? maps.ra : maps.rb;
+    f.same_low = f.out_low = p.parts > 1;
     f.k_acc = it.kind == GRAM ? SA / (SX * SX) : p.c * (SB / (SA * SA));
     f.k_same = p.b * (SB / SA);
   } else {
-    f.ld = p.ldx;
-    f.same = p.X[at];
-    f.out = p.X[at ^ 1];
-    if (!takes_low(it.step, p.steps, p.parts)) f.same.lo = nullptr;
-    if (!takes_low(it.step + 1, p.steps, p.parts)) f.out.lo = nullptr;
+    f.same = maps.rx[at];
+    f.out = maps.rx[at ^ 1];
+    f.same_low = takes_low(it.step, p.steps, p.parts);
+    f.out_low = takes_low(it.step + 1, p.steps, p.parts);
     f.k_acc = it.kind == LAST ? 1.f / (SB * SX) : 1.f / SB;
     f.k_same = it.kind == LAST ? p.a / SX : p.a;
   }
-  const long off = (long)it.mat * it.m * f.ld;
-  f.same.hi += off;
-  f.out.hi += off;
-  if (f.same.lo != nullptr) f.same.lo += off;
-  if (f.out.lo != nullptr) f.out.lo += off;
   return f;
 }
 
-// 32 columns of one output row as they come out of tensor memory.  Rows of the fp16 matrices are whole groups of
-// eight: what lies past the last column is written with it and read by nobody.
+// A box of the last step's result: from shared memory (row r of sizeof(T) * 32 bytes, 16-byte pieces xor-ed with the row)
+// to the rows of X or of the parameters, a lane a column: any alignment, whole rows of the box an instruction.
+template <typename T> __device__ __forceinline__ uint32_t result_at(uint32_t box, int r, int col) {
+  constexpr int PER = 16 / sizeof(T), PIECES = 32 / PER;
+  return box + (uint32_t)(r * 32 * (int)sizeof(T) + (((col / PER) ^ (PIECES == 4 ? r >> 1 & 3 : r & 7)) * 16) + col % PER * (int)sizeof(T));
+}
+template <typename T> __device__ __forceinline__ T lds_as(uint32_t addr);
+template <> __device__ __forceinline__ float lds_as<float>(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+template <> __device__ __forceinline__ bf16 lds_as<bf16>(uint32_t addr) { return __ushort_as_bfloat16(tch::lds_u16(addr)); }
 template <typename T>
-__device__ __forceinline__ void finish_row(const NsPlan& p, const NsItem& it, const Finish& fin, int row, int col0, const uint32_t (&r)[32]) {
-  if (row >= it.m) return;
-  const long at = (long)row * fin.ld + col0;
-  uint4 hi[4], lo[4];
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    hi[g] = lo[g] = make_uint4(0, 0, 0, 0);
-    if (it.kind != GRAM && col0 + 8 * g < it.n) {
-      hi[g] = *reinterpret_cast<const uint4*>(fin.same.hi + at + 8 * g);
-      if (fin.same.lo != nullptr) lo[g] = *reinterpret_cast<const uint4*>(fin.same.lo + at + 8 * g);
-    }
-  }
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int cols = it.n - col0 - 8 * g;
-    if (cols <= 0) break;
-    float f[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = fin.k_acc * __uint_as_float(r[8 * g + j]);
-    add_halves(f, hi[g], fin.k_same);
-    if (fin.same.lo != nullptr) add_halves(f, lo[g], fin.k_same);
-    if (it.kind == LAST) {
-      store8(p, (T*)p.result + (p.offsets != nullptr ? p.offsets[it.mat] : (long)it.mat * p.m * p.n) + (long)row * p.n + col0 + 8 * g,
-             f, cols);
-      continue;
-    }
-    const uint4 h = to_halves(f);
-    *reinterpret_cast<uint4*>(fin.out.hi + at + 8 * g) = h;
-    if (fin.out.lo != nullptr) {
-      add_halves(f, h, -1.f);
-      *reinterpret_cast<uint4*>(fin.out.lo + at + 8 * g) = to_halves(f);
-    }
+__device__ __forceinline__ void write_result(const NsPlan& p, const NsItem& it, uint32_t box, int row0, int col0) {
+  const int lane = threadIdx.x & 31, rows = it.m - row0 < 32 ? it.m - row0 : 32;
+  if (col0 + lane >= it.n) return;
+  T* dst = (T*)p.result + (p.offsets != nullptr ? p.offsets[it.mat] : (long)it.mat * p.m * p.n) + (long)row0 * p.n + col0 + lane;
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r) {
+    if (r >= rows) break;
+    const T x = lds_as<T>(result_at<T>(box, r, lane));
+    if (p.muon) dst[(long)r * p.n] = from_f<T>(to_f(dst[(long)r * p.n]) * p.decay - p.lr * p.scale * to_f(x));
+    else dst[(long)r * p.n] = x;
   }
 }
 
@@ -306,6 +279,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
   constexpr int EDGE = PAIR ? 256 : 128, BLOCKS = PAIR ? 2 : 1;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2], tk_full[TICKETS], tk_empty[TICKETS];
+  __shared__ __align__(8) uint64_t same_bar[EPI_WARPS][2];
   __shared__ int tk[TICKETS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -328,6 +302,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       ptx::mbar_init(&tk_full[k], 1);
       ptx::mbar_init(&tk_empty[k], 1 + BLOCKS * EPI_WARPS + (BLOCKS - 1));   // products, rows, the odd block's loads
     }
+    for (int k = 0; k < 2 * EPI_WARPS; ++k) ptx::mbar_init(&same_bar[k >> 1][k & 1], 1);
     ptx::mbar_fence_init();
   }
   if (warp == 1) {
@@ -370,6 +345,20 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     else ptx::mbar_arrive(&tk_empty[q % TICKETS]);
   };
 
+  auto finished = [&](const NsItem& it) {              // waits for the products an item reads
+    long spins = 0;
+    unsigned long long t0 = 0;
+    while (ld_acquire_gpu(p.done + it.mat) < it.need * BLOCKS * EPI_WARPS) {
+      if (++spins > p.spin_limit || *abortp != 0) return false;
+      if ((spins & 255) == 0) {
+        const unsigned long long now = ptx::globaltimer_ns();
+        if (t0 == 0) t0 = now;
+        else if (now - t0 > ptx::kWaitDeadlineNs) return false;
+      }
+    }
+    return true;
+  };
+
   if (warp == 0) {
     if (lane == 0) {
       uint32_t s = 0, ph = 0;
@@ -394,20 +383,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         }
         if (index < 0) break;
         const NsItem it = item_of(p, index, EDGE);
-        if (it.need > 0) {                            // the products this one reads
-          long spins = 0;
-          unsigned long long t0 = 0;
-          bool ok = true;
-          while (ld_acquire_gpu(p.done + it.mat) < it.need * BLOCKS) {
-            if (++spins > p.spin_limit || abort_flag != 0) { ok = false; break; }
-            if ((spins & 255) == 0) {
-              const unsigned long long now = ptx::globaltimer_ns();
-              if (t0 == 0) t0 = now;
-              else if (now - t0 > ptx::kWaitDeadlineNs) { ok = false; break; }
-            }
-          }
-          if (!ok) { give_up(0xFFFA); break; }
-        }
+        if (!finished(it)) { give_up(0xFFFA); break; }
         ptx::fence_proxy_async();                     // written by other blocks' stores, read here by TMA
         const int m0 = it.ti * EDGE + 128 * (int)rank, n0 = it.tj * EDGE + 128 * (int)rank;
         const int nk = (it.K + BK - 1) / BK, at = it.step & 1;
@@ -497,8 +473,22 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     __syncwarp();
   } else {
     // warp w may read TMEM lanes [32 (w % 4), +32); the two warps of a quarter split the tile's columns
-    const int quarter = warp & 3, half = (warp - 2) >> 2, et = tid - 64;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
     constexpr int CH = EDGE / 32 / 2;
+    const uint32_t staging = ptx::smem_u32(smem) + STAGES * 2 * OPERAND_BYTES + (uint32_t)((warp - 2) * 2 * BUFFER_BYTES);
+    uint32_t same_phase = 0;
+    int boxes = 0, row0 = 0, col0 = 0;                // boxes taken: they alternate between the warp's buffers
+    Finish fin;
+    // (lane 0) brings box c of `same` into the buffer of box number `box`
+    auto fetch = [&](const Finish& f, const NsItem& it, int c, int box) {
+      const int col = col0 + c * 32;
+      if (it.kind == GRAM || row0 >= it.m || col >= it.n) return;
+      uint64_t* bar = &same_bar[warp - 2][box & 1];
+      uint8_t* to = smem + (staging - ptx::smem_u32(smem)) + (box & 1) * BUFFER_BYTES;
+      ptx::mbar_arrive_expect_tx(bar, f.same_low ? 2 * BOX_BYTES : BOX_BYTES);
+      tch::tma_load_3d(to, f.same, col, row0, it.mat, bar);
+      if (f.same_low) tch::tma_load_3d(to + BOX_BYTES, f.same + 1, col, row0, it.mat, bar);
+    };
     for (int q = 0;; ++q) {
       bool ok = wait_ticket(q);
       const int index = tk[q % TICKETS];
@@ -510,7 +500,19 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         if (index < 0) break;
         it = item_of(p, index, EDGE);
         b = q % sums;
-        ok = ptx::mbar_wait(&acc_full[b], (uint32_t)(q / sums) & 1u, p.spin_limit * 8, abortp);
+        row0 = it.ti * EDGE + 128 * (int)rank + quarter * 32;
+        col0 = it.tj * EDGE + half * (EDGE / 2);
+        fin = finish_of(p, maps, it);
+        if (lane == 0 && it.kind != GRAM) {           // under the products: the first box of `same`
+          ok = finished(it);
+          ptx::fence_proxy_async();
+          if (ok) {
+            tch::bulk_wait_read_all();
+            fetch(fin, it, 0, boxes);
+          }
+        }
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        ok = ok && ptx::mbar_wait(&acc_full[b], (uint32_t)(q / sums) & 1u, p.spin_limit * 8, abortp);
       }
       if (!ok && abort_flag == 0) give_up(0xFFFF);
       uint32_t stop;                                  // one verdict for all of them
@@ -524,15 +526,10 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           : "memory");
       if (stop) break;
       ptx::tc_fence_after();
-      if (lane == 0) (void)ld_acquire_gpu(p.done + it.mat);     // (the loads waited for the value)
-      __syncwarp();
-      const Finish fin = finish_of(p, it);
-      const int row = it.ti * EDGE + 128 * (int)rank + quarter * 32 + lane;
-      const int col0 = it.tj * EDGE + half * (EDGE / 2);
       const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((p.parts > 1 ? 0 : b * EDGE) + half * (EDGE / 2));
       const int nk = (it.K + BK - 1) / BK;
 #pragma unroll 1
-      for (int c = 0; c < CH; ++c) {
+      for (int c = 0; c < CH; ++c, ++boxes) {
         uint32_t r[32];
         ptx::tmem_ld32(tsrc + (uint32_t)(c * 32), r);
         ptx::tmem_ld_wait();
@@ -552,15 +549,72 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
             else ptx::mbar_arrive(&acc_empty[b]);
           }
         }
-        if (col0 + c * 32 < it.n) finish_row<T>(p, it, fin, row, col0 + c * 32, r);
+        const int col = col0 + c * 32;
+        const bool wanted = row0 < it.m && col < it.n;
+        const uint32_t buffer = staging + (uint32_t)((boxes & 1) * BUFFER_BYTES);
+        if (lane == 0) {
+          tch::bulk_wait_read_all();                  // the other buffer's last box has left
+          if (c + 1 < CH) fetch(fin, it, c + 1, boxes + 1);
+        }
+        __syncwarp();
+        if (!wanted) continue;
+        if (it.kind != GRAM && !ptx::mbar_wait(&same_bar[warp - 2][boxes & 1], (same_phase >> (boxes & 1)) & 1u, p.spin_limit * 8, abortp) &&
+            abort_flag == 0)
+          give_up(0xFFF9);                            // (what follows is invalid and reported)
+        if (it.kind != GRAM) same_phase ^= 1u << (boxes & 1);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float f[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = fin.k_acc * __uint_as_float(r[8 * g + j]);
+          const uint32_t piece = buffer + (uint32_t)(lane * 64 + ((g ^ (lane >> 1 & 3)) << 4));
+          if (it.kind != GRAM) {
+            add_halves(f, tch::lds_u4(piece), fin.k_same);
+            if (fin.same_low) add_halves(f, tch::lds_u4(piece + BOX_BYTES), fin.k_same);
+          }
+          if (it.kind == LAST) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[8 * g + j] = __float_as_uint(f[j]);
+            continue;
+          }
+          const uint4 h = to_halves(f);
+          sts_u4(piece, h);
+          if (fin.out_low) {
+            add_halves(f, h, -1.f);
+            sts_u4(piece + BOX_BYTES, to_halves(f));
+          }
+        }
+        if (it.kind == LAST) {
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 32; j += 16 / (int)sizeof(T)) {
+            alignas(16) T x[16 / sizeof(T)];
+#pragma unroll
+            for (int k = 0; k < (int)(16 / sizeof(T)); ++k) x[k] = from_f<T>(__uint_as_float(r[j + k]));
+            sts_u4(result_at<T>(buffer, lane, j), *reinterpret_cast<const uint4*>(x));
+          }
+          __syncwarp();
+          write_result<T>(p, it, buffer, row0, col);
+          ptx::fence_proxy_async_smem();              // read here, next written by TMA
+          __syncwarp();
+        } else {
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tch::tma_store_3d(fin.out, smem + (buffer - ptx::smem_u32(smem)), col, row0, it.mat);
+            if (fin.out_low) tch::tma_store_3d(fin.out + 1, smem + (buffer + BOX_BYTES - ptx::smem_u32(smem)), col, row0, it.mat);
+            tch::bulk_commit();
+          }
+        }
       }
-      if (it.kind != LAST) {
+      if (it.kind != LAST && lane == 0) {
+        tch::bulk_wait_all();                         // written, not only read
         ptx::fence_proxy_async();
         __threadfence();
-        asm volatile("bar.sync 2, %0;" ::"n"(32 * EPI_WARPS) : "memory");
-        if (et == 0) red_release_gpu_add(p.done + it.mat, 1);
+        red_release_gpu_add(p.done + it.mat, 1);
       }
     }
+    if (lane == 0) tch::bulk_wait_read_all();
   }
   if (abort_flag != 0)
     for (int i = 0; i < 2000; ++i) __nanosleep(100);   // copies in flight land before the shared memory goes
@@ -711,18 +765,19 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   p.per_step = p.count * (2 * p.triangle + p.all);
   p.total = p.steps * p.per_step;
   NsMaps maps;
-  auto map = [&](CUtensorMap* out, const __half* base, int rows, int cols, long ld) {
-    return make_tmap_f16_sw128(out, base, cols, rows, p.count, ld, (long)rows * ld);
+  auto map = [&](CUtensorMap* out, CUtensorMap* box, const __half* base, int rows, int cols, long ld) {
+    ELMAN_RETURN_IF(make_tmap_f16(box, base, cols, rows, p.count, ld, (long)rows * ld, 32));
+    return make_tmap_f16(out, base, cols, rows, p.count, ld, (long)rows * ld, 64);
   };
   const bool split = p.parts > 1;
   for (int k = 0; k < 2; ++k) {
-    ELMAN_RETURN_IF(map(&maps.x[k][0], buf.X[k].hi, p.m, p.n, buf.ldx));
-    ELMAN_RETURN_IF(map(&maps.x[k][1], split ? buf.X[k].lo : buf.X[k].hi, p.m, p.n, buf.ldx));
+    ELMAN_RETURN_IF(map(&maps.x[k][0], &maps.rx[k][0], buf.X[k].hi, p.m, p.n, buf.ldx));
+    ELMAN_RETURN_IF(map(&maps.x[k][1], &maps.rx[k][1], buf.X[k].lo, p.m, p.n, buf.ldx));
   }
-  ELMAN_RETURN_IF(map(&maps.a[0], buf.A.hi, p.r, p.r, buf.ldr));
-  ELMAN_RETURN_IF(map(&maps.a[1], split ? buf.A.lo : buf.A.hi, p.r, p.r, buf.ldr));
-  ELMAN_RETURN_IF(map(&maps.b[0], buf.B.hi, p.r, p.r, buf.ldr));
-  ELMAN_RETURN_IF(map(&maps.b[1], split ? buf.B.lo : buf.B.hi, p.r, p.r, buf.ldr));
+  ELMAN_RETURN_IF(map(&maps.a[0], &maps.ra[0], buf.A.hi, p.r, p.r, buf.ldr));
+  ELMAN_RETURN_IF(map(&maps.a[1], &maps.ra[1], split ? buf.A.lo : buf.A.hi, p.r, p.r, buf.ldr));
+  ELMAN_RETURN_IF(map(&maps.b[0], &maps.rb[0], buf.B.hi, p.r, p.r, buf.ldr));
+  ELMAN_RETURN_IF(map(&maps.b[1], &maps.rb[1], split ? buf.B.lo : buf.B.hi, p.r, p.r, buf.ldr));
   const long size = (long)p.m * p.n, blocks = (size + 256 * 8 - 1) / (256 * 8);
   Split x0 = buf.X[0];
   if (!takes_low(0, p.steps, p.parts)) x0.lo = nullptr;
