@@ -128,73 +128,6 @@ __device__ __forceinline__ NsItem item_of(const NsPlan& p, int index, int edge) 
   return it;
 }
 
-__device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
-  hi = __float2half_rn(v);
-  lo = __float2half_rn(v - __half2float(hi));
-}
-
-// ------------------------------------------------------------------ start: norm and scaling
-
-template <typename T> __device__ __forceinline__ float source_at(const NsSource& s, long at, long dense, float gs, bool advance) {
-  float g = to_f(((const T*)s.in)[at]);
-  if (s.momentum == nullptr) return g;
-  g *= gs;
-  float mom = s.momentum[dense];
-  if (advance) {
-    mom += (1.f - s.mu) * (g - mom);
-    s.momentum[dense] = mom;
-  }
-  return s.nesterov ? g + s.mu * (mom - g) : mom;
-}
-
-// Sums of squares in fp64: a sum over millions of elements, of numbers whose squares leave fp32's range.
-template <typename T>
-__global__ void __launch_bounds__(256) ns_norm_kernel(NsSource s, long size, double* partial, int* ticket, int* done) {
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    done[blockIdx.y] = 0;
-    if (blockIdx.y == 0) *ticket = 0;
-  }
-  const long base = s.offsets != nullptr ? s.offsets[blockIdx.y] : (long)blockIdx.y * size;
-  const float gs = s.grad_scale != nullptr ? *s.grad_scale : 1.f;
-  double sum = 0.;
-  for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < size; e += NORM_PARTS * 256) {
-    const double v = source_at<T>(s, base + e, (long)blockIdx.y * size + e, gs, true);
-    sum += v * v;
-  }
-  __shared__ double warp_sum[8];
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_down_sync(0xFFFFFFFFu, sum, o);
-  if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int k = 1; k < 8; ++k) sum += warp_sum[k];
-    partial[(long)blockIdx.y * NORM_PARTS + blockIdx.x] = sum;
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n, long ld, float eps, const double* partial, Split x) {
-  __shared__ double total;
-  if (threadIdx.x == 0) {
-    double t = 0.;
-    for (int k = 0; k < NORM_PARTS; ++k) t += partial[(long)blockIdx.y * NORM_PARTS + k];
-    total = t;
-  }
-  __syncthreads();
-  const float scale = (float)(SX / (sqrt(total) + (double)eps));
-  const float gs = s.grad_scale != nullptr ? *s.grad_scale : 1.f;
-  const long size = (long)m * n, base = s.offsets != nullptr ? s.offsets[blockIdx.y] : (long)blockIdx.y * size;
-  const long to = (long)blockIdx.y * m * ld;
-  for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < size; e += (long)gridDim.x * 256) {
-    const long row = e / n, col = e - row * n;
-    __half hi, lo;
-    split_half(source_at<T>(s, base + e, (long)blockIdx.y * size + e, gs, false) * scale, hi, lo);
-    x.hi[to + row * ld + col] = hi;
-    if (x.lo != nullptr) x.lo[to + row * ld + col] = lo;
-  }
-}
-
-// ------------------------------------------------------------------ products
-
 __device__ __forceinline__ void add_halves(float (&f)[8], uint4 x, float k) {
   const __half2* h = reinterpret_cast<const __half2*>(&x);
 #pragma unroll
@@ -211,6 +144,128 @@ __device__ __forceinline__ uint4 to_halves(const float (&f)[8]) {
   for (int q = 0; q < 4; ++q) h[q] = __floats2half2_rn(f[2 * q], f[2 * q + 1]);
   return x;
 }
+
+// ------------------------------------------------------------------ start: norm and scaling
+
+// Muon's momentum moves by (1 - mu)(g - momentum); the update is it, or Nesterov's look ahead.
+__device__ __forceinline__ float advance(const NsSource& s, float g, float gs, float& momentum) {
+  g *= gs;
+  momentum += (1.f - s.mu) * (g - momentum);
+  return s.nesterov ? g + s.mu * (momentum - g) : momentum;
+}
+__device__ __forceinline__ float look_ahead(const NsSource& s, float g, float gs, float momentum) {
+  g *= gs;
+  return s.nesterov ? g + s.mu * (momentum - g) : momentum;
+}
+// Eight adjacent elements as one or two 16-byte accesses.
+template <typename T> __device__ __forceinline__ void load8(const T* at, float (&f)[8]) {
+  uint4 x[sizeof(T) / 2];
+#pragma unroll
+  for (int q = 0; q < (int)sizeof(T) / 2; ++q) x[q] = reinterpret_cast<const uint4*>(at)[q];
+  const T* v = reinterpret_cast<const T*>(x);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = to_f(v[j]);
+}
+__device__ __forceinline__ void store8(float* at, const float (&f)[8]) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) reinterpret_cast<float4*>(at)[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+}
+
+// Sums of squares in fp64: a sum over millions of elements, of numbers whose squares leave fp32's range.  Also starts
+// the counters of the products.
+template <typename T>
+__global__ void __launch_bounds__(256) ns_norm_kernel(NsSource s, long size, double* partial, int* ticket, int* done) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    done[blockIdx.y] = 0;
+    if (blockIdx.y == 0) *ticket = 0;
+  }
+  const T* in = (const T*)s.in + (s.offsets != nullptr ? s.offsets[blockIdx.y] : (long)blockIdx.y * size);
+  float* momentum = s.momentum != nullptr ? s.momentum + (long)blockIdx.y * size : nullptr;
+  const float gs = s.grad_scale != nullptr ? *s.grad_scale : 1.f;
+  double sum = 0.;
+  const bool vec = (((uintptr_t)in | (uintptr_t)momentum) & 15) == 0;
+  const long whole = vec ? size / 8 : 0;
+  for (long g = (long)blockIdx.x * 256 + threadIdx.x; g < whole; g += NORM_PARTS * 256) {
+    float f[8];
+    load8(in + 8 * g, f);
+    if (momentum != nullptr) {
+      float mom[8];
+      load8(momentum + 8 * g, mom);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = advance(s, f[j], gs, mom[j]);
+      store8(momentum + 8 * g, mom);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = fma((double)f[j], (double)f[j], sum);
+  }
+  for (long e = 8 * whole + (long)blockIdx.x * 256 + threadIdx.x; e < size; e += NORM_PARTS * 256) {
+    float v = to_f(in[e]);
+    if (momentum != nullptr) {
+      float mom = momentum[e];
+      v = advance(s, v, gs, mom);
+      momentum[e] = mom;
+    }
+    sum = fma((double)v, (double)v, sum);
+  }
+  __shared__ double warp_sum[8];
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_down_sync(0xFFFFFFFFu, sum, o);
+  if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < 8; ++k) sum += warp_sum[k];
+    partial[(long)blockIdx.y * NORM_PARTS + blockIdx.x] = sum;
+  }
+}
+
+// A warp a row: X_0, scaled, as the sum of two fp16 numbers.
+template <typename T>
+__global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n, long ld, float eps, const double* partial, Split x) {
+  const int lane = threadIdx.x & 31;
+  static_assert(NORM_PARTS == 64, "two partial sums a lane");
+  double total = partial[(long)blockIdx.y * NORM_PARTS + lane] + partial[(long)blockIdx.y * NORM_PARTS + 32 + lane];
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+  const float scale = (float)(SX / (sqrt(total) + (double)eps));
+  const long size = (long)m * n;
+  const T* in = (const T*)s.in + (s.offsets != nullptr ? s.offsets[blockIdx.y] : (long)blockIdx.y * size);
+  const float* momentum = s.momentum != nullptr ? s.momentum + (long)blockIdx.y * size : nullptr;
+  const float gs = s.grad_scale != nullptr ? *s.grad_scale : 1.f;
+  const bool vec = n % 8 == 0 && (((uintptr_t)in | (uintptr_t)momentum) & 15) == 0;
+  for (long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5); row < m; row += (long)gridDim.x * 8) {
+    const long from = row * n, to = ((long)blockIdx.y * m + row) * ld;
+    if (vec) {
+      for (int col = 8 * lane; col < n; col += 256) {
+        float f[8];
+        load8(in + from + col, f);
+        if (momentum != nullptr) {
+          float mom[8];
+          load8(momentum + from + col, mom);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = look_ahead(s, f[j], gs, mom[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= scale;
+        const uint4 h = to_halves(f);
+        *reinterpret_cast<uint4*>(x.hi + to + col) = h;
+        if (x.lo != nullptr) {
+          add_halves(f, h, -1.f);
+          *reinterpret_cast<uint4*>(x.lo + to + col) = to_halves(f);
+        }
+      }
+    } else {
+      for (int col = lane; col < n; col += 32) {
+        float v = to_f(in[from + col]);
+        if (momentum != nullptr) v = look_ahead(s, v, gs, momentum[from + col]);
+        v *= scale;
+        const __half hi = __float2half_rn(v);
+        x.hi[to + col] = hi;
+        if (x.lo != nullptr) x.lo[to + col] = __float2half_rn(v - __half2float(hi));
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ products
+
 __device__ __forceinline__ void sts_u4(uint32_t addr, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -610,7 +665,6 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       if (it.kind != LAST && lane == 0) {
         tch::bulk_wait_all();                         // written, not only read
         ptx::fence_proxy_async();
-        __threadfence();
         red_release_gpu_add(p.done + it.mat, 1);
       }
     }
@@ -778,7 +832,7 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   ELMAN_RETURN_IF(map(&maps.a[1], &maps.ra[1], split ? buf.A.lo : buf.A.hi, p.r, p.r, buf.ldr));
   ELMAN_RETURN_IF(map(&maps.b[0], &maps.rb[0], buf.B.hi, p.r, p.r, buf.ldr));
   ELMAN_RETURN_IF(map(&maps.b[1], &maps.rb[1], split ? buf.B.lo : buf.B.hi, p.r, p.r, buf.ldr));
-  const long size = (long)p.m * p.n, blocks = (size + 256 * 8 - 1) / (256 * 8);
+  const long size = (long)p.m * p.n, blocks = (p.m + 7) / 8;
   Split x0 = buf.X[0];
   if (!takes_low(0, p.steps, p.parts)) x0.lo = nullptr;
   ns_norm_kernel<T><<<dim3(NORM_PARTS, p.count), 256, 0, st>>>(src, size, buf.partial, buf.ticket, buf.done);
