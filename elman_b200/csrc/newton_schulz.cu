@@ -29,7 +29,7 @@ namespace {
 // One block's share of a tile is 128 rows of the product; a pair of blocks (cta_group::2) makes a tile of 256 x 256,
 // a block by itself one of 128 x 128.  Either way a block loads 128 rows of each operand a stage.
 constexpr int BK = 64, STAGES = 5, TICKETS = 4;
-constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
+constexpr int EPI_WARPS = 8, THREADS = 96 + 32 * EPI_WARPS;
 constexpr int BLOCK_BYTES = 64 * BK * 2;              // one TMA box: 64 x 64 fp16
 constexpr int OPERAND_BYTES = 128 * BK * 2;
 // Rows are finished in boxes of 32 x 32 through shared memory: two buffers a warp, each a box's high and low parts.
@@ -59,11 +59,10 @@ struct NsSource {
   const float* grad_scale;   // device, or null
 };
 
-// [buffer][high, low part]; operands in boxes of 64 x 64, results in boxes of 32 x 32.
-struct NsMaps {
-  CUtensorMap x[2][2], a[2], b[2];
-  CUtensorMap rx[2][2], ra[2], rb[2];
-};
+// [high, low part] of a matrix: operand boxes of 128 rows x 64 (read along the rows) and of 64 x 64 (read MN-major),
+// result boxes of 32 x 32.
+struct NsMap { CUtensorMap rows[2], block[2], box[2]; };
+struct NsMaps { NsMap x[2], a, b; };
 
 // The whole iteration as one list of tiles: step by step, in a step all Gram tiles of all matrices, then the squares',
 // then the updates'.
@@ -273,21 +272,21 @@ __device__ __forceinline__ void sts_u4(uint32_t addr, uint4 v) {
 // What becomes of a product: k_acc * product + k_same * same.
 struct Finish {
   float k_acc, k_same;
-  const CUtensorMap *same, *out;    // [high, low]
+  const CUtensorMap *same, *out;    // [high, low]: boxes
   bool same_low, out_low;
 };
 __device__ __forceinline__ Finish finish_of(const NsPlan& p, const NsMaps& maps, const NsItem& it) {
   Finish f;
   const int at = it.step & 1;
   if (it.kind == GRAM || it.kind == SQUARE) {
-    f.same = maps.ra;
-    f.out = it.kind == GRAM ? maps.ra : maps.rb;
+    f.same = maps.a.box;
+    f.out = it.kind == GRAM ? maps.a.box : maps.b.box;
     f.same_low = f.out_low = p.parts > 1;
     f.k_acc = it.kind == GRAM ? SA / (SX * SX) : p.c * (SB / (SA * SA));
     f.k_same = p.b * (SB / SA);
   } else {
-    f.same = maps.rx[at];
-    f.out = maps.rx[at ^ 1];
+    f.same = maps.x[at].box;
+    f.out = maps.x[at ^ 1].box;
     f.same_low = takes_low(it.step, p.steps, p.parts);
     f.out_low = takes_low(it.step + 1, p.steps, p.parts);
     f.k_acc = it.kind == LAST ? 1.f / (SB * SX) : 1.f / SB;
@@ -327,8 +326,9 @@ __device__ __forceinline__ void write_result(const NsPlan& p, const NsItem& it, 
 // products it reads are finished (`done` of its matrix), which were handed out before it, so whoever waits, waits
 // for someone who runs: no block has to be resident for another's sake, and launches may overlap.  With more than a
 // few matrices the wait is over before it begins.
-// Warp 0 takes the items (the even block of a pair) and loads, warp 1 issues the products (for both blocks), the others
-// finish the rows: two accumulators, so a tile is finished under the next one's products.
+// Warp 0 takes the items (the even block of a pair) and loads the first operand, warp 2 loads the second (one thread
+// issues a stage's copies in about 1000 cycles, twice what its products take), warp 1 issues the products (for
+// both blocks), the others finish the rows: two accumulators, so a tile is finished under the next one's products.
 template <typename T, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ NsMaps maps, const NsPlan p) {
   constexpr int EDGE = PAIR ? 256 : 128, BLOCKS = PAIR ? 2 : 1;
@@ -355,11 +355,12 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     }
     for (int k = 0; k < TICKETS; ++k) {
       ptx::mbar_init(&tk_full[k], 1);
-      ptx::mbar_init(&tk_empty[k], 1 + BLOCKS * EPI_WARPS + (BLOCKS - 1));   // products, rows, the odd block's loads
+      ptx::mbar_init(&tk_empty[k], 1 + BLOCKS * (EPI_WARPS + 1) + (BLOCKS - 1));   // products, rows, loads but the even block's first
     }
     for (int k = 0; k < 2 * EPI_WARPS; ++k) ptx::mbar_init(&same_bar[k >> 1][k & 1], 1);
     ptx::mbar_fence_init();
   }
+  if (warp == 2 && lane < (int)(sizeof(NsMaps) / sizeof(CUtensorMap))) ptx::prefetch_tmap(reinterpret_cast<const CUtensorMap*>(&maps) + lane);
   if (warp == 1) {
     if constexpr (PAIR) {
       ptx::tmem_alloc_pair(&tmem_slot, 512);
@@ -404,6 +405,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     long spins = 0;
     unsigned long long t0 = 0;
     while (ld_acquire_gpu(p.done + it.mat) < it.need * BLOCKS * EPI_WARPS) {
+      __nanosleep(20);
       if (++spins > p.spin_limit || *abortp != 0) return false;
       if ((spins & 255) == 0) {
         const unsigned long long now = ptx::globaltimer_ns();
@@ -414,17 +416,25 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     return true;
   };
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 2) {
     if (lane == 0) {
+      const bool first = warp == 0;                   // operand A, or B
+      uint8_t* const to = first ? sA : sB;
+      const uint32_t bars = PAIR ? tch::mapa(ptx::smem_u32(full_bar), 0) : ptx::smem_u32(full_bar);
       uint32_t s = 0, ph = 0;
       long iteration = 0;
       for (int q = 0; abort_flag == 0; ++q) {
         const int k = q % TICKETS;
         int index;
-        if (rank == 0) {
+        NsItem it;
+        if (first && rank == 0) {
           if (!ptx::mbar_wait(&tk_empty[k], ((uint32_t)(q / TICKETS) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFB); break; }
           index = atomicAdd(p.ticket, 1);
           if (index >= p.total) index = -1;
+          if (index >= 0) {
+            it = item_of(p, index, EDGE);
+            if (!finished(it)) { give_up(0xFFFA); break; }       // the others hear of the item when it can start
+          }
           tk[k] = index;
           ptx::mbar_arrive(&tk_full[k]);
           if constexpr (PAIR) {
@@ -435,41 +445,36 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           if (!wait_ticket(q)) { give_up(0xFFFC); break; }
           index = tk[k];
           free_ticket(q);
+          if (index >= 0) it = item_of(p, index, EDGE);
         }
         if (index < 0) break;
-        const NsItem it = item_of(p, index, EDGE);
-        if (!finished(it)) { give_up(0xFFFA); break; }
-        ptx::fence_proxy_async();                     // written by other blocks' stores, read here by TMA
-        const int m0 = it.ti * EDGE + 128 * (int)rank, n0 = it.tj * EDGE + 128 * (int)rank;
-        const int nk = (it.K + BK - 1) / BK, at = it.step & 1;
-        const CUtensorMap *A, *B;
-        if (it.kind == GRAM) A = B = maps.x[at];
-        else if (it.kind == SQUARE) A = B = maps.a;
-        else { A = p.tall ? maps.x[at] : maps.b; B = p.tall ? maps.b : maps.x[at]; }
+        ptx::fence_proxy_async();                     // written by other blocks, read here by TMA
+        const int at = it.step & 1, form = first ? it.a_form : it.b_form;
+        const int row0 = (first ? it.ti : it.tj) * EDGE + 128 * (int)rank;
+        const NsMap& map = it.kind == GRAM ? maps.x[at] : it.kind == SQUARE ? maps.a : first == (p.tall != 0) ? maps.x[at] : maps.b;
         bool ok = true;
-        for (int i = 0; i < nk * p.parts; ++i, ++iteration) {
-          const int part = i / nk, k0 = (i - part * nk) * BK;    // high x high, high x low, low x high
-          if (!ptx::mbar_wait(&empty_bar[s], ph ^ 1u, p.spin_limit, abortp)) { give_up(i); ok = false; break; }
-          if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[s], BLOCKS * 2 * OPERAND_BYTES);
-          const bool a_mn = mn_major(it.a_form, m0, k0, EDGE), b_mn = mn_major(it.b_form, n0, k0, EDGE);
-          if (!(iteration == p.stall && blockIdx.x == 0)) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint8_t* da = sA + s * OPERAND_BYTES + h * BLOCK_BYTES;
-              uint8_t* db = sB + s * OPERAND_BYTES + h * BLOCK_BYTES;
-              const int ax = a_mn ? m0 + 64 * h : k0, ay = a_mn ? k0 : m0 + 64 * h;
-              const int bx = b_mn ? n0 + 64 * h : k0, by = b_mn ? k0 : n0 + 64 * h;
-              if constexpr (PAIR) {
-                const uint32_t bar = tch::mapa(ptx::smem_u32(&full_bar[s]), 0);
-                ptx::tma_load_3d_pair(da, A + (part == 2), ax, ay, it.mat, bar);
-                ptx::tma_load_3d_pair(db, B + (part == 1), bx, by, it.mat, bar);
+        for (int part = 0; part < p.parts && ok; ++part) {      // high x high, high x low, low x high
+          const int low = first ? part == 2 : part == 1;
+          for (int k0 = 0; k0 < it.K; k0 += BK, ++iteration) {
+            if (!ptx::mbar_wait(&empty_bar[s], ph ^ 1u, p.spin_limit, abortp)) { give_up(k0); ok = false; break; }
+            if (first && rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[s], BLOCKS * 2 * OPERAND_BYTES);
+            const bool mn = mn_major(form, row0, k0, EDGE);
+            const uint32_t bar = bars + 8 * s;
+            if (!(iteration == p.stall && blockIdx.x == 0)) {
+              uint8_t* dst = to + s * OPERAND_BYTES;
+              auto copy = [&](uint8_t* d, const CUtensorMap* m, int x, int y) {
+                if constexpr (PAIR) ptx::tma_load_3d_pair(d, m, x, y, it.mat, bar);
+                else tch::tma_load_3d(d, m, x, y, it.mat, &full_bar[s]);
+              };
+              if (mn) {
+                copy(dst, &map.block[low], row0, k0);
+                copy(dst + BLOCK_BYTES, &map.block[low], row0 + 64, k0);
               } else {
-                tch::tma_load_3d(da, A + (part == 2), ax, ay, it.mat, &full_bar[s]);
-                tch::tma_load_3d(db, B + (part == 1), bx, by, it.mat, &full_bar[s]);
+                copy(dst, &map.rows[low], k0, row0);
               }
             }
+            if (++s == STAGES) { s = 0; ph ^= 1u; }
           }
-          if (++s == STAGES) { s = 0; ph ^= 1u; }
         }
         if (!ok) break;
       }
@@ -528,9 +533,9 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     __syncwarp();
   } else {
     // warp w may read TMEM lanes [32 (w % 4), +32); the two warps of a quarter split the tile's columns
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, mine = warp - 3, half = mine >> 2;
     constexpr int CH = EDGE / 32 / 2;
-    const uint32_t staging = ptx::smem_u32(smem) + STAGES * 2 * OPERAND_BYTES + (uint32_t)((warp - 2) * 2 * BUFFER_BYTES);
+    const uint32_t staging = ptx::smem_u32(smem) + STAGES * 2 * OPERAND_BYTES + (uint32_t)(mine * 2 * BUFFER_BYTES);
     uint32_t same_phase = 0;
     int boxes = 0, row0 = 0, col0 = 0;                // boxes taken: they alternate between the warp's buffers
     Finish fin;
@@ -538,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     auto fetch = [&](const Finish& f, const NsItem& it, int c, int box) {
       const int col = col0 + c * 32;
       if (it.kind == GRAM || row0 >= it.m || col >= it.n) return;
-      uint64_t* bar = &same_bar[warp - 2][box & 1];
+      uint64_t* bar = &same_bar[mine][box & 1];
       uint8_t* to = smem + (staging - ptx::smem_u32(smem)) + (box & 1) * BUFFER_BYTES;
       ptx::mbar_arrive_expect_tx(bar, f.same_low ? 2 * BOX_BYTES : BOX_BYTES);
       tch::tma_load_3d(to, f.same, col, row0, it.mat, bar);
@@ -559,15 +564,12 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         col0 = it.tj * EDGE + half * (EDGE / 2);
         fin = finish_of(p, maps, it);
         if (lane == 0 && it.kind != GRAM) {           // under the products: the first box of `same`
-          ok = finished(it);
           ptx::fence_proxy_async();
-          if (ok) {
-            tch::bulk_wait_read_all();
-            fetch(fin, it, 0, boxes);
-          }
+          tch::bulk_wait_read_all();
+          fetch(fin, it, 0, boxes);
         }
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        ok = ok && ptx::mbar_wait(&acc_full[b], (uint32_t)(q / sums) & 1u, p.spin_limit * 8, abortp);
+        __syncwarp();
+        ok = ptx::mbar_wait(&acc_full[b], (uint32_t)(q / sums) & 1u, p.spin_limit * 8, abortp);
       }
       if (!ok && abort_flag == 0) give_up(0xFFFF);
       uint32_t stop;                                  // one verdict for all of them
@@ -613,7 +615,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         }
         __syncwarp();
         if (!wanted) continue;
-        if (it.kind != GRAM && !ptx::mbar_wait(&same_bar[warp - 2][boxes & 1], (same_phase >> (boxes & 1)) & 1u, p.spin_limit * 8, abortp) &&
+        if (it.kind != GRAM && !ptx::mbar_wait(&same_bar[mine][boxes & 1], (same_phase >> (boxes & 1)) & 1u, p.spin_limit * 8, abortp) &&
             abort_flag == 0)
           give_up(0xFFF9);                            // (what follows is invalid and reported)
         if (it.kind != GRAM) same_phase ^= 1u << (boxes & 1);
@@ -779,9 +781,11 @@ int launch(const NsMaps& maps, const NsPlan& p, cudaStream_t st) {
       if (dev < 64) sized[dev] = true;
     }
   }
-  const int blocks = PAIR ? 2 : 1, units = 148 / blocks;
+  // no more than a product's tiles: the next products run where code and tensor maps are warm
+  const int blocks = PAIR ? 2 : 1, most = p.count * (p.triangle > p.all ? p.triangle : p.all);
+  const int units = most < 148 / blocks ? most : 148 / blocks;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(blocks * (p.total < units ? p.total : units)));
+  cfg.gridDim = dim3((unsigned)(blocks * units));
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = NS_SMEM;
   cfg.stream = st;
@@ -819,19 +823,20 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   p.per_step = p.count * (2 * p.triangle + p.all);
   p.total = p.steps * p.per_step;
   NsMaps maps;
-  auto map = [&](CUtensorMap* out, CUtensorMap* box, const __half* base, int rows, int cols, long ld) {
-    ELMAN_RETURN_IF(make_tmap_f16(box, base, cols, rows, p.count, ld, (long)rows * ld, 32));
-    return make_tmap_f16(out, base, cols, rows, p.count, ld, (long)rows * ld, 64);
+  auto map = [&](NsMap& out, const Split& x, int rows, int cols, long ld) {
+    for (int low = 0; low < 2; ++low) {
+      const __half* base = low && x.lo != nullptr ? x.lo : x.hi;
+      const uint64_t all = (uint64_t)rows * ld;
+      ELMAN_RETURN_IF(make_tmap_f16(&out.rows[low], base, cols, rows, p.count, ld, all, 64, 128));
+      ELMAN_RETURN_IF(make_tmap_f16(&out.block[low], base, cols, rows, p.count, ld, all, 64, 64));
+      ELMAN_RETURN_IF(make_tmap_f16(&out.box[low], base, cols, rows, p.count, ld, all, 32, 32));
+    }
+    return (int)ELMAN_OK;
   };
-  const bool split = p.parts > 1;
-  for (int k = 0; k < 2; ++k) {
-    ELMAN_RETURN_IF(map(&maps.x[k][0], &maps.rx[k][0], buf.X[k].hi, p.m, p.n, buf.ldx));
-    ELMAN_RETURN_IF(map(&maps.x[k][1], &maps.rx[k][1], buf.X[k].lo, p.m, p.n, buf.ldx));
-  }
-  ELMAN_RETURN_IF(map(&maps.a[0], &maps.ra[0], buf.A.hi, p.r, p.r, buf.ldr));
-  ELMAN_RETURN_IF(map(&maps.a[1], &maps.ra[1], split ? buf.A.lo : buf.A.hi, p.r, p.r, buf.ldr));
-  ELMAN_RETURN_IF(map(&maps.b[0], &maps.rb[0], buf.B.hi, p.r, p.r, buf.ldr));
-  ELMAN_RETURN_IF(map(&maps.b[1], &maps.rb[1], split ? buf.B.lo : buf.B.hi, p.r, p.r, buf.ldr));
+  ELMAN_RETURN_IF(map(maps.x[0], buf.X[0], p.m, p.n, buf.ldx));
+  ELMAN_RETURN_IF(map(maps.x[1], buf.X[1], p.m, p.n, buf.ldx));
+  ELMAN_RETURN_IF(map(maps.a, buf.A, p.r, p.r, buf.ldr));
+  ELMAN_RETURN_IF(map(maps.b, buf.B, p.r, p.r, buf.ldr));
   const long size = (long)p.m * p.n, blocks = (p.m + 7) / 8;
   Split x0 = buf.X[0];
   if (!takes_low(0, p.steps, p.parts)) x0.lo = nullptr;
