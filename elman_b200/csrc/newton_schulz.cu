@@ -333,7 +333,7 @@ template <typename T, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ NsMaps maps, const NsPlan p) {
   constexpr int EDGE = PAIR ? 256 : 128, BLOCKS = PAIR ? 2 : 1;
   extern __shared__ uint8_t raw[];
-  __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2], tk_full[TICKETS], tk_empty[TICKETS];
+  __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2], tk_full[TICKETS], tk_empty[TICKETS], go[TICKETS];
   __shared__ __align__(8) uint64_t same_bar[EPI_WARPS][2];
   __shared__ int tk[TICKETS];
   __shared__ uint32_t tmem_slot;
@@ -355,6 +355,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     }
     for (int k = 0; k < TICKETS; ++k) {
       ptx::mbar_init(&tk_full[k], 1);
+      ptx::mbar_init(&go[k], 1);
       ptx::mbar_init(&tk_empty[k], 1 + BLOCKS * (EPI_WARPS + 1) + (BLOCKS - 1));   // products, rows, loads but the even block's first
     }
     for (int k = 0; k < 2 * EPI_WARPS; ++k) ptx::mbar_init(&same_bar[k >> 1][k & 1], 1);
@@ -383,10 +384,10 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tch::mapa(ptx::smem_u32(&abort_flag), rank ^ 1u)), "r"(1) : "memory");
     report_timeout(p.status, KID_NEWTON_SCHULZ, where);
   };
-  auto wait_ticket = [&](int q) {                     // (cluster-wide acquire: a pair's come from the even block)
+  auto wait_for = [&](uint64_t* bar, int q) {         // item q's ticket or start (cluster-wide acquire: a pair's come from the even block)
     long spins = 0;
     unsigned long long t0 = 0;
-    while (!tch::mbar_try_wait_cluster(&tk_full[q % TICKETS], (uint32_t)(q / TICKETS) & 1u)) {
+    while (!tch::mbar_try_wait_cluster(bar, (uint32_t)(q / TICKETS) & 1u)) {
       if (++spins > p.spin_limit * 8 || *abortp != 0) return false;
       if ((spins & 1023) == 0) {
         const unsigned long long now = ptx::globaltimer_ns();
@@ -431,10 +432,6 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           if (!ptx::mbar_wait(&tk_empty[k], ((uint32_t)(q / TICKETS) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFB); break; }
           index = atomicAdd(p.ticket, 1);
           if (index >= p.total) index = -1;
-          if (index >= 0) {
-            it = item_of(p, index, EDGE);
-            if (!finished(it)) { give_up(0xFFFA); break; }       // the others hear of the item when it can start
-          }
           tk[k] = index;
           ptx::mbar_arrive(&tk_full[k]);
           if constexpr (PAIR) {
@@ -442,15 +439,23 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
             ptx::mbar_arrive_cluster(tch::mapa(ptx::smem_u32(&tk_full[k]), 1));
           }
         } else {
-          if (!wait_ticket(q)) { give_up(0xFFFC); break; }
+          if (!wait_for(&tk_full[k], q)) { give_up(0xFFFC); break; }
           index = tk[k];
           free_ticket(q);
-          if (index >= 0) it = item_of(p, index, EDGE);
         }
         if (index < 0) break;
-        ptx::fence_proxy_async();                     // written by other blocks, read here by TMA
+        it = item_of(p, index, EDGE);
         const int at = it.step & 1, form = first ? it.a_form : it.b_form;
         const int row0 = (first ? it.ti : it.tj) * EDGE + 128 * (int)rank;
+        if (first && rank == 0) {                     // everyone knows the item; now it may start
+          if (!finished(it)) { give_up(0xFFFA); break; }
+          ptx::mbar_arrive(&go[k]);
+          if constexpr (PAIR) ptx::mbar_arrive_cluster(tch::mapa(ptx::smem_u32(&go[k]), 1));
+        } else if (!wait_for(&go[k], q)) {
+          give_up(0xFFF8);
+          break;
+        }
+        ptx::fence_proxy_async();                     // written by other blocks, read here by TMA
         const NsMap& map = it.kind == GRAM ? maps.x[at] : it.kind == SQUARE ? maps.a : first == (p.tall != 0) ? maps.x[at] : maps.b;
         bool ok = true;
         for (int part = 0; part < p.parts && ok; ++part) {      // high x high, high x low, low x high
@@ -485,44 +490,47 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       uint32_t s = 0, ph = 0;
       bool ready = false, ok = true;
       for (int q = 0; ok; ++q) {
-        if (!wait_ticket(q)) { give_up(0xFFFD); break; }
+        if (!wait_for(&tk_full[q % TICKETS], q)) { give_up(0xFFFD); break; }
         const int index = tk[q % TICKETS];
         free_ticket(q);
         if (index < 0) break;
         const NsItem it = item_of(p, index, EDGE);
-        const int m0 = it.ti * EDGE, n0 = it.tj * EDGE, nk = (it.K + BK - 1) / BK, iters = nk * p.parts;
+        const int m0 = it.ti * EDGE, n0 = it.tj * EDGE, nk = (it.K + BK - 1) / BK;
         const int b = q % sums;
         if (!ptx::mbar_wait(&acc_empty[b], ((uint32_t)(q / sums) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFE); break; }
         ptx::tc_fence_after();
-        int k0 = 0;
-        for (int i = 0; i < iters; ++i) {
-          if (!ready && !ptx::mbar_wait(&full_bar[s], ph, p.spin_limit, abortp)) { give_up(i); ok = false; break; }
-          const bool a_mn = mn_major(it.a_form, m0, k0, EDGE), b_mn = mn_major(it.b_form, n0, k0, EDGE);
-          const uint32_t idesc = ptx::umma_idesc_f16(EDGE, EDGE) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
-          const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
-          const uint32_t a_addr = ptx::smem_u32(sA) + s * OPERAND_BYTES, b_addr = ptx::smem_u32(sB) + s * OPERAND_BYTES;
-          const uint64_t da = a_mn ? ptx::umma_desc_mn_sw128(a_addr, BLOCK_BYTES) : ptx::umma_desc_k_sw128(a_addr);
-          const uint64_t db = b_mn ? ptx::umma_desc_mn_sw128(b_addr, BLOCK_BYTES) : ptx::umma_desc_k_sw128(b_addr);
-          uint32_t s_next = s + 1, ph_next = ph;
-          if (s_next == STAGES) { s_next = 0; ph_next ^= 1u; }
-          if constexpr (PAIR) {
-            ready = ptx::umma_stage_pair(tmem_base + (uint32_t)(b * EDGE), da, db, a_step, b_step, idesc, i > 0 ? 1u : 0u,
-                                         &empty_bar[s], &full_bar[s_next], ph_next);
-          } else {
-            // fp32: the large products take turns in three sums, the others have a fourth
-            const int sum = p.parts == 1 ? b : i < nk ? i % 3 : 3;
-            const bool opens = p.parts == 1 ? i == 0 : i < 3 ? i <= nk : i == nk;
-            ptx::tc_fence_after();
-#pragma unroll
-            for (int j = 0; j < BK / 16; ++j)
-              ptx::umma_bf16(tmem_base + (uint32_t)(sum * EDGE), da + a_step * j, db + b_step * j, idesc, opens && j == 0 ? 0u : 1u);
-            ptx::umma_commit(&empty_bar[s]);
-            ready = false;
+        const uint32_t sum0 = tmem_base + (uint32_t)(b * EDGE);
+        int i = 0;                                    // stages of this item, over all parts
+        for (int part = 0; part < p.parts && ok; ++part) {
+          for (int k0 = 0; k0 < it.K && ok;) {
+            // the stretch of K in which both operands keep their form: an upper matrix changes at the diagonal
+            int end = it.K;
+            if (it.a_form == UPPER && k0 < m0) end = m0;
+            if (it.b_form == UPPER && k0 < n0 && n0 < end) end = n0;
+            const bool a_mn = mn_major(it.a_form, m0, k0, EDGE), b_mn = mn_major(it.b_form, n0, k0, EDGE);
+            const uint32_t idesc = ptx::umma_idesc_f16(EDGE, EDGE) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+            const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
+            const uint64_t da0 = a_mn ? ptx::umma_desc_mn_sw128(ptx::smem_u32(sA), BLOCK_BYTES) : ptx::umma_desc_k_sw128(ptx::smem_u32(sA));
+            const uint64_t db0 = b_mn ? ptx::umma_desc_mn_sw128(ptx::smem_u32(sB), BLOCK_BYTES) : ptx::umma_desc_k_sw128(ptx::smem_u32(sB));
+            for (; k0 < end; k0 += BK, ++i) {
+              if (!ready && !ptx::mbar_wait(&full_bar[s], ph, p.spin_limit, abortp)) { give_up(i); ok = false; break; }
+              uint32_t s_next = s + 1, ph_next = ph;
+              if (s_next == STAGES) { s_next = 0; ph_next ^= 1u; }
+              const uint64_t da = da0 + (uint64_t)(s * (OPERAND_BYTES / 16)), db = db0 + (uint64_t)(s * (OPERAND_BYTES / 16));
+              if constexpr (PAIR) {
+                ready = ptx::umma_stage_pair(sum0, da, db, a_step, b_step, idesc, i > 0 ? 1u : 0u, &empty_bar[s], &full_bar[s_next],
+                                             ph_next);
+              } else {
+                // fp32: the large products take turns in three sums, the others have a fourth
+                const int sum = p.parts == 1 ? b : part == 0 ? i % 3 : 3;
+                const bool opens = p.parts == 1 ? i == 0 : part == 0 ? i < 3 : i == nk;
+                ready = ptx::umma_stage(tmem_base + (uint32_t)(sum * EDGE), da, db, a_step, b_step, idesc, opens ? 0u : 1u, &empty_bar[s],
+                                        &full_bar[s_next], ph_next);
+              }
+              s = s_next;
+              ph = ph_next;
+            }
           }
-          s = s_next;
-          ph = ph_next;
-          k0 += BK;
-          if (k0 >= it.K) k0 = 0;
         }
         if (ok) {
           if constexpr (PAIR) ptx::umma_commit_pair(&acc_full[b], 3);
@@ -550,7 +558,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       if (f.same_low) tch::tma_load_3d(to + BOX_BYTES, f.same + 1, col, row0, it.mat, bar);
     };
     for (int q = 0;; ++q) {
-      bool ok = wait_ticket(q);
+      bool ok = wait_for(&tk_full[q % TICKETS], q);
       const int index = tk[q % TICKETS];
       NsItem it;
       int b = 0;
@@ -563,7 +571,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         row0 = it.ti * EDGE + 128 * (int)rank + quarter * 32;
         col0 = it.tj * EDGE + half * (EDGE / 2);
         fin = finish_of(p, maps, it);
-        if (lane == 0 && it.kind != GRAM) {           // under the products: the first box of `same`
+        if (lane == 0 && it.kind != GRAM && wait_for(&go[q % TICKETS], q)) {    // under the products: the first box of `same`
           ptx::fence_proxy_async();
           tch::bulk_wait_read_all();
           fetch(fin, it, 0, boxes);
@@ -666,7 +674,6 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       }
       if (it.kind != LAST && lane == 0) {
         tch::bulk_wait_all();                         // written, not only read
-        ptx::fence_proxy_async();
         red_release_gpu_add(p.done + it.mat, 1);
       }
     }

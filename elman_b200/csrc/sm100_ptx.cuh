@@ -335,6 +335,36 @@ __device__ __forceinline__ bool umma_stage_pair(uint32_t tmem_d, uint64_t da, ui
       : "memory");
   return ready != 0;
 }
+// The same for a CTA by itself (cta_group::1).
+__device__ __forceinline__ bool umma_stage(uint32_t tmem_d, uint64_t da, uint64_t db, uint64_t a_step, uint64_t b_step,
+                                           uint32_t idesc, uint32_t accumulate_first, uint64_t* free_bar,
+                                           uint64_t* next_full_bar, uint32_t next_parity) {
+  uint32_t ready;
+  asm volatile(
+      "{\n\t.reg .pred pw, pa, pt;\n\t"
+      ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "tcgen05.fence::after_thread_sync;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 pw, [%9], %10;\n\t"
+      "setp.ne.b32 pa, %6, 0;\n\t"
+      "setp.eq.b32 pt, 0, 0;\n\t"
+      "add.u64 a1, %2, %4;\n\t"
+      "add.u64 b1, %3, %5;\n\t"
+      "add.u64 a2, a1, %4;\n\t"
+      "add.u64 b2, b1, %5;\n\t"
+      "add.u64 a3, a2, %4;\n\t"
+      "add.u64 b3, b2, %5;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], %2, %3, %7, pa;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], a1, b1, %7, pt;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], a2, b2, %7, pt;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], a3, b3, %7, pt;\n\t"
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%8];\n\t"
+      "selp.b32 %0, 1, 0, pw;\n\t}"
+      : "=r"(ready)
+      : "r"(tmem_d), "l"(da), "l"(db), "l"(a_step), "l"(b_step), "r"(accumulate_first), "r"(idesc), "r"(smem_u32(free_bar)),
+        "r"(smem_u32(next_full_bar)), "r"(next_parity)
+      : "memory");
+  return ready != 0;
+}
 // Arrive on the mbarrier at the same shared-memory offset in every CTA of `cta_mask` when
 // all MMAs issued so far by this thread have completed.
 __device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint16_t cta_mask) {
