@@ -29,7 +29,7 @@ namespace {
 // One block's share of a tile is 128 rows of the product; a pair of blocks (cta_group::2) makes a tile of 256 x 256,
 // a block by itself one of 128 x 128.  Either way a block loads 128 rows of each operand a stage.
 constexpr int BK = 64, STAGES = 5, TICKETS = 4;
-constexpr int EPI_WARPS = 8, THREADS = 96 + 32 * EPI_WARPS;
+constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
 constexpr int BLOCK_BYTES = 64 * BK * 2;              // one TMA box: 64 x 64 fp16
 constexpr int OPERAND_BYTES = 128 * BK * 2;
 // Rows are finished in boxes of 32 x 32 through shared memory: two buffers a warp, each a box's high and low parts.
@@ -65,7 +65,8 @@ struct NsMap { CUtensorMap rows[2], block[2], box[2]; };
 struct NsMaps { NsMap x[2], a, b; };
 
 // The whole iteration as one list of tiles: step by step, in a step all Gram tiles of all matrices, then the squares',
-// then the updates'.
+// then the updates'.  (Groups of matrices that stay in L2 from product to product were slower: 18 x 1280 x 1280 as three
+// groups 0.98 ms, as one 0.87: waiting for the matrix one reads costs more than reading it from HBM.)
 struct NsPlan {
   int count, m, n, r, tall, steps, parts;
   int triangle, all;         // tiles of a symmetric product and of an update
@@ -326,9 +327,10 @@ __device__ __forceinline__ void write_result(const NsPlan& p, const NsItem& it, 
 // products it reads are finished (`done` of its matrix), which were handed out before it, so whoever waits, waits
 // for someone who runs: no block has to be resident for another's sake, and launches may overlap.  With more than a
 // few matrices the wait is over before it begins.
-// Warp 0 takes the items (the even block of a pair) and loads the first operand, warp 2 loads the second (one thread
-// issues a stage's copies in about 1000 cycles, twice what its products take), warp 1 issues the products (for
-// both blocks), the others finish the rows: two accumulators, so a tile is finished under the next one's products.
+// Warp 3 of the even block takes items ahead of the others and waits until they may start, warps 0 and 2 load the
+// two operands (one thread issues a stage's copies in about 1000 cycles, twice what its products take), warp 1
+// issues the products (for both blocks), the others finish the rows: two accumulators, so a tile is finished under
+// the next one's products.
 template <typename T, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ NsMaps maps, const NsPlan p) {
   constexpr int EDGE = PAIR ? 256 : 128, BLOCKS = PAIR ? 2 : 1;
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     for (int k = 0; k < TICKETS; ++k) {
       ptx::mbar_init(&tk_full[k], 1);
       ptx::mbar_init(&go[k], 1);
-      ptx::mbar_init(&tk_empty[k], 1 + BLOCKS * (EPI_WARPS + 1) + (BLOCKS - 1));   // products, rows, loads but the even block's first
+      ptx::mbar_init(&tk_empty[k], 1 + BLOCKS * (EPI_WARPS + 2));   // products; rows and loads of both blocks
     }
     for (int k = 0; k < 2 * EPI_WARPS; ++k) ptx::mbar_init(&same_bar[k >> 1][k & 1], 1);
     ptx::mbar_fence_init();
@@ -426,35 +428,14 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       long iteration = 0;
       for (int q = 0; abort_flag == 0; ++q) {
         const int k = q % TICKETS;
-        int index;
-        NsItem it;
-        if (first && rank == 0) {
-          if (!ptx::mbar_wait(&tk_empty[k], ((uint32_t)(q / TICKETS) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFB); break; }
-          index = atomicAdd(p.ticket, 1);
-          if (index >= p.total) index = -1;
-          tk[k] = index;
-          ptx::mbar_arrive(&tk_full[k]);
-          if constexpr (PAIR) {
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tch::mapa(ptx::smem_u32(&tk[k]), 1)), "r"(index) : "memory");
-            ptx::mbar_arrive_cluster(tch::mapa(ptx::smem_u32(&tk_full[k]), 1));
-          }
-        } else {
-          if (!wait_for(&tk_full[k], q)) { give_up(0xFFFC); break; }
-          index = tk[k];
-          free_ticket(q);
-        }
-        if (index < 0) break;
-        it = item_of(p, index, EDGE);
+        if (!wait_for(&tk_full[k], q)) { give_up(0xFFFC); break; }
+        const int index = tk[k];
+        if (index < 0) { free_ticket(q); break; }
+        const NsItem it = item_of(p, index, EDGE);
         const int at = it.step & 1, form = first ? it.a_form : it.b_form;
         const int row0 = (first ? it.ti : it.tj) * EDGE + 128 * (int)rank;
-        if (first && rank == 0) {                     // everyone knows the item; now it may start
-          if (!finished(it)) { give_up(0xFFFA); break; }
-          ptx::mbar_arrive(&go[k]);
-          if constexpr (PAIR) ptx::mbar_arrive_cluster(tch::mapa(ptx::smem_u32(&go[k]), 1));
-        } else if (!wait_for(&go[k], q)) {
-          give_up(0xFFF8);
-          break;
-        }
+        if (!wait_for(&go[k], q)) { give_up(0xFFF8); break; }
+        free_ticket(q);                               // (not before: the start of the slot's next item would hide this one's)
         ptx::fence_proxy_async();                     // written by other blocks, read here by TMA
         const NsMap& map = it.kind == GRAM ? maps.x[at] : it.kind == SQUARE ? maps.a : first == (p.tall != 0) ? maps.x[at] : maps.b;
         bool ok = true;
@@ -482,6 +463,26 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           }
         }
         if (!ok) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    if (lane == 0 && rank == 0) {
+      for (int q = 0; abort_flag == 0; ++q) {
+        const int k = q % TICKETS;
+        if (!ptx::mbar_wait(&tk_empty[k], ((uint32_t)(q / TICKETS) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFB); break; }
+        int index = atomicAdd(p.ticket, 1);
+        if (index >= p.total) index = -1;
+        tk[k] = index;
+        ptx::mbar_arrive(&tk_full[k]);
+        if constexpr (PAIR) {
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tch::mapa(ptx::smem_u32(&tk[k]), 1)), "r"(index) : "memory");
+          ptx::mbar_arrive_cluster(tch::mapa(ptx::smem_u32(&tk_full[k]), 1));
+        }
+        if (index < 0) break;
+        if (!finished(item_of(p, index, EDGE))) { give_up(0xFFFA); break; }
+        ptx::mbar_arrive(&go[k]);
+        if constexpr (PAIR) ptx::mbar_arrive_cluster(tch::mapa(ptx::smem_u32(&go[k]), 1));
       }
     }
     __syncwarp();
@@ -541,7 +542,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     __syncwarp();
   } else {
     // warp w may read TMEM lanes [32 (w % 4), +32); the two warps of a quarter split the tile's columns
-    const int quarter = warp & 3, mine = warp - 3, half = mine >> 2;
+    const int quarter = warp & 3, mine = warp - 4, half = mine >> 2;
     constexpr int CH = EDGE / 32 / 2;
     const uint32_t staging = ptx::smem_u32(smem) + STAGES * 2 * OPERAND_BYTES + (uint32_t)(mine * 2 * BUFFER_BYTES);
     uint32_t same_phase = 0;
@@ -564,20 +565,25 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       int b = 0;
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (ok) {
-        if (lane == 0) free_ticket(q);
-        if (index < 0) break;
+        if (index < 0) {
+          if (lane == 0) free_ticket(q);
+          break;
+        }
         it = item_of(p, index, EDGE);
         b = q % sums;
         row0 = it.ti * EDGE + 128 * (int)rank + quarter * 32;
         col0 = it.tj * EDGE + half * (EDGE / 2);
         fin = finish_of(p, maps, it);
-        if (lane == 0 && it.kind != GRAM && wait_for(&go[q % TICKETS], q)) {    // under the products: the first box of `same`
-          ptx::fence_proxy_async();
-          tch::bulk_wait_read_all();
-          fetch(fin, it, 0, boxes);
+        if (lane == 0) {
+          ok = it.kind == GRAM || wait_for(&go[q % TICKETS], q);
+          free_ticket(q);
+          if (ok && it.kind != GRAM) {                // under the products: the first box of `same`
+            ptx::fence_proxy_async();
+            tch::bulk_wait_read_all();
+            fetch(fin, it, 0, boxes);
+          }
         }
-        __syncwarp();
-        ok = ptx::mbar_wait(&acc_full[b], (uint32_t)(q / sums) & 1u, p.spin_limit * 8, abortp);
+        ok = __all_sync(0xFFFFFFFFu, ok) && ptx::mbar_wait(&acc_full[b], (uint32_t)(q / sums) & 1u, p.spin_limit * 8, abortp);
       }
       if (!ok && abort_flag == 0) give_up(0xFFFF);
       uint32_t stop;                                  // one verdict for all of them
