@@ -28,13 +28,15 @@ namespace {
 
 // One block's share of a tile is 128 rows of the product; a pair of blocks (cta_group::2) makes a tile of 256 x 256,
 // a block by itself one of 128 x 128.  Either way a block loads 128 rows of each operand a stage.
-constexpr int BK = 64, STAGES = 5, TICKETS = 4;
+constexpr int BK = 64, STAGES = 6, TICKETS = 4;
 constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
 constexpr int BLOCK_BYTES = 64 * BK * 2;              // one TMA box: 64 x 64 fp16
 constexpr int OPERAND_BYTES = 128 * BK * 2;
-// Rows are finished in boxes of 32 x 32 through shared memory: two buffers a warp, each a box's high and low parts.
+// Rows are finished in boxes of 32 x 32 through shared memory, a box's high and low parts a warp, with plain 16-byte
+// accesses to global memory: the copy engine takes about two cycles a row of a box, and the operands' rows alone
+// (256 a stage of 512 cycles) fill its time.
 constexpr int BOX_BYTES = 32 * 64, BUFFER_BYTES = 2 * BOX_BYTES;
-constexpr int NS_SMEM = STAGES * 2 * OPERAND_BYTES + EPI_WARPS * 2 * BUFFER_BYTES + 1024;
+constexpr int NS_SMEM = STAGES * 2 * OPERAND_BYTES + EPI_WARPS * BUFFER_BYTES + 1024;
 constexpr float SX = 4096.f, SA = 4096.f, SB = 1024.f;
 constexpr int NORM_PARTS = 64;                        // partial sums of squares a matrix
 
@@ -59,9 +61,8 @@ struct NsSource {
   const float* grad_scale;   // device, or null
 };
 
-// [high, low part] of a matrix: operand boxes of 128 rows x 64 (read along the rows) and of 64 x 64 (read MN-major),
-// result boxes of 32 x 32.
-struct NsMap { CUtensorMap rows[2], block[2], box[2]; };
+// [high, low part] of a matrix: boxes of 128 rows x 64 (read along the rows) and of 64 x 64 (read MN-major).
+struct NsMap { CUtensorMap rows[2], block[2]; };
 struct NsMaps { NsMap x[2], a, b; };
 
 // The whole iteration as one list of tiles: step by step, in a step all Gram tiles of all matrices, then the squares',
@@ -86,46 +87,56 @@ struct NsPlan {
 };
 __host__ __device__ inline bool takes_low(int step, int steps, int parts) { return parts > 1 || step < steps - 2; }
 
-// One item of the list.
+// One item of the list.  Taking it apart costs divisions, a thousand cycles of latency: the warp that takes items does
+// it ahead of time and hands on the four numbers that the rest follows from.
+struct alignas(16) NsSlot { int kind, mat, tile, step; };     // kind -1: no more
+__device__ __forceinline__ NsSlot slot_of(const NsPlan& p, int index, int edge) {
+  NsSlot k;
+  k.step = index / p.per_step;
+  int w = index - k.step * p.per_step, ti, tj;
+  const int gram = p.count * p.triangle;
+  if (w < 2 * gram) {
+    k.kind = w >= gram ? SQUARE : GRAM;
+    if (w >= gram) w -= gram;
+    k.mat = w / p.triangle;
+    const int t = w - k.mat * p.triangle;      // the tiles (i, j >= i), column by column
+    tj = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+    while ((tj + 1) * (tj + 2) / 2 <= t) ++tj;
+    while (tj * (tj + 1) / 2 > t) --tj;
+    ti = t - tj * (tj + 1) / 2;
+  } else {
+    w -= 2 * gram;
+    k.kind = k.step == p.steps - 1 ? LAST : UPDATE;
+    k.mat = w / p.all;
+    const int t = w - k.mat * p.all, tiles_n = (p.n + edge - 1) / edge;
+    ti = t / tiles_n;
+    tj = t - ti * tiles_n;
+  }
+  k.tile = ti << 16 | tj;
+  return k;
+}
 struct NsItem {
   int kind, mat, ti, tj, step;
   int m, n, K, a_form, b_form;
-  int need;                  // tiles of this matrix that have to be finished before
 };
-__device__ __forceinline__ NsItem item_of(const NsPlan& p, int index, int edge) {
+__device__ __forceinline__ NsItem item_of(const NsPlan& p, NsSlot k) {
   NsItem it;
-  it.step = index / p.per_step;
-  int w = index - it.step * p.per_step;
-  const int gram = p.count * p.triangle, before = it.step * (2 * p.triangle + p.all);
-  if (w < 2 * gram) {
-    const bool square = w >= gram;
-    if (square) w -= gram;
-    it.kind = square ? SQUARE : GRAM;
-    it.mat = w / p.triangle;
-    const int t = w - it.mat * p.triangle;     // the tiles (i, j >= i), column by column
-    it.tj = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-    while ((it.tj + 1) * (it.tj + 2) / 2 <= t) ++it.tj;
-    while (it.tj * (it.tj + 1) / 2 > t) --it.tj;
-    it.ti = t - it.tj * (it.tj + 1) / 2;
-    it.m = it.n = p.r;
-    it.K = square ? p.r : p.tall ? p.m : p.n;
-    it.a_form = it.b_form = square ? UPPER : p.tall ? K_ROWS : ROWS_K;
-    it.need = before + (square ? p.triangle : 0);
-  } else {
-    w -= 2 * gram;
-    it.kind = it.step == p.steps - 1 ? LAST : UPDATE;
-    it.mat = w / p.all;
-    const int t = w - it.mat * p.all, tiles_n = (p.n + edge - 1) / edge;
-    it.ti = t / tiles_n;
-    it.tj = t - it.ti * tiles_n;
-    it.m = p.m;
-    it.n = p.n;
-    it.K = p.r;
-    it.a_form = p.tall ? ROWS_K : UPPER;       // X B, or B X
+  it.kind = k.kind; it.mat = k.mat; it.ti = k.tile >> 16; it.tj = k.tile & 0xFFFF; it.step = k.step;
+  const bool symmetric = k.kind == GRAM || k.kind == SQUARE;
+  it.m = symmetric ? p.r : p.m;
+  it.n = symmetric ? p.r : p.n;
+  it.K = k.kind != GRAM ? p.r : p.tall ? p.m : p.n;
+  if (k.kind == GRAM) it.a_form = it.b_form = p.tall ? K_ROWS : ROWS_K;
+  else if (k.kind == SQUARE) it.a_form = it.b_form = UPPER;
+  else {                                       // X B, or B X
+    it.a_form = p.tall ? ROWS_K : UPPER;
     it.b_form = p.tall ? UPPER : K_ROWS;
-    it.need = before + 2 * p.triangle;
   }
   return it;
+}
+// Tiles of its matrix that have to be finished before an item may start.
+__device__ __forceinline__ int needed(const NsPlan& p, NsSlot k) {
+  return k.step * (2 * p.triangle + p.all) + (k.kind == GRAM ? 0 : k.kind == SQUARE ? p.triangle : 2 * p.triangle);
 }
 
 __device__ __forceinline__ void add_halves(float (&f)[8], uint4 x, float k) {
@@ -273,27 +284,48 @@ __device__ __forceinline__ void sts_u4(uint32_t addr, uint4 v) {
 // What becomes of a product: k_acc * product + k_same * same.
 struct Finish {
   float k_acc, k_same;
-  const CUtensorMap *same, *out;    // [high, low]: boxes
-  bool same_low, out_low;
+  Split same, out;                 // at the item's matrix; lo null: not used
+  long ld;
 };
-__device__ __forceinline__ Finish finish_of(const NsPlan& p, const NsMaps& maps, const NsItem& it) {
+__device__ __forceinline__ Finish finish_of(const NsPlan& p, const NsItem& it) {
   Finish f;
   const int at = it.step & 1;
   if (it.kind == GRAM || it.kind == SQUARE) {
-    f.same = maps.a.box;
-    f.out = it.kind == GRAM ? maps.a.box : maps.b.box;
-    f.same_low = f.out_low = p.parts > 1;
+    f.ld = p.ldr;
+    f.same = p.A;
+    f.out = it.kind == GRAM ? p.A : p.B;
     f.k_acc = it.kind == GRAM ? SA / (SX * SX) : p.c * (SB / (SA * SA));
     f.k_same = p.b * (SB / SA);
   } else {
-    f.same = maps.x[at].box;
-    f.out = maps.x[at ^ 1].box;
-    f.same_low = takes_low(it.step, p.steps, p.parts);
-    f.out_low = takes_low(it.step + 1, p.steps, p.parts);
+    f.ld = p.ldx;
+    f.same = p.X[at];
+    f.out = p.X[at ^ 1];
+    if (!takes_low(it.step, p.steps, p.parts)) f.same.lo = nullptr;
+    if (!takes_low(it.step + 1, p.steps, p.parts)) f.out.lo = nullptr;
     f.k_acc = it.kind == LAST ? 1.f / (SB * SX) : 1.f / SB;
     f.k_same = it.kind == LAST ? p.a / SX : p.a;
   }
+  const long off = (long)it.mat * it.m * f.ld;
+  f.same.hi += off;
+  f.out.hi += off;
+  if (f.same.lo != nullptr) f.same.lo += off;
+  if (f.out.lo != nullptr) f.out.lo += off;
   return f;
+}
+// A box's 16-byte pieces as a warp moves them: piece (lane & 3) of row 8 k + lane / 4.  Rows are whole groups of eight in
+// memory: what lies past the last column is moved with it and used by nobody.
+__device__ __forceinline__ uint32_t piece_at(uint32_t box, int r, int g) { return box + (uint32_t)(r * 64 + ((g ^ (r >> 1 & 3)) << 4)); }
+struct Box { uint4 hi[4], lo[4]; };
+__device__ __forceinline__ void fetch_box(Box& x, const Finish& f, const NsItem& it, int row0, int col0) {
+  const int lane = threadIdx.x & 31, col = col0 + 8 * (lane & 3);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int row = row0 + 8 * k + (lane >> 2);
+    if (it.kind == GRAM || row >= it.m || col >= it.n) continue;
+    // (written by other blocks of this launch: from L2)
+    x.hi[k] = __ldcg(reinterpret_cast<const uint4*>(f.same.hi + (long)row * f.ld + col));
+    if (f.same.lo != nullptr) x.lo[k] = __ldcg(reinterpret_cast<const uint4*>(f.same.lo + (long)row * f.ld + col));
+  }
 }
 
 // A box of the last step's result: from shared memory (row r of sizeof(T) * 32 bytes, 16-byte pieces xor-ed with the row)
@@ -336,8 +368,8 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
   constexpr int EDGE = PAIR ? 256 : 128, BLOCKS = PAIR ? 2 : 1;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2], tk_full[TICKETS], tk_empty[TICKETS], go[TICKETS];
-  __shared__ __align__(8) uint64_t same_bar[EPI_WARPS][2];
-  __shared__ int tk[TICKETS];
+
+  __shared__ NsSlot tk[TICKETS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -360,7 +392,6 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       ptx::mbar_init(&go[k], 1);
       ptx::mbar_init(&tk_empty[k], 1 + BLOCKS * (EPI_WARPS + 2));   // products; rows and loads of both blocks
     }
-    for (int k = 0; k < 2 * EPI_WARPS; ++k) ptx::mbar_init(&same_bar[k >> 1][k & 1], 1);
     ptx::mbar_fence_init();
   }
   if (warp == 2 && lane < (int)(sizeof(NsMaps) / sizeof(CUtensorMap))) ptx::prefetch_tmap(reinterpret_cast<const CUtensorMap*>(&maps) + lane);
@@ -404,10 +435,11 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     else ptx::mbar_arrive(&tk_empty[q % TICKETS]);
   };
 
-  auto finished = [&](const NsItem& it) {              // waits for the products an item reads
+  auto finished = [&](NsSlot item) {                   // waits for the products an item reads
+    const int want = needed(p, item) * BLOCKS * EPI_WARPS;
     long spins = 0;
     unsigned long long t0 = 0;
-    while (ld_acquire_gpu(p.done + it.mat) < it.need * BLOCKS * EPI_WARPS) {
+    while (ld_acquire_gpu(p.done + item.mat) < want) {
       __nanosleep(20);
       if (++spins > p.spin_limit || *abortp != 0) return false;
       if ((spins & 255) == 0) {
@@ -429,9 +461,9 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       for (int q = 0; abort_flag == 0; ++q) {
         const int k = q % TICKETS;
         if (!wait_for(&tk_full[k], q)) { give_up(0xFFFC); break; }
-        const int index = tk[k];
-        if (index < 0) { free_ticket(q); break; }
-        const NsItem it = item_of(p, index, EDGE);
+        const NsSlot slot = tk[k];
+        if (slot.kind < 0) { free_ticket(q); break; }
+        const NsItem it = item_of(p, slot);
         const int at = it.step & 1, form = first ? it.a_form : it.b_form;
         const int row0 = (first ? it.ti : it.tj) * EDGE + 128 * (int)rank;
         if (!wait_for(&go[k], q)) { give_up(0xFFF8); break; }
@@ -471,16 +503,18 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       for (int q = 0; abort_flag == 0; ++q) {
         const int k = q % TICKETS;
         if (!ptx::mbar_wait(&tk_empty[k], ((uint32_t)(q / TICKETS) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFB); break; }
-        int index = atomicAdd(p.ticket, 1);
-        if (index >= p.total) index = -1;
-        tk[k] = index;
+        const int index = atomicAdd(p.ticket, 1);
+        NsSlot slot{-1, 0, 0, 0};
+        if (index < p.total) slot = slot_of(p, index, EDGE);
+        tk[k] = slot;
         ptx::mbar_arrive(&tk_full[k]);
         if constexpr (PAIR) {
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tch::mapa(ptx::smem_u32(&tk[k]), 1)), "r"(index) : "memory");
+          asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tch::mapa(ptx::smem_u32(&tk[k]), 1)), "r"(slot.kind),
+                       "r"(slot.mat), "r"(slot.tile), "r"(slot.step) : "memory");
           ptx::mbar_arrive_cluster(tch::mapa(ptx::smem_u32(&tk_full[k]), 1));
         }
-        if (index < 0) break;
-        if (!finished(item_of(p, index, EDGE))) { give_up(0xFFFA); break; }
+        if (slot.kind < 0) break;
+        if (!finished(slot)) { give_up(0xFFFA); break; }
         ptx::mbar_arrive(&go[k]);
         if constexpr (PAIR) ptx::mbar_arrive_cluster(tch::mapa(ptx::smem_u32(&go[k]), 1));
       }
@@ -492,10 +526,10 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       bool ready = false, ok = true;
       for (int q = 0; ok; ++q) {
         if (!wait_for(&tk_full[q % TICKETS], q)) { give_up(0xFFFD); break; }
-        const int index = tk[q % TICKETS];
+        const NsSlot slot = tk[q % TICKETS];
         free_ticket(q);
-        if (index < 0) break;
-        const NsItem it = item_of(p, index, EDGE);
+        if (slot.kind < 0) break;
+        const NsItem it = item_of(p, slot);
         const int m0 = it.ti * EDGE, n0 = it.tj * EDGE, nk = (it.K + BK - 1) / BK;
         const int b = q % sums;
         if (!ptx::mbar_wait(&acc_empty[b], ((uint32_t)(q / sums) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFE); break; }
@@ -544,46 +578,29 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     // warp w may read TMEM lanes [32 (w % 4), +32); the two warps of a quarter split the tile's columns
     const int quarter = warp & 3, mine = warp - 4, half = mine >> 2;
     constexpr int CH = EDGE / 32 / 2;
-    const uint32_t staging = ptx::smem_u32(smem) + STAGES * 2 * OPERAND_BYTES + (uint32_t)(mine * 2 * BUFFER_BYTES);
-    uint32_t same_phase = 0;
-    int boxes = 0, row0 = 0, col0 = 0;                // boxes taken: they alternate between the warp's buffers
-    Finish fin;
-    // (lane 0) brings box c of `same` into the buffer of box number `box`
-    auto fetch = [&](const Finish& f, const NsItem& it, int c, int box) {
-      const int col = col0 + c * 32;
-      if (it.kind == GRAM || row0 >= it.m || col >= it.n) return;
-      uint64_t* bar = &same_bar[mine][box & 1];
-      uint8_t* to = smem + (staging - ptx::smem_u32(smem)) + (box & 1) * BUFFER_BYTES;
-      ptx::mbar_arrive_expect_tx(bar, f.same_low ? 2 * BOX_BYTES : BOX_BYTES);
-      tch::tma_load_3d(to, f.same, col, row0, it.mat, bar);
-      if (f.same_low) tch::tma_load_3d(to + BOX_BYTES, f.same + 1, col, row0, it.mat, bar);
-    };
+    const uint32_t buffer = ptx::smem_u32(smem) + STAGES * 2 * OPERAND_BYTES + (uint32_t)(mine * BUFFER_BYTES);
     for (int q = 0;; ++q) {
-      bool ok = wait_for(&tk_full[q % TICKETS], q);
-      const int index = tk[q % TICKETS];
+      bool ok = __all_sync(0xFFFFFFFFu, wait_for(&tk_full[q % TICKETS], q));
       NsItem it;
-      int b = 0;
-      ok = __all_sync(0xFFFFFFFFu, ok);
+      Finish fin;
+      Box same;
+      int b = 0, row0 = 0, col0 = 0;
       if (ok) {
-        if (index < 0) {
+        const NsSlot slot = tk[q % TICKETS];
+        __syncwarp();
+        if (slot.kind < 0) {
           if (lane == 0) free_ticket(q);
           break;
         }
-        it = item_of(p, index, EDGE);
+        it = item_of(p, slot);
         b = q % sums;
         row0 = it.ti * EDGE + 128 * (int)rank + quarter * 32;
         col0 = it.tj * EDGE + half * (EDGE / 2);
-        fin = finish_of(p, maps, it);
-        if (lane == 0) {
-          ok = it.kind == GRAM || wait_for(&go[q % TICKETS], q);
-          free_ticket(q);
-          if (ok && it.kind != GRAM) {                // under the products: the first box of `same`
-            ptx::fence_proxy_async();
-            tch::bulk_wait_read_all();
-            fetch(fin, it, 0, boxes);
-          }
-        }
-        ok = __all_sync(0xFFFFFFFFu, ok) && ptx::mbar_wait(&acc_full[b], (uint32_t)(q / sums) & 1u, p.spin_limit * 8, abortp);
+        fin = finish_of(p, it);
+        ok = __all_sync(0xFFFFFFFFu, it.kind == GRAM || wait_for(&go[q % TICKETS], q));
+        if (lane == 0) free_ticket(q);
+        if (ok) fetch_box(same, fin, it, row0, col0);  // under the products
+        ok = ok && ptx::mbar_wait(&acc_full[b], (uint32_t)(q / sums) & 1u, p.spin_limit * 8, abortp);
       }
       if (!ok && abort_flag == 0) give_up(0xFFFF);
       uint32_t stop;                                  // one verdict for all of them
@@ -600,9 +617,20 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((p.parts > 1 ? 0 : b * EDGE) + half * (EDGE / 2));
       const int nk = (it.K + BK - 1) / BK;
 #pragma unroll 1
-      for (int c = 0; c < CH; ++c, ++boxes) {
+      for (int c = 0; c < CH; ++c) {
         uint32_t r[32];
         ptx::tmem_ld32(tsrc + (uint32_t)(c * 32), r);
+        const int col = col0 + c * 32;
+        if (it.kind != GRAM) {                        // `same`, from the lanes that fetched it to the rows' lanes
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t at = piece_at(buffer, 8 * k + (lane >> 2), lane & 3);
+            sts_u4(at, same.hi[k]);
+            if (fin.same.lo != nullptr) sts_u4(at + BOX_BYTES, same.lo[k]);
+          }
+          __syncwarp();
+          if (c + 1 < CH) fetch_box(same, fin, it, row0, col + 32);
+        }
         ptx::tmem_ld_wait();
         for (int sum = 1; sum < 4 && p.parts > 1; ++sum) {
           if (sum < 3 && sum >= nk) continue;
@@ -620,28 +648,16 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
             else ptx::mbar_arrive(&acc_empty[b]);
           }
         }
-        const int col = col0 + c * 32;
-        const bool wanted = row0 < it.m && col < it.n;
-        const uint32_t buffer = staging + (uint32_t)((boxes & 1) * BUFFER_BYTES);
-        if (lane == 0) {
-          tch::bulk_wait_read_all();                  // the other buffer's last box has left
-          if (c + 1 < CH) fetch(fin, it, c + 1, boxes + 1);
-        }
-        __syncwarp();
-        if (!wanted) continue;
-        if (it.kind != GRAM && !ptx::mbar_wait(&same_bar[mine][boxes & 1], (same_phase >> (boxes & 1)) & 1u, p.spin_limit * 8, abortp) &&
-            abort_flag == 0)
-          give_up(0xFFF9);                            // (what follows is invalid and reported)
-        if (it.kind != GRAM) same_phase ^= 1u << (boxes & 1);
+        if (row0 >= it.m || col >= it.n) continue;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           float f[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) f[j] = fin.k_acc * __uint_as_float(r[8 * g + j]);
-          const uint32_t piece = buffer + (uint32_t)(lane * 64 + ((g ^ (lane >> 1 & 3)) << 4));
+          const uint32_t piece = piece_at(buffer, lane, g);
           if (it.kind != GRAM) {
             add_halves(f, tch::lds_u4(piece), fin.k_same);
-            if (fin.same_low) add_halves(f, tch::lds_u4(piece + BOX_BYTES), fin.k_same);
+            if (fin.same.lo != nullptr) add_halves(f, tch::lds_u4(piece + BOX_BYTES), fin.k_same);
           }
           if (it.kind == LAST) {
 #pragma unroll
@@ -650,13 +666,13 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           }
           const uint4 h = to_halves(f);
           sts_u4(piece, h);
-          if (fin.out_low) {
+          if (fin.out.lo != nullptr) {
             add_halves(f, h, -1.f);
             sts_u4(piece + BOX_BYTES, to_halves(f));
           }
         }
+        __syncwarp();
         if (it.kind == LAST) {
-          __syncwarp();
 #pragma unroll
           for (int j = 0; j < 32; j += 16 / (int)sizeof(T)) {
             alignas(16) T x[16 / sizeof(T)];
@@ -666,24 +682,20 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           }
           __syncwarp();
           write_result<T>(p, it, buffer, row0, col);
-          ptx::fence_proxy_async_smem();              // read here, next written by TMA
-          __syncwarp();
         } else {
-          ptx::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tch::tma_store_3d(fin.out, smem + (buffer - ptx::smem_u32(smem)), col, row0, it.mat);
-            if (fin.out_low) tch::tma_store_3d(fin.out + 1, smem + (buffer + BOX_BYTES - ptx::smem_u32(smem)), col, row0, it.mat);
-            tch::bulk_commit();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int row = row0 + 8 * k + (lane >> 2), to = col + 8 * (lane & 3);
+            if (row >= it.m || to >= it.n) continue;
+            const uint32_t at = piece_at(buffer, 8 * k + (lane >> 2), lane & 3);
+            *reinterpret_cast<uint4*>(fin.out.hi + (long)row * fin.ld + to) = tch::lds_u4(at);
+            if (fin.out.lo != nullptr) *reinterpret_cast<uint4*>(fin.out.lo + (long)row * fin.ld + to) = tch::lds_u4(at + BOX_BYTES);
           }
         }
+        __syncwarp();
       }
-      if (it.kind != LAST && lane == 0) {
-        tch::bulk_wait_all();                         // written, not only read
-        red_release_gpu_add(p.done + it.mat, 1);
-      }
+      if (it.kind != LAST && lane == 0) red_release_gpu_add(p.done + it.mat, 1);
     }
-    if (lane == 0) tch::bulk_wait_read_all();
   }
   if (abort_flag != 0)
     for (int i = 0; i < 2000; ++i) __nanosleep(100);   // copies in flight land before the shared memory goes
@@ -842,7 +854,6 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
       const uint64_t all = (uint64_t)rows * ld;
       ELMAN_RETURN_IF(make_tmap_f16(&out.rows[low], base, cols, rows, p.count, ld, all, 64, 128));
       ELMAN_RETURN_IF(make_tmap_f16(&out.block[low], base, cols, rows, p.count, ld, all, 64, 64));
-      ELMAN_RETURN_IF(make_tmap_f16(&out.box[low], base, cols, rows, p.count, ld, all, 32, 32));
     }
     return (int)ELMAN_OK;
   };
