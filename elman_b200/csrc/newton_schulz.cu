@@ -781,16 +781,19 @@ bool stays_in_range(int steps, double a, double b, double c) {
   return true;
 }
 
-// Pairs run the tensor cores at their full rate, single blocks (128 columns a product) at about half of it, but
-// in tiles a quarter the size: fewer wasted rows and more blocks where there are few tiles.
+// Pairs make four times the tile in little more than the time of a single block's: about 600 cycles a stage and
+// 11000 a tile against 550 and 7000 (waits, first loads, finishing; measured).  Single blocks waste fewer rows of ragged
+// matrices and spread few tiles over more of the device: 6 x 640 x 1280 takes 257 us in pairs and 211 in single blocks,
+// 4 x 1280 x 1280 takes 316 and 379.
 bool pays_as_pairs(const NsPlan& p) {
   if (p.parts > 1) return false;
-  auto rounds = [&](int edge, int units) {     // rounds of tiles a step, in K steps of a tile
-    const double side = (p.r + edge - 1) / edge, q = (p.tall ? p.m : p.n);
-    const double tri = p.count * side * (side + 1) / 2, all = p.count * side * ceil(q / edge);
-    return ceil(tri / units) * q + ceil(tri / units) * p.r + ceil(all / units) * p.r;
+  auto cost = [&](int edge, int units, double stage, double tile) {     // of a step
+    const double side = (p.r + edge - 1) / edge, q = p.tall ? p.m : p.n;
+    const double tri = p.count * side * (side + 1) / 2 / units, all = p.count * side * ceil(q / edge) / units;
+    const double gram = ceil(q / BK) * stage + tile, other = ceil((double)p.r / BK) * stage + tile;
+    return fmax(tri, 1.) * (gram + other) + fmax(all, 1.) * other;
   };
-  return rounds(256, 74) * 512 < rounds(128, 148) * 440;
+  return cost(256, 74, 600, 11000) < cost(128, 148, 550, 7000);
 }
 
 template <typename T, bool PAIR>

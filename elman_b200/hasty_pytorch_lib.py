@@ -14,7 +14,8 @@ to this module, so the reference's model files pick it up unchanged.
 """
 from __future__ import annotations
 
-import ctypes
+import array
+import contextlib
 
 import torch
 
@@ -59,6 +60,19 @@ def _workspace(nbytes, device):
 
 def _stream(device):
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """The tensors' device as the current one; nothing to enter where it is already (a generation step is as
+    short as the calls around it)."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 # --------------------------------------------------------------------------- E1
@@ -817,6 +831,14 @@ GATED_LINEAR_CHUNK = 64   # ELMAN_GATED_LINEAR_CHUNK: steps between the states k
 def _check_sequences(fn, ref, **tensors):
     """[T, B, d] tensors of one dtype and device whose channels are dense; the strides over t and b are
     free (slices of one projection, batch-major tensors seen through transpose(0, 1))."""
+    if isinstance(ref, torch.Tensor) and ref.is_cuda and ref.dim() == 3 and ref.dtype in _DT:
+        dtype, device, shape = ref.dtype, ref.device, ref.shape
+        for t in tensors.values():       # the short way to see that nothing is wrong
+            if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == shape
+                    and (t.stride(2) == 1 or shape[2] <= 1)):
+                break
+        else:
+            return _DT[dtype]
     for name, t in tensors.items():
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{fn}: {name} must be a Tensor")
@@ -831,9 +853,7 @@ def _check_sequences(fn, ref, **tensors):
         _shape(fn, t, ref.shape, name)
         if t.shape[2] > 1 and t.stride(2) != 1:
             raise RuntimeError(f"{fn}: {name} must have dense channels (stride 1 over the last dimension)")
-    if ref.dtype not in _DT:
-        raise RuntimeError(f"{fn}: dtype {ref.dtype} is not supported (float32 and bfloat16 are)")
-    return _DT[ref.dtype]
+    raise RuntimeError(f"{fn}: dtype {ref.dtype} is not supported (float32 and bfloat16 are)")
 
 
 def _check_state(fn, t, name, shape, device):
@@ -868,8 +888,7 @@ def _sequence_like(x):
 
 
 def _tb_strides(*tensors):
-    flat = [s for t in tensors for s in (t.stride(0), t.stride(1))]
-    return (ctypes.c_long * len(flat))(*flat)
+    return array.array("l", [s for t in tensors for s in t.stride()[:2]])
 
 
 def gated_linear_forward(training, f, c, z, h0=None, reset=None):
@@ -885,16 +904,19 @@ def gated_linear_forward(training, f, c, z, h0=None, reset=None):
     _check_state(fn, h0, "h0", (B, d), f.device)
     _check_reset(fn, reset, T, B, f.device)
     lib = _lib.load()
-    with torch.cuda.device(f.device):
+    device = f.device
+    with _on(device):
         y = _sequence_like(f)
-        h_last = torch.empty(B, d, dtype=torch.float32, device=f.device)
+        h_last = torch.empty(B, d, dtype=torch.float32, device=device)
         rows = -(-T // GATED_LINEAR_CHUNK) if training else 0
-        saved = torch.empty((rows, B, d) if training else (0,), dtype=torch.float32, device=f.device)
-        ws = _workspace(lib.elman_gated_linear_workspace(dt, T, B, d), f.device)
+        saved = torch.empty((rows, B, d) if training else (0,), dtype=torch.float32, device=device)
+        need = lib.elman_gated_linear_workspace(dt, T, B, d)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+        strides = _tb_strides(f, c, z, y)
         rc = lib.elman_gated_linear_forward(
             dt, 1 if training else 0, T, B, d, f.data_ptr(), c.data_ptr(), z.data_ptr(), _opt(h0),
-            _opt(reset), _tb_strides(f, c, z, y), y.data_ptr(), h_last.data_ptr(), saved.data_ptr(),
-            ws.data_ptr(), ws.numel(), _stream(f.device))
+            _opt(reset), strides.buffer_info()[0], y.data_ptr(), h_last.data_ptr(), saved.data_ptr(),
+            _opt(ws), need, _raw_stream(device))
         _lib.check(rc, fn)
     return [y, h_last, saved]
 
@@ -913,7 +935,8 @@ def gated_linear_backward(f, c, z, saved, d_output, dh_last=None, reset=None, ou
         raise RuntimeError(f"{fn}: saved is empty: run the forward pass with training=True")
     _check_state(fn, saved, "saved", (-(-T // GATED_LINEAR_CHUNK), B, d), f.device)
     lib = _lib.load()
-    with torch.cuda.device(f.device):
+    device = f.device
+    with _on(device):
         if out is None:
             df, dc, dz = (_sequence_like(f) for _ in range(3))
         else:
@@ -922,13 +945,14 @@ def gated_linear_backward(f, c, z, saved, d_output, dh_last=None, reset=None, ou
             used = {t.untyped_storage().data_ptr() for t in (f, c, z, saved, d_output)}
             if any(t.untyped_storage().data_ptr() in used for t in out if t.numel() > 0):
                 raise RuntimeError(f"{fn}: out must not share storage with the inputs")
-        dh0 = torch.empty(B, d, dtype=torch.float32, device=f.device)
-        ws = _workspace(lib.elman_gated_linear_workspace(dt, T, B, d), f.device)
+        dh0 = torch.empty(B, d, dtype=torch.float32, device=device)
+        need = lib.elman_gated_linear_workspace(dt, T, B, d)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+        strides = _tb_strides(f, c, z, d_output, df, dc, dz)
         rc = lib.elman_gated_linear_backward(
             dt, T, B, d, f.data_ptr(), c.data_ptr(), z.data_ptr(), saved.data_ptr(),
-            d_output.data_ptr(), _opt(dh_last), _opt(reset),
-            _tb_strides(f, c, z, d_output, df, dc, dz), df.data_ptr(), dc.data_ptr(), dz.data_ptr(),
-            dh0.data_ptr(), ws.data_ptr(), ws.numel(), _stream(f.device))
+            d_output.data_ptr(), _opt(dh_last), _opt(reset), strides.buffer_info()[0], df.data_ptr(),
+            dc.data_ptr(), dz.data_ptr(), dh0.data_ptr(), _opt(ws), need, _raw_stream(device))
         _lib.check(rc, fn)
     return [df, dc, dz, dh0]
 
@@ -950,10 +974,10 @@ def newton_schulz(G, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7)
     count = G.numel() // (m * n) if m * n > 0 else 0
     a, b, c = coefficients
     lib = _lib.load()
-    with torch.cuda.device(G.device):
+    with _on(G.device):
         out = torch.empty_like(G)
         ws = _workspace(lib.elman_newton_schulz_workspace(dt, count, m, n), G.device)
         rc = lib.elman_newton_schulz(dt, count, m, n, G.data_ptr(), out.data_ptr(), int(steps), float(a), float(b),
-                                     float(c), float(eps), ws.data_ptr(), ws.numel(), _stream(G.device))
+                                     float(c), float(eps), ws.data_ptr(), ws.numel(), _raw_stream(G.device))
         _lib.check(rc, fn)
     return out
