@@ -6,6 +6,7 @@ Layout:
   mamba_gated_elman.py     E1: autograd Function, cell, layer (same API as the reference)
   stock_elman.py           E0
   pure_lowrank_elman.py    E5
+  gated_linear.py          the layer of the gated linear recurrence
   ladder_lm.py             the byte-level LM wrapper that calls the layers (caller of the path)
 """
 import sys

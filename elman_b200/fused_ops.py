@@ -7,6 +7,7 @@ one GEMM) of the CUDA library instead of a chain of framework ops:
                           (elman/models/mamba_gated_elman.py:283-297)
   linear()                out_proj / lm_head through the library's GEMMs
                           (mamba_gated_elman.py:306, ladder_lm.py:929-933, :1062)
+  gated_linear()          the gated linear recurrence on its packed projection
 
 They change no arithmetic beyond rounding order and are used by the layers' fused paths and
 by LadderLM; CPU tensors are refused like everywhere else in the package.
@@ -250,6 +251,15 @@ def linear(x, weight, bias=None):
     """y = x W^T (+ b) over the last dimension through the library's GEMMs."""
     from .mamba_gated_elman import LinearFunction
     return LinearFunction.apply(x, weight, bias)
+
+
+def gated_linear(fcz, h0=None, reset=None):
+    """The gated linear recurrence on a projection fcz [T,B,3d] = (f, c, z): (y [T,B,d], h_last [B,d]
+    float32), differentiable in fcz and h0.  reset [T,B] bool: True where a step starts anew."""
+    from .gated_linear import GatedLinearFunction
+    if fcz.dim() != 3 or fcz.shape[2] % 3 != 0:
+        raise RuntimeError("gated_linear: fcz must be [T, B, 3 * dim]")
+    return GatedLinearFunction.apply(fcz, h0, reset)
 
 
 def library_handles(x):

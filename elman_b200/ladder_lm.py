@@ -19,6 +19,7 @@ import torch.nn.functional as F
 from torch.autograd import forward_ad
 
 from . import _lib, _spectral, fused_ops
+from .gated_linear import GatedLinearElman
 from .mamba_gated_elman import MambaGatedElman, MambaGatedElmanCell
 from .pure_lowrank_elman import PureLowRankElman
 from .siblings import E32NoPresilu, E33SelfGate, E57LearnedRadius, LowRankElman
@@ -31,7 +32,7 @@ _BF16 = {torch.bfloat16}
 _dtype_of = operator.attrgetter("dtype")
 
 _LEVELS = {0: StockElman, 1: MambaGatedElman, 4: LowRankElman, 5: PureLowRankElman,
-           32: E32NoPresilu, 33: E33SelfGate, 57: E57LearnedRadius}
+           32: E32NoPresilu, 33: E33SelfGate, 57: E57LearnedRadius, "gated_linear": GatedLinearElman}
 
 
 def _runs_only(module, cls):
@@ -62,12 +63,12 @@ def _transformed():
 def get_ladder_level(level):
     """Layer class of an ablation-ladder level (0 = E0, 1 = E1, 4 = E1 with a low-rank recurrent
     matrix, 5 = E5, 32 / 33 / 57 = the E1 siblings without pre-silu, with a self gate, with a
-    learned spectral radius)."""
+    learned spectral radius), or "gated_linear", which the reference does not have."""
     try:
-        return _LEVELS[int(level)]
+        return _LEVELS[level if level == "gated_linear" else int(level)]
     except (KeyError, ValueError):
         raise ValueError(f"level {level!r} is not implemented here "
-                         f"(available: {sorted(_LEVELS)})")
+                         f"(available: {sorted(_LEVELS, key=str)})")
 
 
 class LadderLM(nn.Module):
@@ -109,14 +110,21 @@ class LadderLM(nn.Module):
         nn.init.normal_(self.embedding.weight, std=0.02)
 
     def forward(self, x, return_loss=False, return_prev_hiddens=False, prev_hiddens=None,
-                prev_conv_buffers=None, actual_length=None, doc_boundaries=None):
-        """x: [B,T] token ids ([B,T+1] with return_loss: inputs and shifted targets)."""
+                prev_conv_buffers=None, actual_length=None, doc_boundaries=None, reset=None):
+        """x: [B,T] token ids ([B,T+1] with return_loss: inputs and shifted targets).  reset (not a
+        reference argument): bool like x, True where a token starts a new document and the layers forget
+        what came before; level "gated_linear" only."""
         if return_loss:
             inp, target = x[:, :-1], x[:, 1:]
         else:
             inp = x
         if prev_hiddens is None:
             prev_hiddens = [None] * self.depth
+        more = {}
+        if reset is not None:
+            if not all(isinstance(layer, GatedLinearElman) for layer in self.layers):
+                raise ValueError("reset: only the layers of level \"gated_linear\" start anew inside a sequence")
+            more["reset"] = reset[:, :inp.size(1)]
         if not return_loss and inp.size(1) == 1 and not torch.is_grad_enabled():
             token = self._one_token(inp, prev_hiddens)
             if token is not None:
@@ -156,7 +164,7 @@ class LadderLM(nn.Module):
             residual = None
             for i, (ln, layer) in enumerate(zip(self.layer_norms, self.layers)):
                 h, residual = self._add_norm(ln, h, residual, group=i)
-                h, h_final = layer(h, prev_hiddens[i])
+                h, h_final = layer(h, prev_hiddens[i], **more)
                 new_hiddens.append(h_final)
         h, _ = self._add_norm(self.norm, h, residual, last=True)
         if time_major and (not return_loss or self.loss_chunk_size > 0):

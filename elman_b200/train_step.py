@@ -74,7 +74,7 @@ class GraphedTrainStep:
             self.reducer.finish()
         if self.after_backward is not None:
             self.after_backward(self.params)
-        if isinstance(self.opt, FlatAdamW) and self.reducer is not None:
+        if isinstance(self.opt, (FlatAdamW, FlatMuon)) and self.reducer is not None:
             # clipping folded into the update: the factor is applied as the gradients are read
             coef = self.reducer.clip_coef(self.max_grad_norm)[0] if self.max_grad_norm else None
             self.opt.step(grad_scale=coef)
@@ -370,6 +370,111 @@ class FlatAdamW:
         self.exp_avg.copy_(sd["exp_avg"])
         self.exp_avg_sq.copy_(sd["exp_avg_sq"])
         self.param_groups[0].update(sd["param_groups"][0])
+
+
+def hidden_matrices(model):
+    """The weight matrices inside a model's layers (not the embedding, the head or vectors): what Muon updates."""
+    return [p for layer in getattr(model, "layers", []) for p in layer.parameters()
+            if p.dim() == 2 and p.requires_grad]
+
+
+class FlatMuon:
+    """Muon over the flat buffers of a FlatGradients: each of `matrices` moves along its momentum-weighted gradient
+    with the singular values brought near one by Newton-Schulz products (elman_muon_step: all matrices of one shape
+    in one call), scaled by sqrt(max(1, rows / columns)); every other parameter takes an AdamW step.  The clipping
+    factor is applied while the gradients are read.  Momentum is float32; nothing is read back by the host, so the
+    step can be captured."""
+
+    def __init__(self, grads, matrices, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
+                 coefficients=None, eps=1e-7, adamw_lr=3e-4, betas=(0.9, 0.95), adamw_eps=1e-8,
+                 adamw_weight_decay=0.0):
+        from . import hasty_pytorch_lib as H
+        if not grads.flat.is_cuda:
+            raise RuntimeError("FlatMuon runs on CUDA buffers only (no CPU fallback)")
+        matrices = list(matrices)
+        known = {id(p) for p in grads.params}
+        if len({id(p) for p in matrices}) != len(matrices):
+            raise ValueError("a matrix appears more than once")
+        for p in matrices:
+            if p.dim() != 2 or id(p) not in known:
+                raise ValueError("matrices must be 2-D parameters of the gradients' owner")
+        self.grads = grads
+        self.flat_params = flat = grads.flatten_parameters()
+        lo, size = grads.flat.data_ptr(), grads.flat.element_size()
+        at = {id(p): (p.grad.data_ptr() - lo) // size for p in grads.params}
+        mine = {id(p) for p in matrices}
+        shapes = {}
+        for p in matrices:
+            if p.numel() > 0:
+                shapes.setdefault(tuple(p.shape), []).append(at[id(p)])
+        self.groups = []      # (m, n, where each matrix starts in the flat buffers, momentum)
+        for (m, n), offsets in shapes.items():
+            self.groups.append((m, n, torch.tensor(offsets, dtype=torch.int64, device=flat.device),
+                                torch.zeros(len(offsets), m, n, dtype=torch.float32, device=flat.device)))
+        runs = []             # stretches of the flat buffers that are no matrix
+        for off, n in sorted((at[id(p)], p.numel()) for p in grads.params if id(p) not in mine):
+            if runs and runs[-1][1] == off:
+                runs[-1][1] = off + n
+            else:
+                runs.append([off, off + n])
+        self.runs = [tuple(r) for r in runs]
+        rest = sum(b - a for a, b in self.runs)
+        self.exp_avg = torch.zeros(rest, dtype=flat.dtype, device=flat.device)
+        self.exp_avg_sq = torch.zeros_like(self.exp_avg)
+        self.step_count = torch.zeros(max(1, len(self.runs)), dtype=torch.float32, device=flat.device)
+        coefficients = tuple(coefficients or H.NEWTON_SCHULZ_COEFFICIENTS)
+        self.param_groups = [
+            dict(params=matrices, lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                 coefficients=coefficients, eps=eps),
+            dict(params=[p for p in grads.params if id(p) not in mine], lr=adamw_lr, betas=betas, eps=adamw_eps,
+                 weight_decay=adamw_weight_decay)]
+
+    def zero_grad(self, set_to_none=False):
+        self.grads.zero()
+
+    def step(self, grad_scale=None):
+        from . import _lib
+        from . import hasty_pytorch_lib as H
+        flat, grad = self.flat_params, self.grads.flat
+        if grad_scale is not None and (grad_scale.dtype != torch.float32 or not grad_scale.is_cuda):
+            raise RuntimeError("FlatMuon.step: grad_scale must be a float32 CUDA tensor")
+        lib, dt, size = _lib.load(), H._DT[flat.dtype], flat.element_size()
+        scale = None if grad_scale is None else grad_scale.data_ptr()
+        with torch.cuda.device(flat.device):
+            stream = torch.cuda.current_stream(flat.device).cuda_stream
+            g = self.param_groups[0]
+            for m, n, offsets, momentum in self.groups:
+                count = offsets.numel()
+                ws = H._workspace(lib.elman_newton_schulz_workspace(dt, count, m, n), flat.device)
+                rc = lib.elman_muon_step(
+                    dt, count, m, n, offsets.data_ptr(), flat.data_ptr(), grad.data_ptr(), momentum.data_ptr(),
+                    float(g["lr"]), float(g["momentum"]), 1 if g["nesterov"] else 0, float(g["weight_decay"]),
+                    max(1.0, m / n) ** 0.5, scale, int(g["steps"]), *(float(c) for c in g["coefficients"]),
+                    float(g["eps"]), ws.data_ptr(), ws.numel(), stream)
+                _lib.check(rc, "elman_muon_step")
+            g, done = self.param_groups[1], 0
+            for k, (a, b) in enumerate(self.runs):
+                rc = lib.elman_adamw_step(
+                    dt, b - a, flat.data_ptr() + a * size, grad.data_ptr() + a * size,
+                    self.exp_avg.data_ptr() + done * size, self.exp_avg_sq.data_ptr() + done * size, float(g["lr"]),
+                    float(g["betas"][0]), float(g["betas"][1]), float(g["eps"]), float(g["weight_decay"]),
+                    self.step_count.data_ptr() + 4 * k, scale, stream)
+                _lib.check(rc, "elman_adamw_step")
+                done += b - a
+
+    def state_dict(self):
+        return {"step": self.step_count.clone(), "exp_avg": self.exp_avg.clone(),
+                "exp_avg_sq": self.exp_avg_sq.clone(), "momentum": [m.clone() for *_, m in self.groups],
+                "param_groups": [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]}
+
+    def load_state_dict(self, sd):
+        self.step_count.copy_(sd["step"])
+        self.exp_avg.copy_(sd["exp_avg"])
+        self.exp_avg_sq.copy_(sd["exp_avg_sq"])
+        for (*_, mine), kept in zip(self.groups, sd["momentum"], strict=True):
+            mine.copy_(kept)
+        for mine, kept in zip(self.param_groups, sd["param_groups"], strict=True):
+            mine.update(kept)
 
 
 def ladder_buckets(model):
