@@ -94,6 +94,36 @@ def test_strided_inputs(T, B, d, packed, batch_major, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("packed,batch_major", [(False, False), (True, False), (True, True)])
+@pytest.mark.parametrize("T,B,d,reset", [(9, 2, 64, None), (64, 1, 120, 0.05), (129, 3, 128, None), (200, 2, 1000, 0.01), (2100, 2, 120, None),
+                                         (5000, 1, 64, 0.002), (4097, 1, 60, None), (300, 9, 1280, None)])
+def test_rows_on_16_bytes(T, B, d, reset, packed, batch_major, dtype):
+    """The shapes whose rows TMA copies: whole and ragged channel groups, one tile and several groups of them."""
+    check(make(T, B, d, dtype, seed=T, packed=packed, batch_major=batch_major, reset=reset), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [128, 62, 61])
+def test_calls_on_two_streams_at_once(d, dtype):
+    """Long chains in several launches that share the device: none waits for another's blocks."""
+    sets = [make(3000, 4, d, dtype, seed=40 + k, reset=0.001) for k in range(3)]
+    want = [[t.clone() for t in H.gated_linear_forward(True, s["f"], s["c"], s["z"], s["h0"], s["reset"])] for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for s, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                out = H.gated_linear_forward(True, s["f"], s["c"], s["z"], s["h0"], s["reset"])
+                got.append(out + H.gated_linear_backward(s["f"], s["c"], s["z"], out[2], s["dy"], s["dh"], s["reset"]))
+    torch.cuda.synchronize()
+    for k, out in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(out[:3], want[k % 3]))
+        assert all(torch.equal(a, b) for a, b in zip(out[3:], got[k % 3][3:]))
+    assert _lib.device_status()[0] == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("share", [0.01, 0.3, 1.0])
 @pytest.mark.parametrize("T,B,d", [(3, 2, 16), (200, 3, 65), (1500, 1, 64)])
 def test_resets(T, B, d, share, dtype):

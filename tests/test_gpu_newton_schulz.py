@@ -122,6 +122,29 @@ def test_two_runs_and_two_batches_give_the_same_bits():
     assert torch.equal(torch.stack([H.newton_schulz(g) for g in G]), X)
 
 
+def test_calls_on_two_streams_at_once():
+    """Launches that share the device: none waits for another's blocks."""
+    sets = [make(6, 640, 700, torch.bfloat16, seed=1), make(2, 1100, 1024, torch.bfloat16, seed=2), make(3, 300, 400, torch.float32, seed=3)]
+    want = [H.newton_schulz(G) for G in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for G, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append(H.newton_schulz(G))
+    torch.cuda.synchronize()
+    assert all(torch.equal(X, want[k % 3]) for k, X in enumerate(got))
+    assert _lib.device_status()[0] == 0
+
+
+@pytest.mark.parametrize("count,m,n", [(18, 512, 512), (3, 1280, 1280), (4, 2560, 1024), (1, 2048, 4096)])
+def test_tiles_of_block_pairs(count, m, n):
+    """Sizes at which pairs of blocks make tiles of 256 x 256."""
+    G = make(count, m, n, torch.bfloat16, kind="lowrank", seed=m)
+    assert rel(H.newton_schulz(G), reference(G)) < TOL[torch.bfloat16]
+
+
 def test_captured_on_another_stream():
     a, b = make(2, 200, 300, torch.bfloat16, seed=7), make(1, 330, 130, torch.bfloat16, seed=8)
     side, graphs, outs, pool = torch.cuda.Stream(), [], [], None
