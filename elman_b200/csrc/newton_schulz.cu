@@ -70,6 +70,7 @@ struct NsMaps { NsMap x[2], a, b; };
 // groups 0.98 ms, as one 0.87: waiting for the matrix one reads costs more than reading it from HBM.)
 struct NsPlan {
   int count, m, n, r, tall, steps, parts;
+  int split;                 // bf16: both parts of A and of B go into the products
   int triangle, all;         // tiles of a symmetric product and of an update
   int per_step, total;       // items of the list
   float a, b, c;
@@ -118,11 +119,13 @@ __device__ __forceinline__ NsSlot slot_of(const NsPlan& p, int index, int edge) 
 struct NsItem {
   int kind, mat, ti, tj, step;
   int m, n, K, a_form, b_form;
+  int parts;                                   // products of high and low parts
 };
 __device__ __forceinline__ NsItem item_of(const NsPlan& p, NsSlot k) {
   NsItem it;
   it.kind = k.kind; it.mat = k.mat; it.ti = k.tile >> 16; it.tj = k.tile & 0xFFFF; it.step = k.step;
   const bool symmetric = k.kind == GRAM || k.kind == SQUARE;
+  it.parts = !p.split || k.kind == GRAM ? p.parts : k.kind == SQUARE ? 3 : 2;
   it.m = symmetric ? p.r : p.m;
   it.n = symmetric ? p.r : p.n;
   it.K = k.kind != GRAM ? p.r : p.tall ? p.m : p.n;
@@ -471,8 +474,8 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         ptx::fence_proxy_async();                     // written by other blocks, read here by TMA
         const NsMap& map = it.kind == GRAM ? maps.x[at] : it.kind == SQUARE ? maps.a : first == (p.tall != 0) ? maps.x[at] : maps.b;
         bool ok = true;
-        for (int part = 0; part < p.parts && ok; ++part) {      // high x high, high x low, low x high
-          const int low = first ? part == 2 : part == 1;
+        for (int part = 0; part < it.parts && ok; ++part) {     // high x high, high x low, low x high; or B's low part
+          const int low = it.parts == 2 ? part == 1 && first == (p.tall == 0) : first ? part == 2 : part == 1;
           for (int k0 = 0; k0 < it.K; k0 += BK, ++iteration) {
             if (!ptx::mbar_wait(&empty_bar[s], ph ^ 1u, p.spin_limit, abortp)) { give_up(k0); ok = false; break; }
             if (first && rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[s], BLOCKS * 2 * OPERAND_BYTES);
@@ -536,7 +539,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         ptx::tc_fence_after();
         const uint32_t sum0 = tmem_base + (uint32_t)(b * EDGE);
         int i = 0;                                    // stages of this item, over all parts
-        for (int part = 0; part < p.parts && ok; ++part) {
+        for (int part = 0; part < it.parts && ok; ++part) {
           for (int k0 = 0; k0 < it.K && ok;) {
             // the stretch of K in which both operands keep their form: an upper matrix changes at the diagonal
             int end = it.K;
@@ -713,6 +716,12 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
 
 long padded(long x) { return (x + 7) / 8 * 8; }       // rows start on 16 bytes
 
+// Where r is small A and B are mostly diagonal, all of it rounded alike, and B X is nearly three times the result it
+// becomes part of: 24 x 800 comes out 2.2e-3 off before the last rounding (with it 2.8e-3; a rounded exact result is
+// 1.7e-3 off).  The second parts of A and B in their products make that 0.9e-3, for three stages of latency a step where
+// r is one stage long (101 us become 108).
+bool splits(int r) { return r <= BK; }
+
 struct NsBuffers {
   Split X[2], A, B;
   double* partial;
@@ -740,7 +749,7 @@ NsBuffers carve(void* ws, int dtype, int count, int m, int n) {
   }
   b.A.hi = (__half*)take(a);
   b.B.hi = (__half*)take(a);
-  if (dtype == ELMAN_F32) {
+  if (dtype == ELMAN_F32 || splits(r)) {
     b.A.lo = (__half*)take(a);
     b.B.lo = (__half*)take(a);
   }
@@ -835,6 +844,7 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   p.r = p.tall ? g.n : g.m;
   p.steps = g.steps;
   p.parts = g.dtype == ELMAN_F32 ? 3 : 1;
+  p.split = p.parts == 1 && splits(p.r);
   p.a = g.a; p.b = g.b; p.c = g.c;
   p.X[0] = buf.X[0]; p.X[1] = buf.X[1]; p.A = buf.A; p.B = buf.B;
   p.ldx = buf.ldx; p.ldr = buf.ldr;
