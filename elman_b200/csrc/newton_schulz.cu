@@ -70,7 +70,7 @@ struct NsMaps { NsMap x[2], a, b; };
 // groups 0.98 ms, as one 0.87: waiting for the matrix one reads costs more than reading it from HBM.)
 struct NsPlan {
   int count, m, n, r, tall, steps, parts;
-  int split;                 // bf16: both parts of A and of B go into the products
+  int split;                 // bf16: 1: both parts of B go into the products, 2: of A as well
   int triangle, all;         // tiles of a symmetric product and of an update
   int per_step, total;       // items of the list
   float a, b, c;
@@ -125,7 +125,7 @@ __device__ __forceinline__ NsItem item_of(const NsPlan& p, NsSlot k) {
   NsItem it;
   it.kind = k.kind; it.mat = k.mat; it.ti = k.tile >> 16; it.tj = k.tile & 0xFFFF; it.step = k.step;
   const bool symmetric = k.kind == GRAM || k.kind == SQUARE;
-  it.parts = !p.split || k.kind == GRAM ? p.parts : k.kind == SQUARE ? 3 : 2;
+  it.parts = p.split == 0 || k.kind == GRAM ? p.parts : k.kind != SQUARE ? 2 : p.split == 2 ? 3 : 1;
   it.m = symmetric ? p.r : p.m;
   it.n = symmetric ? p.r : p.n;
   it.K = k.kind != GRAM ? p.r : p.tall ? p.m : p.n;
@@ -718,9 +718,9 @@ long padded(long x) { return (x + 7) / 8 * 8; }       // rows start on 16 bytes
 
 // Where r is small A and B are mostly diagonal, all of it rounded alike, and B X is nearly three times the result it
 // becomes part of: 24 x 800 comes out 2.2e-3 off before the last rounding (with it 2.8e-3; a rounded exact result is
-// 1.7e-3 off).  The second parts of A and B in their products make that 0.9e-3, for three stages of latency a step where
-// r is one stage long (101 us become 108).
-bool splits(int r) { return r <= BK; }
+// 1.7e-3 off).  The second part of B in the update's product, one or two stages of latency a step, makes that 1.4e-3,
+// that of A as well, where r is a single stage, 0.9e-3 (101 us become 108).
+int splits(int dtype, int r) { return dtype == ELMAN_F32 || r > 128 ? 0 : r > BK ? 1 : 2; }
 
 struct NsBuffers {
   Split X[2], A, B;
@@ -749,10 +749,8 @@ NsBuffers carve(void* ws, int dtype, int count, int m, int n) {
   }
   b.A.hi = (__half*)take(a);
   b.B.hi = (__half*)take(a);
-  if (dtype == ELMAN_F32 || splits(r)) {
-    b.A.lo = (__half*)take(a);
-    b.B.lo = (__half*)take(a);
-  }
+  if (dtype == ELMAN_F32 || splits(dtype, r) == 2) b.A.lo = (__half*)take(a);
+  if (dtype == ELMAN_F32 || splits(dtype, r) > 0) b.B.lo = (__half*)take(a);
   b.partial = (double*)take((size_t)count * NORM_PARTS * sizeof(double));
   b.ticket = (int*)take(sizeof(int));
   b.done = (int*)take((size_t)count * sizeof(int));
@@ -844,7 +842,7 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   p.r = p.tall ? g.n : g.m;
   p.steps = g.steps;
   p.parts = g.dtype == ELMAN_F32 ? 3 : 1;
-  p.split = p.parts == 1 && splits(p.r);
+  p.split = splits(g.dtype, p.r);
   p.a = g.a; p.b = g.b; p.c = g.c;
   p.X[0] = buf.X[0]; p.X[1] = buf.X[1]; p.A = buf.A; p.B = buf.B;
   p.ldx = buf.ldx; p.ldr = buf.ldr;
