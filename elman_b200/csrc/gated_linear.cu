@@ -633,9 +633,12 @@ struct GlTma {
   int tiles, groups_per_row, total;   // tiles in time; channel groups of a batch row; all tiles
   long cols;                          // channels as the chain counts them: whole groups
 };
-struct Feed {                          // shared: producer <-> scanning warps
+// Where a tile lies: its ticket (-1: no more tiles), its place in the scan's order, its batch row and channel group.
+// The producer takes tickets apart; the divisions were a tenth of the backward tile's instructions.
+struct alignas(16) TileAt { int ticket, n, b, group; };
+struct Feed {                          // shared: producer <-> scanning and linking warps
   uint64_t full[2], done[2];
-  int ticket[2];
+  TileAt tile[2];
   int gave_up;
 };
 
@@ -645,77 +648,67 @@ __device__ __forceinline__ void produce(Feed& fd, uint8_t* smem, const CUtensorM
                                         const GlTma& g, const GlChain& ch) {
   constexpr int TENSOR = Stages<IN, ROWS>::TENSOR, STAGE = Stages<IN, ROWS>::STAGE;
   volatile int* gave_up = &fd.gave_up;
-  int ticket[2] = {-1, -1};
+  TileAt tile[2] = {{-1, 0, 0, 0}, {-1, 0, 0, 0}};
+  const int per_time = g.total / g.tiles;
+  auto row_of = [&](const TileAt& t) { return (backward ? g.tiles - 1 - t.n : t.n) * ROWS; };
+  auto store = [&](int s) {
+#pragma unroll
+    for (int k = 0; k < OUT; ++k)
+      tch::tma_store_3d(out[k], smem + s * STAGE + k * TENSOR, tile[s].group * channels, tile[s].b, row_of(tile[s]));
+    tch::bulk_commit();
+  };
   for (int it = 0;; ++it) {
     const int s = it & 1;
-    uint8_t* stage = smem + s * STAGE;
-    auto corner = [&](int tk, int& c0, int& c1, int& c2) {
-      const int n = tk / g.groups_per_row / (g.total / g.tiles / g.groups_per_row);
-      const int group = tk - n * (g.total / g.tiles);
-      c1 = group / g.groups_per_row;
-      c0 = (group - c1 * g.groups_per_row) * channels;
-      c2 = (backward ? g.tiles - 1 - n : n) * ROWS;
-    };
-    int c0, c1, c2;
     if (it >= 2) {                                  // the tile that was here: its results leave
       if (!ptx::mbar_wait(&fd.done[s], (uint32_t)((it >> 1) - 1) & 1u, ch.spin_limit * 8, gave_up)) break;
-      corner(ticket[s], c0, c1, c2);
-#pragma unroll
-      for (int k = 0; k < OUT; ++k) tch::tma_store_3d(out[k], stage + k * TENSOR, c0, c1, c2);
-      tch::bulk_commit();
-      tch::bulk_wait_read_all();
+      store(s);
     }
     const uint32_t next = g.tiles > 1 ? atomicAdd(ch.ctrl, 1u) + 1u
                                       : (uint32_t)(it == 0 ? blockIdx.x : g.total);
-    const bool any = next < (uint32_t)g.total;
-    ticket[s] = any ? (int)next : -1;
-    fd.ticket[s] = ticket[s];
-    if (!any) {
+    TileAt t{-1, 0, 0, 0};
+    if (next < (uint32_t)g.total) {
+      t.ticket = (int)next;
+      t.n = t.ticket / per_time;
+      const int column = t.ticket - t.n * per_time;
+      t.b = column / g.groups_per_row;
+      t.group = column - t.b * g.groups_per_row;
+    }
+    tile[s] = t;
+    fd.tile[s] = t;
+    if (t.ticket < 0) {
       ptx::mbar_arrive(&fd.full[s]);                // nothing more: the scanning warps end here
-      if (it >= 1 && ticket[s ^ 1] >= 0) {          // the last tile's results
-        if (ptx::mbar_wait(&fd.done[s ^ 1], (uint32_t)((it - 1) >> 1) & 1u, ch.spin_limit * 8, gave_up)) {
-          corner(ticket[s ^ 1], c0, c1, c2);
-#pragma unroll
-          for (int k = 0; k < OUT; ++k) tch::tma_store_3d(out[k], smem + (s ^ 1) * STAGE + k * TENSOR, c0, c1, c2);
-          tch::bulk_commit();
-        }
-      }
+      // the last tile's results
+      if (it >= 1 && tile[s ^ 1].ticket >= 0 &&
+          ptx::mbar_wait(&fd.done[s ^ 1], (uint32_t)((it - 1) >> 1) & 1u, ch.spin_limit * 8, gave_up))
+        store(s ^ 1);
       break;
     }
-    corner(ticket[s], c0, c1, c2);
+    tch::bulk_wait_read_all();                      // the stage has been read out
     ptx::mbar_arrive_expect_tx(&fd.full[s], STAGE);
 #pragma unroll
-    for (int k = 0; k < IN; ++k) tch::tma_load_3d(stage + k * TENSOR, in[k], c0, c1, c2, &fd.full[s]);
+    for (int k = 0; k < IN; ++k)
+      tch::tma_load_3d(smem + s * STAGE + k * TENSOR, in[k], t.group * channels, t.b, row_of(t), &fd.full[s]);
   }
   if (*gave_up != 0)
     for (int i = 0; i < 2000; ++i) __nanosleep(100);   // loads in flight land before the shared memory goes
   tch::bulk_wait_read_all();
 }
 
-// What a scanning warp knows of the tile it is at.
-template <int V> struct TmaTile {
-  int n, b, i;
-  long base;
-  __device__ __forceinline__ TmaTile(int ticket, const GlTma& g) {
-    const int per_time = g.total / g.tiles;
-    n = ticket / per_time;
-    const int group = ticket - n * per_time;
-    base = (long)group * (32 * V);
-    b = group / g.groups_per_row;
-    i = (group - b * g.groups_per_row) * (32 * V) + (threadIdx.x & 31) * V;
-  }
-};
+// V channels of a state [B, d] from channel i on.
 template <int V> __device__ __forceinline__ Vec<V> read_state(const float* from, int b, int i, int d) {
   Vec<V> x(0.f);
+  if (from == nullptr) return x;
+  from += (long)b * d + i;
 #pragma unroll
   for (int v = 0; v < V; ++v)
-    if (from != nullptr && i + v < d) x.set(v, from[(long)b * d + i + v]);
+    if (i + v < d) x.set(v, from[v]);
   return x;
 }
 template <int V> __device__ __forceinline__ void write_state(float* to, int b, int i, int d, Vec<V> x) {
+  to += (long)b * d + i;
 #pragma unroll
   for (int v = 0; v < V; ++v)
-    if (i + v < d) to[(long)b * d + i + v] = x.get(v);
+    if (i + v < d) to[v] = x.get(v);
 }
 template <typename T, int V> __device__ __forceinline__ Vec<V> word_at(uint32_t addr) {
   uint32_t w;
@@ -816,12 +809,12 @@ __device__ __forceinline__ void link_tiles(Links<V, W>& sh, Feed& fd, const GlPa
     const int s = it & 1;
     const bool here = ptx::mbar_wait(&fd.full[s], (uint32_t)(it >> 1) & 1u, ch.spin_limit * 8, &fd.gave_up);
     if (!__all_sync(0xFFFFFFFFu, here)) return;      // (the scanning warps see it too)
-    const int ticket = fd.ticket[s];
-    if (ticket < 0) return;
-    const int per_time = g.total / g.tiles, n = ticket / per_time, group = ticket - n * per_time;
-    const int b = group / g.groups_per_row, i = (group - b * g.groups_per_row) * (32 * V) + x;
-    const float start = n < GROUP && initial != nullptr && i < p.d ? initial[(long)b * p.d + i] : 0.f;
-    const bool ok = link<V, W, RESET>(sh, x, n, g.tiles, (long)group * (32 * V), g.cols, start, ch, ticket);
+    const TileAt t = fd.tile[s];
+    if (t.ticket < 0) return;
+    const int i = t.group * (32 * V) + x;
+    const long base = ((long)t.b * g.groups_per_row + t.group) * (32 * V);
+    const float start = t.n < GROUP && initial != nullptr && i < p.d ? initial[(long)t.b * p.d + i] : 0.f;
+    const bool ok = link<V, W, RESET>(sh, x, t.n, g.tiles, base, g.cols, start, ch, t.ticket);
     if (threadIdx.x % 32 == 0) ptx::mbar_arrive(&fd.done[s]);
     if (!ok) return;
   }
@@ -872,9 +865,9 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
       report_timeout(ch.status, KID_GATED_LINEAR, 0xFFFF);
       return;
     }
-    const int ticket = fd.ticket[s];
-    if (ticket < 0) return;
-    const TmaTile<V> at(ticket, g);
+    const TileAt at = fd.tile[s];
+    if (at.ticket < 0) return;
+    const int i = at.group * (32 * V) + lane * V;
     const int t0 = at.n * ROWS + w * FL, steps = p.T - t0;
     const uint32_t row = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * FL * ROW_BYTES + lane * 4);
     const uint32_t cut = RESET ? reset_bits<FL>(p, t0, at.b) : 0;
@@ -905,14 +898,14 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
       return;
     }
     if (p.saved != nullptr && t0 % GL_CHUNK == 0 && steps > 0)
-      write_state<V>(p.saved + (long)(t0 / GL_CHUNK) * p.B * p.d, at.b, at.i, p.d, h);
+      write_state<V>(p.saved + (long)(t0 / GL_CHUNK) * p.B * p.d, at.b, i, p.d, h);
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
       if (RESET) h = unless(cut >> l & 1, h);
       h = vfma(u[l], vsub(word_at<T, V>(row + TENSOR + l * ROW_BYTES), h), h);
       word_to<T, V>(row + l * ROW_BYTES, vmul(h, zs[l]));
     }
-    if (steps > 0 && steps <= FL) write_state<V>(p.h_last, at.b, at.i, p.d, h);
+    if (steps > 0 && steps <= FL) write_state<V>(p.h_last, at.b, i, p.d, h);
     ptx::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(&fd.done[s]);
@@ -963,13 +956,13 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
       report_timeout(ch.status, KID_GATED_LINEAR, 0xFFFF);
       return;
     }
-    const int ticket = fd.ticket[s];
-    if (ticket < 0) return;
-    const TmaTile<V> at(ticket, g);
+    const TileAt at = fd.tile[s];
+    if (at.ticket < 0) return;
+    const int i = at.group * (32 * V) + lane * V;
     const int chunk = g.tiles - 1 - at.n, t0 = chunk * ROWS + w * BL, steps = p.T - t0;
     const uint32_t row = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * BL * ROW_BYTES + lane * 4);
     const uint32_t cut = RESET ? reset_bits<BL>(p, t0, at.b) : 0;
-    F h = read_state<V>(p.saved + (long)chunk * p.B * p.d, at.b, at.i, p.d);
+    F h = read_state<V>(p.saved + (long)chunk * p.B * p.d, at.b, i, p.d);
     F u[BL], a[BL];
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
@@ -993,12 +986,11 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
 #pragma unroll
     for (int v = 0; v < V; ++v) ahead[w][lane * V + v] = Pair{R.get(v), H.get(v)};
     asm volatile("bar.sync 3, %0;" ::"n"(32 * BW) : "memory");
+#pragma unroll 1
+    for (int k = 0; k < w; ++k) {
 #pragma unroll
-    for (int k = 0; k < BW - 1; ++k)
-      if (k < w) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) h.set(v, pass<RESET>(h.get(v), ahead[k][lane * V + v]));
-      }
+      for (int v = 0; v < V; ++v) h.set(v, pass<RESET>(h.get(v), ahead[k][lane * V + v]));
+    }
     F q[BL];                              // a becomes (p - c) u (1 - u): df = g a
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
@@ -1037,7 +1029,7 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
       D = vsub(gt, gu);
       if (RESET) D = unless(cut >> l & 1, D);
     }
-    if (t0 == 0) write_state<V>(p.dh0, at.b, at.i, p.d, D);
+    if (t0 == 0) write_state<V>(p.dh0, at.b, i, p.d, D);
     ptx::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(&fd.done[s]);
