@@ -6,6 +6,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <initializer_list>
 #include <mutex>
 
 #include "common.cuh"
@@ -1698,6 +1699,12 @@ int elman_adamw_step(int dtype, long n, void* params, const void* grads, void* e
 // ---------------------------------------------------------------------------
 // gated linear recurrence
 // ---------------------------------------------------------------------------
+// Every pointer lies on a boundary of its elements.
+static bool on_elements(int dtype, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (((uintptr_t)p & (esize(dtype) - 1)) != 0) return false;
+  return true;
+}
 // No two elements of a [T, B, d] output may share an address.
 static bool distinct_elements(int T, int B, int d, const long* s) {
   if (T > 1 && s[0] < d) return false;
@@ -1734,6 +1741,7 @@ int elman_gated_linear_forward(int dtype, int training, int T, int B, int d, con
   if (T > 0) {
     REQUIRE_PTR(f); REQUIRE_PTR(c); REQUIRE_PTR(z); REQUIRE_PTR(y);
     if (training) REQUIRE_PTR(saved);
+    ELMAN_ARG_CHECK(on_elements(dtype, {f, c, z, y}), "misaligned tensor");
   }
   const size_t need = gated_linear_workspace(dtype, T, B, d);
   if (need > 0) REQUIRE_PTR(workspace);
@@ -1759,6 +1767,7 @@ int elman_gated_linear_backward(int dtype, int T, int B, int d, const void* f, c
   if (T > 0) {
     REQUIRE_PTR(f); REQUIRE_PTR(c); REQUIRE_PTR(z); REQUIRE_PTR(saved); REQUIRE_PTR(d_output);
     REQUIRE_PTR(df); REQUIRE_PTR(dc); REQUIRE_PTR(dz);
+    ELMAN_ARG_CHECK(on_elements(dtype, {f, c, z, d_output, df, dc, dz}), "misaligned tensor");
   }
   const size_t need = gated_linear_workspace(dtype, T, B, d);
   if (need > 0) REQUIRE_PTR(workspace);

@@ -617,18 +617,25 @@ __global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p
 }
 
 // ---------------------------------------------------------------------------
-// The same tiles fed by TMA, for tensors whose base and row strides are multiples of 16 bytes: the next
-// tile's rows arrive in one shared-memory stage while this tile is scanned from the other, so the loads
-// never pause for the arithmetic, and results leave from the stage as bulk stores.  One producer thread
-// takes tiles from the counter, loads, and stores; the other warps scan.  A lane owns the same 4-byte
-// word of every row (two bf16 channels or one fp32 channel) throughout, so results overwrite the inputs
-// that made them.  A tile lies within one batch row; rows past T and channels past d are zero-filled
-// and clipped by the copies.
+// The same tiles fed by asynchronous copies: the next tile's rows arrive in one shared-memory stage while
+// this tile is scanned from the other, so the loads never pause for the arithmetic.  A producer takes
+// tiles from the counter and loads them; the other warps scan and link.  A tile lies within one batch row.
+//
+// FEED_TMA, for tensors whose base and row strides are multiples of 16 bytes: a box a tensor, rows past T and
+// channels past d zero-filled; a lane owns the same 4-byte word of every row (two bf16 channels or one
+// fp32 channel), results overwrite the inputs that made them and leave as bulk stores.
+// FEED_ROWS4 and FEED_ROWS2, for all others, by what their rows' starts are multiples of: a copy a row, of the
+// 16-byte blocks it touches, read at the row's own offset in them; results go out by plain stores.
 // ---------------------------------------------------------------------------
 constexpr int ROW_BYTES = 128;
-template <int IN, int ROWS> struct Stages {
-  static constexpr int TENSOR = ROWS * ROW_BYTES, STAGE = IN * TENSOR, BYTES = 2 * STAGE + 128;   // + alignment
+enum FeedKind { FEED_TMA, FEED_ROWS4, FEED_ROWS2 };
+constexpr int pitch_of(int feed) { return feed == FEED_TMA ? ROW_BYTES : ROW_BYTES + 16; }
+template <int IN, int ROWS, int FEED> struct Stages {
+  static constexpr int TENSOR = ROWS * pitch_of(FEED), STAGE = IN * TENSOR, BYTES = 2 * STAGE + 128;   // + alignment
 };
+// Scanning warps of the forward tile (16 steps each; two stages of longer rows leave room for seven).
+constexpr int forward_warps(int feed) { return feed == FEED_TMA ? FW : 7; }
+constexpr int producer_threads(int feed) { return feed == FEED_TMA ? 32 : 64; }
 struct GlTma {
   int tiles, groups_per_row, total;   // tiles in time; channel groups of a batch row; all tiles
   long cols;                          // channels as the chain counts them: whole groups
@@ -646,7 +653,7 @@ template <int IN, int OUT, int ROWS>
 __device__ __forceinline__ void produce(Feed& fd, uint8_t* smem, const CUtensorMap* const (&in)[IN],
                                         const CUtensorMap* const (&out)[OUT], int channels, bool backward,
                                         const GlTma& g, const GlChain& ch) {
-  constexpr int TENSOR = Stages<IN, ROWS>::TENSOR, STAGE = Stages<IN, ROWS>::STAGE;
+  constexpr int TENSOR = Stages<IN, ROWS, FEED_TMA>::TENSOR, STAGE = Stages<IN, ROWS, FEED_TMA>::STAGE;
   volatile int* gave_up = &fd.gave_up;
   TileAt tile[2] = {{-1, 0, 0, 0}, {-1, 0, 0, 0}};
   const int per_time = g.total / g.tiles;
@@ -694,6 +701,67 @@ __device__ __forceinline__ void produce(Feed& fd, uint8_t* smem, const CUtensorM
   tch::bulk_wait_read_all();
 }
 
+// The two producer warps for rows of any alignment: 16-byte copies of the blocks a row touches (eight, or nine), a
+// warp every second four rows.  (A bulk copy a row was measured too: three times slower, some 50 cycles each.)
+template <typename T, int V, int IN, int ROWS, int FEED>
+__device__ __forceinline__ void produce_rows(Feed& fd, uint8_t* smem, const void* const (&in)[IN], const Strides (&st)[IN], int which,
+                                             const GlParams& p, bool backward, const GlTma& g, const GlChain& ch) {
+  constexpr int PITCH = pitch_of(FEED), TENSOR = Stages<IN, ROWS, FEED>::TENSOR, STAGE = Stages<IN, ROWS, FEED>::STAGE;
+  static_assert(ROWS % 8 == 0, "four rows a warp in turn");
+  volatile int* gave_up = &fd.gave_up;
+  const int lane = threadIdx.x & 31, per_time = g.total / g.tiles;
+  for (int it = 0;; ++it) {
+    const int s = it & 1;
+    if (which == 0 && lane == 0) {
+      TileAt t{-1, 0, 0, 0};
+      if (it >= 2 && !ptx::mbar_wait(&fd.done[s], (uint32_t)((it >> 1) - 1) & 1u, ch.spin_limit * 8, gave_up)) {
+        t.ticket = -2;                              // given up: nobody waits for the stage any more
+      } else {
+        const uint32_t next = g.tiles > 1 ? atomicAdd(ch.ctrl, 1u) + 1u : (uint32_t)(it == 0 ? blockIdx.x : g.total);
+        if (next < (uint32_t)g.total) {
+          t.ticket = (int)next;
+          t.n = t.ticket / per_time;
+          const int column = t.ticket - t.n * per_time;
+          t.b = column / g.groups_per_row;
+          t.group = column - t.b * g.groups_per_row;
+        }
+      }
+      fd.tile[s] = t;
+    }
+    asm volatile("bar.sync 4, 64;" ::: "memory");
+    const TileAt t = fd.tile[s];
+    if (t.ticket >= 0) {
+      const int row0 = (backward ? g.tiles - 1 - t.n : t.n) * ROWS, i0 = t.group * (32 * V);
+      const int rows = p.T - row0 < ROWS ? p.T - row0 : ROWS;
+      const uintptr_t width = (uintptr_t)((p.d - i0 < 32 * V ? p.d - i0 : 32 * V) * (int)sizeof(T));
+#pragma unroll
+      for (int k = 0; k < IN; ++k) {
+        const long step = st[k].t * (long)sizeof(T);
+        const uintptr_t first = (uintptr_t)in[k] + (uintptr_t)((long)row0 * step + (t.b * st[k].b + i0) * (long)sizeof(T));
+        const uint32_t to = ptx::smem_u32(smem + s * STAGE + k * TENSOR);
+        auto copy = [&](int r, int block) {         // one 16-byte block of row r, if the row reaches into it
+          const uintptr_t start = first + (uintptr_t)((long)r * step), from = (start & ~(uintptr_t)15) + 16u * block;
+          if (r < rows && from < start + width)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + r * PITCH + 16 * block), "l"(from) : "memory");
+        };
+#pragma unroll 4
+        for (int r = 4 * which + (lane >> 3); r < ROWS; r += 8) copy(r, lane & 7);
+        for (int r = 32 * which + lane; r < ROWS; r += 64) copy(r, 8);
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ptx::smem_u32(&fd.full[s])) : "memory");
+      if (which == 0 && lane == 0) ptx::mbar_arrive(&fd.full[s]);       // what it wrote of the tile is visible
+    } else {
+      if (t.ticket == -1) {
+        ptx::mbar_arrive(&fd.full[s]);
+        if (which == 0 && lane == 0) ptx::mbar_arrive(&fd.full[s]);
+      }
+      break;
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+constexpr int full_arrivals(int feed) { return feed == FEED_TMA ? 1 : 65; }
+
 // V channels of a state [B, d] from channel i on.
 template <int V> __device__ __forceinline__ Vec<V> read_state(const float* from, int b, int i, int d) {
   Vec<V> x(0.f);
@@ -710,25 +778,87 @@ template <int V> __device__ __forceinline__ void write_state(float* to, int b, i
   for (int v = 0; v < V; ++v)
     if (i + v < d) to[v] = x.get(v);
 }
-template <typename T, int V> __device__ __forceinline__ Vec<V> word_at(uint32_t addr) {
+__device__ __forceinline__ uint32_t lds_word(uint32_t addr) {
   uint32_t w;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(addr));
+  return w;
+}
+__device__ __forceinline__ void sts_word(uint32_t addr, uint32_t w) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(w) : "memory");
+}
+template <typename T, int V> __device__ __forceinline__ Vec<V> from_word(uint32_t w) {
   typename Lane<T, V>::Raw r;
   memcpy(&r, &w, 4);
   return Lane<T, V>::get(r);
 }
-template <typename T, int V> __device__ __forceinline__ void word_to(uint32_t addr, Vec<V> x) {
+template <typename T, int V> __device__ __forceinline__ uint32_t to_word(Vec<V> x) {
   const typename Lane<T, V>::Raw r = Lane<T, V>::put(x);
   uint32_t w;
   memcpy(&w, &r, 4);
-  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(w) : "memory");
+  return w;
 }
+// A lane's words of a warp's rows of one tensor in a stage.
+template <typename T, int V, int FEED> struct RowsIn {
+  uint32_t at, low, step;            // low, step: where the rows start (their low bits count)
+  __device__ __forceinline__ RowsIn(uint32_t rows, const void* base, Strides s, int t0, int b, int i0) : at(rows + (threadIdx.x & 31) * 4) {
+    low = (uint32_t)(uintptr_t)base + (uint32_t)(((long)t0 * s.t + b * s.b + i0) * (long)sizeof(T));
+    step = (uint32_t)(s.t * (long)sizeof(T));
+  }
+  __device__ __forceinline__ uint32_t addr(int l) const {
+    return FEED == FEED_TMA ? at + l * ROW_BYTES : at + l * pitch_of(FEED) + ((low + l * step) & 15u);
+  }
+  __device__ __forceinline__ Vec<V> get(int l) const {
+    if constexpr (FEED == FEED_ROWS2)
+      return from_word<T, V>((uint32_t)tch::lds_u16(addr(l)) | (uint32_t)tch::lds_u16(addr(l) + 2) << 16);
+    else
+      return from_word<T, V>(lds_word(addr(l)));
+  }
+  // rows from `steps` on were not copied: zeros (a zero gate alone would not keep what is not a number out)
+  template <int L> __device__ __forceinline__ void clear_after(int steps) const {
+    if (FEED == FEED_TMA || steps >= L) return;
+#pragma unroll 1
+    for (int l = steps > 0 ? steps : 0; l < L; ++l) {
+      if constexpr (FEED == FEED_ROWS2) {
+        tch::sts_u16(addr(l), 0);
+        tch::sts_u16(addr(l) + 2, 0);
+      } else {
+        sts_word(addr(l), 0);
+      }
+    }
+  }
+};
+// Where a lane's results go: into the stage, or out.
+template <typename T, int V, int FEED> struct RowsOut {
+  uint32_t stage;
+  char* at;
+  long step;
+  int channels, steps;
+  __device__ __forceinline__ RowsOut(uint32_t rows, void* base, Strides s, int t0, int b, int i, int d, int steps_)
+      : stage(rows + (threadIdx.x & 31) * 4), steps(steps_) {
+    at = (char*)base + ((long)t0 * s.t + b * s.b + i) * (long)sizeof(T);
+    step = s.t * (long)sizeof(T);
+    channels = d - i;
+  }
+  __device__ __forceinline__ void put(int l, Vec<V> x) const {
+    const uint32_t w = to_word<T, V>(x);
+    if constexpr (FEED == FEED_TMA) {
+      sts_word(stage + l * ROW_BYTES, w);
+    } else if (l < steps && channels > 0) {
+      if constexpr (FEED == FEED_ROWS4) {
+        __stcs(reinterpret_cast<uint32_t*>(at + l * step), w);
+      } else {
+        __stcs(reinterpret_cast<unsigned short*>(at + l * step), (unsigned short)w);
+        if (channels > 1) __stcs(reinterpret_cast<unsigned short*>(at + l * step) + 1, (unsigned short)(w >> 16));
+      }
+    }
+  }
+};
 
-// What the warps of a TMA block share.  The scanning warps leave their pairs (barrier 1, where they only
+// What the warps of such a block share.  The scanning warps leave their pairs (barrier 1, where they only
 // arrive), warps of their own link the tile into the chain, one thread per channel, and hand back the
 // state that enters each scanning warp (barrier 2).  Meanwhile the scanning warps work on what needs no
-// state.  (The general kernel below 128-bit rows folds in the scanning warps: the pass over the pairs was
-// a third of the instructions of the backward tile.)
+// state.  (Where the scanning warps folded the pairs themselves, that was a third of the backward tile's
+// instructions.)
 template <int V, int W> struct Links {
   Pair own[W][32 * V];             // the warps' pairs, in the scan's direction
   float enters[W][32 * V];         // state that enters each warp
@@ -820,18 +950,17 @@ __device__ __forceinline__ void link_tiles(Links<V, W>& sh, Feed& fd, const GlPa
   }
 }
 
-constexpr int TMA_THREADS_EXTRA = 32;     // the producer's warp, after the linking ones
 
-template <typename T, int V, bool RESET>
-__global__ void __launch_bounds__(32 * (FW + V) + TMA_THREADS_EXTRA, 2)
-gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_constant__ CUtensorMap tc,
+template <typename T, int V, bool RESET, int FEED>
+__global__ void __launch_bounds__(32 * (forward_warps(FEED) + V) + producer_threads(FEED), 2)
+gl_forward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_constant__ CUtensorMap tc,
                       const __grid_constant__ CUtensorMap tz, const __grid_constant__ CUtensorMap ty, GlParams p,
                       GlChain ch, GlTma g) {
   typedef Vec<V> F;
   static_assert(32 * V * sizeof(T) == ROW_BYTES, "a lane owns 4 bytes of a row");
-  constexpr int ROWS = FW * FL, TENSOR = Stages<3, ROWS>::TENSOR, STAGE = Stages<3, ROWS>::STAGE;
+  constexpr int W = forward_warps(FEED), ROWS = W * FL, TENSOR = Stages<3, ROWS, FEED>::TENSOR, STAGE = Stages<3, ROWS, FEED>::STAGE;
   extern __shared__ uint8_t raw[];
-  __shared__ Links<V, FW> sh;
+  __shared__ Links<V, W> sh;
   __shared__ Feed fd;
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 127) & ~(uintptr_t)127);
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -839,22 +968,26 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
     sh.gave_up = 0;
     fd.gave_up = 0;
     for (int s = 0; s < 2; ++s) {
-      ptx::mbar_init(&fd.full[s], 1);
-      ptx::mbar_init(&fd.done[s], FW + V);
+      ptx::mbar_init(&fd.full[s], full_arrivals(FEED));
+      ptx::mbar_init(&fd.done[s], W + V);
     }
     ptx::mbar_fence_init();
   }
   __syncthreads();
-  if (w == FW + V) {
-    if (lane == 0) {
+  if (w >= W + V) {
+    if constexpr (FEED != FEED_TMA) {
+      const void* const in[3] = {p.f, p.c, p.z};
+      const Strides st[3] = {p.sf, p.sc, p.sz};
+      produce_rows<T, V, 3, ROWS, FEED>(fd, smem, in, st, w - (W + V), p, false, g, ch);
+    } else if (lane == 0) {
       const CUtensorMap* const in[3] = {&tf, &tc, &tz};
       const CUtensorMap* const out[1] = {&ty};
       produce<3, 1, ROWS>(fd, smem, in, out, 32 * V, false, g, ch);
     }
     return;
   }
-  if (w >= FW) {
-    link_tiles<V, FW, RESET>(sh, fd, p, ch, g, p.h0);
+  if (w >= W) {
+    link_tiles<V, W, RESET>(sh, fd, p, ch, g, p.h0);
     return;
   }
   for (int it = 0;; ++it) {
@@ -869,11 +1002,16 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
     if (at.ticket < 0) return;
     const int i = at.group * (32 * V) + lane * V;
     const int t0 = at.n * ROWS + w * FL, steps = p.T - t0;
-    const uint32_t row = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * FL * ROW_BYTES + lane * 4);
+    const uint32_t rows = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * FL * pitch_of(FEED));
+    const RowsIn<T, V, FEED> f(rows, p.f, p.sf, t0, at.b, i - lane * V), c(rows + TENSOR, p.c, p.sc, t0, at.b, i - lane * V),
+        z(rows + 2 * TENSOR, p.z, p.sz, t0, at.b, i - lane * V);
+    f.template clear_after<FL>(steps);
+    c.template clear_after<FL>(steps);
+    z.template clear_after<FL>(steps);
     const uint32_t cut = RESET ? reset_bits<FL>(p, t0, at.b) : 0;
     F u[FL], zs[FL], e;
 #pragma unroll
-    for (int l = 0; l < FL; ++l) u[l] = gate_of(vmul(word_at<T, V>(row + l * ROW_BYTES), F(LOG2E)), e);
+    for (int l = 0; l < FL; ++l) u[l] = gate_of(vmul(f.get(l), F(LOG2E)), e);
     if (steps < FL) {
 #pragma unroll
       for (int l = 0; l < FL; ++l)
@@ -883,27 +1021,28 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
       if (RESET) H = unless(cut >> l & 1, H);
-      H = vfma(u[l], vsub(word_at<T, V>(row + TENSOR + l * ROW_BYTES), H), H);
+      H = vfma(u[l], vsub(c.get(l), H), H);
       R = vfma(u[l], vsub(F(1.f), R), R);
     }
     if (RESET && cut) R = F(-1.f);
-    leave_pair<V, FW>(sh, w, R, H);
+    leave_pair<V, W>(sh, w, R, H);
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
-      const F z = word_at<T, V>(row + 2 * TENSOR + l * ROW_BYTES);
-      zs[l] = vmul(z, gate_of(vmul(z, F(-LOG2E)), e));
+      const F x = z.get(l);
+      zs[l] = vmul(x, gate_of(vmul(x, F(-LOG2E)), e));
     }
-    if (!take_state<V, FW>(sh, w, h)) {
+    if (!take_state<V, W>(sh, w, h)) {
       fd.gave_up = 1;
       return;
     }
+    const RowsOut<T, V, FEED> y(rows, p.y, p.sy, t0, at.b, i, p.d, steps);
     if (p.saved != nullptr && t0 % GL_CHUNK == 0 && steps > 0)
       write_state<V>(p.saved + (long)(t0 / GL_CHUNK) * p.B * p.d, at.b, i, p.d, h);
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
       if (RESET) h = unless(cut >> l & 1, h);
-      h = vfma(u[l], vsub(word_at<T, V>(row + TENSOR + l * ROW_BYTES), h), h);
-      word_to<T, V>(row + l * ROW_BYTES, vmul(h, zs[l]));
+      h = vfma(u[l], vsub(c.get(l), h), h);
+      y.put(l, vmul(h, zs[l]));
     }
     if (steps > 0 && steps <= FL) write_state<V>(p.h_last, at.b, i, p.d, h);
     ptx::fence_proxy_async_smem();
@@ -912,14 +1051,14 @@ gl_forward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
   }
 }
 
-template <typename T, int V, bool RESET>
-__global__ void __launch_bounds__(32 * (BW + V) + TMA_THREADS_EXTRA, 2)
-gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_constant__ CUtensorMap tc,
+template <typename T, int V, bool RESET, int FEED>
+__global__ void __launch_bounds__(32 * (BW + V) + producer_threads(FEED), 2)
+gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_constant__ CUtensorMap tc,
                        const __grid_constant__ CUtensorMap tz, const __grid_constant__ CUtensorMap tdy,
                        const __grid_constant__ CUtensorMap tdf, const __grid_constant__ CUtensorMap tdc,
                        const __grid_constant__ CUtensorMap tdz, GlParams p, GlChain ch, GlTma g) {
   typedef Vec<V> F;
-  constexpr int ROWS = BW * BL, TENSOR = Stages<4, ROWS>::TENSOR, STAGE = Stages<4, ROWS>::STAGE;
+  constexpr int ROWS = BW * BL, TENSOR = Stages<4, ROWS, FEED>::TENSOR, STAGE = Stages<4, ROWS, FEED>::STAGE;
   extern __shared__ uint8_t raw[];
   __shared__ Links<V, BW> sh;
   __shared__ Pair ahead[BW][32 * V];
@@ -930,14 +1069,18 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
     sh.gave_up = 0;
     fd.gave_up = 0;
     for (int s = 0; s < 2; ++s) {
-      ptx::mbar_init(&fd.full[s], 1);
+      ptx::mbar_init(&fd.full[s], full_arrivals(FEED));
       ptx::mbar_init(&fd.done[s], BW + V);
     }
     ptx::mbar_fence_init();
   }
   __syncthreads();
-  if (w == BW + V) {
-    if (lane == 0) {
+  if (w >= BW + V) {
+    if constexpr (FEED != FEED_TMA) {
+      const void* const in[4] = {p.f, p.c, p.z, p.dy};
+      const Strides st[4] = {p.sf, p.sc, p.sz, p.sy};
+      produce_rows<T, V, 4, ROWS, FEED>(fd, smem, in, st, w - (BW + V), p, true, g, ch);
+    } else if (lane == 0) {
       const CUtensorMap* const in[4] = {&tf, &tc, &tz, &tdy};
       const CUtensorMap* const out[3] = {&tdf, &tdc, &tdz};
       produce<4, 3, ROWS>(fd, smem, in, out, 32 * V, true, g, ch);
@@ -960,14 +1103,20 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
     if (at.ticket < 0) return;
     const int i = at.group * (32 * V) + lane * V;
     const int chunk = g.tiles - 1 - at.n, t0 = chunk * ROWS + w * BL, steps = p.T - t0;
-    const uint32_t row = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * BL * ROW_BYTES + lane * 4);
+    const uint32_t rows = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * BL * pitch_of(FEED));
+    const RowsIn<T, V, FEED> f(rows, p.f, p.sf, t0, at.b, i - lane * V), c(rows + TENSOR, p.c, p.sc, t0, at.b, i - lane * V),
+        z(rows + 2 * TENSOR, p.z, p.sz, t0, at.b, i - lane * V), dy(rows + 3 * TENSOR, p.dy, p.sy, t0, at.b, i - lane * V);
+    f.template clear_after<BL>(steps);
+    c.template clear_after<BL>(steps);
+    z.template clear_after<BL>(steps);
+    dy.template clear_after<BL>(steps);
     const uint32_t cut = RESET ? reset_bits<BL>(p, t0, at.b) : 0;
     F h = read_state<V>(p.saved + (long)chunk * p.B * p.d, at.b, i, p.d);
     F u[BL], a[BL];
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
       F e;
-      u[l] = gate_of(held(vmul(word_at<T, V>(row + l * ROW_BYTES), F(LOG2E))), e);
+      u[l] = gate_of(held(vmul(f.get(l), F(LOG2E))), e);
       a[l] = vmul(vmul(e, u[l]), u[l]);
     }
     if (steps < BL) {
@@ -979,7 +1128,7 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
       if (RESET) H = unless(cut >> l & 1, H);
-      H = vfma(u[l], vsub(word_at<T, V>(row + TENSOR + l * ROW_BYTES), H), H);
+      H = vfma(u[l], vsub(c.get(l), H), H);
       R = vfma(u[l], vsub(F(1.f), R), R);
     }
     if (RESET && cut) R = F(-1.f);
@@ -991,18 +1140,19 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
 #pragma unroll
       for (int v = 0; v < V; ++v) h.set(v, pass<RESET>(h.get(v), ahead[k][lane * V + v]));
     }
+    const RowsOut<T, V, FEED> dz(rows + 2 * TENSOR, p.dz, p.sdz, t0, at.b, i, p.d, steps);
     F q[BL];                              // a becomes (p - c) u (1 - u): df = g a
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
       if (RESET) h = unless(cut >> l & 1, h);
-      const F prev = vsub(h, word_at<T, V>(row + TENSOR + l * ROW_BYTES));
+      const F prev = vsub(h, c.get(l));
       a[l] = vmul(a[l], prev);
       h = vsub(h, vmul(u[l], prev));
-      const F z = word_at<T, V>(row + 2 * TENSOR + l * ROW_BYTES), dy = word_at<T, V>(row + 3 * TENSOR + l * ROW_BYTES);
+      const F x = z.get(l), gy = dy.get(l);
       F e;
-      const F sg = gate_of(vmul(z, F(-LOG2E)), e), zs = vmul(z, sg);
-      q[l] = vmul(dy, zs);
-      word_to<T, V>(row + 2 * TENSOR + l * ROW_BYTES, vmul(vmul(dy, h), vfma(zs, vsub(F(1.f), sg), sg)));
+      const F sg = gate_of(vmul(x, F(-LOG2E)), e), zs = vmul(x, sg);
+      q[l] = vmul(gy, zs);
+      dz.put(l, vmul(vmul(gy, h), vfma(zs, vsub(F(1.f), sg), sg)));
     }
     if (steps < BL) {
 #pragma unroll
@@ -1021,11 +1171,12 @@ gl_backward_tma_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
       fd.gave_up = 1;
       return;
     }
+    const RowsOut<T, V, FEED> df(rows, p.df, p.sdf, t0, at.b, i, p.d, steps), dc(rows + TENSOR, p.dc, p.sdc, t0, at.b, i, p.d, steps);
 #pragma unroll
     for (int l = BL - 1; l >= 0; --l) {
       const F gt = vadd(q[l], D), gu = vmul(gt, u[l]);
-      word_to<T, V>(row + l * ROW_BYTES, vmul(gt, a[l]));
-      word_to<T, V>(row + TENSOR + l * ROW_BYTES, gu);
+      df.put(l, vmul(gt, a[l]));
+      dc.put(l, gu);
       D = vsub(gt, gu);
       if (RESET) D = unless(cut >> l & 1, D);
     }
@@ -1073,12 +1224,11 @@ long whole_groups(int dtype, int d) {
   const int width = dtype == ELMAN_F32 ? 32 : 64;
   return ((long)d + width - 1) / width * width;
 }
-// TMA copies need rows that start on 16 bytes; a batch row's last group should not be mostly empty.
-bool tma_width(int dtype, int d) { return whole_groups(dtype, d) <= d + d / 4; }
-bool tma_rows(int dtype, const GatedLinearArgs& a, bool bwd) {
-  if (!tma_width(dtype, a.d) || a.T > (1 << 30) || a.B > (1 << 30)) return false;
+// A batch row's last group should not be mostly empty: narrower rows go to the kernels that count channels through.
+bool whole_width(int dtype, int d) { return whole_groups(dtype, d) <= d + d / 4; }
+FeedKind feed_of(int dtype, const GatedLinearArgs& a, bool bwd) {
   const long per16 = dtype == ELMAN_F32 ? 4 : 8, most = (1L << 39) / 4;
-  bool ok = true;
+  bool ok = a.T <= (1 << 30) && a.B <= (1 << 30);
   auto see = [&](const void* base, const long* s) {
     ok = ok && ((uintptr_t)base & 15) == 0 && s[0] % per16 == 0 && s[0] < most &&
          (a.B <= 1 || (s[1] % per16 == 0 && s[1] > 0 && s[1] < most)) && s[0] > 0;
@@ -1086,7 +1236,7 @@ bool tma_rows(int dtype, const GatedLinearArgs& a, bool bwd) {
   see(a.f, a.f_strides); see(a.c, a.c_strides); see(a.z, a.z_strides);
   see(bwd ? a.dy : a.y, a.y_strides);
   if (bwd) { see(a.df, a.df_strides); see(a.dc, a.dc_strides); see(a.dz, a.dz_strides); }
-  return ok;
+  return ok ? FEED_TMA : dtype == ELMAN_F32 || pairs_of_channels(a, bwd) ? FEED_ROWS4 : FEED_ROWS2;
 }
 
 void prepare_chain(GlChain& ch, const GatedLinearArgs& a, int tiles, long cols) {
@@ -1100,11 +1250,11 @@ void prepare_chain(GlChain& ch, const GatedLinearArgs& a, int tiles, long cols) 
   ch.states = (float*)(ws + 256 + (size_t)tiles * cols * sizeof(float2));
 }
 
-template <typename T, int V, bool RESET>
-int launch_tma(int dtype, const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
+template <typename T, int V, bool RESET, int FEED>
+int launch_fed(int dtype, const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
   static std::mutex mutex;
   static bool sized[2][64];      // the kernel's shared-memory limit is set, per direction and device
-  const int rows = bwd ? BW * BL : FW * FL;
+  const int rows = bwd ? BW * BL : forward_warps(FEED) * FL;
   GlTma g{};
   g.tiles = tiles_of(a.T, rows);
   g.groups_per_row = (int)(whole_groups(dtype, a.d) / (32 * V));
@@ -1112,8 +1262,8 @@ int launch_tma(int dtype, const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
   ELMAN_ARG_CHECK(total + 148 * 8 < (1L << 31), "too many channels for one call");
   g.total = (int)total;
   g.cols = (long)g.groups_per_row * a.B * 32 * V;
-  const int smem = bwd ? Stages<4, BW * BL>::BYTES : Stages<3, FW * FL>::BYTES;
-  const void* kernel = bwd ? (const void*)&gl_backward_tma_kernel<T, V, RESET> : (const void*)&gl_forward_tma_kernel<T, V, RESET>;
+  const int smem = bwd ? Stages<4, BW * BL, FEED>::BYTES : Stages<3, forward_warps(FEED) * FL, FEED>::BYTES;
+  const void* kernel = bwd ? (const void*)&gl_backward_fed_kernel<T, V, RESET, FEED> : (const void*)&gl_forward_fed_kernel<T, V, RESET, FEED>;
   int dev = 0;
   ELMAN_CUDA_CHECK(cudaGetDevice(&dev));
   {
@@ -1124,18 +1274,21 @@ int launch_tma(int dtype, const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
     }
   }
   CUtensorMap m[7];
-  auto map = [&](int k, const void* base, const long* s) {
-    const uint64_t one = a.B > 1 ? s[1] : s[0];     // (a single batch row: any valid stride)
-    return make_tmap_3d(&m[k], dtype, base, a.d, a.B, a.T, one, s[0], 32 * V, 1, rows);
-  };
-  ELMAN_RETURN_IF(map(0, a.f, a.f_strides));
-  ELMAN_RETURN_IF(map(1, a.c, a.c_strides));
-  ELMAN_RETURN_IF(map(2, a.z, a.z_strides));
-  ELMAN_RETURN_IF(map(3, bwd ? a.dy : a.y, a.y_strides));
-  if (bwd) {
-    ELMAN_RETURN_IF(map(4, a.df, a.df_strides));
-    ELMAN_RETURN_IF(map(5, a.dc, a.dc_strides));
-    ELMAN_RETURN_IF(map(6, a.dz, a.dz_strides));
+  memset(m, 0, sizeof(m));
+  if (FEED == FEED_TMA) {
+    auto map = [&](int k, const void* base, const long* s) {
+      const uint64_t one = a.B > 1 ? s[1] : s[0];     // (a single batch row: any valid stride)
+      return make_tmap_3d(&m[k], dtype, base, a.d, a.B, a.T, one, s[0], 32 * V, 1, rows);
+    };
+    ELMAN_RETURN_IF(map(0, a.f, a.f_strides));
+    ELMAN_RETURN_IF(map(1, a.c, a.c_strides));
+    ELMAN_RETURN_IF(map(2, a.z, a.z_strides));
+    ELMAN_RETURN_IF(map(3, bwd ? a.dy : a.y, a.y_strides));
+    if (bwd) {
+      ELMAN_RETURN_IF(map(4, a.df, a.df_strides));
+      ELMAN_RETURN_IF(map(5, a.dc, a.dc_strides));
+      ELMAN_RETURN_IF(map(6, a.dz, a.dz_strides));
+    }
   }
   GlChain ch{};
   prepare_chain(ch, a, g.tiles, g.cols);
@@ -1143,9 +1296,9 @@ int launch_tma(int dtype, const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
   const GlParams p = params_of(a);
   const unsigned grid = (unsigned)(g.tiles > 1 && total > 148 * 2 ? 148 * 2 : total);
   if (bwd)
-    gl_backward_tma_kernel<T, V, RESET><<<grid, 32 * (BW + V) + TMA_THREADS_EXTRA, smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], p, ch, g);
+    gl_backward_fed_kernel<T, V, RESET, FEED><<<grid, 32 * (BW + V) + producer_threads(FEED), smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], p, ch, g);
   else
-    gl_forward_tma_kernel<T, V, RESET><<<grid, 32 * (FW + V) + TMA_THREADS_EXTRA, smem, st>>>(m[0], m[1], m[2], m[3], p, ch, g);
+    gl_forward_fed_kernel<T, V, RESET, FEED><<<grid, 32 * (forward_warps(FEED) + V) + producer_threads(FEED), smem, st>>>(m[0], m[1], m[2], m[3], p, ch, g);
   count_launch(false);
   ELMAN_CUDA_CHECK(cudaGetLastError());
   return ELMAN_OK;
@@ -1179,8 +1332,15 @@ int launch_tiles(const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
 
 template <bool RESET>
 int launch_tiles(int dtype, const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
-  if (tma_rows(dtype, a, bwd))
-    return dtype == ELMAN_F32 ? launch_tma<float, 1, RESET>(dtype, a, bwd, st) : launch_tma<bf16, 2, RESET>(dtype, a, bwd, st);
+  if (whole_width(dtype, a.d)) {
+    const FeedKind feed = feed_of(dtype, a, bwd);
+    if (dtype == ELMAN_F32)
+      return feed == FEED_TMA ? launch_fed<float, 1, RESET, FEED_TMA>(dtype, a, bwd, st)
+                              : launch_fed<float, 1, RESET, FEED_ROWS4>(dtype, a, bwd, st);
+    return feed == FEED_TMA     ? launch_fed<bf16, 2, RESET, FEED_TMA>(dtype, a, bwd, st)
+           : feed == FEED_ROWS4 ? launch_fed<bf16, 2, RESET, FEED_ROWS4>(dtype, a, bwd, st)
+                                : launch_fed<bf16, 2, RESET, FEED_ROWS2>(dtype, a, bwd, st);
+  }
   if (dtype == ELMAN_F32) return launch_tiles<float, 1, RESET>(a, bwd, st);
   if (pairs_of_channels(a, bwd)) return launch_tiles<bf16, 2, RESET>(a, bwd, st);
   return launch_tiles<bf16, 1, RESET>(a, bwd, st);
@@ -1216,7 +1376,7 @@ int gated_linear_bwd(int dtype, const GatedLinearArgs& a, cudaStream_t st) {
 
 size_t gated_linear_workspace(int dtype, int T, int B, int d) {
   // the backward pass has the shorter tiles
-  return T > SEQ_STEPS ? chain_bytes(tiles_of(T, BW * BL), B * (tma_width(dtype, d) ? whole_groups(dtype, d) : (long)d)) : 0;
+  return T > SEQ_STEPS ? chain_bytes(tiles_of(T, BW * BL), B * (whole_width(dtype, d) ? whole_groups(dtype, d) : (long)d)) : 0;
 }
 
 }  // namespace elman

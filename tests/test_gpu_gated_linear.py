@@ -103,7 +103,53 @@ def test_rows_on_16_bytes(T, B, d, reset, packed, batch_major, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("d", [128, 62, 61])
+@pytest.mark.parametrize("packed,batch_major", [(False, False), (True, False), (True, True)])
+@pytest.mark.parametrize("T,B,d,reset", [(9, 2, 63, None), (112, 1, 62, 0.05), (113, 3, 61, None), (200, 2, 1001, 0.01), (2100, 2, 126, None),
+                                         (5000, 1, 55, 0.002), (300, 9, 1279, None), (130, 2, 118, 0.02)])
+def test_rows_of_any_alignment(T, B, d, reset, packed, batch_major, dtype):
+    """The shapes whose rows are copied one by one: starts on 4 and on 2 bytes, changing from row to row."""
+    check(make(T, B, d, dtype, seed=T, packed=packed, batch_major=batch_major, reset=reset), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shift", [1, 2, 3, 5])
+def test_tensors_off_their_16_byte_boundary(shift, dtype):
+    """The same values from storages that start elsewhere, and outputs that leave their neighbours alone."""
+    T, B, d = 150, 2, 128
+    s = make(T, B, d, dtype, seed=12)
+    def moved(t):
+        room = torch.full((t.numel() + 64,), float("nan"), device="cuda", dtype=dtype)
+        room[16 + shift:16 + shift + t.numel()] = t.reshape(-1)
+        return room[16 + shift:16 + shift + t.numel()].view(t.shape)
+    f, c, z, dy = (moved(s[k]) for k in ("f", "c", "z", "dy"))
+    y, h, saved = H.gated_linear_forward(True, f, c, z, s["h0"])
+    want = H.gated_linear_forward(True, s["f"], s["c"], s["z"], s["h0"])
+    tol = TOL[dtype]
+    assert rel(y, want[0].cpu()) < 2 * tol and rel(h, want[1].cpu()) < 2 * STATE_TOL
+    outs = [torch.full((T * B * d + 64,), 7.0, device="cuda", dtype=dtype) for _ in range(3)]
+    views = tuple(o[16 + shift:16 + shift + T * B * d].view(T, B, d) for o in outs)
+    H.gated_linear_backward(f, c, z, saved, dy, out=views)
+    ref = H.gated_linear_backward(s["f"], s["c"], s["z"], want[2], s["dy"])
+    for o, v, r in zip(outs, views, ref):
+        assert rel(v, r.cpu()) < 2 * tol
+        assert (o[:16 + shift] == 7).all() and (o[16 + shift + T * B * d:] == 7).all()
+
+
+@pytest.mark.parametrize("T,d", [(200, 128), (200, 62), (200, 24)])
+def test_expanded_inputs(T, d):
+    """Inputs broadcast over time or batch (stride 0): full gradients come back."""
+    s = make(T, 3, d, torch.float32, seed=13)
+    f, c, z = s["f"][:1].expand(T, 3, d), s["c"][:, :1].expand(T, 3, d), s["z"]
+    y, h, saved = H.gated_linear_forward(True, f, c, z, s["h0"])
+    g = H.gated_linear_backward(f, c, z, saved, s["dy"], s["dh"])
+    y2, h2, saved2 = H.gated_linear_forward(True, f.contiguous(), c.contiguous(), z, s["h0"])
+    g2 = H.gated_linear_backward(f.contiguous(), c.contiguous(), z, saved2, s["dy"], s["dh"])
+    for a, b in zip([y, h] + g, [y2, h2] + g2):
+        assert rel(a, b.cpu()) < 2 * TOL[torch.float32]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [128, 62, 61, 40])
 def test_calls_on_two_streams_at_once(d, dtype):
     """Long chains in several launches that share the device: none waits for another's blocks."""
     sets = [make(3000, 4, d, dtype, seed=40 + k, reset=0.001) for k in range(3)]
