@@ -635,7 +635,10 @@ template <int IN, int ROWS, int FEED> struct Stages {
 };
 // Scanning warps of the forward tile (16 steps each; two stages of longer rows leave room for seven).
 constexpr int forward_warps(int feed) { return feed == FEED_TMA ? FW : 7; }
-constexpr int producer_threads(int feed) { return feed == FEED_TMA ? 32 : 64; }
+// Producer warps for rows copied in blocks: two channels a lane are short of registers (T4096 B16 d1001 bf16 forward 166 us
+// with one, 193 with two, 213 with four), one is not (fp32 289, 247, 217).
+constexpr int row_producers(int V) { return V == 2 ? 1 : 4; }
+constexpr int producer_threads(int feed, int V) { return feed == FEED_TMA ? 32 : 32 * row_producers(V); }
 struct GlTma {
   int tiles, groups_per_row, total;   // tiles in time; channel groups of a batch row; all tiles
   long cols;                          // channels as the chain counts them: whole groups
@@ -701,13 +704,12 @@ __device__ __forceinline__ void produce(Feed& fd, uint8_t* smem, const CUtensorM
   tch::bulk_wait_read_all();
 }
 
-// The two producer warps for rows of any alignment: 16-byte copies of the blocks a row touches (eight, or nine), a
-// warp every second four rows.  (A bulk copy a row was measured too: three times slower, some 50 cycles each.)
+// The producer warps for rows of any alignment: 16-byte copies of the blocks a row touches (eight, or nine), four rows
+// an instruction.  (A bulk copy a row was measured too: T777 B5 d1001 fp32 forward 53 us instead of 21.)
 template <typename T, int V, int IN, int ROWS, int FEED>
 __device__ __forceinline__ void produce_rows(Feed& fd, uint8_t* smem, const void* const (&in)[IN], const Strides (&st)[IN], int which,
                                              const GlParams& p, bool backward, const GlTma& g, const GlChain& ch) {
   constexpr int PITCH = pitch_of(FEED), TENSOR = Stages<IN, ROWS, FEED>::TENSOR, STAGE = Stages<IN, ROWS, FEED>::STAGE;
-  static_assert(ROWS % 8 == 0, "four rows a warp in turn");
   volatile int* gave_up = &fd.gave_up;
   const int lane = threadIdx.x & 31, per_time = g.total / g.tiles;
   for (int it = 0;; ++it) {
@@ -728,7 +730,7 @@ __device__ __forceinline__ void produce_rows(Feed& fd, uint8_t* smem, const void
       }
       fd.tile[s] = t;
     }
-    asm volatile("bar.sync 4, 64;" ::: "memory");
+    asm volatile("bar.sync 4, %0;" ::"n"(32 * row_producers(V)) : "memory");
     const TileAt t = fd.tile[s];
     if (t.ticket >= 0) {
       const int row0 = (backward ? g.tiles - 1 - t.n : t.n) * ROWS, i0 = t.group * (32 * V);
@@ -745,8 +747,8 @@ __device__ __forceinline__ void produce_rows(Feed& fd, uint8_t* smem, const void
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + r * PITCH + 16 * block), "l"(from) : "memory");
         };
 #pragma unroll 4
-        for (int r = 4 * which + (lane >> 3); r < ROWS; r += 8) copy(r, lane & 7);
-        for (int r = 32 * which + lane; r < ROWS; r += 64) copy(r, 8);
+        for (int r = 4 * which + (lane >> 3); r < ROWS; r += 4 * row_producers(V)) copy(r, lane & 7);
+        for (int r = 32 * which + lane; r < ROWS; r += 32 * row_producers(V)) copy(r, 8);
       }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ptx::smem_u32(&fd.full[s])) : "memory");
       if (which == 0 && lane == 0) ptx::mbar_arrive(&fd.full[s]);       // what it wrote of the tile is visible
@@ -760,7 +762,7 @@ __device__ __forceinline__ void produce_rows(Feed& fd, uint8_t* smem, const void
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
-constexpr int full_arrivals(int feed) { return feed == FEED_TMA ? 1 : 65; }
+constexpr int full_arrivals(int feed, int V) { return feed == FEED_TMA ? 1 : 32 * row_producers(V) + 1; }
 
 // V channels of a state [B, d] from channel i on.
 template <int V> __device__ __forceinline__ Vec<V> read_state(const float* from, int b, int i, int d) {
@@ -952,7 +954,7 @@ __device__ __forceinline__ void link_tiles(Links<V, W>& sh, Feed& fd, const GlPa
 
 
 template <typename T, int V, bool RESET, int FEED>
-__global__ void __launch_bounds__(32 * (forward_warps(FEED) + V) + producer_threads(FEED), 2)
+__global__ void __launch_bounds__(32 * (forward_warps(FEED) + V) + producer_threads(FEED, V), 2)
 gl_forward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_constant__ CUtensorMap tc,
                       const __grid_constant__ CUtensorMap tz, const __grid_constant__ CUtensorMap ty, GlParams p,
                       GlChain ch, GlTma g) {
@@ -968,7 +970,7 @@ gl_forward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
     sh.gave_up = 0;
     fd.gave_up = 0;
     for (int s = 0; s < 2; ++s) {
-      ptx::mbar_init(&fd.full[s], full_arrivals(FEED));
+      ptx::mbar_init(&fd.full[s], full_arrivals(FEED, V));
       ptx::mbar_init(&fd.done[s], W + V);
     }
     ptx::mbar_fence_init();
@@ -1052,7 +1054,7 @@ gl_forward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
 }
 
 template <typename T, int V, bool RESET, int FEED>
-__global__ void __launch_bounds__(32 * (BW + V) + producer_threads(FEED), 2)
+__global__ void __launch_bounds__(32 * (BW + V) + producer_threads(FEED, V), 2)
 gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_constant__ CUtensorMap tc,
                        const __grid_constant__ CUtensorMap tz, const __grid_constant__ CUtensorMap tdy,
                        const __grid_constant__ CUtensorMap tdf, const __grid_constant__ CUtensorMap tdc,
@@ -1069,7 +1071,7 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
     sh.gave_up = 0;
     fd.gave_up = 0;
     for (int s = 0; s < 2; ++s) {
-      ptx::mbar_init(&fd.full[s], full_arrivals(FEED));
+      ptx::mbar_init(&fd.full[s], full_arrivals(FEED, V));
       ptx::mbar_init(&fd.done[s], BW + V);
     }
     ptx::mbar_fence_init();
@@ -1224,8 +1226,9 @@ long whole_groups(int dtype, int d) {
   const int width = dtype == ELMAN_F32 ? 32 : 64;
   return ((long)d + width - 1) / width * width;
 }
-// A batch row's last group should not be mostly empty: narrower rows go to the kernels that count channels through.
-bool whole_width(int dtype, int d) { return whole_groups(dtype, d) <= d + d / 4; }
+// A batch row's last group should not be mostly empty: narrower rows go to the kernels that count channels through, which
+// reach about two thirds of the speed.
+bool whole_width(int dtype, int d) { return whole_groups(dtype, d) <= d + d / 2; }
 FeedKind feed_of(int dtype, const GatedLinearArgs& a, bool bwd) {
   const long per16 = dtype == ELMAN_F32 ? 4 : 8, most = (1L << 39) / 4;
   bool ok = a.T <= (1 << 30) && a.B <= (1 << 30);
@@ -1296,9 +1299,9 @@ int launch_fed(int dtype, const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
   const GlParams p = params_of(a);
   const unsigned grid = (unsigned)(g.tiles > 1 && total > 148 * 2 ? 148 * 2 : total);
   if (bwd)
-    gl_backward_fed_kernel<T, V, RESET, FEED><<<grid, 32 * (BW + V) + producer_threads(FEED), smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], p, ch, g);
+    gl_backward_fed_kernel<T, V, RESET, FEED><<<grid, 32 * (BW + V) + producer_threads(FEED, V), smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], p, ch, g);
   else
-    gl_forward_fed_kernel<T, V, RESET, FEED><<<grid, 32 * (forward_warps(FEED) + V) + producer_threads(FEED), smem, st>>>(m[0], m[1], m[2], m[3], p, ch, g);
+    gl_forward_fed_kernel<T, V, RESET, FEED><<<grid, 32 * (forward_warps(FEED) + V) + producer_threads(FEED, V), smem, st>>>(m[0], m[1], m[2], m[3], p, ch, g);
   count_launch(false);
   ELMAN_CUDA_CHECK(cudaGetLastError());
   return ELMAN_OK;
