@@ -883,12 +883,25 @@ def _sequence_like(x):
     """A dense [T, B, d] tensor in x's order of t and b (batch-major x: a view of a [B, T, d] one)."""
     T, B, d = x.shape
     if T > 1 and B > 1 and x.stride(0) < x.stride(1):
-        return torch.empty(B, T, d, dtype=x.dtype, device=x.device).transpose(0, 1)
-    return torch.empty(T, B, d, dtype=x.dtype, device=x.device)
+        return x.new_empty((B, T, d)).transpose(0, 1)
+    return x.new_empty((T, B, d))
 
 
 def _tb_strides(*tensors):
-    return array.array("l", [s for t in tensors for s in t.stride()[:2]])
+    flat = ()
+    for t in tensors:
+        flat += t.stride()[:2]
+    return array.array("l", flat)
+
+
+_NOTHING = {}     # per device: the empty tensor that inference returns in place of saved states
+
+
+def _nothing(device):
+    empty = _NOTHING.get(device)
+    if empty is None:
+        empty = _NOTHING[device] = torch.empty(0, dtype=torch.float32, device=device)
+    return empty
 
 
 def gated_linear_forward(training, f, c, z, h0=None, reset=None):
@@ -901,15 +914,17 @@ def gated_linear_forward(training, f, c, z, h0=None, reset=None):
     fn = "gated_linear_forward"
     dt = _check_sequences(fn, f, f=f, c=c, z=z)
     T, B, d = f.shape
-    _check_state(fn, h0, "h0", (B, d), f.device)
-    _check_reset(fn, reset, T, B, f.device)
-    lib = _lib.load()
     device = f.device
+    if h0 is not None:
+        _check_state(fn, h0, "h0", (B, d), device)
+    if reset is not None:
+        _check_reset(fn, reset, T, B, device)
+    lib = _lib.load()
     with _on(device):
         y = _sequence_like(f)
         h_last = torch.empty(B, d, dtype=torch.float32, device=device)
-        rows = -(-T // GATED_LINEAR_CHUNK) if training else 0
-        saved = torch.empty((rows, B, d) if training else (0,), dtype=torch.float32, device=device)
+        saved = torch.empty(-(-T // GATED_LINEAR_CHUNK), B, d, dtype=torch.float32, device=device) if training \
+            else _nothing(device)
         need = lib.elman_gated_linear_workspace(dt, T, B, d)
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
         strides = _tb_strides(f, c, z, y)
