@@ -1713,6 +1713,23 @@ static bool distinct_elements(int T, int B, int d, const long* s) {
   return s[0] >= (B - 1) * s[1] + d || s[1] >= (T - 1) * s[0] + d;
 }
 
+// Two outputs of equal sizes are apart: one behind the other, or slices of the same rows.
+static bool outputs_apart(int dtype, int T, int B, int d, const void* x, const long* sx, const void* y, const long* sy) {
+  if ((uintptr_t)x > (uintptr_t)y) return outputs_apart(dtype, T, B, d, y, sy, x, sx);
+  const unsigned long delta = ((uintptr_t)y - (uintptr_t)x) / esize(dtype);
+  if (delta >= (unsigned long)((T - 1) * sx[0] + (B - 1) * sx[1] + d)) return true;
+  if ((T > 1 && sx[0] != sy[0]) || (B > 1 && sx[1] != sy[1])) return false;
+  if (T <= 1 && B <= 1) return false;
+  long row = T > 1 ? sx[0] : sx[1];
+  if (T > 1 && B > 1) {
+    const long other = sx[1];
+    if (row > other ? row % other != 0 : other % row != 0) return false;
+    if (other < row) row = other;
+  }
+  const long at = (long)(delta % (unsigned long)row);
+  return at >= d && row - at >= d;
+}
+
 static int check_gated_linear(int dtype, int T, int B, int d, const long* strides, int n_in, int n_out) {
   ELMAN_RETURN_IF(check_common(dtype, T, B, d));
   REQUIRE_PTR(strides);
@@ -1768,6 +1785,9 @@ int elman_gated_linear_backward(int dtype, int T, int B, int d, const void* f, c
     REQUIRE_PTR(f); REQUIRE_PTR(c); REQUIRE_PTR(z); REQUIRE_PTR(saved); REQUIRE_PTR(d_output);
     REQUIRE_PTR(df); REQUIRE_PTR(dc); REQUIRE_PTR(dz);
     ELMAN_ARG_CHECK(on_elements(dtype, {f, c, z, d_output, df, dc, dz}), "misaligned tensor");
+    ELMAN_ARG_CHECK(outputs_apart(dtype, T, B, d, df, strides + 8, dc, strides + 10) &&
+                        outputs_apart(dtype, T, B, d, df, strides + 8, dz, strides + 12) &&
+                        outputs_apart(dtype, T, B, d, dc, strides + 10, dz, strides + 12), "df, dc and dz overlap");
   }
   const size_t need = gated_linear_workspace(dtype, T, B, d);
   if (need > 0) REQUIRE_PTR(workspace);

@@ -110,7 +110,6 @@ __global__ void __launch_bounds__(128) gl_backward_seq_kernel(GlParams p) {
   p.dh0[col] = D;
 }
 
-
 // ---------------------------------------------------------------------------
 // Sequences of more than a few steps: tiles of (W warps x L steps) x (32 V channels), each read once.
 //
@@ -951,7 +950,6 @@ __device__ __forceinline__ void link_tiles(Links<V, W>& sh, Feed& fd, const GlPa
     if (!ok) return;
   }
 }
-
 
 template <typename T, int V, bool RESET, int FEED>
 __global__ void __launch_bounds__(32 * (forward_warps(FEED) + V) + producer_threads(FEED, V), 2)

@@ -978,16 +978,16 @@ int make_tmap_bf16_sw128(CUtensorMap* out, const void* base, uint64_t rows, uint
 }
 
 int make_tmap_f16(CUtensorMap* out, const void* base, uint64_t cols, uint64_t rows, uint64_t count, uint64_t ld,
-                  uint64_t stride, uint32_t box_cols, uint32_t box_rows) {
+                  uint64_t stride, uint32_t box_rows) {
   EncodeTiledFn fn = get_encode_fn();
   if (fn == nullptr)
     return set_error(ELMAN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint64_t dims[3] = {cols, rows, count};
   cuuint64_t strides[2] = {ld * 2, stride * 2};
-  cuuint32_t box[3] = {box_cols, box_rows, 1};
+  cuuint32_t box[3] = {64, box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult rc = fn(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (rc != CUDA_SUCCESS)
     return set_error(ELMAN_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for [%llu x %llu x %llu]", (int)rc,

@@ -371,7 +371,6 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
   constexpr int EDGE = PAIR ? 256 : 128, BLOCKS = PAIR ? 2 : 1;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2], tk_full[TICKETS], tk_empty[TICKETS], go[TICKETS];
-
   __shared__ NsSlot tk[TICKETS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -863,8 +862,8 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
     for (int low = 0; low < 2; ++low) {
       const __half* base = low && x.lo != nullptr ? x.lo : x.hi;
       const uint64_t all = (uint64_t)rows * ld;
-      ELMAN_RETURN_IF(make_tmap_f16(&out.rows[low], base, cols, rows, p.count, ld, all, 64, 128));
-      ELMAN_RETURN_IF(make_tmap_f16(&out.block[low], base, cols, rows, p.count, ld, all, 64, 64));
+      ELMAN_RETURN_IF(make_tmap_f16(&out.rows[low], base, cols, rows, p.count, ld, all, 128));
+      ELMAN_RETURN_IF(make_tmap_f16(&out.block[low], base, cols, rows, p.count, ld, all, 64));
     }
     return (int)ELMAN_OK;
   };

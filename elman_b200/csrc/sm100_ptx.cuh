@@ -396,9 +396,9 @@ __device__ __forceinline__ bool elect_one() {
 int make_tmap_bf16_sw128(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols,
                          uint64_t ld, uint32_t box_rows);
 // 3D fp16 tensor map over `count` row-major matrices [rows, cols] of row stride `ld` and matrix stride `stride`
-// (elements, multiples of 8); box 1 x box_rows x box_cols, swizzled over its rows' bytes: box_cols 64 or 32.
+// (elements, multiples of 8); box 1 x box_rows x 64 columns, 128-byte swizzle.
 int make_tmap_f16(CUtensorMap* out, const void* base, uint64_t cols, uint64_t rows, uint64_t count, uint64_t ld,
-                  uint64_t stride, uint32_t box_cols, uint32_t box_rows);
+                  uint64_t stride, uint32_t box_rows);
 // 3D tensor map over [n2, n1, n0] elements of `dtype` (n0 dense, s1 and s2 the element strides of the outer
 // dimensions), box b2 x b1 x b0, without swizzle.
 int make_tmap_3d(CUtensorMap* out, int dtype, const void* base, uint64_t n0, uint64_t n1, uint64_t n2, uint64_t s1,

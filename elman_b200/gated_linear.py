@@ -11,6 +11,7 @@ inside a sequence are given as a reset mask.  LadderLM runs it as level "gated_l
 """
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import fused_ops, hasty_pytorch_lib
 
@@ -29,6 +30,7 @@ class GatedLinearFunction(torch.autograd.Function):
         return y, h_last
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh_last):
         fcz, saved, reset = ctx.saved_tensors
         f, c, z = fcz.chunk(3, dim=-1)

@@ -940,7 +940,7 @@ def gated_linear_backward(f, c, z, saved, d_output, dh_last=None, reset=None, ou
     """-> [df, dc, dz, dh0 [B,d] float32] for the forward call on the same f, c, z and reset.
 
     dh_last [B,d] float32 or None: gradient of the last state.  out: three [T,B,d] tensors with dense
-    channels to write df, dc, dz to (slices of one gradient buffer), sharing no storage with the inputs."""
+    channels to write df, dc, dz to, apart or slices of one buffer's rows, sharing no storage with the inputs."""
     fn = "gated_linear_backward"
     dt = _check_sequences(fn, f, f=f, c=c, z=z, d_output=d_output)
     T, B, d = f.shape
@@ -980,7 +980,7 @@ NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # singular values of (0
 def newton_schulz(G, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7):
     """The matrices G [..., m, n] with their singular values moved towards one and their singular vectors kept:
     X = G / (|G| + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T.  float32 or bfloat16,
-    contiguous; returns a tensor like G.  No counterpart in the reference."""
+    contiguous; returns a tensor like G, which carries no gradient.  No counterpart in the reference."""
     fn = "newton_schulz"
     dt = _check_inputs(fn, G, G=G)
     if G.dim() < 2:

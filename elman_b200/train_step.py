@@ -412,7 +412,7 @@ class FlatMuon:
             self.groups.append((m, n, torch.tensor(offsets, dtype=torch.int64, device=flat.device),
                                 torch.zeros(len(offsets), m, n, dtype=torch.float32, device=flat.device)))
         runs = []             # stretches of the flat buffers that are no matrix
-        for off, n in sorted((at[id(p)], p.numel()) for p in grads.params if id(p) not in mine):
+        for off, n in sorted((at[id(p)], p.numel()) for p in grads.params if id(p) not in mine and p.numel() > 0):
             if runs and runs[-1][1] == off:
                 runs[-1][1] = off + n
             else:

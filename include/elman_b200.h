@@ -578,7 +578,8 @@ int elman_e1_lm_token(int dtype, int depth, int B, int d, int vocab, const long 
  * f, c, z, y, d_output, df, dc, dz are [T,B,d] of `dtype` with dense channels and any element strides
  * over t and b: `strides` holds a (t, b) pair for f, c, z, y (forward) resp. f, c, z, d_output, df, dc,
  * dz (backward), read on the host.  Slices of one projection and batch-major tensors are read in place.
- * Outputs must not overlap anything else of the call.  The states are fp32 in either dtype: h0 [B,d] (NULL:
+ * Outputs must not overlap anything else of the call (df, dc and dz may be slices of one tensor's rows, with equal
+ * strides of which one is a multiple of the other; what else lies among one another's rows is refused).  The states are fp32 in either dtype: h0 [B,d] (NULL:
  * zeros), h_last [B,d] (the state after step T-1), dh_last [B,d] (NULL: zeros), dh0 [B,d].
  * reset [T,B] (NULL: none): non-zero where step t starts a new sequence and forgets the state.
  * saved [ceil(T / ELMAN_GATED_LINEAR_CHUNK), B, d] fp32: written by the forward call with `training`, read

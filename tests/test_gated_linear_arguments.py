@@ -64,3 +64,16 @@ def test_python_refuses():
         H.gated_linear_forward(False, x.tolist(), x, x)
     with pytest.raises(RuntimeError, match="CUDA"):
         H.gated_linear_backward(x, x, x, x, x)
+
+
+@pytest.mark.parametrize("dc,dz,strides,refused", [
+    (8, 16, (48, 24), False), (8, 24, (48, 24), True), (8, 12, (48, 24), True), (0, 16, (48, 24), True),
+    (48, 16, (48, 24), True), (16, 8, (24, 1680), False), (8, 16, (50, 24), True), (4096, 8192, (50, 24), False)])
+def test_c_backward_refuses_gradients_among_one_another(dc, dz, strides, refused):
+    """df, dc, dz at these elements of one buffer.  What is apart gets as far as the missing workspace."""
+    lib = _lib.load()
+    p = 1 << 20
+    assert lib.elman_gated_linear_workspace(_lib.ELMAN_F32, 70, 2, 8) > 0
+    assert lib.elman_gated_linear_backward(_lib.ELMAN_F32, 70, 2, 8, p, p, p, p, p, None, None,
+                                           _strides(*[48, 24] * 4, *strides * 3), p, p + 4 * dc, p + 4 * dz, p, None, 0, None) == 1
+    assert (b"df, dc and dz overlap" if refused else b"workspace is NULL") in lib.elman_b200_last_error()

@@ -83,6 +83,43 @@ def test_node_accepts_what_autograd_hands_it():
         fused_ops.gated_linear(torch.zeros(3, 2, 9, device="cuda", dtype=torch.float16))
 
 
+def test_second_derivatives_are_refused():
+    x = torch.randn(20, 2, 3 * 16, device="cuda", requires_grad=True)
+    y, _ = fused_ops.gated_linear(x)
+    (grad,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice|once_differentiable"):
+        (grad.square().sum() + x.sum()).backward()
+
+
+def test_gradient_slices_that_overlap_are_refused():
+    x = torch.zeros(70, 2, 8, device="cuda")
+    saved = H.gated_linear_forward(True, x, x, x)[2]
+    one = torch.empty_like(x)
+    with pytest.raises(_lib.ElmanB200Error, match="overlap"):
+        H.gated_linear_backward(x, x, x, saved, x, out=(one, one, torch.empty_like(x)))
+    rows = torch.empty(70, 2, 20, device="cuda")
+    with pytest.raises(_lib.ElmanB200Error, match="overlap"):
+        H.gated_linear_backward(x, x, x, saved, x, out=(rows[..., :8], rows[..., 6:14], torch.empty_like(x)))
+
+
+def test_flat_muon_with_a_parameter_of_no_elements():
+    """The empty parameter lies between others; the step is that of the same model without it."""
+    def run(empty):
+        torch.manual_seed(3)
+        ps = [torch.nn.Parameter(torch.randn(s, device="cuda")) for s in ((5,), (8, 12), (7,))]
+        if empty:
+            ps.insert(1, torch.nn.Parameter(torch.empty(0, device="cuda")))
+        grads = FlatGradients([ps])
+        opt = FlatMuon(grads, [p for p in ps if p.dim() == 2])
+        for p in ps:
+            p.grad.fill_(0.5)
+        opt.step()
+        return [p.detach() for p in ps if p.numel() > 0]
+
+    for a, b in zip(run(False), run(True)):
+        assert torch.equal(a, b)
+
+
 def test_python_entry_refuses_on_the_device():
     x = torch.zeros(70, 2, 8, device="cuda")
     y, h, saved = H.gated_linear_forward(True, x, x, x)
