@@ -11,7 +11,6 @@ inside a sequence are given as a reset mask.  LadderLM runs it as level "gated_l
 """
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import fused_ops, hasty_pytorch_lib
 
@@ -30,8 +29,9 @@ class GatedLinearFunction(torch.autograd.Function):
         return y, h_last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh_last):
+        if torch.is_grad_enabled():      # create_graph: the result would silently be a constant
+            raise RuntimeError("gated_linear: second derivatives are not supported")
         fcz, saved, reset = ctx.saved_tensors
         f, c, z = fcz.chunk(3, dim=-1)
         if dy is None:

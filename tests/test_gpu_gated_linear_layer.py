@@ -86,9 +86,8 @@ def test_node_accepts_what_autograd_hands_it():
 def test_second_derivatives_are_refused():
     x = torch.randn(20, 2, 3 * 16, device="cuda", requires_grad=True)
     y, _ = fused_ops.gated_linear(x)
-    (grad,) = torch.autograd.grad(y.sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError, match="twice|once_differentiable"):
-        (grad.square().sum() + x.sum()).backward()
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
 
 
 def test_gradient_slices_that_overlap_are_refused():
