@@ -27,7 +27,7 @@ namespace elman {
 namespace {
 
 // One block's share of a tile is 128 rows of the product; a pair of blocks (cta_group::2) makes a tile of 256 x 256,
-// a block by itself one of 128 x 128.  Either way a block loads 128 rows of each operand a stage.
+// a block by itself one of 128 x 128 or of 128 x 64.
 constexpr int BK = 64, STAGES = 6, TICKETS = 4;
 constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
 constexpr int BLOCK_BYTES = 64 * BK * 2;              // one TMA box: 64 x 64 fp16
@@ -71,6 +71,7 @@ struct NsMaps { NsMap x[2], a, b; };
 struct NsPlan {
   int count, m, n, r, tall, steps, parts;
   int split;                 // bf16: 1: both parts of B go into the products, 2: of A as well
+  int edge, n_sym, n_upd;    // rows of a tile; columns of a symmetric product's tiles and of an update's
   int triangle, all;         // tiles of a symmetric product and of an update
   int per_step, total;       // items of the list
   float a, b, c;
@@ -91,7 +92,7 @@ __host__ __device__ inline bool takes_low(int step, int steps, int parts) { retu
 // One item of the list.  Taking it apart costs divisions, a thousand cycles of latency: the warp that takes items does
 // it ahead of time and hands on the four numbers that the rest follows from.
 struct alignas(16) NsSlot { int kind, mat, tile, step; };     // kind -1: no more
-__device__ __forceinline__ NsSlot slot_of(const NsPlan& p, int index, int edge) {
+__device__ __forceinline__ NsSlot slot_of(const NsPlan& p, int index) {
   NsSlot k;
   k.step = index / p.per_step;
   int w = index - k.step * p.per_step, ti, tj;
@@ -100,16 +101,19 @@ __device__ __forceinline__ NsSlot slot_of(const NsPlan& p, int index, int edge) 
     k.kind = w >= gram ? SQUARE : GRAM;
     if (w >= gram) w -= gram;
     k.mat = w / p.triangle;
-    const int t = w - k.mat * p.triangle;      // the tiles (i, j >= i), column by column
-    tj = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-    while ((tj + 1) * (tj + 2) / 2 <= t) ++tj;
-    while (tj * (tj + 1) / 2 > t) --tj;
-    ti = t - tj * (tj + 1) / 2;
+    // column by column of blocks the blocks (i, j >= i), `per` tiles each
+    const int t = w - k.mat * p.triangle, per = p.edge / p.n_sym, s = t / per;
+    int j = (int)((sqrtf(8.f * (float)s + 1.f) - 1.f) * 0.5f);
+    while ((j + 1) * (j + 2) / 2 <= s) ++j;
+    while (j * (j + 1) / 2 > s) --j;
+    const int rest = t - per * (j * (j + 1) / 2);
+    tj = per * j + rest / (j + 1);
+    ti = rest % (j + 1);
   } else {
     w -= 2 * gram;
     k.kind = k.step == p.steps - 1 ? LAST : UPDATE;
     k.mat = w / p.all;
-    const int t = w - k.mat * p.all, tiles_n = (p.n + edge - 1) / edge;
+    const int t = w - k.mat * p.all, tiles_n = (p.n + p.n_upd - 1) / p.n_upd;
     ti = t / tiles_n;
     tj = t - ti * tiles_n;
   }
@@ -118,6 +122,7 @@ __device__ __forceinline__ NsSlot slot_of(const NsPlan& p, int index, int edge) 
 }
 struct NsItem {
   int kind, mat, ti, tj, step;
+  int columns;                                 // of the tile
   int m, n, K, a_form, b_form;
   int parts;                                   // products of high and low parts
 };
@@ -126,6 +131,7 @@ __device__ __forceinline__ NsItem item_of(const NsPlan& p, NsSlot k) {
   it.kind = k.kind; it.mat = k.mat; it.ti = k.tile >> 16; it.tj = k.tile & 0xFFFF; it.step = k.step;
   const bool symmetric = k.kind == GRAM || k.kind == SQUARE;
   it.parts = p.split == 0 || k.kind == GRAM ? p.parts : k.kind != SQUARE ? 2 : p.split == 2 ? 3 : 1;
+  it.columns = symmetric ? p.n_sym : p.n_upd;
   it.m = symmetric ? p.r : p.m;
   it.n = symmetric ? p.r : p.n;
   it.K = k.kind != GRAM ? p.r : p.tall ? p.m : p.n;
@@ -422,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
   auto wait_for = [&](uint64_t* bar, int q) {         // item q's ticket or start (cluster-wide acquire: a pair's come from the even block)
     long spins = 0;
     unsigned long long t0 = 0;
-    while (!tch::mbar_try_wait_cluster(bar, (uint32_t)(q / TICKETS) & 1u)) {
+    while (!(PAIR ? tch::mbar_try_wait_cluster(bar, (uint32_t)(q / TICKETS) & 1u) : ptx::mbar_try_wait(bar, (uint32_t)(q / TICKETS) & 1u))) {
       if (++spins > p.spin_limit * 8 || *abortp != 0) return false;
       if ((spins & 1023) == 0) {
         const unsigned long long now = ptx::globaltimer_ns();
@@ -467,17 +473,23 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         if (slot.kind < 0) { free_ticket(q); break; }
         const NsItem it = item_of(p, slot);
         const int at = it.step & 1, form = first ? it.a_form : it.b_form;
-        const int row0 = (first ? it.ti : it.tj) * EDGE + 128 * (int)rank;
+        const int row0 = (first ? it.ti * EDGE : it.tj * it.columns) + 128 * (int)rank;
+        const NsMap& map = it.kind == GRAM ? maps.x[at] : it.kind == SQUARE ? maps.a : first == (p.tall != 0) ? maps.x[at] : maps.b;
+        auto claim = [&]() {                          // a stage to fill
+          if (!ptx::mbar_wait(&empty_bar[s], ph ^ 1u, p.spin_limit, abortp)) return false;
+          if (first && rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[s], BLOCKS * OPERAND_BYTES + (uint32_t)it.columns * (BK * 2));
+          return true;
+        };
+        bool claimed = claim(), ok = true;            // the first one before the item may start
+        if (!claimed) { give_up(0xFFF9); break; }
         if (!wait_for(&go[k], q)) { give_up(0xFFF8); break; }
         free_ticket(q);                               // (not before: the start of the slot's next item would hide this one's)
-        ptx::fence_proxy_async();                     // written by other blocks, read here by TMA
-        const NsMap& map = it.kind == GRAM ? maps.x[at] : it.kind == SQUARE ? maps.a : first == (p.tall != 0) ? maps.x[at] : maps.b;
-        bool ok = true;
+        ptx::fence_proxy_async_global();              // written by other blocks, read here by TMA
         for (int part = 0; part < it.parts && ok; ++part) {     // high x high, high x low, low x high; or B's low part
           const int low = it.parts == 2 ? part == 1 && first == (p.tall == 0) : first ? part == 2 : part == 1;
           for (int k0 = 0; k0 < it.K; k0 += BK, ++iteration) {
-            if (!ptx::mbar_wait(&empty_bar[s], ph ^ 1u, p.spin_limit, abortp)) { give_up(k0); ok = false; break; }
-            if (first && rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[s], BLOCKS * 2 * OPERAND_BYTES);
+            if (!claimed && !claim()) { give_up(k0); ok = false; break; }
+            claimed = false;
             const bool mn = mn_major(form, row0, k0, EDGE);
             const uint32_t bar = bars + 8 * s;
             if (!(iteration == p.stall && blockIdx.x == 0)) {
@@ -486,7 +498,9 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
                 if constexpr (PAIR) ptx::tma_load_3d_pair(d, m, x, y, it.mat, bar);
                 else tch::tma_load_3d(d, m, x, y, it.mat, &full_bar[s]);
               };
-              if (mn) {
+              if (!PAIR && !first && it.columns == 64) {
+                copy(dst, &map.block[low], mn ? row0 : k0, mn ? k0 : row0);
+              } else if (mn) {
                 copy(dst, &map.block[low], row0, k0);
                 copy(dst + BLOCK_BYTES, &map.block[low], row0 + 64, k0);
               } else {
@@ -507,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         if (!ptx::mbar_wait(&tk_empty[k], ((uint32_t)(q / TICKETS) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFB); break; }
         const int index = atomicAdd(p.ticket, 1);
         NsSlot slot{-1, 0, 0, 0};
-        if (index < p.total) slot = slot_of(p, index, EDGE);
+        if (index < p.total) slot = slot_of(p, index);
         tk[k] = slot;
         ptx::mbar_arrive(&tk_full[k]);
         if constexpr (PAIR) {
@@ -532,7 +546,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         free_ticket(q);
         if (slot.kind < 0) break;
         const NsItem it = item_of(p, slot);
-        const int m0 = it.ti * EDGE, n0 = it.tj * EDGE, nk = (it.K + BK - 1) / BK;
+        const int m0 = it.ti * EDGE, n0 = it.tj * it.columns / EDGE * EDGE, nk = (it.K + BK - 1) / BK;
         const int b = q % sums;
         if (!ptx::mbar_wait(&acc_empty[b], ((uint32_t)(q / sums) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFE); break; }
         ptx::tc_fence_after();
@@ -545,7 +559,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
             if (it.a_form == UPPER && k0 < m0) end = m0;
             if (it.b_form == UPPER && k0 < n0 && n0 < end) end = n0;
             const bool a_mn = mn_major(it.a_form, m0, k0, EDGE), b_mn = mn_major(it.b_form, n0, k0, EDGE);
-            const uint32_t idesc = ptx::umma_idesc_f16(EDGE, EDGE) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+            const uint32_t idesc = ptx::umma_idesc_f16(EDGE, PAIR ? EDGE : it.columns) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
             const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
             const uint64_t da0 = a_mn ? ptx::umma_desc_mn_sw128(ptx::smem_u32(sA), BLOCK_BYTES) : ptx::umma_desc_k_sw128(ptx::smem_u32(sA));
             const uint64_t db0 = b_mn ? ptx::umma_desc_mn_sw128(ptx::smem_u32(sB), BLOCK_BYTES) : ptx::umma_desc_k_sw128(ptx::smem_u32(sB));
@@ -579,7 +593,6 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
   } else {
     // warp w may read TMEM lanes [32 (w % 4), +32); the two warps of a quarter split the tile's columns
     const int quarter = warp & 3, mine = warp - 4, half = mine >> 2;
-    constexpr int CH = EDGE / 32 / 2;
     const uint32_t buffer = ptx::smem_u32(smem) + STAGES * 2 * OPERAND_BYTES + (uint32_t)(mine * BUFFER_BYTES);
     for (int q = 0;; ++q) {
       bool ok = __all_sync(0xFFFFFFFFu, wait_for(&tk_full[q % TICKETS], q));
@@ -597,7 +610,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         it = item_of(p, slot);
         b = q % sums;
         row0 = it.ti * EDGE + 128 * (int)rank + quarter * 32;
-        col0 = it.tj * EDGE + half * (EDGE / 2);
+        col0 = it.tj * it.columns + half * (it.columns / 2);
         fin = finish_of(p, it);
         ok = __all_sync(0xFFFFFFFFu, it.kind == GRAM || wait_for(&go[q % TICKETS], q));
         if (lane == 0) free_ticket(q);
@@ -616,10 +629,10 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           : "memory");
       if (stop) break;
       ptx::tc_fence_after();
-      const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((p.parts > 1 ? 0 : b * EDGE) + half * (EDGE / 2));
-      const int nk = (it.K + BK - 1) / BK;
+      const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((p.parts > 1 ? 0 : b * EDGE) + half * (it.columns / 2));
+      const int nk = (it.K + BK - 1) / BK, boxes = it.columns / 64;
 #pragma unroll 1
-      for (int c = 0; c < CH; ++c) {
+      for (int c = 0; c < boxes; ++c) {
         uint32_t r[32];
         ptx::tmem_ld32(tsrc + (uint32_t)(c * 32), r);
         const int col = col0 + c * 32;
@@ -631,7 +644,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
             if (fin.same.lo != nullptr) sts_u4(at + BOX_BYTES, same.lo[k]);
           }
           __syncwarp();
-          if (c + 1 < CH) fetch_box(same, fin, it, row0, col + 32);
+          if (c + 1 < boxes) fetch_box(same, fin, it, row0, col + 32);
         }
         ptx::tmem_ld_wait();
         for (int sum = 1; sum < 4 && p.parts > 1; ++sum) {
@@ -642,7 +655,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(more[j]));
         }
-        if (c == CH - 1) {                            // the accumulator is free again
+        if (c == boxes - 1) {                            // the accumulator is free again
           ptx::tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -787,19 +800,31 @@ bool stays_in_range(int steps, double a, double b, double c) {
   return true;
 }
 
-// Pairs make four times the tile in little more than the time of a single block's: about 600 cycles a stage and
-// 11000 a tile against 550 and 7000 (waits, first loads, finishing; measured).  Single blocks waste fewer rows of ragged
-// matrices and spread few tiles over more of the device: 6 x 640 x 1280 takes 257 us in pairs and 211 in single blocks,
-// 4 x 1280 x 1280 takes 316 and 379.
+// Pairs make four times the tile in little more than the time of a single block's: about 600 cycles a stage and 11000 a
+// tile against 550 and 7000 where tiles follow one another; 16000 a tile against 10400 for a matrix whose products wait for
+// one another, 800 a stage with single blocks (measured).  Single blocks also waste fewer rows of ragged matrices.
+// 6 x 640 x 1280 takes 257 us in pairs and 204 in single blocks, 18 x 512 x 512 209 and 178, 4 x 1280 x 1280 316 and 379,
+// 1 x 2048 x 2048 350 and 367.
 bool pays_as_pairs(const NsPlan& p) {
   if (p.parts > 1) return false;
-  auto cost = [&](int edge, int units, double stage, double tile) {     // of a step
-    const double side = (p.r + edge - 1) / edge, q = p.tall ? p.m : p.n;
+  auto cost = [&](int edge, int units, double stage, double tile, double alone, double latency) {     // of a step
+    const double side = (p.r + edge - 1) / edge, q = p.tall ? p.m : p.n, k_gram = ceil(q / BK), k = ceil((double)p.r / BK);
     const double tri = p.count * side * (side + 1) / 2 / units, all = p.count * side * ceil(q / edge) / units;
-    const double gram = ceil(q / BK) * stage + tile, other = ceil((double)p.r / BK) * stage + tile;
-    return fmax(tri, 1.) * (gram + other) + fmax(all, 1.) * other;
+    return fmax(tri * (k_gram * stage + tile) + (tri + all) * (k * stage + tile), (k_gram + 2 * k) * alone + 3 * latency);
   };
-  return cost(256, 74, 600, 11000) < cost(128, 148, 550, 7000);
+  return cost(256, 74, 600, 11000, 600, 16000) < cost(128, 148, 550, 7000, 800, 10400);
+}
+// Tiles of the blocks (i, j >= i) of a symmetric product.
+int triangle_of(int r, int edge, int columns) {
+  const int per = edge / columns, strips = (r + columns - 1) / columns, whole = strips / per;
+  return per * (whole * (whole + 1) / 2) + strips % per * (whole + 1);
+}
+// Single blocks: tiles of 64 columns where they spread a product over more of the device.  They take about 2500 cycles
+// less from start to end, most of it in finishing rows: 1 x 256 x 256 89 us against 112, 4 x 512 x 512 122 and 140; but
+// 18 x 512 x 512 219 and 178.
+int columns_of(const NsPlan& p, int wide, int narrow, int stages) {
+  auto cost = [&](int tiles, double tile) { return ceil((double)tiles * p.count / 148) * (800. * stages * p.parts + tile); };
+  return cost(narrow, 7900) < cost(wide, 10400) ? 64 : 128;
 }
 
 template <typename T, bool PAIR>
@@ -850,9 +875,16 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   p.spin_limit = options().spin_limit;
   p.stall = (int)options().test_stall_step;
   const bool pair = pays_as_pairs(p);
-  const int edge = pair ? 256 : 128, side = (p.r + edge - 1) / edge;
-  p.triangle = side * (side + 1) / 2;
-  p.all = ((p.m + edge - 1) / edge) * ((p.n + edge - 1) / edge);
+  const int edge = pair ? 256 : 128;
+  p.edge = p.n_sym = p.n_upd = edge;
+  const int upd_rows = (p.m + edge - 1) / edge;
+  if (!pair) {
+    const int gram = ((p.tall ? p.m : p.n) + BK - 1) / BK, inner = (p.r + BK - 1) / BK;
+    p.n_sym = columns_of(p, triangle_of(p.r, 128, 128), triangle_of(p.r, 128, 64), (gram + inner) / 2);
+    p.n_upd = columns_of(p, upd_rows * ((p.n + 127) / 128), upd_rows * ((p.n + 63) / 64), inner);
+  }
+  p.triangle = triangle_of(p.r, edge, p.n_sym);
+  p.all = upd_rows * ((p.n + p.n_upd - 1) / p.n_upd);
   const double total = (double)p.steps * p.count * (2. * p.triangle + p.all);
   ELMAN_ARG_CHECK(total + 1024 < (double)(1L << 31), "matrices too large");
   p.per_step = p.count * (2 * p.triangle + p.all);
