@@ -126,7 +126,10 @@ __global__ void __launch_bounds__(128) gl_backward_seq_kernel(GlParams p) {
 // (NaN goes out as 0x7fffffff), so an exchange is one store and one load.  Tiles are handed out in time
 // order by a counter: whoever a tile waits for has started before it and waits for nobody behind it.
 // ---------------------------------------------------------------------------
-constexpr int GROUP = 16;
+// Long groups make the chain of states short, short ones leave fewer pairs to fold and registers to hold them.  Forward and
+// backward, us, with 8 / 10 / 16: T65536 B1 d1280 bf16 525 / 520 / 534, T65536 B1 d256 179 / 166 / 160, T4096 B64 d1536
+// 1649 / 1659 / 1693.
+constexpr int GROUP = 10;
 constexpr uint32_t NOT_YET = 0xFFFFFFFFu;
 
 struct GlChain {             // workspace; all of it starts as NOT_YET

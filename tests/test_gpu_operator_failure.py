@@ -25,7 +25,7 @@ def _expect_timeout(kernel_id):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("d", [128, 62, 61, 20])
-@pytest.mark.parametrize("tile", [0, 15])      # a pair, or a group's state
+@pytest.mark.parametrize("tile", [0, 9, 15])      # a pair, or a group's state
 def test_recurrence_gives_up_when_a_tile_withholds_its_share_and_recovers(tile, d, dtype):
     g = torch.Generator(device="cuda").manual_seed(1)
     f, c, z, dy = (torch.randn(4200, 1, d, generator=g, device="cuda").to(dtype) for _ in range(4))
