@@ -9,6 +9,8 @@
 //
 // Bound by HBM: forward 4 values an element, backward 7 (each of f, c, z, dy read once, each result
 // written once); the backward pass recomputes the states from one in GL_CHUNK that the forward saved.
+// Measured, calls on bf16: T4096 B64 d1536 549 us forward (5.9 TB/s), 1110 backward (5.1 TB/s; instruction issue is next);
+// T65536 B1 d1280, where the columns are few and the tiles wait for the chain of states, 185 (3.6) and 339 (3.5).
 #include <string.h>
 
 #include <mutex>
@@ -111,7 +113,9 @@ __global__ void __launch_bounds__(128) gl_backward_seq_kernel(GlParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Sequences of more than a few steps: tiles of (W warps x L steps) x (32 V channels), each read once.
+// Sequences of more than a few steps: tiles of (W warps x L steps) x (32 V channels), each read once.  The kernels
+// of this section take the rows whose last 128 bytes would be mostly empty (whole_width below) and count channels through
+// batch rows; the next section's take all others.
 //
 // A warp holds L steps of 32 lanes x V channels in registers and scans them from a zero state: the pair (R, H)
 // with  h_out = h_in + (H - R h_in),  R = 1 - prod(1 - u) kept as the scan of the constant 1, so that
@@ -621,7 +625,8 @@ __global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p
 // ---------------------------------------------------------------------------
 // The same tiles fed by asynchronous copies: the next tile's rows arrive in one shared-memory stage while
 // this tile is scanned from the other, so the loads never pause for the arithmetic.  A producer takes
-// tiles from the counter and loads them; the other warps scan and link.  A tile lies within one batch row.
+// tiles from the counter and loads them; the other warps scan and link.  A tile lies within one batch row.  (Tiles loaded
+// into registers by the scanning warps: T512 B32 d1280 forward and backward 165 us, fed 123.)
 //
 // FEED_TMA, for tensors whose base and row strides are multiples of 16 bytes: a box a tensor, rows past T and
 // channels past d zero-filled; a lane owns the same 4-byte word of every row (two bf16 channels or one
