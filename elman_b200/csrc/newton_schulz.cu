@@ -2,10 +2,10 @@
 //   X = G / (|G|_F + eps);  steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X
 // (tall matrices: A = X^T X and X <- a X + X B, so that A has the smaller of the two extents, r).
 // A and B are symmetric: only the tiles on and above the diagonal are computed and stored.  Per step 3 r^2 q + r^3
-// flops with q the larger extent: bound by the tensor cores.  Measured, five steps on bf16: 18 x 1280 x 1280 850 us (889
-// TFLOP/s), 2 x 4096 x 4096 2.27 ms (1210); each block of a pair takes in 64 bytes a cycle of products, about what an SM gets from L2, and
-// a stage of 512 cycles lasts 600 to 700.  Small matrices are bound by the latency of 15 products one after
-// another: 1 x 256 x 256 90 us, 6 us each (about: loads 2, products 1.4, rows 1.2, stores made visible and seen 1.2).
+// flops with q the larger extent: bound by the tensor cores.  Measured, five steps on bf16: 18 x 1280 x 1280 872 us (866
+// TFLOP/s), 2 x 4096 x 4096 2.2 ms (1246); each block of a pair takes in 64 bytes a cycle of products, about what an SM
+// gets from L2, and a stage of 512 cycles lasts 600 to 700.  Small matrices are bound by the latency of 15 products one
+// after another: 1 x 256 x 256 90 us, 6 us each (about: loads 2, products 1.4, rows 1.2, stores made visible and seen 1.2).
 //
 // Numbers.  The operands are fp16 (11 significant bits; bf16 has 8), scaled by powers of two into its
 // range: X by 2^12, A by 2^12, B by 2^10; every sum is fp32.  The polynomial multiplies small singular
@@ -15,7 +15,9 @@
 // the polynomial's slope is small and rounding a X and B X alike is what keeps the error small.
 // fp32 matrices take both parts of X, A and B into the products as well (three products for one): 5e-6.  The tensor
 // cores cut their fp32 sums off rather than rounding them, which over a long contraction adds up (2.5e-5 at
-// 33 x 2000 with one sum): there the large products take turns in three sums and the small ones have a fourth.
+// 33 x 2000 with one sum): there the large products take turns in three sums and the small ones have a fourth (3.4e-6 at
+// 200 x 2000, 1.2e-5 at 200 x 9000, 2.9e-5 at 1000 x 20000).  A step along K brings the high parts of both operands in one
+// stage and the low parts in the next, for all three products: 4 x 1000 x 257 250 us with a stage a product, now 188.
 #include <math.h>
 
 #include <mutex>
@@ -489,9 +491,10 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         if (!wait_for(&go[k], q)) { give_up(0xFFF8); break; }
         free_ticket(q);                               // (not before: the start of the slot's next item would hide this one's)
         ptx::fence_proxy_async_global();              // written by other blocks, read here by TMA
-        for (int part = 0; part < it.parts && ok; ++part) {     // high x high, high x low, low x high; or B's low part
-          const int low = it.parts == 2 ? part == 1 && first == (p.tall == 0) : first ? part == 2 : part == 1;
-          for (int k0 = 0; k0 < it.K; k0 += BK, ++iteration) {
+        const int both = it.parts == 3, stages = (it.K + BK - 1) / BK << both;   // both: a stage of high parts, one of low parts
+        for (int part = 0; part < (both ? 1 : it.parts) && ok; ++part) {
+          for (int i = 0; i < stages; ++i, ++iteration) {
+            const int k0 = (i >> both) * BK, low = both ? i & 1 : part == 1 && first == (p.tall == 0);   // (two parts: B's)
             if (!claimed && !claim()) { give_up(k0); ok = false; break; }
             claimed = false;
             const bool mn = mn_major(form, row0, k0, EDGE);
@@ -550,13 +553,13 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         free_ticket(q);
         if (slot.kind < 0) break;
         const NsItem it = item_of(p, slot);
-        const int m0 = it.ti * EDGE, n0 = it.tj * it.columns / EDGE * EDGE, nk = (it.K + BK - 1) / BK;
+        const int m0 = it.ti * EDGE, n0 = it.tj * it.columns / EDGE * EDGE;
         const int b = q % sums;
         if (!ptx::mbar_wait(&acc_empty[b], ((uint32_t)(q / sums) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFE); break; }
         ptx::tc_fence_after();
         const uint32_t sum0 = tmem_base + (uint32_t)(b * EDGE);
-        int i = 0;                                    // stages of this item, over all parts
-        for (int part = 0; part < it.parts && ok; ++part) {
+        int i = 0;                                    // steps of this item along K, over all parts
+        for (int part = 0; part < (it.parts == 3 ? 1 : it.parts) && ok; ++part) {
           for (int k0 = 0; k0 < it.K && ok;) {
             // the stretch of K in which both operands keep their form: an upper matrix changes at the diagonal
             int end = it.K;
@@ -575,12 +578,21 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
               if constexpr (PAIR) {
                 ready = ptx::umma_stage_pair(sum0, da, db, a_step, b_step, idesc, i > 0 ? 1u : 0u, &empty_bar[s], &full_bar[s_next],
                                              ph_next);
+              } else if (it.parts == 3) {
+                // high x high, high x low, low x high, from two stages.  fp32: the large products take turns in three sums,
+                // the others have a fourth
+                const uint32_t large = tmem_base + (uint32_t)((p.parts > 1 ? i % 3 : b) * EDGE), small = tmem_base + (uint32_t)((p.parts > 1 ? 3 : b) * EDGE);
+                const bool opens = i < (p.parts > 1 ? 3 : 1);
+                if (!ptx::umma_stage<false>(large, da, db, a_step, b_step, idesc, opens ? 0u : 1u, &empty_bar[s], &full_bar[s_next], ph_next) &&
+                    !ptx::mbar_wait(&full_bar[s_next], ph_next, p.spin_limit, abortp)) { give_up(i); ok = false; break; }
+                const uint32_t low = s_next;
+                const uint64_t da_low = da0 + (uint64_t)(low * (OPERAND_BYTES / 16)), db_low = db0 + (uint64_t)(low * (OPERAND_BYTES / 16));
+                if (++s_next == STAGES) { s_next = 0; ph_next ^= 1u; }
+                ptx::umma_stage<false>(small, da, db_low, a_step, b_step, idesc, p.parts > 1 && i == 0 ? 0u : 1u, &empty_bar[s], &full_bar[s_next], ph_next);
+                ready = ptx::umma_stage(small, da_low, db, a_step, b_step, idesc, 1u, &empty_bar[s], &full_bar[s_next], ph_next);
+                ptx::umma_commit(&empty_bar[low]);
               } else {
-                // fp32: the large products take turns in three sums, the others have a fourth
-                const int sum = p.parts == 1 ? b : part == 0 ? i % 3 : 3;
-                const bool opens = p.parts == 1 ? i == 0 : part == 0 ? i < 3 : i == nk;
-                ready = ptx::umma_stage(tmem_base + (uint32_t)(sum * EDGE), da, db, a_step, b_step, idesc, opens ? 0u : 1u, &empty_bar[s],
-                                        &full_bar[s_next], ph_next);
+                ready = ptx::umma_stage(sum0, da, db, a_step, b_step, idesc, i > 0 ? 1u : 0u, &empty_bar[s], &full_bar[s_next], ph_next);
               }
               s = s_next;
               ph = ph_next;
@@ -810,7 +822,7 @@ bool stays_in_range(int steps, double a, double b, double c) {
 // 6 x 640 x 1280 takes 257 us in pairs and 204 in single blocks, 18 x 512 x 512 209 and 178, 4 x 1280 x 1280 316 and 379,
 // 1 x 2048 x 2048 350 and 367.
 bool pays_as_pairs(const NsPlan& p) {
-  if (p.parts > 1) return false;
+  if (p.parts > 1 || p.split > 0) return false;
   auto cost = [&](int edge, int units, double stage, double tile, double alone, double latency) {     // of a step
     const double side = (p.r + edge - 1) / edge, q = p.tall ? p.m : p.n, k_gram = ceil(q / BK), k = ceil((double)p.r / BK);
     const double tri = p.count * side * (side + 1) / 2 / units, all = p.count * side * ceil(q / edge) / units;

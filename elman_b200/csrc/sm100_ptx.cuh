@@ -338,7 +338,8 @@ __device__ __forceinline__ bool umma_stage_pair(uint32_t tmem_d, uint64_t da, ui
       : "memory");
   return ready != 0;
 }
-// The same for a CTA by itself (cta_group::1).
+// The same for a CTA by itself (cta_group::1); FREE false: the stage is still needed.
+template <bool FREE = true>
 __device__ __forceinline__ bool umma_stage(uint32_t tmem_d, uint64_t da, uint64_t db, uint64_t a_step, uint64_t b_step,
                                            uint32_t idesc, uint32_t accumulate_first, uint64_t* free_bar,
                                            uint64_t* next_full_bar, uint32_t next_parity) {
@@ -360,11 +361,13 @@ __device__ __forceinline__ bool umma_stage(uint32_t tmem_d, uint64_t da, uint64_
       "tcgen05.mma.cta_group::1.kind::f16 [%1], a1, b1, %7, pt;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%1], a2, b2, %7, pt;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%1], a3, b3, %7, pt;\n\t"
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%8];\n\t"
+      "setp.ne.b32 pa, %11, 0;\n\t"
+      "@pa tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%8];\n\t"
       "selp.b32 %0, 1, 0, pw;\n\t}"
       : "=r"(ready)
       : "r"(tmem_d), "l"(da), "l"(db), "l"(a_step), "l"(b_step), "r"(accumulate_first), "r"(idesc), "r"(smem_u32(free_bar)),
-        "r"(smem_u32(next_full_bar)), "r"(next_parity)
+        "r"(smem_u32(next_full_bar)), "r"(next_parity),
+        "n"(FREE ? 1 : 0)
       : "memory");
   return ready != 0;
 }

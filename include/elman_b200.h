@@ -605,6 +605,7 @@ int elman_gated_linear_backward(int dtype, int T, int B, int d, const void* f, c
  * A = X X^T, which moves every singular value by s -> a s + b s^3 + c s^5 and keeps the singular
  * vectors; out[count,m,n] of `dtype` (may be `in`).  Products take fp16 operands with fp32 sums (fp32
  * matrices: two fp16 numbers an element), so coefficients that take singular values beyond 3.5 are refused.
+ * fp32 results are about 1.5e-9 times the longer extent off (3e-6 at least), in norm.
  * A zero matrix stays zero; a matrix with a NaN or an infinity becomes NaN; the others of the call
  * are not touched by it.
  *

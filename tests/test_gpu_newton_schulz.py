@@ -164,3 +164,15 @@ def test_captured_on_another_stream():
             torch.cuda.synchronize()
             got = X.clone()
             assert torch.equal(got, H.newton_schulz(G))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n", [(64, 9000), (9000, 100), (200, 9000)])
+def test_long_and_narrow_matrices(m, n, dtype):
+    """The tile's shape follows both extents: these are where the longer one, q, decides.  The fp32 sums are cut off, not
+    rounded: each of the q / 48 additions to one of the three sums loses 2^-24 of it on average, half of that over a sum
+    that grows, and a relative error of A enters X with a factor of up to two in each of five steps."""
+    G = make(2, m, n, dtype, seed=7)
+    X, want = H.newton_schulz(G), reference(G)
+    for k in range(2):
+        assert rel(X[k], want[k]) < TOL[dtype] + 10 * (9000 / 48) * 2 ** -25, (k, rel(X[k], want[k]))
