@@ -173,6 +173,11 @@ __device__ __forceinline__ uint4 to_halves(const float (&f)[8]) {
 
 // ------------------------------------------------------------------ start: norm and scaling
 
+// The three launches of a call overlap: each lets the next one start when its own blocks have, and that one waits here
+// before it touches memory (all of what came before has ended then).
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Muon's momentum moves by (1 - mu)(g - momentum); the update is it, or Nesterov's look ahead.
 __device__ __forceinline__ float advance(const NsSource& s, float g, float gs, float& momentum) {
   g *= gs;
@@ -201,6 +206,7 @@ __device__ __forceinline__ void store8(float* at, const float (&f)[8]) {
 // the counters of the products.
 template <typename T>
 __global__ void __launch_bounds__(256) ns_norm_kernel(NsSource s, long size, double* partial, int* ticket, int* done) {
+  let_next_start();
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     done[blockIdx.y] = 0;
     if (blockIdx.y == 0) *ticket = 0;
@@ -246,6 +252,8 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsSource s, long size, dou
 // A warp a row: X_0, scaled, as the sum of two fp16 numbers.
 template <typename T>
 __global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n, long ld, float eps, const double* partial, Split x) {
+  let_next_start();
+  wait_for_previous();
   const int lane = threadIdx.x & 31;
   static_assert(NORM_PARTS == 64, "two partial sums a lane");
   double total = partial[(long)blockIdx.y * NORM_PARTS + lane] + partial[(long)blockIdx.y * NORM_PARTS + 32 + lane];
@@ -424,6 +432,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
   ptx::tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
   volatile int* abortp = &abort_flag;
+  wait_for_previous();
   const int sums = p.parts > 1 ? 1 : 2;              // accumulators in turn (fp32: one of four partial sums)
   auto give_up = [&](int where) {
     abort_flag = 1;
@@ -843,6 +852,13 @@ int columns_of(const NsPlan& p, int wide, int narrow, int stages) {
   return cost(narrow, 7900) < cost(wide, 10400) ? 64 : 128;
 }
 
+cudaLaunchAttribute after_its_start() {              // of the launch before, rather than after its end
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  return attr;
+}
+
 template <typename T, bool PAIR>
 int launch(const NsMaps& maps, const NsPlan& p, cudaStream_t st) {
   static std::mutex mutex;
@@ -864,12 +880,13 @@ int launch(const NsMaps& maps, const NsPlan& p, cudaStream_t st) {
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = NS_SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = blocks;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = PAIR ? 1 : 0;
+  cudaLaunchAttribute attrs[2];
+  attrs[0] = after_its_start();
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = blocks;
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = PAIR ? 2 : 1;
   ELMAN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ns_kernel<T, PAIR>, maps, p));
   count_launch(true);
   return ELMAN_OK;
@@ -924,7 +941,14 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   if (!takes_low(0, p.steps, p.parts)) x0.lo = nullptr;
   ns_norm_kernel<T><<<dim3(NORM_PARTS, p.count), 256, 0, st>>>(src, size, buf.partial, buf.ticket, buf.done);
   count_launch(false);
-  ns_scale_kernel<T><<<dim3((unsigned)(blocks < 1024 ? blocks : 1024), p.count), 256, 0, st>>>(src, p.m, p.n, buf.ldx, g.eps, buf.partial, x0);
+  cudaLaunchAttribute attr = after_its_start();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(blocks < 1024 ? blocks : 1024), p.count);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  ELMAN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ns_scale_kernel<T>, src, p.m, p.n, buf.ldx, g.eps, (const double*)buf.partial, x0));
   count_launch(false);
   ELMAN_CUDA_CHECK(cudaGetLastError());
   return pair ? launch<T, true>(maps, p, st) : launch<T, false>(maps, p, st);
