@@ -1700,11 +1700,12 @@ int elman_adamw_step(int dtype, long n, void* params, const void* grads, void* e
 // gated linear recurrence
 // ---------------------------------------------------------------------------
 // Every pointer lies on a boundary of its elements.
-static bool on_elements(int dtype, std::initializer_list<const void*> pointers) {
+static bool on_boundary(size_t bytes, std::initializer_list<const void*> pointers) {
   for (const void* p : pointers)
-    if (((uintptr_t)p & (esize(dtype) - 1)) != 0) return false;
+    if (((uintptr_t)p & (bytes - 1)) != 0) return false;
   return true;
 }
+static bool on_elements(int dtype, std::initializer_list<const void*> pointers) { return on_boundary(esize(dtype), pointers); }
 // No two elements of a [T, B, d] output may share an address.
 static bool distinct_elements(int T, int B, int d, const long* s) {
   if (T > 1 && s[0] < d) return false;
@@ -1760,10 +1761,12 @@ int elman_gated_linear_forward(int dtype, int training, int T, int B, int d, con
     if (training) REQUIRE_PTR(saved);
     ELMAN_ARG_CHECK(on_elements(dtype, {f, c, z, y}), "misaligned tensor");
   }
+  ELMAN_ARG_CHECK(on_boundary(4, {h0, h_last, saved}), "misaligned state");
   const size_t need = gated_linear_workspace(dtype, T, B, d);
   if (need > 0) REQUIRE_PTR(workspace);
   if (workspace_bytes < need)
     return set_error(ELMAN_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  ELMAN_ARG_CHECK(on_boundary(16, {workspace}), "workspace must be 16-byte aligned");
   GatedLinearArgs a{};
   a.T = T; a.B = B; a.d = d; a.f = f; a.c = c; a.z = z;
   a.f_strides = strides; a.c_strides = strides + 2; a.z_strides = strides + 4; a.y_strides = strides + 6;
@@ -1789,10 +1792,12 @@ int elman_gated_linear_backward(int dtype, int T, int B, int d, const void* f, c
                         outputs_apart(dtype, T, B, d, df, strides + 8, dz, strides + 12) &&
                         outputs_apart(dtype, T, B, d, dc, strides + 10, dz, strides + 12), "df, dc and dz overlap");
   }
+  ELMAN_ARG_CHECK(on_boundary(4, {saved, dh_last, dh0}), "misaligned state");
   const size_t need = gated_linear_workspace(dtype, T, B, d);
   if (need > 0) REQUIRE_PTR(workspace);
   if (workspace_bytes < need)
     return set_error(ELMAN_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  ELMAN_ARG_CHECK(on_boundary(16, {workspace}), "workspace must be 16-byte aligned");
   GatedLinearArgs a{};
   a.T = T; a.B = B; a.d = d; a.f = f; a.c = c; a.z = z; a.dy = d_output;
   a.f_strides = strides; a.c_strides = strides + 2; a.z_strides = strides + 4; a.y_strides = strides + 6;
@@ -1839,6 +1844,7 @@ int elman_newton_schulz(int dtype, int count, int m, int n, const void* in, void
   ELMAN_RETURN_IF(check_newton_schulz(dtype, count, m, n, steps, a, b, c, eps, workspace, workspace_bytes));
   if (count == 0 || m == 0 || n == 0) return ELMAN_OK;
   REQUIRE_PTR(in); REQUIRE_PTR(out);
+  ELMAN_ARG_CHECK(on_elements(dtype, {in, out}), "misaligned matrix");
   const NewtonSchulzArgs args{dtype, count, m, n, steps, a, b, c, eps, in, out, workspace};
   return newton_schulz(args, (cudaStream_t)stream);
 }
@@ -1850,6 +1856,8 @@ int elman_muon_step(int dtype, int count, int m, int n, const long long* offsets
   ELMAN_RETURN_IF(check_newton_schulz(dtype, count, m, n, steps, a, b, c, eps, workspace, workspace_bytes));
   if (count == 0 || m == 0 || n == 0) return ELMAN_OK;
   REQUIRE_PTR(offsets); REQUIRE_PTR(params); REQUIRE_PTR(grads); REQUIRE_PTR(momentum);
+  ELMAN_ARG_CHECK(on_elements(dtype, {params, grads}) && on_boundary(4, {momentum, grad_scale}) && on_boundary(8, {offsets}),
+                  "misaligned parameters, gradients, momentum, scale or offsets");
   const NewtonSchulzArgs args{dtype, count, m, n, steps, a, b, c, eps, nullptr, nullptr, workspace};
   const MuonArgs u{offsets, params, grads, momentum, lr, mu, weight_decay, scale, nesterov, grad_scale};
   return muon_step(args, u, (cudaStream_t)stream);

@@ -77,3 +77,20 @@ def test_c_backward_refuses_gradients_among_one_another(dc, dz, strides, refused
     assert lib.elman_gated_linear_backward(_lib.ELMAN_F32, 70, 2, 8, p, p, p, p, p, None, None,
                                            _strides(*[48, 24] * 4, *strides * 3), p, p + 4 * dc, p + 4 * dz, p, None, 0, None) == 1
     assert (b"df, dc and dz overlap" if refused else b"workspace is NULL") in lib.elman_b200_last_error()
+
+
+@pytest.mark.parametrize("kw,message", [(dict(f=(1 << 20) + 2), b"misaligned tensor"), (dict(y=(1 << 20) + 1), b"misaligned tensor"),
+                                        (dict(h_last=(1 << 20) + 2), b"misaligned state"),
+                                        (dict(training=1, saved=(1 << 20) + 1), b"misaligned state")])
+def test_c_entry_refuses_pointers_between_elements(kw, message):
+    lib = _lib.load()
+    assert _forward(lib, **kw) == 1
+    assert message in lib.elman_b200_last_error()
+
+
+def test_c_entry_refuses_a_workspace_off_its_boundary():
+    lib = _lib.load()
+    p, need = 1 << 20, lib.elman_gated_linear_workspace(_lib.ELMAN_F32, 70, 2, 8)
+    s = _strides(*[16, 8] * 4)
+    assert lib.elman_gated_linear_forward(_lib.ELMAN_F32, 0, 70, 2, 8, p, p, p, None, None, s, 2 * p, p, None, p + 8, need, None) == 1
+    assert b"16-byte" in lib.elman_b200_last_error()

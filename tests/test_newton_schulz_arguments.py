@@ -17,7 +17,7 @@ def _call(lib, dtype=_lib.ELMAN_BF16, count=1, m=4, n=4, steps=5, abc=H.NEWTON_S
     (dict(steps=101), 1, b"steps"), (dict(eps=-1.0), 1, b"eps"), (dict(abc=(10.0, 0.0, 0.0)), 1, b"beyond 3.5"),
     (dict(abc=(2.0, 70.0, -70.0), steps=1), 1, b"beyond"), (dict(abc=(float("nan"), 0.0, 0.0)), 1, b"beyond"),
     (dict(G=None), 1, b"NULL"), (dict(out=None), 1, b"NULL"), (dict(ws=None), 1, b"NULL"), (dict(ws_bytes=100), 4, b"workspace"),
-    (dict(ws=P + 8), 1, b"aligned"),
+    (dict(ws=P + 8), 1, b"aligned"), (dict(G=P + 1), 1, b"misaligned"), (dict(out=P + 2, dtype=_lib.ELMAN_F32), 1, b"misaligned"),
 ])
 def test_c_entry_refuses(kw, rc, message):
     lib = _lib.load()
@@ -37,6 +37,8 @@ def test_muon_entry_refuses():
         _lib.ELMAN_F32, 1, 4, 4, offsets, params, grads, mom, 0.1, 0.9, 1, 0.0, 1.0, None, 5, *H.NEWTON_SCHULZ_COEFFICIENTS, 1e-7, ws, 1 << 30, None)
     for name in ("offsets", "params", "grads", "mom", "ws"):
         assert call(**{name: None}) == 1 and b"NULL" in lib.elman_b200_last_error()
+    for name in ("offsets", "params", "grads", "mom"):
+        assert call(**{name: P + (4 if name == "offsets" else 2)}) == 1 and b"misaligned" in lib.elman_b200_last_error()
 
 
 def test_nothing_to_do_is_no_error_and_needs_no_workspace():
