@@ -366,6 +366,14 @@ int lowrank_tc(const LowRankTcArgs& a, cudaStream_t stream);
 int gemm_tc_dual_tn(int M, int N, int K, const bf16* A, const bf16* B1, const bf16* B2, void* C1,
                     void* C2, cudaStream_t stream);
 
+// A launch that starts with the one before it rather than after its end.
+inline cudaLaunchAttribute after_its_start() {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  return attr;
+}
+
 // Gated linear recurrence (gated_linear.cu).  Strides are element strides over (t, b); channels are dense.
 constexpr int GL_CHUNK = ELMAN_GATED_LINEAR_CHUNK;
 struct GatedLinearArgs {

@@ -448,6 +448,7 @@ __global__ void __launch_bounds__(32 * FW, 2) gl_forward_tile_kernel(GlParams p,
   const int w = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const long cols = (long)p.B * p.d;
   const int total = tiles * col_groups;
+  ptx::wait_for_previous();
   if (threadIdx.x == 0) {
     sh.gave_up = 0;
     sh.next = tiles > 1 ? (int)(atomicAdd(ch.ctrl, 1u) + 1u) : (int)blockIdx.x;
@@ -516,6 +517,7 @@ __global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const long cols = (long)p.B * p.d;
   const int total = tiles * col_groups;
+  ptx::wait_for_previous();
   if (threadIdx.x == 0) {
     sh.gave_up = 0;
     sh.next = tiles > 1 ? (int)(atomicAdd(ch.ctrl, 1u) + 1u) : (int)blockIdx.x;
@@ -982,6 +984,7 @@ gl_forward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
     ptx::mbar_fence_init();
   }
   __syncthreads();
+  ptx::wait_for_previous();
   if (w >= W + V) {
     if constexpr (FEED != FEED_TMA) {
       const void* const in[3] = {p.f, p.c, p.z};
@@ -1083,6 +1086,7 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
     ptx::mbar_fence_init();
   }
   __syncthreads();
+  ptx::wait_for_previous();
   if (w >= BW + V) {
     if constexpr (FEED != FEED_TMA) {
       const void* const in[4] = {p.f, p.c, p.z, p.dy};
@@ -1211,7 +1215,7 @@ int tiles_of(int T, int steps) { return (int)(((long)T + steps - 1) / steps); }
 
 size_t chain_bytes(int tiles, long cols) {
   if (tiles <= 1) return 0;
-  return 256 + (size_t)tiles * cols * sizeof(float2) + (size_t)((tiles + GROUP - 1) / GROUP) * cols * sizeof(float);
+  return (256 + (size_t)tiles * cols * sizeof(float2) + (size_t)((tiles + GROUP - 1) / GROUP) * cols * sizeof(float) + 15) / 16 * 16;
 }
 
 // Two channels a lane where every row of every tensor allows 4-byte accesses.
@@ -1246,6 +1250,36 @@ FeedKind feed_of(int dtype, const GatedLinearArgs& a, bool bwd) {
   see(bwd ? a.dy : a.y, a.y_strides);
   if (bwd) { see(a.df, a.df_strides); see(a.dc, a.dc_strides); see(a.dz, a.dz_strides); }
   return ok ? FEED_TMA : dtype == ELMAN_F32 || pairs_of_channels(a, bwd) ? FEED_ROWS4 : FEED_ROWS2;
+}
+
+// The workspace's start; the scan's launch overlaps it (T512 B32 d1280: a call takes 2 us less than behind a memset).
+__global__ void __launch_bounds__(256) gl_fill_kernel(uint4* ws, long n) {
+  ptx::let_next_start();
+  const uint4 x = make_uint4(NOT_YET, NOT_YET, NOT_YET, NOT_YET);
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) ws[i] = x;
+}
+
+// The scan's launch, behind the workspace's where there is a chain.
+template <typename... P, typename... A>
+int launch_scan(void (*kernel)(P...), int tiles, long cols, void* workspace, unsigned grid, int threads, int smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr = after_its_start();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 0;
+  if (tiles > 1) {
+    const long pieces = (long)(chain_bytes(tiles, cols) / 16), blocks = (pieces + 255) / 256;
+    gl_fill_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, st>>>((uint4*)workspace, pieces);
+    count_launch(false);
+    cfg.numAttrs = 1;
+  }
+  ELMAN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
+  count_launch(false);
+  ELMAN_CUDA_CHECK(cudaGetLastError());
+  return ELMAN_OK;
 }
 
 void prepare_chain(GlChain& ch, const GatedLinearArgs& a, int tiles, long cols) {
@@ -1301,16 +1335,13 @@ int launch_fed(int dtype, const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
   }
   GlChain ch{};
   prepare_chain(ch, a, g.tiles, g.cols);
-  if (g.tiles > 1) ELMAN_CUDA_CHECK(cudaMemsetAsync(a.workspace, 0xFF, chain_bytes(g.tiles, g.cols), st));
   const GlParams p = params_of(a);
   const unsigned grid = (unsigned)(g.tiles > 1 && total > 148 * 2 ? 148 * 2 : total);
   if (bwd)
-    gl_backward_fed_kernel<T, V, RESET, FEED><<<grid, 32 * (BW + V) + producer_threads(FEED, V), smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], p, ch, g);
-  else
-    gl_forward_fed_kernel<T, V, RESET, FEED><<<grid, 32 * (forward_warps(FEED) + V) + producer_threads(FEED, V), smem, st>>>(m[0], m[1], m[2], m[3], p, ch, g);
-  count_launch(false);
-  ELMAN_CUDA_CHECK(cudaGetLastError());
-  return ELMAN_OK;
+    return launch_scan(&gl_backward_fed_kernel<T, V, RESET, FEED>, g.tiles, g.cols, a.workspace, grid,
+                       32 * (BW + V) + producer_threads(FEED, V), smem, st, m[0], m[1], m[2], m[3], m[4], m[5], m[6], p, ch, g);
+  return launch_scan(&gl_forward_fed_kernel<T, V, RESET, FEED>, g.tiles, g.cols, a.workspace, grid,
+                     32 * (forward_warps(FEED) + V) + producer_threads(FEED, V), smem, st, m[0], m[1], m[2], m[3], p, ch, g);
 }
 
 template <typename T, int V, bool RESET>
@@ -1328,15 +1359,11 @@ int launch_tiles(const GatedLinearArgs& a, bool bwd, cudaStream_t st) {
   prepare_chain(ch, a, tiles, cols);
   long grid = total;
   if (tiles > 1) {
-    ELMAN_CUDA_CHECK(cudaMemsetAsync(a.workspace, 0xFF, chain_bytes(tiles, cols), st));
     const long resident = 148 * 2;       // the counter hands out the tiles
     if (grid > resident) grid = resident;
   }
   GlParams p = params_of(a);
-  kernel<<<(unsigned)grid, 32 * warps, 0, st>>>(p, ch, tiles, (int)col_groups);
-  count_launch(false);
-  ELMAN_CUDA_CHECK(cudaGetLastError());
-  return ELMAN_OK;
+  return launch_scan(kernel, tiles, cols, a.workspace, (unsigned)grid, 32 * warps, 0, st, p, ch, tiles, (int)col_groups);
 }
 
 template <bool RESET>

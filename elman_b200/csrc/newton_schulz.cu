@@ -173,11 +173,6 @@ __device__ __forceinline__ uint4 to_halves(const float (&f)[8]) {
 
 // ------------------------------------------------------------------ start: norm and scaling
 
-// The three launches of a call overlap: each lets the next one start when its own blocks have, and that one waits here
-// before it touches memory (all of what came before has ended then).
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // Muon's momentum moves by (1 - mu)(g - momentum); the update is it, or Nesterov's look ahead.
 __device__ __forceinline__ float advance(const NsSource& s, float g, float gs, float& momentum) {
   g *= gs;
@@ -206,7 +201,7 @@ __device__ __forceinline__ void store8(float* at, const float (&f)[8]) {
 // the counters of the products.
 template <typename T>
 __global__ void __launch_bounds__(256) ns_norm_kernel(NsSource s, long size, double* partial, int* ticket, int* done) {
-  let_next_start();
+  ptx::let_next_start();
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     done[blockIdx.y] = 0;
     if (blockIdx.y == 0) *ticket = 0;
@@ -252,8 +247,8 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsSource s, long size, dou
 // A warp a row: X_0, scaled, as the sum of two fp16 numbers.
 template <typename T>
 __global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n, long ld, float eps, const double* partial, Split x) {
-  let_next_start();
-  wait_for_previous();
+  ptx::let_next_start();
+  ptx::wait_for_previous();
   const int lane = threadIdx.x & 31;
   static_assert(NORM_PARTS == 64, "two partial sums a lane");
   double total = partial[(long)blockIdx.y * NORM_PARTS + lane] + partial[(long)blockIdx.y * NORM_PARTS + 32 + lane];
@@ -432,7 +427,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
   ptx::tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
   volatile int* abortp = &abort_flag;
-  wait_for_previous();
+  ptx::wait_for_previous();
   const int sums = p.parts > 1 ? 1 : 2;              // accumulators in turn (fp32: one of four partial sums)
   auto give_up = [&](int where) {
     abort_flag = 1;
@@ -850,13 +845,6 @@ int triangle_of(int r, int edge, int columns) {
 int columns_of(const NsPlan& p, int wide, int narrow, int stages) {
   auto cost = [&](int tiles, double tile) { return ceil((double)tiles * p.count / 148) * (800. * stages * p.parts + tile); };
   return cost(narrow, 7900) < cost(wide, 10400) ? 64 : 128;
-}
-
-cudaLaunchAttribute after_its_start() {              // of the launch before, rather than after its end
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  return attr;
 }
 
 template <typename T, bool PAIR>
