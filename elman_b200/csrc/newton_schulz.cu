@@ -3,7 +3,7 @@
 // (tall matrices: A = X^T X and X <- a X + X B, so that A has the smaller of the two extents, r).
 // A and B are symmetric: only the tiles on and above the diagonal are computed and stored.  Per step 3 r^2 q + r^3
 // flops with q the larger extent: bound by the tensor cores.  Measured, five steps on bf16: 18 x 1280 x 1280 872 us (866
-// TFLOP/s), 2 x 4096 x 4096 2.2 ms (1246); each block of a pair takes in 64 bytes a cycle of products, about what an SM
+// TFLOP/s), 2 x 4096 x 4096 2.2 ms (1240); each block of a pair takes in 64 bytes a cycle of products, about what an SM
 // gets from L2, and a stage of 512 cycles lasts 600 to 700.  Small matrices are bound by the latency of 15 products one
 // after another: 1 x 256 x 256 90 us, 6 us each (about: loads 2, products 1.4, rows 1.2, stores made visible and seen 1.2).
 //
