@@ -2,25 +2,23 @@
 //   X = G / (|G|_F + eps);  steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X
 // (tall matrices: A = X^T X and X <- a X + X B, so that A has the smaller of the two extents, r).
 // A and B are symmetric: only the tiles on and above the diagonal are computed and stored.  Per step 3 r^2 q + r^3
-// flops with q the larger extent: bound by the tensor cores.  Measured, five steps on bf16: 18 x 1280 x 1280 872 us (866
-// TFLOP/s), 2 x 4096 x 4096 2.2 ms (1240); each block of a pair takes in 64 bytes a cycle of products, about what an SM
-// gets from L2, and a stage of 512 cycles lasts 600 to 700.  Small matrices are bound by the latency of 15 products one
-// after another: 1 x 256 x 256 90 us, 6 us each (about: loads 2, products 1.4, rows 1.2, stores made visible and seen 1.2).
+// flops with q the larger extent, three products for each of them (Numbers, below): bound by the tensor cores.
+// Measured, five steps on bf16, the same inputs again and again: 18 x 1280 x 1280 1.79 ms (1260 TFLOP/s of such products),
+// 1 x 4096 x 4096 2.98 ms (1380), at the power limit.  Small matrices are bound by the latency of 15 products one after
+// another: 1 x 256 x 256 109 us, 7 us each (about: loads 2, products 2, rows 1.5, stores made visible and seen 1.2).
 //
-// Numbers.  The operands are fp16 (11 significant bits; bf16 has 8), scaled by powers of two into its
-// range: X by 2^12, A by 2^12, B by 2^10; every sum is fp32.  The polynomial multiplies small singular
-// values by a (3.44) a step, and with them what rounding X puts into their directions: a gradient with a
-// few strong directions above noise comes out 1.1e-2 off with X in fp16 alone (8e-2 in bf16).  So X is kept
-// as the sum of two fp16 numbers, and the term a X takes both, in all but the last two steps: 7e-4.  Near the end
-// the polynomial's slope is small and rounding a X and B X alike is what keeps the error small.
-// fp32 matrices take both parts of X, A and B into the products as well (three products for one): 5e-6.  The tensor
-// cores cut their fp32 sums off rather than rounding them, which over a long contraction adds up (2.5e-5 at
-// 33 x 2000 with one sum): there the large products take turns in three sums and the small ones have a fourth (3.4e-6 at
-// 200 x 2000, 1.2e-5 at 200 x 9000, 2.9e-5 at 1000 x 20000).  A step along K brings the high parts of both operands in one
-// stage and the low parts in the next, for all three products: 4 x 1000 x 257 250 us with a stage a product, now 188.
+// Numbers.  X, A and B are each kept as the sum of two fp16 numbers (22 significant bits), scaled by powers of two into
+// their range: X by 2^12, A by 2^12, B by 2^10.  A product is three: high x high, high x low, low x high; every sum is
+// fp32.  So a bf16 result is the exact one rounded (one fp16 number an operand leaves 1.3e-3 before that rounding,
+// as much as the rounding itself), and an fp32 result is 5e-6 off.  The tensor cores cut their fp32 sums off rather than
+// rounding them, which over a long contraction adds up (2.5e-5 at 33 x 2000 with one sum): for fp32 matrices the large
+// products take turns in three sums and the small ones have a fourth (3.4e-6 at 200 x 2000, 1.2e-5 at 200 x 9000, 2.9e-5 at
+// 1000 x 20000).  A step along K brings the high parts of both operands in one stage and the low parts in the next, for all
+// three products: 4 x 1000 x 257 fp32 250 us with a stage a product, now 188.
 #include <math.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "sm100_ptx.cuh"
@@ -55,7 +53,7 @@ __device__ __forceinline__ bool mn_major(int form, int row0, int k0, int edge) {
   return form == K_ROWS || (form == UPPER && row0 / edge > k0 / edge);
 }
 
-struct Split { __half* hi; __half* lo; };             // lo may be null
+struct Split { __half* hi; __half* lo; };
 
 // The matrix a step starts from: G, or Muon's momentum-weighted gradient.
 struct NsSource {
@@ -75,8 +73,7 @@ struct NsMaps { NsMap x[2], a, b; };
 // then the updates'.  (Groups of matrices that stay in L2 from product to product were slower: 18 x 1280 x 1280 as three
 // groups 0.98 ms, as one 0.87: waiting for the matrix one reads costs more than reading it from HBM.)
 struct NsPlan {
-  int count, m, n, r, tall, steps, parts;
-  int split;                 // bf16: 1: both parts of B go into the products, 2: of A as well
+  int count, m, n, r, tall, steps;
   int edge, n_sym, n_upd;    // rows of a tile; columns of a symmetric product's tiles and of an update's
   int triangle, all;         // tiles of a symmetric product and of an update
   int per_step, total;       // items of the list
@@ -93,7 +90,6 @@ struct NsPlan {
   long spin_limit;
   int stall;                 // test hook
 };
-__host__ __device__ inline bool takes_low(int step, int steps, int parts) { return parts > 1 || step < steps - 2; }
 
 // One item of the list.  Taking it apart costs divisions, a thousand cycles of latency: the warp that takes items does
 // it ahead of time and hands on the four numbers that the rest follows from.
@@ -130,13 +126,11 @@ struct NsItem {
   int kind, mat, ti, tj, step;
   int columns;                                 // of the tile
   int m, n, K, a_form, b_form;
-  int parts;                                   // products of high and low parts
 };
 __device__ __forceinline__ NsItem item_of(const NsPlan& p, NsSlot k) {
   NsItem it;
   it.kind = k.kind; it.mat = k.mat; it.ti = k.tile >> 16; it.tj = k.tile & 0xFFFF; it.step = k.step;
   const bool symmetric = k.kind == GRAM || k.kind == SQUARE;
-  it.parts = p.split == 0 || k.kind == GRAM ? p.parts : k.kind != SQUARE ? 2 : p.split == 2 ? 3 : 1;
   it.columns = symmetric ? p.n_sym : p.n_upd;
   it.m = symmetric ? p.r : p.m;
   it.n = symmetric ? p.r : p.n;
@@ -275,10 +269,8 @@ __global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n,
         for (int j = 0; j < 8; ++j) f[j] *= scale;
         const uint4 h = to_halves(f);
         *reinterpret_cast<uint4*>(x.hi + to + col) = h;
-        if (x.lo != nullptr) {
-          add_halves(f, h, -1.f);
-          *reinterpret_cast<uint4*>(x.lo + to + col) = to_halves(f);
-        }
+        add_halves(f, h, -1.f);
+        *reinterpret_cast<uint4*>(x.lo + to + col) = to_halves(f);
       }
     } else {
       for (int col = lane; col < n; col += 32) {
@@ -287,7 +279,7 @@ __global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n,
         v *= scale;
         const __half hi = __float2half_rn(v);
         x.hi[to + col] = hi;
-        if (x.lo != nullptr) x.lo[to + col] = __float2half_rn(v - __half2float(hi));
+        x.lo[to + col] = __float2half_rn(v - __half2float(hi));
       }
     }
   }
@@ -302,7 +294,7 @@ __device__ __forceinline__ void sts_u4(uint32_t addr, uint4 v) {
 // What becomes of a product: k_acc * product + k_same * same.
 struct Finish {
   float k_acc, k_same;
-  Split same, out;                 // at the item's matrix; lo null: not used
+  Split same, out;                 // at the item's matrix
   long ld;
 };
 __device__ __forceinline__ Finish finish_of(const NsPlan& p, const NsItem& it) {
@@ -318,16 +310,14 @@ __device__ __forceinline__ Finish finish_of(const NsPlan& p, const NsItem& it) {
     f.ld = p.ldx;
     f.same = p.X[at];
     f.out = p.X[at ^ 1];
-    if (!takes_low(it.step, p.steps, p.parts)) f.same.lo = nullptr;
-    if (!takes_low(it.step + 1, p.steps, p.parts)) f.out.lo = nullptr;
     f.k_acc = it.kind == LAST ? 1.f / (SB * SX) : 1.f / SB;
     f.k_same = it.kind == LAST ? p.a / SX : p.a;
   }
   const long off = (long)it.mat * it.m * f.ld;
   f.same.hi += off;
+  f.same.lo += off;
   f.out.hi += off;
-  if (f.same.lo != nullptr) f.same.lo += off;
-  if (f.out.lo != nullptr) f.out.lo += off;
+  f.out.lo += off;
   return f;
 }
 // A box's 16-byte pieces as a warp moves them: piece (lane & 3) of row 8 k + lane / 4.  Rows are whole groups of eight in
@@ -342,7 +332,7 @@ __device__ __forceinline__ void fetch_box(Box& x, const Finish& f, const NsItem&
     if (it.kind == GRAM || row >= it.m || col >= it.n) continue;
     // (written by other blocks of this launch: from L2)
     x.hi[k] = __ldcg(reinterpret_cast<const uint4*>(f.same.hi + (long)row * f.ld + col));
-    if (f.same.lo != nullptr) x.lo[k] = __ldcg(reinterpret_cast<const uint4*>(f.same.lo + (long)row * f.ld + col));
+    x.lo[k] = __ldcg(reinterpret_cast<const uint4*>(f.same.lo + (long)row * f.ld + col));
   }
 }
 
@@ -359,7 +349,8 @@ template <> __device__ __forceinline__ float lds_as<float>(uint32_t addr) {
   return v;
 }
 template <> __device__ __forceinline__ bf16 lds_as<bf16>(uint32_t addr) { return __ushort_as_bfloat16(tch::lds_u16(addr)); }
-template <typename T>
+// A parameter that Muon moves is rounded once: its share of X comes in fp32 (S).
+template <typename T, typename S>
 __device__ __forceinline__ void write_result(const NsPlan& p, const NsItem& it, uint32_t box, int row0, int col0) {
   const int lane = threadIdx.x & 31, rows = it.m - row0 < 32 ? it.m - row0 : 32;
   if (col0 + lane >= it.n) return;
@@ -367,9 +358,9 @@ __device__ __forceinline__ void write_result(const NsPlan& p, const NsItem& it, 
 #pragma unroll 8
   for (int r = 0; r < 32; ++r) {
     if (r >= rows) break;
-    const T x = lds_as<T>(result_at<T>(box, r, lane));
+    const S x = lds_as<S>(result_at<S>(box, r, lane));
     if (p.muon) dst[(long)r * p.n] = from_f<T>(to_f(dst[(long)r * p.n]) * p.decay - p.lr * p.scale * to_f(x));
-    else dst[(long)r * p.n] = x;
+    else dst[(long)r * p.n] = from_f<T>(to_f(x));
   }
 }
 
@@ -384,6 +375,10 @@ __device__ __forceinline__ void write_result(const NsPlan& p, const NsItem& it, 
 template <typename T, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ NsMaps maps, const NsPlan p) {
   constexpr int EDGE = PAIR ? 256 : 128, BLOCKS = PAIR ? 2 : 1;
+  constexpr bool SUMS = sizeof(T) == 4;              // fp32: four partial sums; else two accumulators in turn
+  static_assert((SUMS ? 4 : 2) * EDGE <= 512, "tensor memory");
+  static_assert(STAGES % 2 == 0, "high and low parts lie side by side");
+  constexpr int sums = SUMS ? 1 : 2;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2], tk_full[TICKETS], tk_empty[TICKETS], go[TICKETS];
   __shared__ NsSlot tk[TICKETS];
@@ -428,7 +423,6 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
   const uint32_t tmem_base = tmem_slot;
   volatile int* abortp = &abort_flag;
   ptx::wait_for_previous();
-  const int sums = p.parts > 1 ? 1 : 2;              // accumulators in turn (fp32: one of four partial sums)
   auto give_up = [&](int where) {
     abort_flag = 1;
     if constexpr (PAIR)
@@ -495,31 +489,29 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         if (!wait_for(&go[k], q)) { give_up(0xFFF8); break; }
         free_ticket(q);                               // (not before: the start of the slot's next item would hide this one's)
         ptx::fence_proxy_async_global();              // written by other blocks, read here by TMA
-        const int both = it.parts == 3, stages = (it.K + BK - 1) / BK << both;   // both: a stage of high parts, one of low parts
-        for (int part = 0; part < (both ? 1 : it.parts) && ok; ++part) {
-          for (int i = 0; i < stages; ++i, ++iteration) {
-            const int k0 = (i >> both) * BK, low = both ? i & 1 : part == 1 && first == (p.tall == 0);   // (two parts: B's)
-            if (!claimed && !claim()) { give_up(k0); ok = false; break; }
-            claimed = false;
-            const bool mn = mn_major(form, row0, k0, EDGE);
-            const uint32_t bar = bars + 8 * s;
-            if (!(iteration == p.stall && blockIdx.x == 0)) {
-              uint8_t* dst = to + s * OPERAND_BYTES;
-              auto copy = [&](uint8_t* d, const CUtensorMap* m, int x, int y) {
-                if constexpr (PAIR) ptx::tma_load_3d_pair(d, m, x, y, it.mat, bar);
-                else tch::tma_load_3d(d, m, x, y, it.mat, &full_bar[s]);
-              };
-              if (!PAIR && !first && it.columns == 64) {
-                copy(dst, &map.block[low], mn ? row0 : k0, mn ? k0 : row0);
-              } else if (mn) {
-                copy(dst, &map.block[low], row0, k0);
-                copy(dst + BLOCK_BYTES, &map.block[low], row0 + 64, k0);
-              } else {
-                copy(dst, &map.rows[low], k0, row0);
-              }
+        const int stages = 2 * ((it.K + BK - 1) / BK);   // high parts, low parts
+        for (int i = 0; i < stages; ++i, ++iteration) {
+          const int k0 = (i >> 1) * BK, low = i & 1;
+          if (!claimed && !claim()) { give_up(k0); ok = false; break; }
+          claimed = false;
+          const bool mn = mn_major(form, row0, k0, EDGE);
+          const uint32_t bar = bars + 8 * s;
+          if (!(iteration == p.stall && blockIdx.x == 0)) {
+            uint8_t* dst = to + s * OPERAND_BYTES;
+            auto copy = [&](uint8_t* d, const CUtensorMap* m, int x, int y) {
+              if constexpr (PAIR) ptx::tma_load_3d_pair(d, m, x, y, it.mat, bar);
+              else tch::tma_load_3d(d, m, x, y, it.mat, &full_bar[s]);
+            };
+            if (!PAIR && !first && it.columns == 64) {
+              copy(dst, &map.block[low], mn ? row0 : k0, mn ? k0 : row0);
+            } else if (mn) {
+              copy(dst, &map.block[low], row0, k0);
+              copy(dst + BLOCK_BYTES, &map.block[low], row0 + 64, k0);
+            } else {
+              copy(dst, &map.rows[low], k0, row0);
             }
-            if (++s == STAGES) { s = 0; ph ^= 1u; }
           }
+          if (++s == STAGES) { s = 0; ph ^= 1u; }
         }
         if (!ok) break;
       }
@@ -561,46 +553,38 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
         const int b = q % sums;
         if (!ptx::mbar_wait(&acc_empty[b], ((uint32_t)(q / sums) & 1u) ^ 1u, p.spin_limit * 8, abortp)) { give_up(0xFFFE); break; }
         ptx::tc_fence_after();
-        const uint32_t sum0 = tmem_base + (uint32_t)(b * EDGE);
-        int i = 0;                                    // steps of this item along K, over all parts
-        for (int part = 0; part < (it.parts == 3 ? 1 : it.parts) && ok; ++part) {
-          for (int k0 = 0; k0 < it.K && ok;) {
-            // the stretch of K in which both operands keep their form: an upper matrix changes at the diagonal
-            int end = it.K;
-            if (it.a_form == UPPER && k0 < m0) end = m0;
-            if (it.b_form == UPPER && k0 < n0 && n0 < end) end = n0;
-            const bool a_mn = mn_major(it.a_form, m0, k0, EDGE), b_mn = mn_major(it.b_form, n0, k0, EDGE);
-            const uint32_t idesc = ptx::umma_idesc_f16(EDGE, PAIR ? EDGE : it.columns) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
-            const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
-            const uint64_t da0 = a_mn ? ptx::umma_desc_mn_sw128(ptx::smem_u32(sA), BLOCK_BYTES) : ptx::umma_desc_k_sw128(ptx::smem_u32(sA));
-            const uint64_t db0 = b_mn ? ptx::umma_desc_mn_sw128(ptx::smem_u32(sB), BLOCK_BYTES) : ptx::umma_desc_k_sw128(ptx::smem_u32(sB));
-            for (; k0 < end; k0 += BK, ++i) {
-              if (!ready && !ptx::mbar_wait(&full_bar[s], ph, p.spin_limit, abortp)) { give_up(i); ok = false; break; }
-              uint32_t s_next = s + 1, ph_next = ph;
-              if (s_next == STAGES) { s_next = 0; ph_next ^= 1u; }
-              const uint64_t da = da0 + (uint64_t)(s * (OPERAND_BYTES / 16)), db = db0 + (uint64_t)(s * (OPERAND_BYTES / 16));
-              if constexpr (PAIR) {
-                ready = ptx::umma_stage_pair(sum0, da, db, a_step, b_step, idesc, i > 0 ? 1u : 0u, &empty_bar[s], &full_bar[s_next],
-                                             ph_next);
-              } else if (it.parts == 3) {
-                // high x high, high x low, low x high, from two stages.  fp32: the large products take turns in three sums,
-                // the others have a fourth
-                const uint32_t large = tmem_base + (uint32_t)((p.parts > 1 ? i % 3 : b) * EDGE), small = tmem_base + (uint32_t)((p.parts > 1 ? 3 : b) * EDGE);
-                const bool opens = i < (p.parts > 1 ? 3 : 1);
-                if (!ptx::umma_stage<false>(large, da, db, a_step, b_step, idesc, opens ? 0u : 1u, &empty_bar[s], &full_bar[s_next], ph_next) &&
-                    !ptx::mbar_wait(&full_bar[s_next], ph_next, p.spin_limit, abortp)) { give_up(i); ok = false; break; }
-                const uint32_t low = s_next;
-                const uint64_t da_low = da0 + (uint64_t)(low * (OPERAND_BYTES / 16)), db_low = db0 + (uint64_t)(low * (OPERAND_BYTES / 16));
-                if (++s_next == STAGES) { s_next = 0; ph_next ^= 1u; }
-                ptx::umma_stage<false>(small, da, db_low, a_step, b_step, idesc, p.parts > 1 && i == 0 ? 0u : 1u, &empty_bar[s], &full_bar[s_next], ph_next);
-                ready = ptx::umma_stage(small, da_low, db, a_step, b_step, idesc, 1u, &empty_bar[s], &full_bar[s_next], ph_next);
-                ptx::umma_commit(&empty_bar[low]);
-              } else {
-                ready = ptx::umma_stage(sum0, da, db, a_step, b_step, idesc, i > 0 ? 1u : 0u, &empty_bar[s], &full_bar[s_next], ph_next);
-              }
-              s = s_next;
-              ph = ph_next;
-            }
+        // high x high, high x low, low x high, from two stages
+        for (int k0 = 0, i = 0; k0 < it.K && ok;) {
+          // the stretch of K in which both operands keep their form: an upper matrix changes at the diagonal
+          int end = it.K;
+          if (it.a_form == UPPER && k0 < m0) end = m0;
+          if (it.b_form == UPPER && k0 < n0 && n0 < end) end = n0;
+          const bool a_mn = mn_major(it.a_form, m0, k0, EDGE), b_mn = mn_major(it.b_form, n0, k0, EDGE);
+          const uint32_t idesc = ptx::umma_idesc_f16(EDGE, PAIR ? EDGE : it.columns) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+          const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
+          const uint64_t da0 = a_mn ? ptx::umma_desc_mn_sw128(ptx::smem_u32(sA), BLOCK_BYTES) : ptx::umma_desc_k_sw128(ptx::smem_u32(sA));
+          const uint64_t db0 = b_mn ? ptx::umma_desc_mn_sw128(ptx::smem_u32(sB), BLOCK_BYTES) : ptx::umma_desc_k_sw128(ptx::smem_u32(sB));
+          for (; k0 < end; k0 += BK, ++i) {
+            if (!ready && !ptx::mbar_wait(&full_bar[s], ph, p.spin_limit, abortp)) { give_up(i); ok = false; break; }
+            const uint32_t low = s + 1;                 // (stages are even in number)
+            const uint32_t next = low + 1 == STAGES ? 0 : low + 1, next_ph = ph ^ (next == 0 ? 1u : 0u);
+            const uint64_t da = da0 + (uint64_t)(s * (OPERAND_BYTES / 16)), db = db0 + (uint64_t)(s * (OPERAND_BYTES / 16));
+            const uint64_t da_low = da + OPERAND_BYTES / 16, db_low = db + OPERAND_BYTES / 16;
+            const uint32_t large = tmem_base + (uint32_t)((SUMS ? i % 3 : b) * EDGE), small = tmem_base + (uint32_t)((SUMS ? 3 : b) * EDGE);
+            const uint32_t large_on = i < (SUMS ? 3 : 1) ? 0u : 1u, small_on = SUMS && i == 0 ? 0u : 1u;
+            auto products = [&](auto free, uint32_t sum, uint64_t x, uint64_t y, uint32_t on, uint32_t test, uint32_t test_ph) {
+              constexpr bool FREE = decltype(free)::value;
+              if constexpr (PAIR) return ptx::umma_stage_pair<FREE>(sum, x, y, a_step, b_step, idesc, on, &empty_bar[s], &full_bar[test], test_ph);
+              else return ptx::umma_stage<FREE>(sum, x, y, a_step, b_step, idesc, on, &empty_bar[s], &full_bar[test], test_ph);
+            };
+            if (!products(std::false_type(), large, da, db, large_on, low, ph) &&
+                !ptx::mbar_wait(&full_bar[low], ph, p.spin_limit, abortp)) { give_up(i); ok = false; break; }
+            products(std::false_type(), small, da, db_low, small_on, next, next_ph);
+            ready = products(std::true_type(), small, da_low, db, 1u, next, next_ph);
+            if constexpr (PAIR) ptx::umma_commit_pair(&empty_bar[low], 3);
+            else ptx::umma_commit(&empty_bar[low]);
+            s = next;
+            ph = next_ph;
           }
         }
         if (ok) {
@@ -649,7 +633,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           : "memory");
       if (stop) break;
       ptx::tc_fence_after();
-      const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((p.parts > 1 ? 0 : b * EDGE) + half * (it.columns / 2));
+      const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * EDGE + half * (it.columns / 2));
       const int nk = (it.K + BK - 1) / BK, boxes = it.columns / 64;
 #pragma unroll 1
       for (int c = 0; c < boxes; ++c) {
@@ -661,13 +645,13 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           for (int k = 0; k < 4; ++k) {
             const uint32_t at = piece_at(buffer, 8 * k + (lane >> 2), lane & 3);
             sts_u4(at, same.hi[k]);
-            if (fin.same.lo != nullptr) sts_u4(at + BOX_BYTES, same.lo[k]);
+            sts_u4(at + BOX_BYTES, same.lo[k]);
           }
           __syncwarp();
           if (c + 1 < boxes) fetch_box(same, fin, it, row0, col + 32);
         }
         ptx::tmem_ld_wait();
-        for (int sum = 1; sum < 4 && p.parts > 1; ++sum) {
+        for (int sum = 1; sum < (SUMS ? 4 : 1); ++sum) {
           if (sum < 3 && sum >= nk) continue;
           uint32_t more[32];
           ptx::tmem_ld32(tsrc + (uint32_t)(sum * EDGE + c * 32), more);
@@ -692,7 +676,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           const uint32_t piece = piece_at(buffer, lane, g);
           if (it.kind != GRAM) {
             add_halves(f, tch::lds_u4(piece), fin.k_same);
-            if (fin.same.lo != nullptr) add_halves(f, tch::lds_u4(piece + BOX_BYTES), fin.k_same);
+            add_halves(f, tch::lds_u4(piece + BOX_BYTES), fin.k_same);
           }
           if (it.kind == LAST) {
 #pragma unroll
@@ -701,22 +685,25 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           }
           const uint4 h = to_halves(f);
           sts_u4(piece, h);
-          if (fin.out.lo != nullptr) {
-            add_halves(f, h, -1.f);
-            sts_u4(piece + BOX_BYTES, to_halves(f));
-          }
+          add_halves(f, h, -1.f);
+          sts_u4(piece + BOX_BYTES, to_halves(f));
         }
         __syncwarp();
         if (it.kind == LAST) {
+          auto leave = [&](auto as) {
+            typedef decltype(as) S;
 #pragma unroll
-          for (int j = 0; j < 32; j += 16 / (int)sizeof(T)) {
-            alignas(16) T x[16 / sizeof(T)];
+            for (int j = 0; j < 32; j += 16 / (int)sizeof(S)) {
+              alignas(16) S x[16 / sizeof(S)];
 #pragma unroll
-            for (int k = 0; k < (int)(16 / sizeof(T)); ++k) x[k] = from_f<T>(__uint_as_float(r[j + k]));
-            sts_u4(result_at<T>(buffer, lane, j), *reinterpret_cast<const uint4*>(x));
-          }
-          __syncwarp();
-          write_result<T>(p, it, buffer, row0, col);
+              for (int k = 0; k < (int)(16 / sizeof(S)); ++k) x[k] = from_f<S>(__uint_as_float(r[j + k]));
+              sts_u4(result_at<S>(buffer, lane, j), *reinterpret_cast<const uint4*>(x));
+            }
+            __syncwarp();
+            write_result<T, S>(p, it, buffer, row0, col);
+          };
+          if (p.muon) leave(0.f);
+          else leave(T());
         } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -724,7 +711,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
             if (row >= it.m || to >= it.n) continue;
             const uint32_t at = piece_at(buffer, 8 * k + (lane >> 2), lane & 3);
             *reinterpret_cast<uint4*>(fin.out.hi + (long)row * fin.ld + to) = tch::lds_u4(at);
-            if (fin.out.lo != nullptr) *reinterpret_cast<uint4*>(fin.out.lo + (long)row * fin.ld + to) = tch::lds_u4(at + BOX_BYTES);
+            *reinterpret_cast<uint4*>(fin.out.lo + (long)row * fin.ld + to) = tch::lds_u4(at + BOX_BYTES);
           }
         }
         __syncwarp();
@@ -748,12 +735,6 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
 
 long padded(long x) { return (x + 7) / 8 * 8; }       // rows start on 16 bytes
 
-// Where r is small A and B are mostly diagonal, all of it rounded alike, and B X is nearly three times the result it
-// becomes part of: 24 x 800 comes out 2.2e-3 off before the last rounding (with it 2.8e-3; a rounded exact result is
-// 1.7e-3 off).  The second part of B in the update's product, one or two stages of latency a step, makes that 1.4e-3,
-// that of A as well, where r is a single stage, 0.9e-3 (101 us become 108).
-int splits(int dtype, int r) { return dtype == ELMAN_F32 || r > 128 ? 0 : r > BK ? 1 : 2; }
-
 struct NsBuffers {
   Split X[2], A, B;
   double* partial;
@@ -762,7 +743,7 @@ struct NsBuffers {
   long ldx, ldr;
   size_t bytes;
 };
-NsBuffers carve(void* ws, int dtype, int count, int m, int n) {
+NsBuffers carve(void* ws, int count, int m, int n) {
   NsBuffers b{};
   char* base = (char*)ws;
   size_t off = 0;
@@ -780,9 +761,9 @@ NsBuffers carve(void* ws, int dtype, int count, int m, int n) {
     b.X[k].lo = (__half*)take(x);
   }
   b.A.hi = (__half*)take(a);
+  b.A.lo = (__half*)take(a);
   b.B.hi = (__half*)take(a);
-  if (dtype == ELMAN_F32 || splits(dtype, r) == 2) b.A.lo = (__half*)take(a);
-  if (dtype == ELMAN_F32 || splits(dtype, r) > 0) b.B.lo = (__half*)take(a);
+  b.B.lo = (__half*)take(a);
   b.partial = (double*)take((size_t)count * NORM_PARTS * sizeof(double));
   b.ticket = (int*)take(sizeof(int));
   b.done = (int*)take((size_t)count * sizeof(int));
@@ -820,31 +801,32 @@ bool stays_in_range(int steps, double a, double b, double c) {
   return true;
 }
 
-// Pairs make four times the tile in little more than the time of a single block's: about 600 cycles a stage and 11000 a
-// tile against 550 and 7000 where tiles follow one another; 16000 a tile against 10400 for a matrix whose products wait for
-// one another, 800 a stage with single blocks (measured).  Single blocks also waste fewer rows of ragged matrices.
-// 6 x 640 x 1280 takes 257 us in pairs and 204 in single blocks, 18 x 512 x 512 209 and 178, 4 x 1280 x 1280 316 and 379,
-// 1 x 2048 x 2048 350 and 367.
+// Pairs make four times the tile of a single block with half as many units.  Measured, us: a step along K (three products)
+// 1.32 in pairs and 0.95 in single blocks where tiles follow one another, 0.5 and 1.5 a tile on top; where a matrix's products
+// wait for one another a step 0.9 and 0.7 and a product 9.8 and 5.9 more.  The smaller of the two times is covered by the
+// other but for a fifth.  Single blocks also waste fewer rows of ragged matrices.
+// 18 x 1280 x 1280 takes 1.79 ms in pairs and 2.31 in single blocks, 4 x 1280 x 1280 484 us and 572, 3 x 1280 x 1280 459 and 461,
+// 6 x 640 x 1280 363 and 273, 18 x 512 x 512 282 and 217, 2 x 200 x 9000 869 and 617, 1 x 2048 x 2048 690 and 610.
 bool pays_as_pairs(const NsPlan& p) {
-  if (p.parts > 1 || p.split > 0) return false;
   auto cost = [&](int edge, int units, double stage, double tile, double alone, double latency) {     // of a step
     const double side = (p.r + edge - 1) / edge, q = p.tall ? p.m : p.n, k_gram = ceil(q / BK), k = ceil((double)p.r / BK);
     const double tri = p.count * side * (side + 1) / 2 / units, all = p.count * side * ceil(q / edge) / units;
-    return fmax(tri * (k_gram * stage + tile) + (tri + all) * (k * stage + tile), (k_gram + 2 * k) * alone + 3 * latency);
+    const double busy = tri * (k_gram * stage + tile) + (tri + all) * (k * stage + tile), chain = (k_gram + 2 * k) * alone + 3 * latency;
+    return fmax(busy, chain) + 0.2 * fmin(busy, chain);
   };
-  return cost(256, 74, 600, 11000, 600, 16000) < cost(128, 148, 550, 7000, 800, 10400);
+  return cost(256, 74, 1.32, 0.5, 0.9, 9.8) < cost(128, 148, 0.95, 1.5, 0.7, 5.9);
 }
 // Tiles of the blocks (i, j >= i) of a symmetric product.
 int triangle_of(int r, int edge, int columns) {
   const int per = edge / columns, strips = (r + columns - 1) / columns, whole = strips / per;
   return per * (whole * (whole + 1) / 2) + strips % per * (whole + 1);
 }
-// Single blocks: tiles of 64 columns where they spread a product over more of the device.  They take about 2500 cycles
-// less from start to end, most of it in finishing rows: 1 x 256 x 256 89 us against 112, 4 x 512 x 512 122 and 140; but
-// 18 x 512 x 512 219 and 178.
+// Single blocks: tiles of 64 columns where they spread a product over more of the device.  From start to end they take
+// 8700 cycles and 1270 a step along K, tiles of 128 columns 11300 and 1330 (measured): 1 x 256 x 256 109 us against 131,
+// 4 x 512 x 512 156 and 176; but 18 x 512 x 512 309 and 217.
 int columns_of(const NsPlan& p, int wide, int narrow, int stages) {
-  auto cost = [&](int tiles, double tile) { return ceil((double)tiles * p.count / 148) * (800. * stages * p.parts + tile); };
-  return cost(narrow, 7900) < cost(wide, 10400) ? 64 : 128;
+  auto cost = [&](int tiles, double stage, double tile) { return ceil((double)tiles * p.count / 148) * (stage * stages + tile); };
+  return cost(narrow, 1270, 8700) < cost(wide, 1330, 11300) ? 64 : 128;
 }
 
 template <typename T, bool PAIR>
@@ -882,12 +864,10 @@ int launch(const NsMaps& maps, const NsPlan& p, cudaStream_t st) {
 
 template <typename T>
 int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t st) {
-  const NsBuffers buf = carve(g.workspace, g.dtype, g.count, g.m, g.n);
+  const NsBuffers buf = carve(g.workspace, g.count, g.m, g.n);
   p.count = g.count; p.m = g.m; p.n = g.n; p.tall = g.m > g.n;
   p.r = p.tall ? g.n : g.m;
   p.steps = g.steps;
-  p.parts = g.dtype == ELMAN_F32 ? 3 : 1;
-  p.split = splits(g.dtype, p.r);
   p.a = g.a; p.b = g.b; p.c = g.c;
   p.X[0] = buf.X[0]; p.X[1] = buf.X[1]; p.A = buf.A; p.B = buf.B;
   p.ldx = buf.ldx; p.ldr = buf.ldr;
@@ -895,7 +875,7 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   p.status = device_status_ptr();
   p.spin_limit = options().spin_limit;
   p.stall = (int)options().test_stall_step;
-  const bool pair = pays_as_pairs(p);
+  const bool pair = sizeof(T) == 2 && pays_as_pairs(p);
   const int edge = pair ? 256 : 128;
   p.edge = p.n_sym = p.n_upd = edge;
   const int upd_rows = (p.m + edge - 1) / edge;
@@ -913,7 +893,7 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   NsMaps maps;
   auto map = [&](NsMap& out, const Split& x, int rows, int cols, long ld) {
     for (int low = 0; low < 2; ++low) {
-      const __half* base = low && x.lo != nullptr ? x.lo : x.hi;
+      const __half* base = low ? x.lo : x.hi;
       const uint64_t all = (uint64_t)rows * ld;
       ELMAN_RETURN_IF(make_tmap_f16(&out.rows[low], base, cols, rows, p.count, ld, all, 128));
       ELMAN_RETURN_IF(make_tmap_f16(&out.block[low], base, cols, rows, p.count, ld, all, 64));
@@ -925,8 +905,6 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   ELMAN_RETURN_IF(map(maps.a, buf.A, p.r, p.r, buf.ldr));
   ELMAN_RETURN_IF(map(maps.b, buf.B, p.r, p.r, buf.ldr));
   const long size = (long)p.m * p.n, blocks = (p.m + 7) / 8;
-  Split x0 = buf.X[0];
-  if (!takes_low(0, p.steps, p.parts)) x0.lo = nullptr;
   ns_norm_kernel<T><<<dim3(NORM_PARTS, p.count), 256, 0, st>>>(src, size, buf.partial, buf.ticket, buf.done);
   count_launch(false);
   cudaLaunchAttribute attr = after_its_start();
@@ -936,15 +914,17 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  ELMAN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ns_scale_kernel<T>, src, p.m, p.n, buf.ldx, g.eps, (const double*)buf.partial, x0));
+  ELMAN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ns_scale_kernel<T>, src, p.m, p.n, buf.ldx, g.eps, (const double*)buf.partial, buf.X[0]));
   count_launch(false);
   ELMAN_CUDA_CHECK(cudaGetLastError());
-  return pair ? launch<T, true>(maps, p, st) : launch<T, false>(maps, p, st);
+  if constexpr (sizeof(T) == 2)
+    if (pair) return launch<T, true>(maps, p, st);
+  return launch<T, false>(maps, p, st);
 }
 
 }  // namespace
 
-size_t newton_schulz_workspace(int dtype, int count, int m, int n) { return carve(nullptr, dtype, count, m, n).bytes; }
+size_t newton_schulz_workspace(int, int count, int m, int n) { return carve(nullptr, count, m, n).bytes; }
 bool newton_schulz_in_range(int steps, float a, float b, float c) { return stays_in_range(steps, a, b, c); }
 
 int newton_schulz(const NewtonSchulzArgs& a, cudaStream_t st) {

@@ -311,6 +311,8 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t tmem_d, uint64_t desc_a,
 // "free" barrier in both CTAs, and only then read the test's result.  An MMA costs its issuing
 // thread about as long as it runs, so whatever else that thread does between MMAs is time
 // the tensor pipe idles; the barrier test's latency is spent under the MMAs this way.
+// FREE false: the stage is still needed, nothing is committed.
+template <bool FREE = true>
 __device__ __forceinline__ bool umma_stage_pair(uint32_t tmem_d, uint64_t da, uint64_t db,
                                                 uint64_t a_step, uint64_t b_step, uint32_t idesc,
                                                 uint32_t accumulate_first, uint64_t* free_bar,
@@ -333,17 +335,18 @@ __device__ __forceinline__ bool umma_stage_pair(uint32_t tmem_d, uint64_t da, ui
       "tcgen05.mma.cta_group::2.kind::f16 [%1], a1, b1, %7, pt;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%1], a2, b2, %7, pt;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%1], a3, b3, %7, pt;\n\t"
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "setp.ne.b32 pa, %12, 0;\n\t"
+      "@pa tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
       "[%8], %11;\n\t"
       "selp.b32 %0, 1, 0, pw;\n\t}"
       : "=r"(ready)
       : "r"(tmem_d), "l"(da), "l"(db), "l"(a_step), "l"(b_step), "r"(accumulate_first),
         "r"(idesc), "r"(smem_u32(free_bar)), "r"(smem_u32(next_full_bar)), "r"(next_parity),
-        "h"((uint16_t)3)
+        "h"((uint16_t)3), "n"(FREE ? 1 : 0)
       : "memory");
   return ready != 0;
 }
-// The same for a CTA by itself (cta_group::1); FREE false: the stage is still needed.
+// The same for a CTA by itself (cta_group::1).
 template <bool FREE = true>
 __device__ __forceinline__ bool umma_stage(uint32_t tmem_d, uint64_t da, uint64_t db, uint64_t a_step, uint64_t b_step,
                                            uint32_t idesc, uint32_t accumulate_first, uint64_t* free_bar,

@@ -604,9 +604,9 @@ int elman_gated_linear_backward(int dtype, int T, int B, int d, const void* f, c
  * Newton-Schulz orthogonalisation of `count` dense row-major matrices in[count,m,n] (an extension without a
  * counterpart in the reference): X = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A A) X with
  * A = X X^T, which moves every singular value by s -> a s + b s^3 + c s^5 and keeps the singular
- * vectors; out[count,m,n] of `dtype` (may be `in`).  Products take fp16 operands with fp32 sums (fp32
- * matrices: two fp16 numbers an element), so coefficients that take singular values beyond 3.5 are refused.
- * fp32 results are about 1.5e-9 times the longer extent off (3e-6 at least), in norm.
+ * vectors; out[count,m,n] of `dtype` (may be `in`).  Products take every element as the sum of two fp16 numbers, with
+ * fp32 sums, so coefficients that take singular values beyond 3.5 are refused.  fp32 results are about 1.5e-9 times
+ * the longer extent off (3e-6 at least), in norm; bf16 results are such ones rounded (sums of theirs: 1e-8 times the extent).
  * A zero matrix stays zero; a matrix with a NaN or an infinity becomes NaN; the others of the call
  * are not touched by it.
  *
@@ -615,6 +615,7 @@ int elman_gated_linear_backward(int dtype, int T, int B, int d, const void* f, c
  *     g = grads * (*grad_scale);  momentum += (1 - mu) (g - momentum)
  *     u = nesterov ? g + mu (momentum - g) : momentum
  *     params = params (1 - lr weight_decay) - lr scale newton_schulz(u)
+ * all in fp32 but for the parameters themselves.
  */
 size_t elman_newton_schulz_workspace(int dtype, int count, int m, int n);
 int elman_newton_schulz(int dtype, int count, int m, int n, const void* in, void* out, int steps, float a,
