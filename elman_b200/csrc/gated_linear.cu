@@ -889,6 +889,7 @@ template <int V, int W> __device__ __forceinline__ bool take_state(Links<V, W>& 
   return sh.gave_up == 0;
 }
 // One linking warp, one tile; x is the thread's channel in the tile.  False: a wait gave up.
+// (`initial` is the caller's and may be any NaN: NOT_YET would send its lane to a state before the first.)
 template <int V, int W, bool RESET>
 __device__ __forceinline__ bool link(Links<V, W>& sh, int x, int n, int tiles, long base, long cols, float initial,
                                      const GlChain& ch, int ticket) {
@@ -896,7 +897,7 @@ __device__ __forceinline__ bool link(Links<V, W>& sh, int x, int n, int tiles, l
   const bool ends_group = in_group == GROUP - 1, more = n + 1 < tiles && ticket != ch.stall;
   const float2* pairs = ch.pairs + (long)first * cols + base + x;
   const float* state = ch.states + (long)(first / GROUP - 1) * cols + base + x;
-  uint32_t g[GROUP - 1][2], at_start = first > 0 ? NOT_YET : __float_as_uint(initial);
+  uint32_t g[GROUP - 1][2], at_start = first > 0 ? NOT_YET : word_of(initial);
 #pragma unroll
   for (int k = 0; k < GROUP - 1; ++k) g[k][0] = g[k][1] = k < in_group ? NOT_YET : 0u;
   auto fetch = [&]() {                             // what is missing: every load in flight before any is looked at
