@@ -359,6 +359,7 @@ int elman_b200_set_option(const char* name, long value) {
   else if (!strcmp(name, "gemm_pair")) o.gemm_pair = value;
   else if (!strcmp(name, "test_resident_blocks")) o.test_resident_blocks = value;
   else if (!strcmp(name, "test_stall_step")) o.test_stall_step = value;
+  else if (!strcmp(name, "test_leave_warp")) o.test_leave_warp = value;
   else if (!strcmp(name, "rec_replicas")) o.rec_replicas = value;
   else if (!strcmp(name, "rec_group_cap")) o.rec_group_cap = value;
   else return set_error(ELMAN_ERR_ARG, "unknown option '%s'", name);
@@ -384,6 +385,7 @@ long elman_b200_get_option(const char* name) {
   if (!strcmp(name, "gemm_pair")) return o.gemm_pair;
   if (!strcmp(name, "test_resident_blocks")) return o.test_resident_blocks;
   if (!strcmp(name, "test_stall_step")) return o.test_stall_step;
+  if (!strcmp(name, "test_leave_warp")) return o.test_leave_warp;
   if (!strcmp(name, "rec_replicas")) return o.rec_replicas;
   if (!strcmp(name, "rec_group_cap")) return o.rec_group_cap;
   return -1;

@@ -143,6 +143,7 @@ struct GlChain {             // workspace; all of it starts as NOT_YET
   int* status;
   long spin_limit;
   int stall;                 // test hook: this tile publishes nothing
+  int leave;                 // test hook: 32 k + w: at a block's tile k its warp w gives up the wait for the stage
 };
 
 struct Pair { float R, H; };
@@ -873,25 +874,39 @@ template <typename T, int V, int FEED> struct RowsOut {
 template <int V, int W> struct Links {
   Pair own[W][32 * V];             // the warps' pairs, in the scan's direction
   float enters[W][32 * V];         // state that enters each warp
-  int gave_up;
+  int gave_up[2];                  // somebody did, at this tile (even and odd ones apart: a slow warp may still look at the last)
 };
+// Each warp waits for a stage by itself, so one may give up (or leave early for another that did) where the rest still
+// see it land.  The barriers have no limit: whoever leaves passes those of the tile first, whoever sees the end as
+// well, and all the others leave behind the last of them.
+template <int V, int W> __device__ __forceinline__ void leave_scan(Links<V, W>& sh, int s, bool given_up, bool backward) {
+  if (given_up) sh.gave_up[s] = 1;
+  if (backward) asm volatile("bar.sync 3, %0;" ::"n"(32 * W) : "memory");
+  asm volatile("bar.arrive 1, %0;" ::"n"(32 * (W + V)) : "memory");
+  asm volatile("bar.sync 2, %0;" ::"n"(32 * (W + V)) : "memory");
+}
+template <int V, int W> __device__ __forceinline__ void leave_link(Links<V, W>& sh, int s, bool given_up) {
+  if (given_up) sh.gave_up[s] = 1;
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * (W + V)) : "memory");
+  asm volatile("bar.sync 2, %0;" ::"n"(32 * (W + V)) : "memory");
+}
 template <int V, int W> __device__ __forceinline__ void leave_pair(Links<V, W>& sh, int w, Vec<V> R, Vec<V> H) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int v = 0; v < V; ++v) sh.own[w][lane * V + v] = Pair{R.get(v), H.get(v)};
   asm volatile("bar.arrive 1, %0;" ::"n"(32 * (W + V)) : "memory");
 }
-template <int V, int W> __device__ __forceinline__ bool take_state(Links<V, W>& sh, int w, Vec<V>& S) {
+template <int V, int W> __device__ __forceinline__ bool take_state(Links<V, W>& sh, int s, int w, Vec<V>& S) {
   const int lane = threadIdx.x & 31;
   asm volatile("bar.sync 2, %0;" ::"n"(32 * (W + V)) : "memory");
 #pragma unroll
   for (int v = 0; v < V; ++v) S.set(v, sh.enters[w][lane * V + v]);
-  return sh.gave_up == 0;
+  return sh.gave_up[s] == 0;
 }
 // One linking warp, one tile; x is the thread's channel in the tile.  False: a wait gave up.
 // (`initial` is the caller's and may be any NaN: NOT_YET would send its lane to a state before the first.)
 template <int V, int W, bool RESET>
-__device__ __forceinline__ bool link(Links<V, W>& sh, int x, int n, int tiles, long base, long cols, float initial,
+__device__ __forceinline__ bool link(Links<V, W>& sh, int stage, int x, int n, int tiles, long base, long cols, float initial,
                                      const GlChain& ch, int ticket) {
   const int first = n / GROUP * GROUP, in_group = n - first;
   const bool ends_group = in_group == GROUP - 1, more = n + 1 < tiles && ticket != ch.stall;
@@ -938,9 +953,9 @@ __device__ __forceinline__ bool link(Links<V, W>& sh, int x, int n, int tiles, l
     s = pass<RESET>(s, own[k]);
   }
   if (more && ends_group) publish(ch.states + (long)(first / GROUP) * cols + base + x, s);
-  if (!ok) sh.gave_up = 1;
+  if (!ok) sh.gave_up[stage] = 1;
   asm volatile("bar.sync 2, %0;" ::"n"(32 * (W + V)) : "memory");
-  return sh.gave_up == 0;
+  return sh.gave_up[stage] == 0;
 }
 // The linking warps' loop over the block's tiles.
 template <int V, int W, bool RESET>
@@ -950,13 +965,21 @@ __device__ __forceinline__ void link_tiles(Links<V, W>& sh, Feed& fd, const GlPa
   for (int it = 0;; ++it) {
     const int s = it & 1;
     const bool here = ptx::mbar_wait(&fd.full[s], (uint32_t)(it >> 1) & 1u, ch.spin_limit * 8, &fd.gave_up);
-    if (!__all_sync(0xFFFFFFFFu, here)) return;      // (the scanning warps see it too)
+    if (!__all_sync(0xFFFFFFFFu, here && 32 * it + (int)(threadIdx.x >> 5) != ch.leave)) {
+      fd.gave_up = 1;
+      report_timeout(ch.status, KID_GATED_LINEAR, 0xFFFF);
+      leave_link(sh, s, true);
+      return;
+    }
     const TileAt t = fd.tile[s];
-    if (t.ticket < 0) return;
+    if (t.ticket < 0) {
+      leave_link(sh, s, false);
+      return;
+    }
     const int i = t.group * (32 * V) + x;
     const long base = ((long)t.b * g.groups_per_row + t.group) * (32 * V);
     const float start = t.n < GROUP && initial != nullptr && i < p.d ? initial[(long)t.b * p.d + i] : 0.f;
-    const bool ok = link<V, W, RESET>(sh, x, t.n, g.tiles, base, g.cols, start, ch, t.ticket);
+    const bool ok = link<V, W, RESET>(sh, s, x, t.n, g.tiles, base, g.cols, start, ch, t.ticket);
     if (threadIdx.x % 32 == 0) ptx::mbar_arrive(&fd.done[s]);
     if (!ok) return;
   }
@@ -976,7 +999,7 @@ gl_forward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 127) & ~(uintptr_t)127);
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    sh.gave_up = 0;
+    sh.gave_up[0] = sh.gave_up[1] = 0;
     fd.gave_up = 0;
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(&fd.full[s], full_arrivals(FEED, V));
@@ -1005,13 +1028,17 @@ gl_forward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
   for (int it = 0;; ++it) {
     const int s = it & 1;
     const bool here = ptx::mbar_wait(&fd.full[s], (uint32_t)(it >> 1) & 1u, ch.spin_limit * 8, &fd.gave_up);
-    if (!__all_sync(0xFFFFFFFFu, here)) {
+    if (!__all_sync(0xFFFFFFFFu, here && 32 * it + w != ch.leave)) {
       fd.gave_up = 1;
       report_timeout(ch.status, KID_GATED_LINEAR, 0xFFFF);
+      leave_scan(sh, s, true, false);
       return;
     }
     const TileAt at = fd.tile[s];
-    if (at.ticket < 0) return;
+    if (at.ticket < 0) {
+      leave_scan(sh, s, false, false);
+      return;
+    }
     const int i = at.group * (32 * V) + lane * V;
     const int t0 = at.n * ROWS + w * FL, steps = p.T - t0;
     const uint32_t rows = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * FL * pitch_of(FEED));
@@ -1043,7 +1070,7 @@ gl_forward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
       const F x = z.get(l);
       zs[l] = vmul(x, gate_of(vmul(x, F(-LOG2E)), e));
     }
-    if (!take_state<V, W>(sh, w, h)) {
+    if (!take_state<V, W>(sh, s, w, h)) {
       fd.gave_up = 1;
       return;
     }
@@ -1078,7 +1105,7 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 127) & ~(uintptr_t)127);
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    sh.gave_up = 0;
+    sh.gave_up[0] = sh.gave_up[1] = 0;
     fd.gave_up = 0;
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(&fd.full[s], full_arrivals(FEED, V));
@@ -1107,13 +1134,17 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
   for (int it = 0;; ++it) {
     const int s = it & 1;
     const bool here = ptx::mbar_wait(&fd.full[s], (uint32_t)(it >> 1) & 1u, ch.spin_limit * 8, &fd.gave_up);
-    if (!__all_sync(0xFFFFFFFFu, here)) {
+    if (!__all_sync(0xFFFFFFFFu, here && 32 * it + w != ch.leave)) {
       fd.gave_up = 1;
       report_timeout(ch.status, KID_GATED_LINEAR, 0xFFFF);
+      leave_scan(sh, s, true, true);
       return;
     }
     const TileAt at = fd.tile[s];
-    if (at.ticket < 0) return;
+    if (at.ticket < 0) {
+      leave_scan(sh, s, false, true);
+      return;
+    }
     const int i = at.group * (32 * V) + lane * V;
     const int chunk = g.tiles - 1 - at.n, t0 = chunk * ROWS + w * BL, steps = p.T - t0;
     const uint32_t rows = ptx::smem_u32(smem + s * STAGE) + (uint32_t)(w * BL * pitch_of(FEED));
@@ -1180,7 +1211,7 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
       if (RESET) E = unless(cut >> l & 1, E);
     }
     leave_pair<V, BW>(sh, BW - 1 - w, R, E);
-    if (!take_state<V, BW>(sh, BW - 1 - w, D)) {
+    if (!take_state<V, BW>(sh, s, BW - 1 - w, D)) {
       fd.gave_up = 1;
       return;
     }
@@ -1288,6 +1319,7 @@ void prepare_chain(GlChain& ch, const GatedLinearArgs& a, int tiles, long cols) 
   ch.status = device_status_ptr();
   ch.spin_limit = options().spin_limit;
   ch.stall = (int)options().test_stall_step;
+  ch.leave = (int)options().test_leave_warp;
   if (tiles <= 1) return;
   ch.ctrl = (uint32_t*)ws;
   ch.pairs = (float2*)(ws + 256);

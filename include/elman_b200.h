@@ -102,6 +102,9 @@ int elman_b200_device_status(int* detail, int clear);
  *                    nothing delivers.  The wait runs out after "spin_limit" polls, the
  *                    kernel records ELMAN_ERR_TIMEOUT in the status word, every block gives
  *                    up and the launch returns; its results are invalid.  Nothing faults.
+ *   "test_leave_warp" the same for one warp alone, -1 (default) = off: in the gated linear recurrence
+ *                    32 k + w makes warp w of every block give up its wait at the block's k-th tile
+ *                    while the other warps see that wait end well
  * Returns ELMAN_OK or ELMAN_ERR_ARG for an unknown name.
  */
 int elman_b200_set_option(const char* name, long value);
