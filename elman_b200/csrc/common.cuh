@@ -62,7 +62,7 @@ struct Options {
   long rec_group_cap = 0;      // widest batch group of the throughput plan: 0 auto (64), 16 / 32 / 64
   long rec_replicas = 0;       // batch replicas of the throughput plan: 0 auto, 1 off, n = at most n
   long test_stall_step = -1;
-  long test_leave_warp = -1;   // gated linear recurrence: 32 k + w: warp w gives up a wait at its block's k-th tile
+  long test_leave_warp = -1;   // gated linear recurrence, Newton-Schulz: 32 k + w: warp w gives up a wait at its block's k-th tile
 };
 Options& options();
 // `kernel`: for the kernels that carry a recurrence, so that a test can tell which of them ran.

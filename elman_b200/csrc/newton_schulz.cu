@@ -88,7 +88,7 @@ struct NsPlan {
   int* done;                 // [count]: warps' shares of tiles finished
   int* status;
   long spin_limit;
-  int stall;                 // test hook
+  int stall, leave;          // test hooks: a stage that is not loaded; 32 q + w: warp w gives up the wait for its block's item q
 };
 
 // One item of the list.  Taking it apart costs divisions, a thousand cycles of latency: the warp that takes items does
@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
     const int quarter = warp & 3, mine = warp - 4, half = mine >> 2;
     const uint32_t buffer = ptx::smem_u32(smem) + STAGES * 2 * OPERAND_BYTES + (uint32_t)(mine * BUFFER_BYTES);
     for (int q = 0;; ++q) {
-      bool ok = __all_sync(0xFFFFFFFFu, wait_for(&tk_full[q % TICKETS], q));
+      bool ok = __all_sync(0xFFFFFFFFu, wait_for(&tk_full[q % TICKETS], q) && 32 * q + warp != p.leave), end = false;
       NsItem it;
       Finish fin;
       Box same;
@@ -607,29 +607,31 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
       if (ok) {
         const NsSlot slot = tk[q % TICKETS];
         __syncwarp();
-        if (slot.kind < 0) {
-          if (lane == 0) free_ticket(q);
-          break;
+        end = slot.kind < 0;
+        if (!end) {
+          it = item_of(p, slot);
+          b = q % sums;
+          row0 = it.ti * EDGE + 128 * (int)rank + quarter * 32;
+          col0 = it.tj * it.columns + half * (it.columns / 2);
+          fin = finish_of(p, it);
+          ok = __all_sync(0xFFFFFFFFu, it.kind == GRAM || wait_for(&go[q % TICKETS], q));
         }
-        it = item_of(p, slot);
-        b = q % sums;
-        row0 = it.ti * EDGE + 128 * (int)rank + quarter * 32;
-        col0 = it.tj * it.columns + half * (it.columns / 2);
-        fin = finish_of(p, it);
-        ok = __all_sync(0xFFFFFFFFu, it.kind == GRAM || wait_for(&go[q % TICKETS], q));
         if (lane == 0) free_ticket(q);
-        if (ok) fetch_box(same, fin, it, row0, col0);  // under the products
-        ok = ok && ptx::mbar_wait(&acc_full[b], (uint32_t)(q / sums) & 1u, p.spin_limit * 8, abortp);
+        if (ok && !end) {
+          fetch_box(same, fin, it, row0, col0);        // under the products
+          ok = ptx::mbar_wait(&acc_full[b], (uint32_t)(q / sums) & 1u, p.spin_limit * 8, abortp);
+        }
       }
       if (!ok && abort_flag == 0) give_up(0xFFFF);
-      uint32_t stop;                                  // one verdict for all of them
+      // One verdict for all of them, at the end too: a warp that gave up there would wait for those that have left.
+      uint32_t stop;
       asm volatile(
           "{\n\t.reg .pred pp, qq;\n\t"
           "setp.ne.b32 pp, %1, 0;\n\t"
           "bar.red.or.pred qq, 1, %2, pp;\n\t"
           "selp.b32 %0, 1, 0, qq;\n\t}"
           : "=r"(stop)
-          : "r"((uint32_t)(!ok || abort_flag != 0)), "n"(32 * EPI_WARPS)
+          : "r"((uint32_t)(!ok || end || abort_flag != 0)), "n"(32 * EPI_WARPS)
           : "memory");
       if (stop) break;
       ptx::tc_fence_after();
@@ -875,6 +877,7 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   p.status = device_status_ptr();
   p.spin_limit = options().spin_limit;
   p.stall = (int)options().test_stall_step;
+  p.leave = (int)options().test_leave_warp;
   const bool pair = sizeof(T) == 2 && pays_as_pairs(p);
   const int edge = pair ? 256 : 128;
   p.edge = p.n_sym = p.n_upd = edge;

@@ -104,7 +104,8 @@ int elman_b200_device_status(int* detail, int clear);
  *                    up and the launch returns; its results are invalid.  Nothing faults.
  *   "test_leave_warp" the same for one warp alone, -1 (default) = off: in the gated linear recurrence
  *                    32 k + w makes warp w of every block give up its wait at the block's k-th tile
- *                    while the other warps see that wait end well
+ *                    while the other warps see that wait end well; in the Newton-Schulz products
+ *                    one of the warps 4 to 11, which finish tiles
  * Returns ELMAN_OK or ELMAN_ERR_ARG for an unknown name.
  */
 int elman_b200_set_option(const char* name, long value);
