@@ -117,10 +117,11 @@ __global__ void __launch_bounds__(128) gl_backward_seq_kernel(GlParams p) {
 // of this section take the rows whose last 128 bytes would be mostly empty (whole_width below) and count channels through
 // batch rows; the next section's take all others.
 //
-// A warp holds L steps of 32 lanes x V channels in registers and scans them from a zero state: the pair (R, H)
-// with  h_out = h_in + (H - R h_in),  R = 1 - prod(1 - u) kept as the scan of the constant 1, so that
-// it too keeps what 1 - u would lose.  R = -1 says that a reset lies inside: h_out = H, and h_in (which
-// may be anything) is not read.  The tile's own pair goes to the tiles that follow in time through L2;
+// A warp holds L steps of 32 lanes x V channels in registers and scans them from a zero state: h_out = P h_in + H with
+// P = prod(1 - u).  Where P is near one its distance from one has to be exact, or what the steps add is lost; where it
+// is small P itself, or a state that has long been forgotten leaves 2^-24 of itself behind.  So both are scanned, and
+// the pair (K, H) keeps the one that counts: K = P where P < 1/2, else P - 1 (kept() below).  K = -1 says that a reset lies
+// inside: h_out = H, and h_in (which may be anything) is not read.  The tile's own pair goes to the tiles that follow in time through L2;
 // they fold the pairs of their group of GROUP tiles onto the state at the group's start, which the last
 // tile of the group before has published.  The association is fixed, so results do not depend on
 // timing; the chain of dependent exchanges is one per GROUP tiles.  Backwards the same with time
@@ -146,13 +147,34 @@ struct GlChain {             // workspace; all of it starts as NOT_YET
   int leave;                 // test hook: 32 k + w: at a block's tile k its warp w gives up the wait for the stage
 };
 
-struct Pair { float R, H; };
+struct Pair { float K, H; };
+// K from P and P - 1: P only above zero (2^-149 stands for less), P - 1 from -1/2 up to zero.
+__device__ __forceinline__ float kept(float P, float P_1) { return P_1 >= -0.5f ? P_1 : fmaxf(P, 1.4e-45f); }
 template <bool RESET> __device__ __forceinline__ float pass(float S, Pair a) {
-  return RESET && a.R < 0.f ? a.H : S + fmaf(-a.R, S, a.H);
+  const float rest = a.K > 0.f ? 0.f : 1.f;      // (known before S is: two dependent instructions a pair)
+  const float t = fmaf(rest, S, fmaf(a.K, S, a.H));
+  return RESET && a.K == -1.f ? a.H : t;
 }
 template <bool RESET> __device__ __forceinline__ Pair join(Pair a, Pair b) {       // a, then b
-  const Pair ab = Pair{RESET && a.R < 0.f ? -1.f : a.R + fmaf(-b.R, a.R, b.R), a.H + fmaf(-b.R, a.H, b.H)};
-  return RESET && b.R < 0.f ? b : ab;
+  const float Pa = a.K > 0.f ? a.K : 1.f + a.K, Pa_1 = a.K > 0.f ? a.K - 1.f : a.K;
+  const float Pb = b.K > 0.f ? b.K : 1.f + b.K, Pb_1 = b.K > 0.f ? b.K - 1.f : b.K;
+  const Pair ab = Pair{RESET && a.K == -1.f ? -1.f : kept(Pa * Pb, fmaf(Pa, Pb_1, Pa_1)), pass<false>(a.H, b)};
+  return RESET && b.K == -1.f ? b : ab;
+}
+
+// The same with P and P - 1 both at hand, as a warp has them.  P - 1 = -2 says that a reset lies inside.
+struct Stretch { float P, P_1, H; };
+template <bool RESET> __device__ __forceinline__ float pass(float S, Stretch a) {
+  const bool near = a.P_1 >= -0.5f;
+  const float t = fmaf(near ? 1.f : 0.f, S, fmaf(near ? a.P_1 : a.P, S, a.H));
+  return RESET && a.P_1 < -1.5f ? a.H : t;
+}
+template <bool RESET> __device__ __forceinline__ Stretch join(Stretch a, Stretch b) {
+  const Stretch ab = Stretch{a.P * b.P, RESET && a.P_1 < -1.5f ? -2.f : fmaf(a.P, b.P_1, a.P_1), pass<false>(a.H, b)};
+  return RESET && b.P_1 < -1.5f ? b : ab;
+}
+template <bool RESET> __device__ __forceinline__ Pair pair_of(Stretch a) {
+  return Pair{RESET && a.P_1 < -1.5f ? -1.f : kept(a.P, a.P_1), a.H};
 }
 
 // The V channels of a lane; two of them are one packed fp32x2 operand (half the instructions: at HBM
@@ -210,11 +232,11 @@ __device__ __forceinline__ float rcp_(float x) {
   return y;
 }
 constexpr float LOG2E = 1.4426950408889634f;
-// 1 / (1 + exp2(x)); e receives exp2(x)
-template <int V> __device__ __forceinline__ Vec<V> gate_of(Vec<V> x, Vec<V>& e) {
+// 1 / (1 + exp2(x)), or with MINUS the negative of that; e receives exp2(x)
+template <int V, bool MINUS = false> __device__ __forceinline__ Vec<V> gate_of(Vec<V> x, Vec<V>& e) {
 #pragma unroll
   for (int v = 0; v < V; ++v) e.set(v, exp2_(x.get(v)));
-  const Vec<V> den = vadd(e, Vec<V>(1.f));
+  const Vec<V> den = MINUS ? vfma(e, Vec<V>(-1.f), Vec<V>(-1.f)) : vadd(e, Vec<V>(1.f));
   Vec<V> r;
 #pragma unroll
   for (int v = 0; v < V; ++v) r.set(v, rcp_(den.get(v)));
@@ -226,11 +248,13 @@ template <> struct Lane<float, 1> {
   typedef float Raw;
   static __device__ __forceinline__ Vec<1> get(Raw r) { return Vec<1>(r); }
   static __device__ __forceinline__ Raw put(Vec<1> v) { return v.x; }
+  static __device__ __forceinline__ Raw put_minus(Vec<1> v) { return -v.x; }
 };
 template <> struct Lane<bf16, 1> {
   typedef unsigned short Raw;
   static __device__ __forceinline__ Vec<1> get(Raw r) { return Vec<1>(__uint_as_float((uint32_t)r << 16)); }
   static __device__ __forceinline__ Raw put(Vec<1> v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v.x)); }
+  static __device__ __forceinline__ Raw put_minus(Vec<1> v) { return __bfloat16_as_ushort(__float2bfloat16_rn(-v.x)); }
 };
 template <> struct Lane<bf16, 2> {
   typedef uint32_t Raw;
@@ -243,11 +267,12 @@ template <> struct Lane<bf16, 2> {
     const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const Raw*>(&p);
   }
+  static __device__ __forceinline__ Raw put_minus(Vec<2> v) { return put(v) ^ 0x80008000u; }
 };
 
 __device__ __forceinline__ uint32_t word_of(float x) { return x != x ? 0x7FFFFFFFu : __float_as_uint(x); }
 __device__ __forceinline__ void publish(float2* at, Pair a) {
-  asm volatile("st.relaxed.gpu.global.v2.b32 [%0], {%1, %2};" ::"l"(at), "r"(word_of(a.R)), "r"(word_of(a.H)) : "memory");
+  asm volatile("st.relaxed.gpu.global.v2.b32 [%0], {%1, %2};" ::"l"(at), "r"(word_of(a.K)), "r"(word_of(a.H)) : "memory");
 }
 __device__ __forceinline__ void publish(float* at, float x) {
   asm volatile("st.relaxed.gpu.global.b32 [%0], %1;" ::"l"(at), "r"(word_of(x)) : "memory");
@@ -322,12 +347,12 @@ __device__ __forceinline__ void warps_sync(int warps) {
 // the scan's direction; `initial` is the state at the scan's start.  False: a
 // wait gave up.
 template <int V, int W, bool RESET>
-__device__ __forceinline__ bool enter(Shared<V, W>& sh, int w, int warps, Vec<V> R, Vec<V> H, int n, int tiles,
+__device__ __forceinline__ bool enter(Shared<V, W>& sh, int w, int warps, Vec<V> K, Vec<V> H, int n, int tiles,
                                       long base, long cols, Vec<V> initial, const GlChain& ch, int ticket,
                                       uint32_t grabbed, Vec<V>& S) {
   const int lane = threadIdx.x & 31, x = threadIdx.x;
 #pragma unroll
-  for (int v = 0; v < V; ++v) sh.own[w][lane * V + v] = Pair{R.get(v), H.get(v)};
+  for (int v = 0; v < V; ++v) sh.own[w][lane * V + v] = Pair{K.get(v), H.get(v)};
   const int first = n / GROUP * GROUP, in_group = n - first;
   const bool ends_group = in_group == GROUP - 1, more = n + 1 < tiles && ticket != ch.stall;
   if (w == 0 && first == 0) {
@@ -377,6 +402,23 @@ __device__ __forceinline__ bool enter(Shared<V, W>& sh, int w, int warps, Vec<V>
   for (int v = 0; v < V; ++v) S.set(v, sh.enters[w][lane * V + v]);
   return true;
 }
+
+// A warp's scan from a zero state, from gates `nu` = -u (a packed fma has no negation): P, P - 1 and the state a step on.
+template <int V> struct Scan {
+  Vec<V> H, P, P_1;
+  __device__ __forceinline__ Scan() : H(0.f), P(1.f), P_1(0.f) {}
+  __device__ __forceinline__ void step(Vec<V> nu, Vec<V> c) {
+    H = vfma(nu, vsub(H, c), H);
+    P_1 = vfma(nu, P, P_1);
+    P = vfma(nu, P, P);
+  }
+  __device__ __forceinline__ Vec<V> K() const {
+    Vec<V> k;
+#pragma unroll
+    for (int v = 0; v < V; ++v) k.set(v, kept(P.get(v), P_1.get(v)));
+    return k;
+  }
+};
 
 // exp2's argument held at 115 (u = 2^-115), so that u (1 - u) = e u^2 stays a number; NaN passes.
 template <int V> __device__ __forceinline__ Vec<V> held(Vec<V> x) {
@@ -465,28 +507,26 @@ __global__ void __launch_bounds__(32 * FW, 2) gl_forward_tile_kernel(GlParams p,
     load_rows<T, V, FL>(rc, p.c, p.sc, t0, p.T, at.b, at.i);
     load_rows<T, V, FL>(rz, p.z, p.sz, t0, p.T, at.b, at.i);
     const uint32_t cut = RESET ? reset_bits<FL>(p, t0, at.b) : 0;
-    F u[FL], e, initial(0.f);
+    F nu[FL], e, initial(0.f);
     if (w == 0 && at.n < GROUP && p.h0 != nullptr && at.on) {
 #pragma unroll
       for (int v = 0; v < V; ++v) initial.set(v, p.h0[at.col + v]);
     }
 #pragma unroll
-    for (int l = 0; l < FL; ++l) u[l] = gate_of(vmul(Ln::get(rf[l]), F(LOG2E)), e);
+    for (int l = 0; l < FL; ++l) nu[l] = gate_of<V, true>(vmul(Ln::get(rf[l]), F(LOG2E)), e);
     if (steps < FL) {
 #pragma unroll
       for (int l = 0; l < FL; ++l)
-        if (l >= steps) u[l] = F(0.f);        // beyond the end: the state stays
+        if (l >= steps) nu[l] = F(0.f);       // beyond the end: the state stays
     }
-    F H(0.f), R(0.f);
+    Scan<V> scan;
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
-      if (RESET) H = unless(cut >> l & 1, H);
-      H = vfma(u[l], vsub(Ln::get(rc[l]), H), H);
-      R = vfma(u[l], vsub(F(1.f), R), R);
+      if (RESET) scan.H = unless(cut >> l & 1, scan.H);
+      scan.step(nu[l], Ln::get(rc[l]));
     }
-    if (RESET && cut) R = F(-1.f);
     F h;
-    if (!enter<V, FW, RESET>(sh, w, warps, R, H, at.n, tiles, at.base, cols, initial, ch, ticket, grabbed, h)) return;
+    if (!enter<V, FW, RESET>(sh, w, warps, RESET && cut ? F(-1.f) : scan.K(), scan.H, at.n, tiles, at.base, cols, initial, ch, ticket, grabbed, h)) return;
     ticket = tiles > 1 ? sh.next : total;
     if (at.on && p.saved != nullptr && t0 % GL_CHUNK == 0 && steps > 0) {
 #pragma unroll
@@ -497,7 +537,7 @@ __global__ void __launch_bounds__(32 * FW, 2) gl_forward_tile_kernel(GlParams p,
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
       if (RESET) h = unless(cut >> l & 1, h);
-      h = vfma(u[l], vsub(Ln::get(rc[l]), h), h);
+      h = vfma(nu[l], vsub(h, Ln::get(rc[l])), h);
       const F z = Ln::get(rz[l]);
       const F out = vmul(h, vmul(z, gate_of(vmul(z, F(-LOG2E)), e)));
       if (at.on && l < steps) __stcs(reinterpret_cast<typename Ln::Raw*>(y + l * step), Ln::put(out));
@@ -545,28 +585,27 @@ __global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p
     }
     const uint32_t cut = RESET ? reset_bits<BL>(p, t0, at.b) : 0;
     // the states before the warp's steps
-    F u[BL], a[BL];
+    F nu[BL], a[BL];
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
       F e;
-      u[l] = gate_of(held(vmul(Ln::get(rf[l]), F(LOG2E))), e);
-      a[l] = vmul(vmul(e, u[l]), u[l]);
+      nu[l] = gate_of<V, true>(held(vmul(Ln::get(rf[l]), F(LOG2E))), e);
+      a[l] = vmul(vmul(e, nu[l]), nu[l]);
     }
     if (steps < BL) {
 #pragma unroll
       for (int l = 0; l < BL; ++l)
-        if (l >= steps) u[l] = F(0.f);
+        if (l >= steps) nu[l] = F(0.f);
     }
-    F H(0.f), R(0.f);
+    Scan<V> scan;
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
-      if (RESET) H = unless(cut >> l & 1, H);
-      H = vfma(u[l], vsub(Ln::get(rc[l]), H), H);
-      R = vfma(u[l], vsub(F(1.f), R), R);
+      if (RESET) scan.H = unless(cut >> l & 1, scan.H);
+      scan.step(nu[l], Ln::get(rc[l]));
     }
-    if (RESET && cut) R = F(-1.f);
+    const F K = RESET && cut ? F(-1.f) : scan.K();
 #pragma unroll
-    for (int v = 0; v < V; ++v) ahead[w][lane * V + v] = Pair{R.get(v), H.get(v)};
+    for (int v = 0; v < V; ++v) ahead[w][lane * V + v] = Pair{K.get(v), scan.H.get(v)};
     __syncthreads();
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -582,7 +621,7 @@ __global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p
     for (int l = 0; l < BL; ++l) {
       if (RESET) h = unless(cut >> l & 1, h);
       prev[l] = vsub(h, Ln::get(rc[l]));
-      h = vfma(u[l], vsub(F(0.f), prev[l]), h);
+      h = vfma(nu[l], prev[l], h);
       const F z = Ln::get(rz[l]), dy = Ln::get(rdy[l]);
       F e;
       const F s = gate_of(vmul(z, F(-LOG2E)), e), zs = vmul(z, s);
@@ -599,22 +638,22 @@ __global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p
 #pragma unroll
     for (int l = BL - 1; l >= 0; --l) {
       const F g = vadd(q[l], E);
-      E = vsub(g, vmul(u[l], g));
+      E = vfma(nu[l], g, g);
       if (RESET) E = unless(cut >> l & 1, E);
     }
-    if (!enter<V, BW, RESET>(sh, warps - 1 - w, warps, R, E, at.n, tiles, at.base, cols, initial, ch, ticket, grabbed, D)) return;
+    if (!enter<V, BW, RESET>(sh, warps - 1 - w, warps, K, E, at.n, tiles, at.base, cols, initial, ch, ticket, grabbed, D)) return;
     ticket = tiles > 1 ? sh.next : total;
     char* df = (char*)p.df + ((long)t0 * p.sdf.t + at.b * p.sdf.b + at.i) * (long)sizeof(T);
     char* dc = (char*)p.dc + ((long)t0 * p.sdc.t + at.b * p.sdc.b + at.i) * (long)sizeof(T);
     const long step_f = p.sdf.t * (long)sizeof(T), step_c = p.sdc.t * (long)sizeof(T);
 #pragma unroll
     for (int l = BL - 1; l >= 0; --l) {
-      const F g = vadd(q[l], D), gu = vmul(g, u[l]);
+      const F g = vadd(q[l], D), minus_gu = vmul(g, nu[l]);
       const F of = vmul(vmul(g, prev[l]), a[l]);
-      D = vsub(g, gu);
+      D = vfma(nu[l], g, g);
       if (RESET) D = unless(cut >> l & 1, D);
       if (at.on && l < steps) {
-        __stcs(reinterpret_cast<typename Ln::Raw*>(dc + l * step_c), Ln::put(gu));
+        __stcs(reinterpret_cast<typename Ln::Raw*>(dc + l * step_c), Ln::put_minus(minus_gu));
         __stcs(reinterpret_cast<typename Ln::Raw*>(df + l * step_f), Ln::put(of));
       }
     }
@@ -803,8 +842,8 @@ template <typename T, int V> __device__ __forceinline__ Vec<V> from_word(uint32_
   memcpy(&r, &w, 4);
   return Lane<T, V>::get(r);
 }
-template <typename T, int V> __device__ __forceinline__ uint32_t to_word(Vec<V> x) {
-  const typename Lane<T, V>::Raw r = Lane<T, V>::put(x);
+template <typename T, int V> __device__ __forceinline__ uint32_t to_word(Vec<V> x, bool minus) {
+  const typename Lane<T, V>::Raw r = minus ? Lane<T, V>::put_minus(x) : Lane<T, V>::put(x);
   uint32_t w;
   memcpy(&w, &r, 4);
   return w;
@@ -851,8 +890,8 @@ template <typename T, int V, int FEED> struct RowsOut {
     step = s.t * (long)sizeof(T);
     channels = d - i;
   }
-  __device__ __forceinline__ void put(int l, Vec<V> x) const {
-    const uint32_t w = to_word<T, V>(x);
+  __device__ __forceinline__ void put(int l, Vec<V> x, bool minus = false) const {
+    const uint32_t w = to_word<T, V>(x, minus);
     if constexpr (FEED == FEED_TMA) {
       sts_word(stage + l * ROW_BYTES, w);
     } else if (l < steps && channels > 0) {
@@ -872,7 +911,7 @@ template <typename T, int V, int FEED> struct RowsOut {
 // state.  (Where the scanning warps folded the pairs themselves, that was a third of the backward tile's
 // instructions.)
 template <int V, int W> struct Links {
-  Pair own[W][32 * V];             // the warps' pairs, in the scan's direction
+  Vec<V> P[W][32], P_1[W][32], H[W][32];   // the warps' stretches, in the scan's direction
   float enters[W][32 * V];         // state that enters each warp
   int gave_up[2];                  // somebody did, at this tile (even and odd ones apart: a slow warp may still look at the last)
 };
@@ -890,10 +929,11 @@ template <int V, int W> __device__ __forceinline__ void leave_link(Links<V, W>& 
   asm volatile("bar.sync 1, %0;" ::"n"(32 * (W + V)) : "memory");
   asm volatile("bar.sync 2, %0;" ::"n"(32 * (W + V)) : "memory");
 }
-template <int V, int W> __device__ __forceinline__ void leave_pair(Links<V, W>& sh, int w, Vec<V> R, Vec<V> H) {
+template <int V, int W, bool RESET> __device__ __forceinline__ void leave_stretch(Links<V, W>& sh, int w, const Scan<V>& scan, Vec<V> H, uint32_t cut) {
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int v = 0; v < V; ++v) sh.own[w][lane * V + v] = Pair{R.get(v), H.get(v)};
+  sh.P[w][lane] = scan.P;
+  sh.P_1[w][lane] = RESET && cut ? Vec<V>(-2.f) : scan.P_1;
+  sh.H[w][lane] = H;
   asm volatile("bar.arrive 1, %0;" ::"n"(32 * (W + V)) : "memory");
 }
 template <int V, int W> __device__ __forceinline__ bool take_state(Links<V, W>& sh, int s, int w, Vec<V>& S) {
@@ -928,14 +968,16 @@ __device__ __forceinline__ bool link(Links<V, W>& sh, int stage, int x, int n, i
   };
   fetch();                                         // while the scanning warps scan
   asm volatile("bar.sync 1, %0;" ::"n"(32 * (W + V)) : "memory");
-  Pair own[W];
+  Stretch own[W];
 #pragma unroll
-  for (int k = 0; k < W; ++k) own[k] = sh.own[k][x];
+  for (int k = 0; k < W; ++k)
+    own[k] = Stretch{reinterpret_cast<const float*>(sh.P[k])[x], reinterpret_cast<const float*>(sh.P_1[k])[x],
+                     reinterpret_cast<const float*>(sh.H[k])[x]};
   if (more && !ends_group) {
-    Pair all = own[0];
+    Stretch all = own[0];
 #pragma unroll
     for (int k = 1; k < W; ++k) all = join<RESET>(all, own[k]);
-    publish(ch.pairs + (long)n * cols + base + x, all);
+    publish(ch.pairs + (long)n * cols + base + x, pair_of<RESET>(all));
   }
   Patience patience;
   bool ok = true;
@@ -1048,23 +1090,21 @@ gl_forward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
     c.template clear_after<FL>(steps);
     z.template clear_after<FL>(steps);
     const uint32_t cut = RESET ? reset_bits<FL>(p, t0, at.b) : 0;
-    F u[FL], zs[FL], e;
+    F nu[FL], zs[FL], e, h;
 #pragma unroll
-    for (int l = 0; l < FL; ++l) u[l] = gate_of(vmul(f.get(l), F(LOG2E)), e);
+    for (int l = 0; l < FL; ++l) nu[l] = gate_of<V, true>(vmul(f.get(l), F(LOG2E)), e);
     if (steps < FL) {
 #pragma unroll
       for (int l = 0; l < FL; ++l)
-        if (l >= steps) u[l] = F(0.f);
+        if (l >= steps) nu[l] = F(0.f);
     }
-    F H(0.f), R(0.f), h;
+    Scan<V> scan;
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
-      if (RESET) H = unless(cut >> l & 1, H);
-      H = vfma(u[l], vsub(c.get(l), H), H);
-      R = vfma(u[l], vsub(F(1.f), R), R);
+      if (RESET) scan.H = unless(cut >> l & 1, scan.H);
+      scan.step(nu[l], c.get(l));
     }
-    if (RESET && cut) R = F(-1.f);
-    leave_pair<V, W>(sh, w, R, H);
+    leave_stretch<V, W, RESET>(sh, w, scan, scan.H, cut);
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
       const F x = z.get(l);
@@ -1080,7 +1120,7 @@ gl_forward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
 #pragma unroll
     for (int l = 0; l < FL; ++l) {
       if (RESET) h = unless(cut >> l & 1, h);
-      h = vfma(u[l], vsub(c.get(l), h), h);
+      h = vfma(nu[l], vsub(h, c.get(l)), h);
       y.put(l, vmul(h, zs[l]));
     }
     if (steps > 0 && steps <= FL) write_state<V>(p.h_last, at.b, i, p.d, h);
@@ -1100,7 +1140,7 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
   constexpr int ROWS = BW * BL, TENSOR = Stages<4, ROWS, FEED>::TENSOR, STAGE = Stages<4, ROWS, FEED>::STAGE;
   extern __shared__ uint8_t raw[];
   __shared__ Links<V, BW> sh;
-  __shared__ Pair ahead[BW][32 * V];
+  __shared__ Vec<V> ahead_K[BW][32], ahead_H[BW][32], ahead_rest[BW][32];
   __shared__ Feed fd;
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 127) & ~(uintptr_t)127);
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1156,33 +1196,40 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
     dy.template clear_after<BL>(steps);
     const uint32_t cut = RESET ? reset_bits<BL>(p, t0, at.b) : 0;
     F h = read_state<V>(p.saved + (long)chunk * p.B * p.d, at.b, i, p.d);
-    F u[BL], a[BL];
+    F nu[BL], a[BL];
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
       F e;
-      u[l] = gate_of(held(vmul(f.get(l), F(LOG2E))), e);
-      a[l] = vmul(vmul(e, u[l]), u[l]);
+      nu[l] = gate_of<V, true>(held(vmul(f.get(l), F(LOG2E))), e);
+      a[l] = vmul(vmul(e, nu[l]), nu[l]);
     }
     if (steps < BL) {
 #pragma unroll
       for (int l = 0; l < BL; ++l)
-        if (l >= steps) u[l] = F(0.f);
+        if (l >= steps) nu[l] = F(0.f);
     }
-    F H(0.f), R(0.f);
+    Scan<V> scan;
 #pragma unroll
     for (int l = 0; l < BL; ++l) {
-      if (RESET) H = unless(cut >> l & 1, H);
-      H = vfma(u[l], vsub(c.get(l), H), H);
-      R = vfma(u[l], vsub(F(1.f), R), R);
+      if (RESET) scan.H = unless(cut >> l & 1, scan.H);
+      scan.step(nu[l], c.get(l));
     }
-    if (RESET && cut) R = F(-1.f);
+    F K, rest;                            // pass() of both channels at once: h <- rest h + (K h + H)
 #pragma unroll
-    for (int v = 0; v < V; ++v) ahead[w][lane * V + v] = Pair{R.get(v), H.get(v)};
+    for (int v = 0; v < V; ++v) {
+      const bool near = scan.P_1.get(v) >= -0.5f;
+      K.set(v, near ? scan.P_1.get(v) : scan.P.get(v));
+      rest.set(v, RESET && cut ? -1.f : near ? 1.f : 0.f);
+    }
+    ahead_K[w][lane] = K;
+    ahead_H[w][lane] = scan.H;
+    ahead_rest[w][lane] = rest;
     asm volatile("bar.sync 3, %0;" ::"n"(32 * BW) : "memory");
 #pragma unroll 1
     for (int k = 0; k < w; ++k) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) h.set(v, pass<RESET>(h.get(v), ahead[k][lane * V + v]));
+      const F H = ahead_H[k][lane], r = ahead_rest[k][lane];
+      const F to = vfma(r, h, vfma(ahead_K[k][lane], h, H));
+      h = RESET && r.get(0) < 0.f ? H : to;         // (a reset cuts all of a batch row's channels)
     }
     const RowsOut<T, V, FEED> dz(rows + 2 * TENSOR, p.dz, p.sdz, t0, at.b, i, p.d, steps);
     F q[BL];                              // a becomes (p - c) u (1 - u): df = g a
@@ -1191,7 +1238,7 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
       if (RESET) h = unless(cut >> l & 1, h);
       const F prev = vsub(h, c.get(l));
       a[l] = vmul(a[l], prev);
-      h = vsub(h, vmul(u[l], prev));
+      h = vfma(nu[l], prev, h);
       const F x = z.get(l), gy = dy.get(l);
       F e;
       const F sg = gate_of(vmul(x, F(-LOG2E)), e), zs = vmul(x, sg);
@@ -1207,10 +1254,10 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
 #pragma unroll
     for (int l = BL - 1; l >= 0; --l) {
       const F gt = vadd(q[l], E);
-      E = vsub(gt, vmul(u[l], gt));
+      E = vfma(nu[l], gt, gt);
       if (RESET) E = unless(cut >> l & 1, E);
     }
-    leave_pair<V, BW>(sh, BW - 1 - w, R, E);
+    leave_stretch<V, BW, RESET>(sh, BW - 1 - w, scan, E, cut);
     if (!take_state<V, BW>(sh, s, BW - 1 - w, D)) {
       fd.gave_up = 1;
       return;
@@ -1218,10 +1265,10 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
     const RowsOut<T, V, FEED> df(rows, p.df, p.sdf, t0, at.b, i, p.d, steps), dc(rows + TENSOR, p.dc, p.sdc, t0, at.b, i, p.d, steps);
 #pragma unroll
     for (int l = BL - 1; l >= 0; --l) {
-      const F gt = vadd(q[l], D), gu = vmul(gt, u[l]);
+      const F gt = vadd(q[l], D);
       df.put(l, vmul(gt, a[l]));
-      dc.put(l, gu);
-      D = vsub(gt, gu);
+      dc.put(l, vmul(gt, nu[l]), true);
+      D = vfma(nu[l], gt, gt);
       if (RESET) D = unless(cut >> l & 1, D);
     }
     if (t0 == 0) write_state<V>(p.dh0, at.b, i, p.d, D);
