@@ -465,6 +465,32 @@ constexpr int FW = 8, FL = 16;      // forward tile: 128 steps
 constexpr int BW = 8, BL = 8;       // backward tile: GL_CHUNK steps, so that it starts at a saved state
 static_assert(BW * BL == GL_CHUNK && GL_CHUNK % FL == 0, "saved states lie on tile and warp edges");
 
+// A warp's last steps once more, from memory: for a state that the steps past the sequence's end, whose gates are zero, have
+// turned from infinite into NaN (0 inf).
+template <typename T, int V, bool RESET>
+__device__ __forceinline__ Vec<V> walk(const GlParams& p, Vec<V> h, int t0, int b, int i) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if (i + v >= p.d) continue;
+    const T* f = (const T*)p.f + b * p.sf.b + i + v;
+    const T* c = (const T*)p.c + b * p.sc.b + i + v;
+    Vec<1> x(h.get(v)), e;
+#pragma unroll 1
+    for (int t = t0; t < p.T; ++t) {
+      if (RESET && p.reset[(long)t * p.B + b] != 0) x = Vec<1>(0.f);
+      x = vfma(gate_of<1, true>(vmul(Vec<1>(to_f(f[t * p.sf.t])), Vec<1>(LOG2E)), e), vsub(x, Vec<1>(to_f(c[t * p.sc.t]))), x);
+    }
+    h.set(v, x.x);
+  }
+  return h;
+}
+template <int V> __device__ __forceinline__ bool any_nan(Vec<V> h) {
+  bool nan = false;
+#pragma unroll
+  for (int v = 0; v < V; ++v) nan = nan || h.get(v) != h.get(v);
+  return nan;
+}
+
 // What both kernels know of the tile they are at.
 template <int V> struct Tile {
   int n, b, i;
@@ -543,6 +569,11 @@ __global__ void __launch_bounds__(32 * FW, 2) gl_forward_tile_kernel(GlParams p,
       if (at.on && l < steps) __stcs(reinterpret_cast<typename Ln::Raw*>(y + l * step), Ln::put(out));
     }
     if (at.on && steps > 0 && steps <= FL) {
+      if (steps < FL && any_nan(h)) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) h.set(v, sh.enters[w][(threadIdx.x & 31) * V + v]);
+        h = walk<T, V, RESET>(p, h, t0, at.b, at.i);
+      }
 #pragma unroll
       for (int v = 0; v < V; ++v) p.h_last[at.col + v] = h.get(v);
     }
@@ -574,13 +605,13 @@ __global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p
     load_rows<T, V, BL>(rc, p.c, p.sc, t0, p.T, at.b, at.i);
     load_rows<T, V, BL>(rz, p.z, p.sz, t0, p.T, at.b, at.i);
     load_rows<T, V, BL>(rdy, p.dy, p.sy, t0, p.T, at.b, at.i);
-    F h(0.f), initial(0.f);
+    F h(0.f), last(0.f);
     if (at.on) {
 #pragma unroll
       for (int v = 0; v < V; ++v) h.set(v, p.saved[(long)chunk * cols + at.col + v]);
-      if (w == warps - 1 && at.n < GROUP && p.dh_last != nullptr) {
+      if (steps > 0 && steps <= BL && p.dh_last != nullptr) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) initial.set(v, p.dh_last[at.col + v]);
+        for (int v = 0; v < V; ++v) last.set(v, p.dh_last[at.col + v]);
       }
     }
     const uint32_t cut = RESET ? reset_bits<BL>(p, t0, at.b) : 0;
@@ -629,10 +660,9 @@ __global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p
       const F out = vmul(vmul(dy, h), vfma(zs, vsub(F(1.f), s), s));
       if (at.on && l < steps) __stcs(reinterpret_cast<typename Ln::Raw*>(dz + l * step_z), Ln::put(out));
     }
-    if (steps < BL) {
+    if (steps <= BL) {
 #pragma unroll
-      for (int l = 0; l < BL; ++l)
-        if (l >= steps) q[l] = F(0.f);
+      for (int l = 0; l < BL; ++l) q[l] = l >= steps ? F(0.f) : l == steps - 1 ? vadd(q[l], last) : q[l];
     }
     F E(0.f), D;
 #pragma unroll
@@ -641,7 +671,7 @@ __global__ void __launch_bounds__(32 * BW, 2) gl_backward_tile_kernel(GlParams p
       E = vfma(nu[l], g, g);
       if (RESET) E = unless(cut >> l & 1, E);
     }
-    if (!enter<V, BW, RESET>(sh, warps - 1 - w, warps, K, E, at.n, tiles, at.base, cols, initial, ch, ticket, grabbed, D)) return;
+    if (!enter<V, BW, RESET>(sh, warps - 1 - w, warps, K, E, at.n, tiles, at.base, cols, F(0.f), ch, ticket, grabbed, D)) return;
     ticket = tiles > 1 ? sh.next : total;
     char* df = (char*)p.df + ((long)t0 * p.sdf.t + at.b * p.sdf.b + at.i) * (long)sizeof(T);
     char* dc = (char*)p.dc + ((long)t0 * p.sdc.t + at.b * p.sdc.b + at.i) * (long)sizeof(T);
@@ -1123,7 +1153,14 @@ gl_forward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_const
       h = vfma(nu[l], vsub(h, c.get(l)), h);
       y.put(l, vmul(h, zs[l]));
     }
-    if (steps > 0 && steps <= FL) write_state<V>(p.h_last, at.b, i, p.d, h);
+    if (steps > 0 && steps <= FL) {
+      if (steps < FL && any_nan(h)) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) h.set(v, sh.enters[w][lane * V + v]);
+        h = walk<T, V, RESET>(p, h, t0, at.b, i);
+      }
+      write_state<V>(p.h_last, at.b, i, p.d, h);
+    }
     ptx::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(&fd.done[s]);
@@ -1168,7 +1205,7 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
     return;
   }
   if (w >= BW) {
-    link_tiles<V, BW, RESET>(sh, fd, p, ch, g, p.dh_last);
+    link_tiles<V, BW, RESET>(sh, fd, p, ch, g, nullptr);
     return;
   }
   for (int it = 0;; ++it) {
@@ -1245,10 +1282,10 @@ gl_backward_fed_kernel(const __grid_constant__ CUtensorMap tf, const __grid_cons
       q[l] = vmul(gy, zs);
       dz.put(l, vmul(vmul(gy, h), vfma(zs, vsub(F(1.f), sg), sg)));
     }
-    if (steps < BL) {
+    if (steps <= BL) {                    // dh_last goes in with the last step (passed on to it, an infinite one would meet 0 inf)
+      const F last = steps > 0 ? read_state<V>(p.dh_last, at.b, i, p.d) : F(0.f);
 #pragma unroll
-      for (int l = 0; l < BL; ++l)
-        if (l >= steps) q[l] = F(0.f);
+      for (int l = 0; l < BL; ++l) q[l] = l >= steps ? F(0.f) : l == steps - 1 ? vadd(q[l], last) : q[l];
     }
     F E(0.f), D;
 #pragma unroll

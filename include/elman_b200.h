@@ -588,6 +588,8 @@ int elman_e1_lm_token(int dtype, int depth, int B, int d, int vocab, const long 
  * reset [T,B] (NULL: none): non-zero where step t starts a new sequence and forgets the state.
  * saved [ceil(T / ELMAN_GATED_LINEAR_CHUNK), B, d] fp32: written by the forward call with `training`, read
  * by the backward call, which takes the inputs of that forward call again.  T = 1 is the generation step.
+ * A state or gradient that is infinite is so for the step it arises in (h_last, dc and dh0 included) and NaN from the
+ * next one on, p + u (c - p) having no other value, until a reset.
  * elman_gated_linear_workspace covers both directions; 0 bytes: none is needed.  The workspace is 16-byte aligned, every
  * other pointer on a boundary of its elements.
  */
