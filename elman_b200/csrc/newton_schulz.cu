@@ -247,7 +247,9 @@ __global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n,
   static_assert(NORM_PARTS == 64, "two partial sums a lane");
   double total = partial[(long)blockIdx.y * NORM_PARTS + lane] + partial[(long)blockIdx.y * NORM_PARTS + 32 + lane];
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
-  const float scale = (float)(SX / (sqrt(total) + (double)eps));
+  // (a zero matrix stays zero without eps too; beyond fp32's range, or where it gets thin, the scale is two factors)
+  const double whole = total == 0. ? 0. : SX / (sqrt(total) + (double)eps);
+  const float first = whole > 0x1p90 ? 0x1p100f : whole < 0x1p-90 ? 0x1p-60f : 1.f, scale = (float)(whole / (double)first);
   const long size = (long)m * n;
   const T* in = (const T*)s.in + (s.offsets != nullptr ? s.offsets[blockIdx.y] : (long)blockIdx.y * size);
   const float* momentum = s.momentum != nullptr ? s.momentum + (long)blockIdx.y * size : nullptr;
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n,
           for (int j = 0; j < 8; ++j) f[j] = look_ahead(s, f[j], gs, mom[j]);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= scale;
+        for (int j = 0; j < 8; ++j) f[j] = f[j] * first * scale;
         const uint4 h = to_halves(f);
         *reinterpret_cast<uint4*>(x.hi + to + col) = h;
         add_halves(f, h, -1.f);
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n,
       for (int col = lane; col < n; col += 32) {
         float v = to_f(in[from + col]);
         if (momentum != nullptr) v = look_ahead(s, v, gs, momentum[from + col]);
-        v *= scale;
+        v = v * first * scale;
         const __half hi = __float2half_rn(v);
         x.hi[to + col] = hi;
         x.lo[to + col] = __float2half_rn(v - __half2float(hi));
