@@ -15,6 +15,8 @@
 // products take turns in three sums and the small ones have a fourth (3.4e-6 at 200 x 2000, 1.2e-5 at 200 x 9000, 2.9e-5 at
 // 1000 x 20000).  A step along K brings the high parts of both operands in one stage and the low parts in the next, for all
 // three products: 4 x 1000 x 257 fp32 250 us with a stage a product, now 188.
+// A start below 1e-4 (a norm far below eps) would lose its low parts under fp16's range: X is held as 2^e X, with an e for each
+// matrix and step that follows from the norm and what the polynomial can make of it.
 #include <math.h>
 
 #include <mutex>
@@ -43,6 +45,7 @@ constexpr int BOX_BYTES = 32 * 64, BUFFER_BYTES = 2 * BOX_BYTES;
 constexpr int NS_SMEM = STAGES * 2 * OPERAND_BYTES + EPI_WARPS * BUFFER_BYTES + 1024;
 constexpr float SX = 4096.f, SA = 4096.f, SB = 1024.f;
 constexpr int NORM_PARTS = 64;                        // partial sums of squares a matrix
+constexpr int SHIFTS = 128;                           // exponents kept a matrix: one in front of each of 100 steps at most, and behind
 
 enum Product { GRAM, SQUARE, UPDATE, LAST };
 // An operand block of rows x K: stored [rows, K]; stored [K, rows] and read MN-major in place; or part of a
@@ -86,6 +89,7 @@ struct NsPlan {
   float lr, decay, scale;    // Muon: p = p decay - lr scale X
   int* ticket;               // items handed out
   int* done;                 // [count]: warps' shares of tiles finished
+  const unsigned char* shift;   // [count][SHIFTS]: step k starts from 2^shift X
   int* status;
   long spin_limit;
   int stall, leave;          // test hooks: a stage that is not loaded; 32 q + w: warp w gives up the wait for its block's item q
@@ -93,7 +97,7 @@ struct NsPlan {
 
 // One item of the list.  Taking it apart costs divisions, a thousand cycles of latency: the warp that takes items does
 // it ahead of time and hands on the four numbers that the rest follows from.
-struct alignas(16) NsSlot { int kind, mat, tile, step; };     // kind -1: no more
+struct alignas(16) NsSlot { int kind, mat, tile, step; };     // kind -1: no more; step with the exponents before and after it
 __device__ __forceinline__ NsSlot slot_of(const NsPlan& p, int index) {
   NsSlot k;
   k.step = index / p.per_step;
@@ -120,16 +124,21 @@ __device__ __forceinline__ NsSlot slot_of(const NsPlan& p, int index) {
     tj = t - ti * tiles_n;
   }
   k.tile = ti << 16 | tj;
+  const unsigned char* e = p.shift + (long)k.mat * SHIFTS + k.step;
+  k.step |= e[0] << 8 | e[1] << 16;
   return k;
 }
+__device__ __forceinline__ int step_of(NsSlot k) { return k.step & 0xFF; }
 struct NsItem {
   int kind, mat, ti, tj, step;
   int columns;                                 // of the tile
+  int e, e_next;                               // X is held at 2^e of itself, and the step's result at 2^e_next
   int m, n, K, a_form, b_form;
 };
 __device__ __forceinline__ NsItem item_of(const NsPlan& p, NsSlot k) {
   NsItem it;
-  it.kind = k.kind; it.mat = k.mat; it.ti = k.tile >> 16; it.tj = k.tile & 0xFFFF; it.step = k.step;
+  it.kind = k.kind; it.mat = k.mat; it.ti = k.tile >> 16; it.tj = k.tile & 0xFFFF; it.step = step_of(k);
+  it.e = k.step >> 8 & 0xFF; it.e_next = k.step >> 16;
   const bool symmetric = k.kind == GRAM || k.kind == SQUARE;
   it.columns = symmetric ? p.n_sym : p.n_upd;
   it.m = symmetric ? p.r : p.m;
@@ -145,7 +154,7 @@ __device__ __forceinline__ NsItem item_of(const NsPlan& p, NsSlot k) {
 }
 // Tiles of its matrix that have to be finished before an item may start.
 __device__ __forceinline__ int needed(const NsPlan& p, NsSlot k) {
-  return k.step * (2 * p.triangle + p.all) + (k.kind == GRAM ? 0 : k.kind == SQUARE ? p.triangle : 2 * p.triangle);
+  return step_of(k) * (2 * p.triangle + p.all) + (k.kind == GRAM ? 0 : k.kind == SQUARE ? p.triangle : 2 * p.triangle);
 }
 
 __device__ __forceinline__ void add_halves(float (&f)[8], uint4 x, float k) {
@@ -238,9 +247,33 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsSource s, long size, dou
   }
 }
 
-// A warp a row: X_0, scaled, as the sum of two fp16 numbers.
+struct Quintic { double a, b, c; };
+// The largest |s (a + b s^2 + c s^4)| of s in [0, top].
+__host__ __device__ inline double largest(Quintic q, double top) {
+  auto poly = [&](double s2) { return fabs(sqrt(s2) * (q.a + s2 * (q.b + q.c * s2))); };
+  double most = poly(top * top);
+  auto see = [&](double s2) {
+    if (s2 > 0. && s2 < top * top) most = fmax(most, poly(s2));
+  };
+  if (q.c != 0.) {
+    const double disc = 9. * q.b * q.b - 20. * q.a * q.c;
+    if (disc >= 0.) {
+      see((-3. * q.b + sqrt(disc)) / (10. * q.c));
+      see((-3. * q.b - sqrt(disc)) / (10. * q.c));
+    }
+  } else if (q.b != 0.) {
+    see(-q.a / (3. * q.b));
+  }
+  return most;
+}
+// The exponent that brings values of up to `top` to between 1/2 and 1; those above stay.
+__host__ __device__ inline int lift(double top) { return top >= 0.5 ? 0 : top < 0x1p-126 ? 126 : -ilogb(top) - 1; }
+
+// A warp a row: X_0, scaled, as the sum of two fp16 numbers; and the exponents of the steps.  `shrinks`: the polynomial
+// brings singular values of up to one below one half on its way.
 template <typename T>
-__global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n, long ld, float eps, const double* partial, Split x) {
+__global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n, long ld, float eps, const double* partial, Split x,
+                                                       unsigned char* shift, int steps, Quintic q, int shrinks) {
   ptx::let_next_start();
   ptx::wait_for_previous();
   const int lane = threadIdx.x & 31;
@@ -248,8 +281,22 @@ __global__ void __launch_bounds__(256) ns_scale_kernel(NsSource s, int m, int n,
   double total = partial[(long)blockIdx.y * NORM_PARTS + lane] + partial[(long)blockIdx.y * NORM_PARTS + 32 + lane];
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
   // (a zero matrix stays zero without eps too; beyond fp32's range, or where it gets thin, the scale is two factors)
-  const double whole = total == 0. ? 0. : SX / (sqrt(total) + (double)eps);
+  const double norm = sqrt(total), start = norm / (norm + (double)eps);
+  const bool plain = !(start < 0.5) && !shrinks;      // (NaN as well)
+  const double whole = (total == 0. ? 0. : SX / (norm + (double)eps)) * (plain ? 1. : ldexp(1., lift(start)));
   const float first = whole > 0x1p90 ? 0x1p100f : whole < 0x1p-90 ? 0x1p-60f : 1.f, scale = (float)(whole / (double)first);
+  if (blockIdx.x == 0 && threadIdx.x < 32) {
+    shift += (long)blockIdx.y * SHIFTS;
+    if (plain) {
+      reinterpret_cast<uint32_t*>(shift)[lane] = 0;
+    } else if (lane == 0) {
+      double top = start;
+      for (int k = 0; k <= steps; ++k) {
+        shift[k] = (unsigned char)lift(top);
+        top = largest(q, top);
+      }
+    }
+  }
   const long size = (long)m * n;
   const T* in = (const T*)s.in + (s.offsets != nullptr ? s.offsets[blockIdx.y] : (long)blockIdx.y * size);
   const float* momentum = s.momentum != nullptr ? s.momentum + (long)blockIdx.y * size : nullptr;
@@ -293,9 +340,10 @@ __device__ __forceinline__ void sts_u4(uint32_t addr, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// What becomes of a product: k_acc * product + k_same * same.
+__device__ __forceinline__ float power_of_two(int e) { return e < -126 ? 0.f : __int_as_float((e + 127) << 23); }
+// What becomes of a product: k_acc * product + k_same * same; the last step's result times k_last.
 struct Finish {
-  float k_acc, k_same;
+  float k_acc, k_same, k_last;
   Split same, out;                 // at the item's matrix
   long ld;
 };
@@ -306,14 +354,17 @@ __device__ __forceinline__ Finish finish_of(const NsPlan& p, const NsItem& it) {
     f.ld = p.ldr;
     f.same = p.A;
     f.out = it.kind == GRAM ? p.A : p.B;
-    f.k_acc = it.kind == GRAM ? SA / (SX * SX) : p.c * (SB / (SA * SA));
-    f.k_same = p.b * (SB / SA);
+    // (A is that of 2^e X, B is X's)
+    f.k_acc = it.kind == GRAM ? SA / (SX * SX) : p.c * (SB / (SA * SA)) * power_of_two(-4 * it.e);
+    f.k_same = p.b * (SB / SA) * power_of_two(-2 * it.e);
   } else {
     f.ld = p.ldx;
     f.same = p.X[at];
     f.out = p.X[at ^ 1];
-    f.k_acc = it.kind == LAST ? 1.f / (SB * SX) : 1.f / SB;
-    f.k_same = it.kind == LAST ? p.a / SX : p.a;
+    const float to = it.kind == LAST ? 1.f / SX : power_of_two(it.e_next - it.e);
+    f.k_acc = to / SB;
+    f.k_same = p.a * to;
+    f.k_last = power_of_two(-it.e);
   }
   const long off = (long)it.mat * it.m * f.ld;
   f.same.hi += off;
@@ -684,7 +735,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_kernel(const __grid_constant__ 
           }
           if (it.kind == LAST) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r[8 * g + j] = __float_as_uint(f[j]);
+            for (int j = 0; j < 8; ++j) r[8 * g + j] = __float_as_uint(f[j] * fin.k_last);
             continue;
           }
           const uint4 h = to_halves(f);
@@ -744,6 +795,7 @@ struct NsBuffers {
   double* partial;
   int* ticket;
   int* done;
+  unsigned char* shift;
   long ldx, ldr;
   size_t bytes;
 };
@@ -771,38 +823,29 @@ NsBuffers carve(void* ws, int count, int m, int n) {
   b.partial = (double*)take((size_t)count * NORM_PARTS * sizeof(double));
   b.ticket = (int*)take(sizeof(int));
   b.done = (int*)take((size_t)count * sizeof(int));
+  b.shift = (unsigned char*)take((size_t)count * SHIFTS);
   b.bytes = off;
   return b;
 }
 
 // The largest singular value that `steps` applications make of values in [0, 1], and the largest |B|: both
 // have to stay inside fp16's range at their scales.
-bool stays_in_range(int steps, double a, double b, double c) {
+bool stays_in_range(int steps, Quintic q) {
   double top = 1.;
   for (int k = 0; k < steps; ++k) {
-    auto poly = [&](double s) { return fabs(s * (a + s * s * (b + c * s * s))); };
-    auto inner = [&](double s) { return fabs(s * s * (b + c * s * s)); };
-    double most = poly(top), most_b = inner(top);
-    auto see = [&](double s2) {
-      if (s2 > 0. && s2 < top * top) {
-        most = fmax(most, poly(sqrt(s2)));
-        most_b = fmax(most_b, inner(sqrt(s2)));
-      }
-    };
-    if (c != 0.) {
-      const double disc = 9. * b * b - 20. * a * c;
-      if (disc >= 0.) {
-        see((-3. * b + sqrt(disc)) / (10. * c));
-        see((-3. * b - sqrt(disc)) / (10. * c));
-      }
-      see(-b / (2. * c));
-    } else if (b != 0.) {
-      see(-a / (3. * b));
-    }
+    auto inner = [&](double s2) { return fabs(s2 * (q.b + q.c * s2)); };
+    const double most = largest(q, top), turn = q.c != 0. ? -q.b / (2. * q.c) : 0.;
+    const double most_b = turn > 0. && turn < top * top ? fmax(inner(top * top), inner(turn)) : inner(top * top);
     if (!(most_b <= 60.) || !(most <= 3.5)) return false;
     top = most;
   }
   return true;
+}
+bool shrinks(int steps, Quintic q) {
+  double top = 1.;
+  for (int k = 0; k < steps; ++k)
+    if ((top = largest(q, top)) < 0.5) return true;
+  return false;
 }
 
 // Pairs make four times the tile of a single block with half as many units.  Measured, us: a step along K (three products)
@@ -873,9 +916,10 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   p.r = p.tall ? g.n : g.m;
   p.steps = g.steps;
   p.a = g.a; p.b = g.b; p.c = g.c;
+  const Quintic quintic{g.a, g.b, g.c};
   p.X[0] = buf.X[0]; p.X[1] = buf.X[1]; p.A = buf.A; p.B = buf.B;
   p.ldx = buf.ldx; p.ldr = buf.ldr;
-  p.ticket = buf.ticket; p.done = buf.done;
+  p.ticket = buf.ticket; p.done = buf.done; p.shift = buf.shift;
   p.status = device_status_ptr();
   p.spin_limit = options().spin_limit;
   p.stall = (int)options().test_stall_step;
@@ -919,7 +963,8 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  ELMAN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ns_scale_kernel<T>, src, p.m, p.n, buf.ldx, g.eps, (const double*)buf.partial, buf.X[0]));
+  ELMAN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ns_scale_kernel<T>, src, p.m, p.n, buf.ldx, g.eps, (const double*)buf.partial, buf.X[0],
+                                     buf.shift, p.steps, quintic, (int)shrinks(p.steps, quintic)));
   count_launch(false);
   ELMAN_CUDA_CHECK(cudaGetLastError());
   if constexpr (sizeof(T) == 2)
@@ -930,7 +975,7 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
 }  // namespace
 
 size_t newton_schulz_workspace(int, int count, int m, int n) { return carve(nullptr, count, m, n).bytes; }
-bool newton_schulz_in_range(int steps, float a, float b, float c) { return stays_in_range(steps, a, b, c); }
+bool newton_schulz_in_range(int steps, float a, float b, float c) { return stays_in_range(steps, Quintic{a, b, c}); }
 
 int newton_schulz(const NewtonSchulzArgs& a, cudaStream_t st) {
   NsSource src{};
