@@ -94,6 +94,7 @@ SIGNATURES = {
     "elman_gated_linear_forward": (_I, [_I] * 5 + [_P] * 9 + [_P, _Z, _P]),
     "elman_gated_linear_backward": (_I, [_I] * 4 + [_P] * 12 + [_P, _Z, _P]),
     "elman_newton_schulz_workspace": (_Z, [_I] * 4),
+    "elman_newton_schulz_tile": (_I, [_I] * 4),
     "elman_newton_schulz": (_I, [_I] * 4 + [_P, _P, _I] + [_F] * 4 + [_P, _Z, _P]),
     "elman_muon_step": (_I, [_I] * 4 + [_P] * 4 + [_F, _F, _I, _F, _F, _P, _I] + [_F] * 4 + [_P, _Z, _P]),
     "elman_projection": (_I, [_I, _I, _I, _I, _P, _I, _P, _I, _P, _P, _I, _I, _P]),

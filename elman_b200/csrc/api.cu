@@ -1841,6 +1841,11 @@ size_t elman_newton_schulz_workspace(int dtype, int count, int m, int n) {
   return newton_schulz_workspace(dtype, count, m, n);
 }
 
+int elman_newton_schulz_tile(int dtype, int count, int m, int n) {
+  if ((dtype != ELMAN_F32 && dtype != ELMAN_BF16) || count <= 0 || m <= 0 || n <= 0) return 0;
+  return newton_schulz_tile(dtype, count, m, n);
+}
+
 int elman_newton_schulz(int dtype, int count, int m, int n, const void* in, void* out, int steps, float a,
                         float b, float c, float eps, void* workspace, size_t workspace_bytes, void* stream) {
   ELMAN_RETURN_IF(check_newton_schulz(dtype, count, m, n, steps, a, b, c, eps, workspace, workspace_bytes));

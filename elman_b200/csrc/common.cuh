@@ -408,6 +408,7 @@ struct MuonArgs {
   const float* grad_scale;            // device, or null
 };
 size_t newton_schulz_workspace(int dtype, int count, int m, int n);
+int newton_schulz_tile(int dtype, int count, int m, int n);
 bool newton_schulz_in_range(int steps, float a, float b, float c);
 int newton_schulz(const NewtonSchulzArgs& a, cudaStream_t stream);
 int muon_step(const NewtonSchulzArgs& a, const MuonArgs& u, cudaStream_t stream);

@@ -863,6 +863,7 @@ bool pays_as_pairs(const NsPlan& p) {
   };
   return cost(256, 74, 1.32, 0.5, 0.9, 9.8) < cost(128, 148, 0.95, 1.5, 0.7, 5.9);
 }
+bool as_pairs(int dtype, const NsPlan& p) { return dtype == ELMAN_BF16 && pays_as_pairs(p); }
 // Tiles of the blocks (i, j >= i) of a symmetric product.
 int triangle_of(int r, int edge, int columns) {
   const int per = edge / columns, strips = (r + columns - 1) / columns, whole = strips / per;
@@ -924,7 +925,7 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
   p.spin_limit = options().spin_limit;
   p.stall = (int)options().test_stall_step;
   p.leave = (int)options().test_leave_warp;
-  const bool pair = sizeof(T) == 2 && pays_as_pairs(p);
+  const bool pair = as_pairs(g.dtype, p);
   const int edge = pair ? 256 : 128;
   p.edge = p.n_sym = p.n_upd = edge;
   const int upd_rows = (p.m + edge - 1) / edge;
@@ -975,6 +976,11 @@ int run(const NewtonSchulzArgs& g, const NsSource& src, NsPlan p, cudaStream_t s
 }  // namespace
 
 size_t newton_schulz_workspace(int, int count, int m, int n) { return carve(nullptr, count, m, n).bytes; }
+int newton_schulz_tile(int dtype, int count, int m, int n) {
+  NsPlan p{};
+  p.count = count; p.m = m; p.n = n; p.tall = m > n; p.r = p.tall ? n : m;
+  return as_pairs(dtype, p) ? 256 : 128;
+}
 bool newton_schulz_in_range(int steps, float a, float b, float c) { return stays_in_range(steps, Quintic{a, b, c}); }
 
 int newton_schulz(const NewtonSchulzArgs& a, cudaStream_t st) {

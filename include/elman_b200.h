@@ -624,6 +624,9 @@ int elman_gated_linear_backward(int dtype, int T, int B, int d, const void* f, c
  * all in fp32 but for the parameters themselves.
  */
 size_t elman_newton_schulz_workspace(int dtype, int count, int m, int n);
+/* Rows of the tiles that a call of these sizes makes: 256 on pairs of blocks, 128 on single ones (0: nothing to do).  Two
+ * calls with the same tiles give a matrix the same bits; others may differ in the last ones. */
+int elman_newton_schulz_tile(int dtype, int count, int m, int n);
 int elman_newton_schulz(int dtype, int count, int m, int n, const void* in, void* out, int steps, float a,
                         float b, float c, float eps, void* workspace, size_t workspace_bytes, void* stream);
 int elman_muon_step(int dtype, int count, int m, int n, const long long* offsets, void* params,
