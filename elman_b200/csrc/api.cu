@@ -1,5 +1,6 @@
 // C ABI of the library: argument checks, workspace carving and the sequence of
 // kernels behind each entry point declared in include/elman_b200.h.
+#include <limits.h>
 #include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
@@ -1735,6 +1736,7 @@ static bool outputs_apart(int dtype, int T, int B, int d, const void* x, const l
 
 static int check_gated_linear(int dtype, int T, int B, int d, const long* strides, int n_in, int n_out) {
   ELMAN_RETURN_IF(check_common(dtype, T, B, d));
+  ELMAN_ARG_CHECK(T <= INT_MAX - 1024, "sequence too long");       // (the last tile's steps are counted past the end)
   REQUIRE_PTR(strides);
   for (int k = 0; k < 2 * (n_in + n_out); ++k)
     ELMAN_ARG_CHECK(strides[k] >= 0, "negative stride");

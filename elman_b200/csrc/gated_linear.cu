@@ -1354,7 +1354,7 @@ long whole_groups(int dtype, int d) {
 }
 // A batch row's last group should not be mostly empty: narrower rows go to the kernels that count channels through, which
 // reach about two thirds of the speed.
-bool whole_width(int dtype, int d) { return whole_groups(dtype, d) <= d + d / 2; }
+bool whole_width(int dtype, int d) { return whole_groups(dtype, d) <= (long)d + d / 2; }
 FeedKind feed_of(int dtype, const GatedLinearArgs& a, bool bwd) {
   const long per16 = dtype == ELMAN_F32 ? 4 : 8, most = (1L << 39) / 4;
   bool ok = a.T <= (1 << 30) && a.B <= (1 << 30);

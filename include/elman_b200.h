@@ -590,6 +590,7 @@ int elman_e1_lm_token(int dtype, int depth, int B, int d, int vocab, const long 
  * by the backward call, which takes the inputs of that forward call again.  T = 1 is the generation step.
  * A state or gradient that is infinite is so for the step it arises in (h_last, dc and dh0 included) and NaN from the
  * next one on, p + u (c - p) having no other value, until a reset.
+ * At most 2^31 - 1025 steps.
  * elman_gated_linear_workspace covers both directions; 0 bytes: none is needed.  The workspace is 16-byte aligned, every
  * other pointer on a boundary of its elements.
  */
