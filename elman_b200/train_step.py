@@ -373,9 +373,11 @@ class FlatAdamW:
 
 
 def hidden_matrices(model):
-    """The weight matrices inside a model's layers (not the embedding, the head or vectors): what Muon updates."""
-    return [p for layer in getattr(model, "layers", []) for p in layer.parameters()
-            if p.dim() == 2 and p.requires_grad]
+    """The weight matrices inside a model's layers (not the embedding, the head or vectors), each once: what Muon
+    updates."""
+    found = {id(p): p for layer in getattr(model, "layers", []) for p in layer.parameters()
+             if p.dim() == 2 and p.requires_grad}
+    return list(found.values())
 
 
 class FlatMuon:
