@@ -957,7 +957,7 @@ def gated_linear_backward(f, c, z, saved, d_output, dh_last=None, reset=None, ou
         else:
             df, dc, dz = out
             _check_sequences(fn, f, df=df, dc=dc, dz=dz)
-            used = {t.untyped_storage().data_ptr() for t in (f, c, z, saved, d_output)}
+            used = {t.untyped_storage().data_ptr() for t in (f, c, z, saved, d_output, dh_last, reset) if t is not None}
             if any(t.untyped_storage().data_ptr() in used for t in out if t.numel() > 0):
                 raise RuntimeError(f"{fn}: out must not share storage with the inputs")
         dh0 = torch.empty(B, d, dtype=torch.float32, device=device)
