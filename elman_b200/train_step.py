@@ -32,10 +32,12 @@ class GraphedTrainStep:
                  warmup_steps=3, after_backward=None, reducer=None):
         """`reducer` (a FlatGradients, optional): the gradients live in its flat buffer; it
         zeroes them, all-reduces them bucket by bucket while backward still runs (N > 1) and
-        clips them.  `after_backward(params)` (the older hook), if given, runs between
+        clips them.  A FlatAdamW or FlatMuon brings its own.  `after_backward(params)` (the older hook), if given, runs between
         backward and clipping, inside the captured step."""
         self.net, self.opt = net, optimizer
         self.after_backward = after_backward
+        if reducer is None and isinstance(optimizer, (FlatAdamW, FlatMuon)):
+            reducer = optimizer.grads      # its gradients are views: a step that did not zero them would add to the last one's
         self.reducer = reducer
         self.max_grad_norm = max_grad_norm
         self.autocast_dtype = autocast_dtype
