@@ -29,11 +29,12 @@ def raise_on_device_timeout(where="a replayed step"):
 
 class GraphedTrainStep:
     def __init__(self, net, optimizer, example_tokens, max_grad_norm=1.0, autocast_dtype=None,
-                 warmup_steps=3, after_backward=None, reducer=None):
+                 warmup_steps=3, after_backward=None, reducer=None, example_reset=None):
         """`reducer` (a FlatGradients, optional): the gradients live in its flat buffer; it
         zeroes them, all-reduces them bucket by bucket while backward still runs (N > 1) and
         clips them.  A FlatAdamW or FlatMuon brings its own.  `after_backward(params)` (the older hook), if given, runs between
-        backward and clipping, inside the captured step."""
+        backward and clipping, inside the captured step.  `example_reset` (bool like the tokens, optional): the net
+        is called with a reset mask (level "gated_linear": packed documents), and each step takes its own."""
         self.net, self.opt = net, optimizer
         self.after_backward = after_backward
         if reducer is None and isinstance(optimizer, (FlatAdamW, FlatMuon)):
@@ -42,6 +43,7 @@ class GraphedTrainStep:
         self.max_grad_norm = max_grad_norm
         self.autocast_dtype = autocast_dtype
         self.tokens = example_tokens.clone()
+        self.reset = None if example_reset is None else example_reset.clone()
         self.params = [p for g in optimizer.param_groups for p in g["params"]]
         side = torch.cuda.Stream(device=self.tokens.device)
         side.wait_stream(torch.cuda.current_stream(self.tokens.device))
@@ -66,11 +68,12 @@ class GraphedTrainStep:
             self.reducer.zero()          # also inside the captured step: one memset
         elif zero:
             self.opt.zero_grad(set_to_none=True)
+        more = {} if self.reset is None else {"reset": self.reset}
         if self.autocast_dtype is not None:
             with torch.autocast(device_type="cuda", dtype=self.autocast_dtype):
-                loss = self.net(self.tokens, return_loss=True)
+                loss = self.net(self.tokens, return_loss=True, **more)
         else:
-            loss = self.net(self.tokens, return_loss=True)
+            loss = self.net(self.tokens, return_loss=True, **more)
         loss.backward()
         if self.reducer is not None:
             self.reducer.finish()
@@ -89,11 +92,17 @@ class GraphedTrainStep:
         self.opt.step()
         return loss.detach()
 
-    def __call__(self, tokens):
-        """Copies `tokens` (host or device) into the captured input and replays the step.
-        Returns the captured loss tensor (valid until the next call)."""
+    def __call__(self, tokens, reset=None):
+        """Copies `tokens` (host or device), and the reset mask of a step captured with one, into the captured
+        inputs and replays the step.  Returns the captured loss tensor (valid until the next call)."""
+        if (reset is None) != (self.reset is None):
+            raise ValueError("GraphedTrainStep: this step was captured " + ("without" if self.reset is None else "with") + " a reset mask")
+        if reset is not None and reset.shape != self.reset.shape:
+            raise ValueError(f"GraphedTrainStep: reset has shape {tuple(reset.shape)}, expected {tuple(self.reset.shape)}")
         raise_on_device_timeout("GraphedTrainStep")   # covers every replay up to the last one
         self.tokens.copy_(tokens, non_blocking=True)
+        if reset is not None:
+            self.reset.copy_(reset, non_blocking=True)
         self.graph.replay()
         return self.loss
 
