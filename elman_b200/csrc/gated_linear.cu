@@ -9,8 +9,9 @@
 //
 // Bound by HBM: forward 4 values an element, backward 7 (each of f, c, z, dy read once, each result
 // written once); the backward pass recomputes the states from one in GL_CHUNK that the forward saved.
-// Measured, calls on bf16: T4096 B64 d1536 549 us forward (5.9 TB/s), 1110 backward (5.1 TB/s; instruction issue is next);
-// T65536 B1 d1280, where the columns are few and the tiles wait for the chain of states, 185 (3.6) and 339 (3.5).
+// Measured, calls on bf16, the same inputs again and again: T4096 B64 d1536 562 us forward (5.7 TB/s; 634 among other calls
+// with inputs that change), 1120 backward (5.0; instruction issue is next); T65536 B1 d1280, where the columns are few and the
+// tiles wait for the chain of states, 188 (3.6) and 340 (3.5).
 #include <string.h>
 
 #include <mutex>
@@ -132,8 +133,8 @@ __global__ void __launch_bounds__(128) gl_backward_seq_kernel(GlParams p) {
 // order by a counter: whoever a tile waits for has started before it and waits for nobody behind it.
 // ---------------------------------------------------------------------------
 // Long groups make the chain of states short, short ones leave fewer pairs to fold and registers to hold them.  Forward and
-// backward, us, with 8 / 10 / 16: T65536 B1 d1280 bf16 525 / 520 / 534, T65536 B1 d256 179 / 166 / 160, T4096 B64 d1536
-// 1649 / 1659 / 1693.
+// backward, us, with 8 / 10 / 16: T65536 B1 d1280 bf16 518 / 527 / 540, T65536 B1 d256 168 / 162 / 157, T4096 B64 d1536
+// 1670 / 1690 / 1736.
 constexpr int GROUP = 10;
 constexpr uint32_t NOT_YET = 0xFFFFFFFFu;
 
@@ -714,8 +715,8 @@ template <int IN, int ROWS, int FEED> struct Stages {
 };
 // Scanning warps of the forward tile (16 steps each; two stages of longer rows leave room for seven).
 constexpr int forward_warps(int feed) { return feed == FEED_TMA ? FW : 7; }
-// Producer warps for rows copied in blocks: two channels a lane are short of registers (T4096 B16 d1001 bf16 forward 166 us
-// with one, 193 with two, 213 with four), one is not (fp32 289, 247, 217).
+// Producer warps for rows copied in blocks: two channels a lane are short of registers (T4096 B16 d1001 bf16 forward 163 us
+// with one, 197 with two, 227 with four), one is not (fp32 288, 245, 215).
 constexpr int row_producers(int V) { return V == 2 ? 1 : 4; }
 constexpr int producer_threads(int feed, int V) { return feed == FEED_TMA ? 32 : 32 * row_producers(V); }
 struct GlTma {

@@ -3,9 +3,9 @@
 // (tall matrices: A = X^T X and X <- a X + X B, so that A has the smaller of the two extents, r).
 // A and B are symmetric: only the tiles on and above the diagonal are computed and stored.  Per step 3 r^2 q + r^3
 // flops with q the larger extent, three products for each of them (Numbers, below): bound by the tensor cores.
-// Measured, five steps on bf16, the same inputs again and again: 18 x 1280 x 1280 1.79 ms (1260 TFLOP/s of such products),
-// 1 x 4096 x 4096 2.98 ms (1380), at the power limit.  Small matrices are bound by the latency of 15 products one after
-// another: 1 x 256 x 256 109 us, 7 us each (about: loads 2, products 2, rows 1.5, stores made visible and seen 1.2).
+// Measured, five steps on bf16, the same inputs again and again: 18 x 1280 x 1280 1.79 ms (1260 TFLOP/s of such products, the
+// tensor pipe 90 % busy; 2.11 ms with inputs that change, at the power limit), 1 x 4096 x 4096 2.98 ms (1380).  Small matrices
+// are bound by the latency of 15 products one after another: 1 x 256 x 256 109 us, 7 us each.
 //
 // Numbers.  X, A and B are each kept as the sum of two fp16 numbers (22 significant bits), scaled by powers of two into
 // their range: X by 2^12, A by 2^12, B by 2^10.  A product is three: high x high, high x low, low x high; every sum is
@@ -14,7 +14,7 @@
 // rounding them, which over a long contraction adds up (2.5e-5 at 33 x 2000 with one sum): for fp32 matrices the large
 // products take turns in three sums and the small ones have a fourth (3.4e-6 at 200 x 2000, 1.2e-5 at 200 x 9000, 2.9e-5 at
 // 1000 x 20000).  A step along K brings the high parts of both operands in one stage and the low parts in the next, for all
-// three products: 4 x 1000 x 257 fp32 250 us with a stage a product, now 188.
+// three products: 4 x 1000 x 257 fp32 250 us with a stage a product, now 176.
 // A start below 1e-4 (a norm far below eps) would lose its low parts under fp16's range: X is held as 2^e X, with an e for each
 // matrix and step that follows from the norm and what the polynomial can make of it.
 #include <math.h>
@@ -39,8 +39,8 @@ constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
 constexpr int BLOCK_BYTES = 64 * BK * 2;              // one TMA box: 64 x 64 fp16
 constexpr int OPERAND_BYTES = 128 * BK * 2;
 // Rows are finished in boxes of 32 x 32 through shared memory, a box's high and low parts a warp, with plain 16-byte
-// accesses to global memory: the copy engine takes about two cycles a row of a box, and the operands' rows alone
-// (256 a stage of 512 cycles) fill its time.
+// accesses to global memory: the copy engine takes about two cycles a row of a box, and the operands' rows (512 a step
+// along K of 1536 cycles) take most of its time already.
 constexpr int BOX_BYTES = 32 * 64, BUFFER_BYTES = 2 * BOX_BYTES;
 constexpr int NS_SMEM = STAGES * 2 * OPERAND_BYTES + EPI_WARPS * BUFFER_BYTES + 1024;
 constexpr float SX = 4096.f, SA = 4096.f, SB = 1024.f;
@@ -73,8 +73,9 @@ struct NsMap { CUtensorMap rows[2], block[2]; };
 struct NsMaps { NsMap x[2], a, b; };
 
 // The whole iteration as one list of tiles: step by step, in a step all Gram tiles of all matrices, then the squares',
-// then the updates'.  (Groups of matrices that stay in L2 from product to product were slower: 18 x 1280 x 1280 as three
-// groups 0.98 ms, as one 0.87: waiting for the matrix one reads costs more than reading it from HBM.)
+// then the updates'.  (Groups of matrices that stay in L2 from product to product were slower, with one product where
+// there are three now: 18 x 1280 x 1280 as three groups 0.98 ms, as one 0.87: waiting for the matrix one reads costs more
+// than reading it from HBM.)
 struct NsPlan {
   int count, m, n, r, tall, steps;
   int edge, n_sym, n_upd;    // rows of a tile; columns of a symmetric product's tiles and of an update's
@@ -266,8 +267,8 @@ __host__ __device__ inline double largest(Quintic q, double top) {
   }
   return most;
 }
-// The exponent that brings values of up to `top` to between 1/2 and 1; those above stay.
-__host__ __device__ inline int lift(double top) { return top >= 0.5 ? 0 : top < 0x1p-126 ? 126 : -ilogb(top) - 1; }
+// The exponent that brings values of up to `top` to between 1/2 and 1; those above stay, and NaN.
+__host__ __device__ inline int lift(double top) { return !(top < 0.5) ? 0 : top < 0x1p-126 ? 126 : -ilogb(top) - 1; }
 
 // A warp a row: X_0, scaled, as the sum of two fp16 numbers; and the exponents of the steps.  `shrinks`: the polynomial
 // brings singular values of up to one below one half on its way.
@@ -422,7 +423,7 @@ __device__ __forceinline__ void write_result(const NsPlan& p, const NsItem& it, 
 // for someone who runs: no block has to be resident for another's sake, and launches may overlap.  With more than a
 // few matrices the wait is over before it begins.
 // Warp 3 of the even block takes items ahead of the others and waits until they may start, warps 0 and 2 load the
-// two operands (one thread issues a stage's copies in about 1000 cycles, twice what its products take), warp 1
+// two operands (one thread issues a stage's copies in about 1000 cycles, and a step's 1536 have two stages), warp 1
 // issues the products (for both blocks), the others finish the rows: two accumulators, so a tile is finished under
 // the next one's products.
 template <typename T, bool PAIR>
