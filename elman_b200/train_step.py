@@ -28,6 +28,8 @@ def raise_on_device_timeout(where="a replayed step"):
 
 
 class GraphedTrainStep:
+    reset = None
+
     def __init__(self, net, optimizer, example_tokens, max_grad_norm=1.0, autocast_dtype=None,
                  warmup_steps=3, after_backward=None, reducer=None, example_reset=None):
         """`reducer` (a FlatGradients, optional): the gradients live in its flat buffer; it
