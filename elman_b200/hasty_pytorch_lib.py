@@ -980,7 +980,8 @@ NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # singular values of (0
 def newton_schulz(G, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7):
     """The matrices G [..., m, n] with their singular values moved towards one and their singular vectors kept:
     X = G / (|G| + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T.  float32 or bfloat16,
-    contiguous; returns a tensor like G, which carries no gradient.  No counterpart in the reference."""
+    contiguous; returns a tensor like G, which carries no gradient: what products in 32 bits give, rounded once.  No
+    counterpart in the reference."""
     fn = "newton_schulz"
     dt = _check_inputs(fn, G, G=G)
     if G.dim() < 2:
