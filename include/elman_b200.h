@@ -588,6 +588,7 @@ int elman_e1_lm_token(int dtype, int depth, int B, int d, int vocab, const long 
  * reset [T,B] (NULL: none): non-zero where step t starts a new sequence and forgets the state.
  * saved [ceil(T / ELMAN_GATED_LINEAR_CHUNK), B, d] fp32: written by the forward call with `training`, read
  * by the backward call, which takes the inputs of that forward call again.  T = 1 is the generation step.
+ * A step rounds to 2^-24 of the larger of the states before and after it; what a state has left behind is forgotten with it.
  * A state or gradient that is infinite is so for the step it arises in (h_last, dc and dh0 included) and NaN from the
  * next one on, p + u (c - p) having no other value, until a reset.
  * At most 2^31 - 1025 steps.
